@@ -179,9 +179,9 @@ def run(s):
 
 
 def _run_own(case, s):
-    from compactwarprnntloss_b200 import distill_loss, fused_linear, token_scores
     x = s["x"]
     if case["op"] == "scores":
+        from compactwarprnntloss_b200 import token_scores
         r = token_scores(x, s["targets"], top_k=case["top"], entropy=case["entropy"], temperature=case["tau"])
         out = {"log_probs": r.log_probs, "entropy": r.entropy, "top": r.top_log_probs, "index": r.top_indices}
         if case["grad"]:
@@ -190,10 +190,12 @@ def _run_own(case, s):
             out["grad"], = torch.autograd.grad([o for o, _ in pairs], [x], [d for _, d in pairs])
         return out
     if case["op"] == "distill":
+        from compactwarprnntloss_b200 import distill_loss
         loss = distill_loss(x, s["teacher"], s["index"], weight=s["weight"], tail=case["tail"],
                             temperature=case["tau"], reduction="mean")
         grad, = torch.autograd.grad(loss, [x])
         return {"loss": loss, "grad": grad}
+    from compactwarprnntloss_b200 import fused_linear
     y = fused_linear(x, s["weight"], s["bias"], s["residual"], activation=s["activation"])
     out = {"y": y}
     if case["grad"]:
