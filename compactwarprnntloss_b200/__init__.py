@@ -7,6 +7,8 @@ Sub-modules:
   synth     seeded synthetic workloads of the benchmark configurations
   joint     `compact_joint` - the joint network's broadcast-add written directly as compact rows
   graphs    `GraphedStep` - a whole training step of the loss as one replayed CUDA graph per shape bucket
+  scores    `token_scores` - log-probabilities of given tokens, entropy and best alternatives of logits rows
+  distill   `distill_loss` - distillation from a teacher's top entries, loss and gradient in one pass
   analysis  `analyse` - best alignment, node posteriors and padded alpha / beta from a forward pass
   build     in-tree build of the native parts
 
@@ -29,4 +31,10 @@ def __getattr__(name):
     if name == "compact_joint":
         from . import joint
         return joint.compact_joint
+    if name in ("token_scores", "TokenScores"):
+        from . import scores
+        return getattr(scores, name)
+    if name == "distill_loss":
+        from . import distill
+        return distill.distill_loss
     raise AttributeError(name)

@@ -17,6 +17,7 @@ FUSED_LOG_SOFTMAX, COSTS_ONLY, REDUCE_MEAN, REDUCE_SUM, AVERAGE_FRAMES = 0x01, 0
 ST_BAD_LENGTH, ST_ROW_MISMATCH, ST_BAD_LABEL, ST_FWD_BWD_GAP = 0x01, 0x02, 0x04, 0x08
 MAX_COLUMNS = 4096
 STATIC_MAX_ROWS, STATIC_MAX_SEQUENCES = 131072, 1024
+MAX_LIST = 32
 ERR_CAPACITY = 5
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float64: F64}
@@ -30,6 +31,7 @@ EXPORTS = [
     "cwrnnt_scale_grad", "cwrnnt_pipeline_groups", "cwrnnt_joint_forward", "cwrnnt_joint_backward",
     "cwrnnt_pipe_wait_costs", "cwrnnt_validate", "cwrnnt_validate_async", "cwrnnt_static_status", "cwrnnt_fill_costs", "cwrnnt_recursion", "cwrnnt_alignment_scratch_bytes", "cwrnnt_export_alignment",
     "cwrnnt_export_posteriors", "cwrnnt_pipe_create_traced", "cwrnnt_pipe_timeline",
+    "cwrnnt_token_scores", "cwrnnt_token_scores_backward", "cwrnnt_distill_workspace_bytes", "cwrnnt_distill",
 ]
 
 
@@ -37,6 +39,13 @@ class Problem(ctypes.Structure):
     _fields_ = [("n_rows", ctypes.c_int64), ("V", ctypes.c_int32), ("B", ctypes.c_int32),
                 ("y_stride", ctypes.c_int32), ("max_u", ctypes.c_int32), ("blank", ctypes.c_int32),
                 ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32), ("mean_denominator", ctypes.c_int32)]
+
+
+class Rows(ctypes.Structure):
+    """cwrnnt_rows: what the operators on rows of logits (token scores, distillation) are told about them."""
+    _fields_ = [("n_rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("grad_stride", ctypes.c_int64),
+                ("temperature", ctypes.c_double), ("V", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("n_list", ctypes.c_int32), ("top_k", ctypes.c_int32)]
 
 
 class CwrnntError(RuntimeError):
@@ -100,6 +109,12 @@ def lib():
         L.cwrnnt_host_ctx_error.restype = ctypes.c_char_p
         L.cwrnnt_host_ctx_error.argtypes = [vp]
         L.cwrnnt_loss_grad_host.argtypes = [vp, pp, vp, vp, vp, vp, vp, i32, vp, vp, vp, i64, ctypes.POINTER(i32 * 4)]
+        rp = ctypes.POINTER(Rows)
+        L.cwrnnt_token_scores.argtypes = [rp, vp, vp, vp, vp, vp, vp, vp, vp]
+        L.cwrnnt_token_scores_backward.argtypes = [rp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        L.cwrnnt_distill_workspace_bytes.restype = i64
+        L.cwrnnt_distill_workspace_bytes.argtypes = [rp]
+        L.cwrnnt_distill.argtypes = [rp, i32, vp, vp, vp, vp, vp, i32, ctypes.c_double, vp, i64, vp, vp, vp, vp]
         _lib = L
     return _lib
 

@@ -80,6 +80,19 @@ int check_workspace(const cwrnnt_problem *p, const void *ws, int64_t bytes, Work
     return CWRNNT_OK;
 }
 
+int check_rows(const cwrnnt_rows *p)
+{
+    if (!p) return CWRNNT_ERR_ARGUMENT;
+    if (p->n_rows < 0 || p->n_rows > INT32_MAX || p->V < 1 || p->V > INT32_MAX - 64) return CWRNNT_ERR_ARGUMENT;
+    if (p->x_stride < p->V) return CWRNNT_ERR_ARGUMENT;
+    if (p->dtype < CWRNNT_F32 || p->dtype > CWRNNT_F64) return CWRNNT_ERR_ARGUMENT;
+    // log2(e) / tau is a factor of single-precision exponents: far from both ends of their range
+    if (!(p->temperature >= 1e-4 && p->temperature <= 1e4)) return CWRNNT_ERR_ARGUMENT;
+    if (p->n_list < 0 || p->n_list > CWRNNT_MAX_LIST) return CWRNNT_ERR_ARGUMENT;
+    if (p->top_k < 0 || p->top_k > CWRNNT_MAX_LIST || p->top_k > p->V) return CWRNNT_ERR_ARGUMENT;
+    return CWRNNT_OK;
+}
+
 }  // namespace
 
 void cwrnnt::set_last_error(const char *text) { std::snprintf(g_last_error, sizeof g_last_error, "%s", text); }
@@ -583,6 +596,67 @@ int cwrnnt_read_status(const void *workspace, int32_t out[4], cwrnnt_stream_t st
     cudaError_t e = cudaMemcpyAsync(out, workspace, 4 * sizeof(int32_t), cudaMemcpyDeviceToHost, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     return e == cudaSuccess ? CWRNNT_OK : fail_launch("read_status", e);
+}
+
+int cwrnnt_token_scores(const cwrnnt_rows *p, const void *x, const int32_t *targets, void *log_probs, void *entropy,
+                        void *top_log_probs, int32_t *top_indices, double *stats, cwrnnt_stream_t stream)
+{
+    int st = check_rows(p);
+    if (st) return st;
+    if (p->n_rows == 0) return CWRNNT_OK;
+    if (!x || (p->n_list > 0 && (!targets || !log_probs)) || (p->top_k > 0 && (!top_log_probs || !top_indices)))
+        return CWRNNT_ERR_ARGUMENT;
+    cudaError_t e = launch_token_scores(*p, x, targets, log_probs, entropy, top_log_probs, top_indices, stats,
+                                        reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? CWRNNT_OK : fail_launch("token_scores", e);
+}
+
+int cwrnnt_token_scores_backward(const cwrnnt_rows *p, const void *x, const int32_t *targets,
+                                 const int32_t *top_indices, const double *stats, const void *entropy,
+                                 const void *g_log_probs, const void *g_entropy, const void *g_top, void *grad_x,
+                                 cwrnnt_stream_t stream)
+{
+    int st = check_rows(p);
+    if (st) return st;
+    if (p->grad_stride < p->V) return CWRNNT_ERR_ARGUMENT;
+    if (p->n_rows == 0) return CWRNNT_OK;
+    if (!x || !stats || !grad_x || (g_log_probs && p->n_list > 0 && !targets) ||
+        (g_top && p->top_k > 0 && !top_indices) || (g_entropy && !entropy))
+        return CWRNNT_ERR_ARGUMENT;
+    cudaError_t e = launch_token_scores_grad(*p, x, targets, top_indices, stats, entropy, g_log_probs, g_entropy, g_top,
+                                             grad_x, reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? CWRNNT_OK : fail_launch("token_scores_backward", e);
+}
+
+int64_t cwrnnt_distill_workspace_bytes(const cwrnnt_rows *p)
+{
+    if (check_rows(p) != CWRNNT_OK) return -1;
+    return align_up(8 * (p->n_rows > 0 ? p->n_rows : 1), 256);
+}
+
+int cwrnnt_distill(const cwrnnt_rows *p, int32_t tail, const void *x, const void *teacher, const int32_t *indices,
+                   const void *weight, const void *upstream, int32_t upstream_stride, double scale, void *workspace,
+                   int64_t workspace_bytes, void *row_loss, void *loss, void *grad_x, cwrnnt_stream_t stream)
+{
+    int st = check_rows(p);
+    if (st) return st;
+    if (p->n_list < 1 || p->top_k != 0 || (tail != 0 && tail != 1)) return CWRNNT_ERR_ARGUMENT;
+    if (upstream_stride != 0 && upstream_stride != 1) return CWRNNT_ERR_ARGUMENT;
+    if (grad_x && p->grad_stride < p->V) return CWRNNT_ERR_ARGUMENT;
+    if (p->n_rows > 0 && (!x || !teacher || !indices)) return CWRNNT_ERR_ARGUMENT;
+    if (loss && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8 != 0 ||
+                 workspace_bytes < cwrnnt_distill_workspace_bytes(p)))
+        return CWRNNT_ERR_WORKSPACE;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (p->n_rows == 0) {  // the loss of no rows is zero
+        if (!loss) return CWRNNT_OK;
+        e = cudaMemsetAsync(loss, 0, p->dtype == CWRNNT_F64 ? 8 : 4, s);
+        return e == cudaSuccess ? CWRNNT_OK : fail_launch("distill", e);
+    }
+    e = launch_distill(*p, tail != 0, x, teacher, indices, weight, upstream, upstream_stride, scale,
+                       static_cast<double *>(workspace), row_loss, loss, grad_x, s);
+    return e == cudaSuccess ? CWRNNT_OK : fail_launch("distill", e);
 }
 
 }  // extern "C"

@@ -84,4 +84,18 @@ cudaError_t launch_joint(const cwrnnt_problem &p, int activation, bool backward,
                          const void *pred, int32_t u_max1, const int32_t *lx, const int32_t *ly, int64_t *off_scratch,
                          const void *grad_out, void *out_or_grad_enc, void *grad_pred, cudaStream_t s);
 
+// Scores of logits rows and their gradient (arguments as in the C ABI).
+cudaError_t launch_token_scores(const cwrnnt_rows &p, const void *x, const int32_t *targets, void *log_probs,
+                                void *entropy, void *top_log_probs, int32_t *top_indices, double *stats,
+                                cudaStream_t s);
+cudaError_t launch_token_scores_grad(const cwrnnt_rows &p, const void *x, const int32_t *targets,
+                                     const int32_t *top_indices, const double *stats, const void *entropy,
+                                     const void *g_log_probs, const void *g_entropy, const void *g_top, void *grad_x,
+                                     cudaStream_t s);
+
+// Distillation from a teacher's top entries: `partial` holds one double per row at most.
+cudaError_t launch_distill(const cwrnnt_rows &p, bool tail, const void *x, const void *teacher, const int32_t *index,
+                           const void *weight, const void *upstream, int32_t upstream_stride, double scale,
+                           double *partial, void *row_loss, void *loss, void *grad_x, cudaStream_t s);
+
 }  // namespace cwrnnt

@@ -1,0 +1,265 @@
+// What the row operators (token scores, top-entry distillation) share: how a row of logits of any size and alignment is
+// cut into 16-byte vectors, the softmax statistics of a row, and the selection of its largest entries. Internal.
+#pragma once
+#include "cwrnnt_common.cuh"
+
+namespace cwrnnt {
+
+constexpr int kRowThreads = 256;  // threads of a CTA in the row operators
+
+// ------------------------------------------------------------------------------------------------ rows as vectors
+// Vector i of a row covers the elements [i*VE - head, i*VE - head + VE), where `head` elements lie between the last
+// 16-byte boundary at or below the row's start and that start: vectors are always aligned, whatever V and the row
+// stride. The first and the last vector can reach over the row's ends; they are put together element by element, with
+// `fill` outside, so nothing outside the row is read. ALIGNED: every row starts on a boundary and ends on one.
+template <typename T, bool ALIGNED>
+struct RowVectors {
+    const T *row;
+    int V, head, count;
+    __device__ __forceinline__ RowVectors(const T *row_, int V_) : row(row_), V(V_)
+    {
+        constexpr int VE = Elt<T>::VE;
+        head = ALIGNED ? 0 : int((reinterpret_cast<uintptr_t>(row_) & 15) / sizeof(T));
+        count = (V_ + head + VE - 1) / VE;
+    }
+    __device__ __forceinline__ int first(int i) const { return i * Elt<T>::VE - head; }
+    __device__ __forceinline__ bool whole(int i) const
+    {
+        return ALIGNED || (first(i) >= 0 && first(i) + Elt<T>::VE <= V);
+    }
+    __device__ __forceinline__ uint4 load(int i) const
+    {
+        if (whole(i)) return __ldg(reinterpret_cast<const uint4 *>(row + first(i)));
+        return edge(i);
+    }
+    __device__ __noinline__ uint4 edge(int i) const
+    {
+        using E = Elt<T>;
+        typename E::acc e[E::VE];
+#pragma unroll
+        for (int c = 0; c < E::VE; ++c) {
+            const int k = first(i) + c;
+            e[c] = k >= 0 && k < V ? E::to_acc(__ldg(row + k)) : typename E::acc(-INFINITY);
+        }
+        return E::pack(e);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 vector_of_nothing()
+{
+    typename Elt<T>::acc e[Elt<T>::VE];
+#pragma unroll
+    for (int c = 0; c < Elt<T>::VE; ++c) e[c] = typename Elt<T>::acc(-INFINITY);
+    return Elt<T>::pack(e);
+}
+
+// Stores vector i of a row of gradients. `same`: the output row has the input row's alignment, so that vector i is one
+// 16-byte store; else element by element.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void store_vector(T *out, const RowVectors<T, ALIGNED> &rv, int i, bool same,
+                                             const typename Elt<T>::acc (&e)[Elt<T>::VE])
+{
+    using E = Elt<T>;
+    if (same && rv.whole(i)) {
+        *reinterpret_cast<uint4 *>(out + rv.first(i)) = E::pack(e);
+        return;
+    }
+#pragma unroll
+    for (int c = 0; c < E::VE; ++c) {
+        const int k = rv.first(i) + c;
+        if (k >= 0 && k < rv.V) out[k] = E::from_acc(e[c]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- softmax of a row
+// With temperature tau and kappa = log2(e)/tau, a term of the row's softmax is 2^(x*kappa - shift): one FFMA and one
+// ex2 in float (relative error near 2^-22). The shift is the row's (or thread's) maximum in these units, rounded to
+// float once; where the sum's logarithm is taken, that rounding is undone. Double takes exp2 and log2 of the library.
+template <typename A>
+struct Base2;
+template <>
+struct Base2<float> {
+    static __device__ __forceinline__ float exp2_of(float d) { return ex2_approx(d); }
+    // log2(s): the binary exponent is split off exactly, so the absolute error stays near 2^-24 for large sums
+    static __device__ __forceinline__ double log2_of(float s)
+    {
+        int e;
+        const float f = frexpf(s, &e);
+        return double(e) + double(logf(f)) * 1.4426950408889634;
+    }
+    static __device__ __forceinline__ float fma_of(float a, float b, float c) { return fmaf(a, b, c); }
+    static __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+    // below this exponent a term is zero; it keeps 0 * (-inf) out of sum p log p
+    static constexpr float kFloor = -1000.0f;
+    // largest shift that x*kappa - shift is formed with; beyond it (rows of the type's lowest value) x*kappa overflows
+    static constexpr float kMostShift = 1e38f;
+};
+template <>
+struct Base2<double> {
+    static __device__ __forceinline__ double exp2_of(double d) { return exp2(d); }
+    static __device__ __forceinline__ double log2_of(double s) { return log2(s); }
+    static __device__ __forceinline__ double fma_of(double a, double b, double c) { return fma(a, b, c); }
+    static __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
+    static constexpr double kFloor = -5000.0;
+    static constexpr double kMostShift = 1e307;
+};
+
+constexpr double kLn2 = 0.6931471805599453;
+constexpr double kLog2e = 1.4426950408889634;
+
+// Running statistics of (part of) a row: maximum x, s = sum 2^d and t = sum 2^d d with d = (x - max) * kappa.
+template <typename A>
+struct RowStats {
+    A max, s, t;
+    __device__ __forceinline__ void clear()
+    {
+        max = A(-INFINITY);
+        s = t = A(0);
+    }
+    static __device__ __forceinline__ A shift_of(A max, A kappa)
+    {
+        return max == A(-INFINITY) ? A(0) : max * kappa;
+    }
+    // (true for a maximum of +inf as well: its terms are then inf - inf = NaN, as they must be)
+    static __device__ __forceinline__ bool extreme(A shift) { return !(fabs(shift) <= Base2<A>::kMostShift); }
+    // Brings the sums to a maximum that is at least the present one.
+    template <bool ENT>
+    __device__ __forceinline__ void raise(A new_max, A kappa)
+    {
+        using M = Base2<A>;
+        const A to = shift_of(new_max, kappa);
+        const A by = extreme(to) ? (max - new_max) * kappa : shift_of(max, kappa) - to;  // <= 0, or NaN
+        // nothing summed yet: the sums stay zero whatever the difference is
+        const A f = s == A(0) ? A(1) : M::exp2_of(by);
+        if (ENT && s != A(0)) t = f == A(0) ? A(0) : (t + s * by) * f;
+        s *= f;
+        max = new_max;
+    }
+    template <bool ENT>
+    __device__ __forceinline__ void join(const RowStats &o, A kappa)
+    {
+        RowStats b = o;
+        const A m = Base2<A>::max_of(max, b.max);
+        raise<ENT>(m, kappa);
+        b.raise<ENT>(m, kappa);
+        s += b.s;
+        if (ENT) t += b.t;
+    }
+    // no finite entry (and no NaN either)
+    __device__ __forceinline__ bool nothing() const { return max == A(-INFINITY) && s == s; }
+    // log2 of sum 2^((x - max) * kappa), the rounding of the shift undone
+    __device__ __forceinline__ double log2_sum(A kappa) const
+    {
+        const A shift = shift_of(max, kappa);
+        const double excess = extreme(shift) || max == A(-INFINITY)
+                                  ? 0.0 : double(Base2<A>::fma_of(max, kappa, -shift));
+        return Base2<A>::log2_of(s) - excess;
+    }
+    // entropy of the row's softmax: ln s - ln2 * t / s
+    __device__ __forceinline__ double entropy() const
+    {
+        if (s == A(0)) return 0.0;
+        return kLn2 * (Base2<A>::log2_of(s) - double(t) / double(s));
+    }
+};
+
+// ln of an entry's probability, (x - max) / tau - ln s, in double: log-probabilities near zero keep their digits, and
+// so do those of rows of the type's lowest value.
+template <typename A>
+__device__ __forceinline__ double log_prob_of(A x, double max, double inv_tau, double ln_s)
+{
+    return x == A(-INFINITY) ? (ln_s == ln_s ? -INFINITY : NAN) : (double(x) - max) * inv_tau - ln_s;
+}
+
+// Adds one vector's terms at a fixed maximum and its shift.
+template <typename T, bool ENT>
+__device__ __forceinline__ void add_terms(const uint4 &v, typename Elt<T>::acc kappa, typename Elt<T>::acc max,
+                                          typename Elt<T>::acc shift, typename Elt<T>::acc &s,
+                                          typename Elt<T>::acc &t)
+{
+    using E = Elt<T>;
+    using A = typename E::acc;
+    using M = Base2<A>;
+    A e[E::VE];
+    E::unpack(v, e);
+    if (RowStats<A>::extreme(shift)) {
+#pragma unroll
+        for (int c = 0; c < E::VE; ++c) e[c] = (e[c] - max) * kappa;
+    } else {
+#pragma unroll
+        for (int c = 0; c < E::VE; ++c) e[c] = M::fma_of(e[c], kappa, -shift);
+    }
+#pragma unroll
+    for (int c = 0; c < E::VE; ++c) {
+        const A w = M::exp2_of(e[c]);
+        s += w;
+        if (ENT) t = M::fma_of(w, M::max_of(e[c], M::kFloor), t);
+    }
+}
+
+// ------------------------------------------------------------------------------------------- largest entries
+// A total order of a row's entries in which "first" is the larger value and, among equal values, the lower index; NaN
+// comes before everything, -0 equals +0. Floats and 16-bit types pack value and index into one 64-bit word.
+template <typename A>
+struct TopKey;
+template <>
+struct TopKey<float> {
+    uint64_t k;
+    static __device__ __forceinline__ TopKey of(float v, int index)
+    {
+        v += 0.0f;  // -0 -> +0
+        const uint32_t b = __float_as_uint(v);
+        const uint32_t o = v != v ? 0xfffffffeu : (b & 0x80000000u ? ~b : b | 0x80000000u);
+        return TopKey{(uint64_t(o) << 32) | uint32_t(~uint32_t(index))};
+    }
+    static __device__ __forceinline__ TopKey none() { return TopKey{0}; }            // after every entry
+    static __device__ __forceinline__ TopKey all() { return TopKey{~uint64_t(0)}; }  // before every entry
+    __device__ __forceinline__ bool before(const TopKey &o) const { return k > o.k; }
+    __device__ __forceinline__ int index() const { return int(~uint32_t(k)); }
+};
+template <>
+struct TopKey<double> {
+    uint64_t o;
+    uint32_t i;  // complement of the index
+    static __device__ __forceinline__ TopKey of(double v, int index)
+    {
+        v += 0.0;
+        const uint64_t b = uint64_t(__double_as_longlong(v));
+        const uint64_t ord = v != v ? ~uint64_t(1) : (b >> 63 ? ~b : b | (uint64_t(1) << 63));
+        return TopKey{ord, ~uint32_t(index)};
+    }
+    static __device__ __forceinline__ TopKey none() { return TopKey{0, 0}; }
+    static __device__ __forceinline__ TopKey all() { return TopKey{~uint64_t(0), ~uint32_t(0)}; }
+    __device__ __forceinline__ bool before(const TopKey &x) const { return o > x.o || (o == x.o && i > x.i); }
+    __device__ __forceinline__ int index() const { return int(~i); }
+};
+__device__ __forceinline__ TopKey<float> shfl_xor_key(unsigned mask, const TopKey<float> &k, int by)
+{
+    return TopKey<float>{__shfl_xor_sync(mask, k.k, by)};
+}
+__device__ __forceinline__ TopKey<double> shfl_xor_key(unsigned mask, const TopKey<double> &k, int by)
+{
+    return TopKey<double>{__shfl_xor_sync(mask, k.o, by), __shfl_xor_sync(mask, k.i, by)};
+}
+
+// The best key of vector `i` of a row that comes after `last` in the order.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void best_after(const RowVectors<T, ALIGNED> &rv, int i, const uint4 &v,
+                                           const TopKey<typename Elt<T>::acc> &last,
+                                           TopKey<typename Elt<T>::acc> &best)
+{
+    using E = Elt<T>;
+    using Key = TopKey<typename E::acc>;
+    typename E::acc e[E::VE];
+    E::unpack(v, e);
+#pragma unroll
+    for (int c = 0; c < E::VE; ++c) {
+        const int k = rv.first(i) + c;
+        if (!ALIGNED && (k < 0 || k >= rv.V)) continue;
+        const Key key = Key::of(e[c], k);
+        if (last.before(key) && key.before(best)) best = key;
+    }
+}
+
+}  // namespace cwrnnt

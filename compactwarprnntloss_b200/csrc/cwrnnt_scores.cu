@@ -1,0 +1,577 @@
+// Scores of logits rows: log-probabilities of given tokens, the entropy and the largest entries of every row of a
+// [n_rows, V] matrix, and the gradient of all three. With z = x / tau, lse = ln sum_j exp z_j, p_j = exp(z_j - lse):
+//     log_probs[r][i]     = z[targets[r][i]] - lse
+//     entropy[r]          = lse - sum_j p_j z_j
+//     top_indices[r][:]   = the k largest entries, lowest index first among equals; top_log_probs[r][i] = z[...] - lse
+//     grad_x[r][j]        = (1/tau) ( sum of the upstream gradients of the entries picked at j
+//                                     - p_j (G + g_H (ln p_j + H)) ),   G = sum of all upstream gradients of entries
+// The lattice's own gather (blank and label of every node) is the special case of two targets; here the columns are
+// free, any V and any alignment is taken, and the entropy and the best alternatives come out of the same pass.
+//
+// Bound: HBM. Forward reads V * sizeof(element) per row, backward reads and writes that much; the statistics of a row
+// stay in registers, a row of up to 512 vectors (8 KB) does too, so that the selection of the largest entries reads
+// nothing again. Longer rows go through a CTA each; their selection reads them a second time, from L2.
+//
+// Selection: the k-th largest of the lanes' own maxima is a lower bound of the row's k-th largest entry. The entries at
+// or above it - about as many as k, since each lane's maximum is one of them - are collected in shared memory and
+// ranked by counting how many come before each. Rows with too many equal entries for that, and rows with NaN, are
+// picked one entry at a time instead.
+#include "cwrnnt_kernels.h"
+#include "cwrnnt_rowops.cuh"
+
+namespace cwrnnt {
+
+namespace {
+
+template <typename T>
+struct ScoresArgs {
+    using A = typename Elt<T>::acc;
+    using C = typename Elt<T>::cost;
+    const T *x;
+    int64_t n_rows, x_stride;
+    int V, n_targets, top_k;
+    A kappa;         // log2(e) / tau
+    double inv_tau;  // 1 / tau
+    const int32_t *targets;
+    C *log_probs, *entropy, *top_log_probs;
+    int32_t *top_indices;
+    double *stats;
+};
+
+// What a row's log-probabilities are taken from.
+struct RowLog {
+    double max, ln_s;
+};
+
+template <typename T>
+__device__ __forceinline__ void emit_top(const ScoresArgs<T> &a, const T *row, int64_t r, const RowLog &log,
+                                         int rank, int index)
+{
+    a.top_indices[r * a.top_k + rank] = index;
+    a.top_log_probs[r * a.top_k + rank] =
+        typename Elt<T>::cost(log_prob_of(Elt<T>::to_acc(__ldg(row + index)), log.max, a.inv_tau, log.ln_s));
+}
+
+// One target's log-probability: 0 where there is none (negative), NaN where it lies outside the row.
+template <typename T>
+__device__ __forceinline__ void emit_target(const ScoresArgs<T> &a, const T *row, int64_t r, const RowLog &log,
+                                            int i)
+{
+    const int t = __ldg(a.targets + r * a.n_targets + i);
+    double lp = 0.0;
+    if (t >= a.V)
+        lp = NAN;
+    else if (t >= 0)
+        lp = log_prob_of(Elt<T>::to_acc(__ldg(row + t)), log.max, a.inv_tau, log.ln_s);
+    a.log_probs[r * a.n_targets + i] = typename Elt<T>::cost(lp);
+}
+
+// Rows of at most LPR * NV vectors: LPR lanes hold a row in NV vectors each. All lanes of a warp take every collective
+// step together, whichever of their groups has a row left. Group g of a CTA takes the rows first + g, + GPC, ..
+template <typename T, int LPR, int NV, bool ALIGNED, bool ENT>
+__global__ void __launch_bounds__(kRowThreads)
+scores_rows_kernel(const ScoresArgs<T> a, int run_len)
+{
+    using E = Elt<T>;
+    using A = typename E::acc;
+    using M = Base2<A>;
+    using Key = TopKey<A>;
+    constexpr int GPC = kRowThreads / LPR;
+    constexpr int kCap = 4 * LPR;  // candidates of a group
+    constexpr unsigned kAll = 0xffffffffu;
+    extern __shared__ __align__(16) unsigned char scratch[];  // kCap keys and one counter per group, when top_k > 0
+    const int gl = threadIdx.x % LPR, group = threadIdx.x / LPR;
+    Key *keys = reinterpret_cast<Key *>(scratch) + group * kCap;
+    int *counter = reinterpret_cast<int *>(reinterpret_cast<Key *>(scratch) + GPC * kCap) + group;
+
+    const int64_t first = int64_t(blockIdx.x) * GPC * run_len + group;
+    for (int step = 0; step < run_len; ++step) {
+        const int64_t r = first + int64_t(step) * GPC;
+        const bool active = r < a.n_rows;
+        if (!__any_sync(kAll, active)) break;
+        const T *row = a.x + (active ? r : 0) * a.x_stride;
+        const RowVectors<T, ALIGNED> rv(row, a.V);
+        uint4 v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            v[j] = vector_of_nothing<T>();
+            if (active && j * LPR + gl < rv.count) v[j] = rv.load(j * LPR + gl);
+        }
+        A own = A(-INFINITY);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) own = M::max_of(own, E::vec_max(v[j]));
+        RowStats<A> st;
+        st.clear();
+        st.max = own;
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) st.max = M::max_of(st.max, __shfl_xor_sync(kAll, st.max, o));
+        const A shift = RowStats<A>::shift_of(st.max, a.kappa);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) add_terms<T, ENT>(v[j], a.kappa, st.max, shift, st.s, st.t);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) {
+            st.s += __shfl_xor_sync(kAll, st.s, o);
+            if (ENT) st.t += __shfl_xor_sync(kAll, st.t, o);
+        }
+        const RowLog log{double(st.max), st.nothing() ? 0.0 : kLn2 * st.log2_sum(a.kappa)};
+        if (active) {
+            if (gl == 0) {
+                if (ENT) a.entropy[r] = typename E::cost(st.entropy());
+                if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = log.ln_s;
+            }
+            for (int i = gl; i < a.n_targets; i += LPR) emit_target(a, row, r, log, i);
+        }
+        if (a.top_k > 0) {
+            int rank = 0;
+            for (int j = 0; j < LPR; ++j) {
+                const A other = __shfl_sync(kAll, own, j, LPR);
+                rank += other > own || (other == own && j < gl);
+            }
+            const unsigned hit = __ballot_sync(kAll, rank == a.top_k - 1) >> ((threadIdx.x & 31) / LPR * LPR);
+            const A bar = __shfl_sync(kAll, own, (__ffs(hit) - 1) & (LPR - 1), LPR);
+            if (gl == 0) *counter = 0;
+            __syncwarp();
+            if (active) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int i = j * LPR + gl;
+                    if (i < rv.count && E::vec_max(v[j]) >= bar) {
+                        A e[E::VE];
+                        E::unpack(v[j], e);
+#pragma unroll
+                        for (int c = 0; c < E::VE; ++c) {
+                            const int k = rv.first(i) + c;
+                            if (e[c] >= bar && (ALIGNED || (k >= 0 && k < a.V))) {
+                                const int at = atomicAdd(counter, 1);
+                                if (at < kCap) keys[at] = Key::of(e[c], k);
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            const int n = *counter;
+            const bool slow = active && (n > kCap || n < a.top_k || st.s != st.s);
+            if (active && !slow) {
+                for (int i = gl; i < n; i += LPR) {
+                    const Key mine = keys[i];
+                    int before = 0;
+                    for (int j = 0; j < n; ++j) before += keys[j].before(mine);
+                    if (before < a.top_k) emit_top(a, row, r, log, before, mine.index());
+                }
+            }
+            if (__any_sync(kAll, slow)) {
+                Key last = Key::all();
+                for (int round = 0; round < a.top_k; ++round) {
+                    Key best = Key::none();
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        if (active && j * LPR + gl < rv.count) best_after(rv, j * LPR + gl, v[j], last, best);
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) {
+                        const Key other = shfl_xor_key(kAll, best, o);
+                        if (other.before(best)) best = other;
+                    }
+                    last = best;
+                    if (slow && gl == 0) emit_top(a, row, r, log, round, best.index());
+                }
+            }
+            __syncwarp();  // the next row fills the same buffers
+        }
+    }
+}
+
+// Statistics of a row over the CTA, the same bits in every thread: the warps' parts are joined in warp order.
+template <typename A, bool ENT>
+__device__ __forceinline__ RowStats<A> join_cta(RowStats<A> st, A kappa, RowStats<A> *parts)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        RowStats<A> other;
+        other.max = __shfl_xor_sync(0xffffffffu, st.max, o);
+        other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+        other.t = ENT ? __shfl_xor_sync(0xffffffffu, st.t, o) : A(0);
+        st.template join<ENT>(other, kappa);
+    }
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = st;
+    __syncthreads();
+    st = parts[0];
+#pragma unroll
+    for (int w = 1; w < kRowThreads / 32; ++w) st.template join<ENT>(parts[w], kappa);
+    return st;
+}
+
+// Any row: one CTA each, four vectors of every thread in flight, running statistics.
+template <typename T, bool ALIGNED, bool ENT>
+__global__ void __launch_bounds__(kRowThreads)
+scores_long_kernel(const ScoresArgs<T> a)
+{
+    using E = Elt<T>;
+    using A = typename E::acc;
+    using M = Base2<A>;
+    using Key = TopKey<A>;
+    constexpr int NV = 4, kCap = 512, kBars = 64, kWarps = kRowThreads / 32;
+    __shared__ RowStats<A> parts[kWarps];
+    __shared__ Key keys[kCap];
+    __shared__ Key best_of[kWarps];
+    __shared__ A bars[kBars];
+    __shared__ A bar_shared;
+    __shared__ int counter;
+    const int tid = threadIdx.x;
+    const int64_t r = blockIdx.x;
+    const T *row = a.x + r * a.x_stride;
+    const RowVectors<T, ALIGNED> rv(row, a.V);
+    if (tid == 0) counter = 0;
+
+    RowStats<A> st;
+    st.clear();
+    for (int at = 0; at < rv.count; at += kRowThreads * NV) {
+        uint4 v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = at + j * kRowThreads + tid;
+            v[j] = i < rv.count ? rv.load(i) : vector_of_nothing<T>();
+        }
+        A m = st.max;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) m = M::max_of(m, E::vec_max(v[j]));
+        if (m > st.max) st.template raise<ENT>(m, a.kappa);
+        const A shift = RowStats<A>::shift_of(st.max, a.kappa);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) add_terms<T, ENT>(v[j], a.kappa, st.max, shift, st.s, st.t);
+    }
+    const A own = st.max;
+    st = join_cta<A, ENT>(st, a.kappa, parts);
+    const RowLog log{double(st.max), st.nothing() ? 0.0 : kLn2 * st.log2_sum(a.kappa)};
+    if (tid == 0) {
+        if (ENT) a.entropy[r] = typename E::cost(st.entropy());
+        if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = log.ln_s;
+    }
+    if (tid < a.n_targets) emit_target(a, row, r, log, tid);
+    if (a.top_k == 0) return;
+
+    // the bar: the k-th largest of the maxima of 64 groups of four threads
+    A four = M::max_of(own, __shfl_xor_sync(0xffffffffu, own, 1));
+    four = M::max_of(four, __shfl_xor_sync(0xffffffffu, four, 2));
+    if (tid % 4 == 0) bars[tid / 4] = four;
+    __syncthreads();
+    if (tid < kBars) {
+        const A mine = bars[tid];
+        int rank = 0;
+        for (int j = 0; j < kBars; ++j) rank += bars[j] > mine || (bars[j] == mine && j < tid);
+        if (rank == a.top_k - 1) bar_shared = mine;
+    }
+    __syncthreads();
+    const A bar = bar_shared;
+    for (int at = 0; at < rv.count; at += kRowThreads * NV) {
+        uint4 v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = at + j * kRowThreads + tid;
+            v[j] = i < rv.count ? rv.load(i) : vector_of_nothing<T>();
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = at + j * kRowThreads + tid;
+            if (i < rv.count && E::vec_max(v[j]) >= bar) {
+                A e[E::VE];
+                E::unpack(v[j], e);
+#pragma unroll
+                for (int c = 0; c < E::VE; ++c) {
+                    const int k = rv.first(i) + c;
+                    if (e[c] >= bar && (ALIGNED || (k >= 0 && k < a.V))) {
+                        const int n = atomicAdd(&counter, 1);
+                        if (n < kCap) keys[n] = Key::of(e[c], k);
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int n = counter;
+    if (n <= kCap && n >= a.top_k && st.s == st.s) {
+        for (int i = tid; i < n; i += kRowThreads) {
+            const Key mine = keys[i];
+            int before = 0;
+            for (int j = 0; j < n; ++j) before += keys[j].before(mine);
+            if (before < a.top_k) emit_top(a, row, r, log, before, mine.index());
+        }
+        return;
+    }
+    Key last = Key::all();
+    for (int round = 0; round < a.top_k; ++round) {
+        Key best = Key::none();
+        for (int i = tid; i < rv.count; i += kRowThreads) best_after(rv, i, rv.load(i), last, best);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const Key other = shfl_xor_key(0xffffffffu, best, o);
+            if (other.before(best)) best = other;
+        }
+        if ((tid & 31) == 0) best_of[tid >> 5] = best;
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w)
+            if (best_of[w].before(best)) best = best_of[w];
+        last = best;
+        if (tid == 0) emit_top(a, row, r, log, round, best.index());
+        __syncthreads();  // the next round fills best_of again
+    }
+}
+
+template <typename T>
+struct ScoresGradArgs {
+    using A = typename Elt<T>::acc;
+    using C = typename Elt<T>::cost;
+    const T *x;
+    T *gx;
+    int64_t n_rows, x_stride, g_stride;
+    int V, n_targets, top_k;
+    A kappa;
+    double inv_tau;
+    const int32_t *targets, *top_indices;
+    const double *stats;
+    const C *entropy, *g_log_probs, *g_entropy, *g_top;
+
+    __device__ __forceinline__ int entries() const { return n_targets + top_k; }
+    __device__ __forceinline__ int index(int64_t r, int e) const
+    {
+        const int t = e < n_targets ? __ldg(targets + r * n_targets + e)
+                                    : __ldg(top_indices + r * top_k + (e - n_targets));
+        return t < V ? t : -1;
+    }
+    __device__ __forceinline__ double upstream(int64_t r, int e) const
+    {
+        const bool t = e < n_targets;
+        const C *g = t ? g_log_probs : g_top;
+        return g ? double(__ldg(g + (t ? r * n_targets + e : r * top_k + (e - n_targets)))) : 0.0;
+    }
+};
+
+// Element-wise once the row's log-sum-exp is known: LPR threads a row (a part of a warp, a warp, or a CTA), four vectors
+// of each in flight. The entries that were picked are written a second time behind a barrier, by the first entry that
+// names them, which adds up all that do.
+template <typename T, int LPR, bool ALIGNED>
+__global__ void __launch_bounds__(kRowThreads)
+scores_grad_kernel(const ScoresGradArgs<T> a)
+{
+    using E = Elt<T>;
+    using A = typename E::acc;
+    using M = Base2<A>;
+    constexpr int NV = 4;
+    constexpr int GPC = kRowThreads / LPR;
+    constexpr int kSum = LPR < 32 ? LPR : 32;  // lanes that add up the entries
+    const int gl = threadIdx.x % LPR;
+    const int64_t r = int64_t(blockIdx.x) * GPC + threadIdx.x / LPR;
+    const bool active = r < a.n_rows;
+    if (LPR >= 32 && !active) return;  // whole warps (or the CTA) leave together
+    const int64_t rr = active ? r : 0;
+    const T *row = a.x + rr * a.x_stride;
+    T *out = a.gx + rr * a.g_stride;
+    const RowVectors<T, ALIGNED> rv(row, a.V);
+    const bool same = ALIGNED || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+
+    const int n = active ? a.entries() : 0;
+    double total = 0.0;
+    for (int e = gl % kSum; e < n; e += kSum)
+        if (a.index(rr, e) >= 0) total += a.upstream(rr, e);
+#pragma unroll
+    for (int o = kSum / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const double max = active ? __ldg(a.stats + 2 * rr) : 0.0;
+    const double log2_s = active ? __ldg(a.stats + 2 * rr + 1) * kLog2e : 0.0;
+    const bool nothing = max == -INFINITY && log2_s == log2_s;  // no finite entry: no gradient
+    // p = 2^((x - top) * kappa - low), the rounding of `low` put into the row's factors
+    const A top = nothing ? A(0) : A(max), low = A(log2_s);
+    const double undo = exp2(double(low) - log2_s);
+    const double gh = a.g_entropy && active ? double(__ldg(a.g_entropy + rr)) : 0.0;
+    const double h = a.g_entropy && active ? double(__ldg(a.entropy + rr)) : 0.0;
+    const double scale = nothing ? 0.0 : a.inv_tau;
+    const A c0 = A(-(total + gh * h) * scale * undo), c1 = A(-gh * kLn2 * scale * undo);
+    if (active) {
+        for (int at = 0; at < rv.count; at += LPR * NV) {
+            uint4 v[NV];
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int i = at + j * LPR + gl;
+                if (i < rv.count) v[j] = rv.load(i);
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int i = at + j * LPR + gl;
+                if (i < rv.count) {
+                    A e[E::VE];
+                    E::unpack(v[j], e);
+#pragma unroll
+                    for (int c = 0; c < E::VE; ++c) {
+                        const A d = M::fma_of(e[c] - top, a.kappa, -low);
+                        e[c] = M::exp2_of(d) * M::fma_of(c1, M::max_of(d, M::kFloor), c0);
+                    }
+                    store_vector(out, rv, i, same, e);
+                }
+            }
+        }
+    }
+    if (n == 0 && LPR >= 32) return;
+    if (LPR > 32)
+        __syncthreads();
+    else
+        __syncwarp();
+    for (int e = gl; e < n; e += LPR) {
+        const int t = a.index(rr, e);
+        if (t < 0) continue;
+        double g = 0.0;
+        bool first = true;
+        for (int o = 0; o < n; ++o)
+            if (a.index(rr, o) == t) {
+                g += a.upstream(rr, o);
+                first = first && o >= e;
+            }
+        if (first) {
+            const A d = M::fma_of(E::to_acc(__ldg(row + t)) - top, a.kappa, -low);
+            out[t] = E::from_acc(A(g * scale) + M::exp2_of(d) * M::fma_of(c1, M::max_of(d, M::kFloor), c0));
+        }
+    }
+}
+
+// Most vectors that a row of V elements can touch.
+template <typename T>
+int vectors_of(int V, bool aligned)
+{
+    constexpr int VE = Elt<T>::VE;
+    return aligned ? V / VE : (V + 2 * VE - 2) / VE;
+}
+
+template <typename T>
+bool rows_aligned(const void *x, int64_t stride, int V)
+{
+    constexpr int VE = Elt<T>::VE;
+    return reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride % VE == 0 && V % VE == 0;
+}
+
+template <typename T, int LPR, int NV, bool ALIGNED>
+cudaError_t launch_scores_rows(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
+{
+    constexpr int GPC = kRowThreads / LPR;
+    const int run_len = 1;
+    const int64_t grid = (a.n_rows + int64_t(GPC) * run_len - 1) / (int64_t(GPC) * run_len);
+    const size_t smem = a.top_k > 0 ? GPC * (4 * LPR * sizeof(TopKey<typename Elt<T>::acc>) + sizeof(int)) : 0;
+    if (ent)
+        scores_rows_kernel<T, LPR, NV, ALIGNED, true><<<unsigned(grid), kRowThreads, smem, s>>>(a, run_len);
+    else
+        scores_rows_kernel<T, LPR, NV, ALIGNED, false><<<unsigned(grid), kRowThreads, smem, s>>>(a, run_len);
+    return cudaGetLastError();
+}
+
+template <typename T, bool ALIGNED>
+cudaError_t launch_scores_t(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
+{
+    const int nv = vectors_of<T>(a.V, ALIGNED);
+    // the bar of the selection is taken among the lanes' maxima: at least twice as many lanes as entries, up to a warp
+    const int lanes = 2 * a.top_k;
+    if (nv <= 16 && lanes <= 4) return launch_scores_rows<T, 4, 4, ALIGNED>(a, ent, s);
+    if (nv <= 32 && lanes <= 8) return launch_scores_rows<T, 8, 4, ALIGNED>(a, ent, s);
+    if (nv <= 64 && lanes <= 16) return launch_scores_rows<T, 16, 4, ALIGNED>(a, ent, s);
+    if (nv <= 128) return launch_scores_rows<T, 32, 4, ALIGNED>(a, ent, s);
+    if (nv <= 256) return launch_scores_rows<T, 32, 8, ALIGNED>(a, ent, s);
+    if (nv <= 512) return launch_scores_rows<T, 32, 16, ALIGNED>(a, ent, s);
+    if (ent)
+        scores_long_kernel<T, ALIGNED, true><<<unsigned(a.n_rows), kRowThreads, 0, s>>>(a);
+    else
+        scores_long_kernel<T, ALIGNED, false><<<unsigned(a.n_rows), kRowThreads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_scores_of(const cwrnnt_rows &p, const void *x, const int32_t *targets, void *log_probs,
+                             void *entropy, void *top_log_probs, int32_t *top_indices, double *stats, cudaStream_t s)
+{
+    using C = typename Elt<T>::cost;
+    ScoresArgs<T> a{};
+    a.x = static_cast<const T *>(x);
+    a.n_rows = p.n_rows, a.x_stride = p.x_stride;
+    a.V = p.V, a.n_targets = p.n_list, a.top_k = p.top_k;
+    a.inv_tau = 1.0 / p.temperature;
+    a.kappa = typename Elt<T>::acc(kLog2e / p.temperature);
+    a.targets = targets;
+    a.log_probs = static_cast<C *>(log_probs), a.entropy = static_cast<C *>(entropy);
+    a.top_log_probs = static_cast<C *>(top_log_probs);
+    a.top_indices = top_indices, a.stats = stats;
+    return rows_aligned<T>(x, p.x_stride, p.V) ? launch_scores_t<T, true>(a, entropy != nullptr, s)
+                                               : launch_scores_t<T, false>(a, entropy != nullptr, s);
+}
+
+template <typename T, bool ALIGNED>
+cudaError_t launch_scores_grad_t(const ScoresGradArgs<T> &a, cudaStream_t s)
+{
+    const int nv = vectors_of<T>(a.V, ALIGNED);
+    auto grid = [&](int lpr) { return unsigned((a.n_rows + kRowThreads / lpr - 1) / (kRowThreads / lpr)); };
+    if (nv <= 32)
+        scores_grad_kernel<T, 8, ALIGNED><<<grid(8), kRowThreads, 0, s>>>(a);
+    else if (nv <= 1024)
+        scores_grad_kernel<T, 32, ALIGNED><<<grid(32), kRowThreads, 0, s>>>(a);
+    else
+        scores_grad_kernel<T, kRowThreads, ALIGNED><<<grid(kRowThreads), kRowThreads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_scores_grad_of(const cwrnnt_rows &p, const void *x, const int32_t *targets,
+                                  const int32_t *top_indices, const double *stats, const void *entropy,
+                                  const void *g_log_probs, const void *g_entropy, const void *g_top, void *gx,
+                                  cudaStream_t s)
+{
+    using C = typename Elt<T>::cost;
+    ScoresGradArgs<T> a{};
+    a.x = static_cast<const T *>(x), a.gx = static_cast<T *>(gx);
+    a.n_rows = p.n_rows, a.x_stride = p.x_stride, a.g_stride = p.grad_stride;
+    // entries without an upstream gradient need not be looked at
+    a.V = p.V, a.n_targets = g_log_probs ? p.n_list : 0, a.top_k = g_top ? p.top_k : 0;
+    a.inv_tau = 1.0 / p.temperature;
+    a.kappa = typename Elt<T>::acc(kLog2e / p.temperature);
+    a.targets = targets, a.top_indices = top_indices;
+    a.stats = stats, a.entropy = static_cast<const C *>(entropy);
+    a.g_log_probs = static_cast<const C *>(g_log_probs), a.g_entropy = static_cast<const C *>(g_entropy);
+    a.g_top = static_cast<const C *>(g_top);
+    const bool aligned = rows_aligned<T>(x, p.x_stride, p.V) && rows_aligned<T>(gx, p.grad_stride, p.V);
+    return aligned ? launch_scores_grad_t<T, true>(a, s) : launch_scores_grad_t<T, false>(a, s);
+}
+
+}  // namespace
+
+cudaError_t launch_token_scores(const cwrnnt_rows &p, const void *x, const int32_t *targets, void *log_probs,
+                                void *entropy, void *top_log_probs, int32_t *top_indices, double *stats, cudaStream_t s)
+{
+    switch (p.dtype) {
+    case CWRNNT_F32:
+        return launch_scores_of<float>(p, x, targets, log_probs, entropy, top_log_probs, top_indices, stats, s);
+    case CWRNNT_F16:
+        return launch_scores_of<__half>(p, x, targets, log_probs, entropy, top_log_probs, top_indices, stats, s);
+    case CWRNNT_BF16:
+        return launch_scores_of<__nv_bfloat16>(p, x, targets, log_probs, entropy, top_log_probs, top_indices, stats, s);
+    case CWRNNT_F64:
+        return launch_scores_of<double>(p, x, targets, log_probs, entropy, top_log_probs, top_indices, stats, s);
+    }
+    return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_token_scores_grad(const cwrnnt_rows &p, const void *x, const int32_t *targets,
+                                     const int32_t *top_indices, const double *stats, const void *entropy,
+                                     const void *g_log_probs, const void *g_entropy, const void *g_top, void *grad_x,
+                                     cudaStream_t s)
+{
+    switch (p.dtype) {
+    case CWRNNT_F32:
+        return launch_scores_grad_of<float>(p, x, targets, top_indices, stats, entropy, g_log_probs, g_entropy, g_top,
+                                            grad_x, s);
+    case CWRNNT_F16:
+        return launch_scores_grad_of<__half>(p, x, targets, top_indices, stats, entropy, g_log_probs, g_entropy, g_top,
+                                             grad_x, s);
+    case CWRNNT_BF16:
+        return launch_scores_grad_of<__nv_bfloat16>(p, x, targets, top_indices, stats, entropy, g_log_probs, g_entropy,
+                                                    g_top, grad_x, s);
+    case CWRNNT_F64:
+        return launch_scores_grad_of<double>(p, x, targets, top_indices, stats, entropy, g_log_probs, g_entropy, g_top,
+                                             grad_x, s);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace cwrnnt

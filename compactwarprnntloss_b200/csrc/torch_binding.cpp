@@ -8,6 +8,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <optional>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -284,6 +285,120 @@ torch::Tensor unpack_padded(const torch::Tensor &compact, const torch::Tensor &l
     return out;
 }
 
+// -------------------------------------------------------------------------------------- operators on rows of logits
+
+using OptTensor = std::optional<torch::Tensor>;
+
+void *ptr(const OptTensor &t) { return t && t->numel() ? t->data_ptr() : nullptr; }
+
+// x [rows, V] with unit column stride; rows may lie further apart.
+cwrnnt_rows describe_rows(const torch::Tensor &x, int64_t n_list, int64_t top_k, double temperature)
+{
+    CHECK_CUDA(x);
+    TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1, "x must be [rows, V] with at least one column");
+    TORCH_CHECK(x.size(1) == 1 || x.stride(1) == 1, "x must have unit stride along its columns");
+    TORCH_CHECK(x.size(1) <= INT32_MAX - 64, "too many columns");
+    TORCH_CHECK(x.size(0) < 2 || x.stride(0) >= x.size(1), "rows of x overlap");
+    TORCH_CHECK(n_list <= CWRNNT_MAX_LIST && top_k <= CWRNNT_MAX_LIST, "at most ", CWRNNT_MAX_LIST,
+                " targets, top entries or teacher entries of a row");
+    TORCH_CHECK(top_k >= 0 && top_k <= x.size(1), "top_k must lie in [0, V]");
+    cwrnnt_rows p{};
+    p.n_rows = x.size(0);
+    p.V = static_cast<int32_t>(x.size(1));
+    p.x_stride = x.size(0) < 2 ? x.size(1) : x.stride(0);
+    p.grad_stride = x.size(1);
+    p.temperature = temperature;
+    p.dtype = dtype_code(x);
+    p.n_list = static_cast<int32_t>(n_list);
+    p.top_k = static_cast<int32_t>(top_k);
+    return p;
+}
+
+// [rows, n] int32 / costs-type companion of x on the same device, contiguous.
+void check_companion(const torch::Tensor &t, const torch::Tensor &x, torch::ScalarType type, const char *name)
+{
+    TORCH_CHECK(t.device() == x.device(), name, " must live on the device of x");
+    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+    TORCH_CHECK(t.scalar_type() == type, name, " must be ", type);
+    TORCH_CHECK(t.size(0) == x.size(0), name, " must have one row for each row of x");
+}
+
+// Returns (log_probs [R,P]?, entropy [R]?, top_log_probs [R,k]?, top_indices [R,k]?, stats [R,2]?).
+std::tuple<OptTensor, OptTensor, OptTensor, OptTensor, OptTensor>
+token_scores(const torch::Tensor &x, const OptTensor &targets, int64_t top_k, bool entropy, double temperature,
+             bool keep)
+{
+    const cwrnnt_rows p = describe_rows(x, targets ? targets->size(1) : 0, top_k, temperature);
+    if (targets) check_companion(*targets, x, torch::ScalarType::Int, "targets");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const auto costs = x.options().dtype(cost_type(x));
+    OptTensor lp, ent, top, index, stats;
+    if (targets) lp = torch::empty({p.n_rows, p.n_list}, costs);
+    if (entropy) ent = torch::empty({p.n_rows}, costs);
+    if (top_k > 0) {
+        top = torch::empty({p.n_rows, p.top_k}, costs);
+        index = torch::empty({p.n_rows, p.top_k}, x.options().dtype(torch::kInt32));
+    }
+    if (keep) stats = torch::empty({p.n_rows, 2}, x.options().dtype(torch::kDouble));
+    check_status(cwrnnt_token_scores(&p, x.data_ptr(), static_cast<const int32_t *>(ptr(targets)), ptr(lp), ptr(ent),
+                                     ptr(top), static_cast<int32_t *>(ptr(index)), static_cast<double *>(ptr(stats)),
+                                     current_stream()),
+                 "cwrnnt_token_scores");
+    return {lp, ent, top, index, stats};
+}
+
+torch::Tensor token_scores_backward(const torch::Tensor &x, const OptTensor &targets, const OptTensor &index,
+                                    const torch::Tensor &stats, const OptTensor &entropy, const OptTensor &g_lp,
+                                    const OptTensor &g_ent, const OptTensor &g_top, double temperature)
+{
+    const cwrnnt_rows p = describe_rows(x, targets ? targets->size(1) : 0, index ? index->size(1) : 0, temperature);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const auto type = cost_type(x);
+    for (const OptTensor *t : {&g_lp, &g_ent, &g_top})
+        if (*t) check_companion(**t, x, type, "an upstream gradient");
+    auto gx = torch::empty({x.size(0), x.size(1)}, x.options());
+    check_status(cwrnnt_token_scores_backward(&p, x.data_ptr(), static_cast<const int32_t *>(ptr(targets)),
+                                              static_cast<const int32_t *>(ptr(index)), stats.data_ptr<double>(),
+                                              ptr(entropy), ptr(g_lp), ptr(g_ent), ptr(g_top), gx.data_ptr(),
+                                              current_stream()),
+                 "cwrnnt_token_scores_backward");
+    return gx;
+}
+
+// Returns (row_loss [R]?, loss []?, grad_x [R,V]?).
+std::tuple<OptTensor, OptTensor, OptTensor> distill(const torch::Tensor &x, const torch::Tensor &teacher,
+                                                    const torch::Tensor &indices, const OptTensor &weight,
+                                                    const OptTensor &upstream, bool tail, double temperature,
+                                                    double scale, bool want_rows, bool want_loss, bool want_grad)
+{
+    TORCH_CHECK(teacher.dim() == 2 && indices.dim() == 2 && teacher.size(1) == indices.size(1) && indices.size(1) > 0,
+                "teacher values and indices must both be [rows, K], K >= 1");
+    const cwrnnt_rows p = describe_rows(x, indices.size(1), 0, temperature);
+    const auto type = cost_type(x);
+    check_companion(teacher, x, type, "teacher values");
+    check_companion(indices, x, torch::ScalarType::Int, "indices");
+    if (weight) check_companion(*weight, x, type, "weight");
+    if (upstream)
+        TORCH_CHECK(upstream->device() == x.device() && upstream->scalar_type() == type && upstream->is_contiguous() &&
+                        (upstream->numel() == 1 || upstream->numel() == x.size(0)),
+                    "an upstream gradient must have 1 or N elements");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const auto costs = x.options().dtype(type);
+    OptTensor rows, loss, gx, ws;
+    if (want_rows) rows = torch::empty({p.n_rows}, costs);
+    if (want_loss) {
+        loss = torch::empty({}, costs);
+        ws = torch::empty({cwrnnt_distill_workspace_bytes(&p)}, x.options().dtype(torch::kUInt8));
+    }
+    if (want_grad) gx = torch::empty({x.size(0), x.size(1)}, x.options());
+    check_status(cwrnnt_distill(&p, tail ? 1 : 0, x.data_ptr(), teacher.data_ptr(),
+                                static_cast<const int32_t *>(indices.data_ptr()), ptr(weight), ptr(upstream),
+                                upstream && upstream->numel() > 1 ? 1 : 0, scale, ptr(ws), ws ? ws->numel() : 0,
+                                ptr(rows), ptr(loss), ptr(gx), current_stream()),
+                 "cwrnnt_distill");
+    return {rows, loss, gx};
+}
+
 // ------------------------------------------------------------------- the reference module's functions, same shapes
 
 // cwarp_cuda.cpp:84-108. xs are log-probabilities. Returns (costs [N], grads [STU,2], alphas, betas [N,Tmax,Umax+1]).
@@ -387,6 +502,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("_rnnt_status", &rnnt_status, "Status words of a workspace (synchronises).");
     m.def("_pack_padded", &pack_padded, "Padded [N,T,U+1,V] -> compact [n_rows,V].");
     m.def("_unpack_padded", &unpack_padded, "Compact [n_rows,V] -> zero-padded [N,T,U+1,V].");
+    m.def("_token_scores", &token_scores, "Scores of logits rows: (log_probs, entropy, top_log_probs, top_indices, stats).");
+    m.def("_token_scores_backward", &token_scores_backward, "Gradient of the scores w.r.t. the rows.");
+    m.def("_distill", &distill, "Distillation from a teacher's top entries: (row_loss, loss, grad_x).");
+    m.attr("MAX_LIST") = static_cast<int>(CWRNNT_MAX_LIST);
     m.attr("FUSED_LOG_SOFTMAX") = static_cast<int>(CWRNNT_FUSED_LOG_SOFTMAX);
     m.attr("COSTS_ONLY") = static_cast<int>(CWRNNT_COSTS_ONLY);
     m.attr("REDUCE_MEAN") = static_cast<int>(CWRNNT_REDUCE_MEAN);

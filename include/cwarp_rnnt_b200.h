@@ -347,6 +347,72 @@ CWRNNT_API int cwrnnt_joint_backward(const cwrnnt_problem *p, int32_t activation
                                      void *grad_pred, cwrnnt_stream_t stream);
 
 /*
+ * Operators on rows of logits next to the loss: scores of the rows (log-probabilities of given tokens, entropy, the
+ * best alternatives) and distillation from a teacher's top entries. They take any [n_rows, V] matrix - the compact
+ * lattice rows, a decoder's or a language model's - of any V, row stride and alignment. The reference has no such
+ * functions (its gather, cwarp_cuda_gather_kernel.cu:19-50, picks two fixed columns of log-probabilities).
+ * Nothing here allocates or synchronises; results do not depend on timing (no floating-point atomics). Entries may name
+ * a token twice, or none (a negative index). A row without a finite logit (a mask that leaves nothing) has
+ * log-probabilities of -inf, entropy 0, a divergence of 0 and a zero gradient; a row with a NaN or +inf logit gives
+ * NaN (its best entries are still found: NaN first, then by value). An index of V or more is never followed: its
+ * log-probability, or the divergence and gradient of its row, is NaN.
+ */
+#define CWRNNT_MAX_LIST 32 /* most targets, top entries or teacher entries of a row */
+typedef struct {
+    int64_t n_rows;      /* rows of x (at most 2^31 - 1)                                              */
+    int64_t x_stride;    /* elements from one row of x to the next, >= V                              */
+    int64_t grad_stride; /* the same of grad_x; not read where there is none                          */
+    double temperature;  /* tau in [1e-4, 1e4]: probabilities are softmax(x / tau)                    */
+    int32_t V;           /* columns                                                                   */
+    int32_t dtype;       /* cwrnnt_dtype of x and grad_x; the "costs type" is float, double for F64   */
+    int32_t n_list;      /* targets (scores) or teacher entries (distillation) of a row, <= CWRNNT_MAX_LIST */
+    int32_t top_k;       /* largest entries of a row to find, <= min(V, CWRNNT_MAX_LIST); scores only */
+} cwrnnt_rows;
+
+/*
+ * Scores of every row, in one pass over x:
+ *   log_probs       [n_rows, n_list] ln softmax(x/tau) at targets [n_rows, n_list]; 0 where the target is negative
+ *   entropy         [n_rows] or NULL (not wanted)
+ *   top_log_probs, top_indices  [n_rows, top_k] the largest entries, lowest index first among equal ones
+ *   stats           [n_rows, 2] double or NULL: the row's largest logit and ln sum exp((x - largest) / tau), what
+ *                   cwrnnt_token_scores_backward needs
+ * log_probs, entropy and top_log_probs are of the costs type.
+ */
+CWRNNT_API int cwrnnt_token_scores(const cwrnnt_rows *p, const void *x, const int32_t *targets, void *log_probs,
+                                   void *entropy, void *top_log_probs, int32_t *top_indices, double *stats,
+                                   cwrnnt_stream_t stream);
+/*
+ * grad_x [n_rows, V], fully written, from the upstream gradients of log_probs, entropy and top_log_probs (costs type;
+ * any of them NULL: zero). targets, top_indices, stats and (with g_entropy) entropy are the forward's. The choice of the
+ * top entries is not differentiated. A target outside the row gets no gradient.
+ */
+CWRNNT_API int cwrnnt_token_scores_backward(const cwrnnt_rows *p, const void *x, const int32_t *targets,
+                                            const int32_t *top_indices, const double *stats, const void *entropy,
+                                            const void *g_log_probs, const void *g_entropy, const void *g_top,
+                                            void *grad_x, cwrnnt_stream_t stream);
+
+/*
+ * Distillation from a teacher's top entries: loss and gradient in one pass over x. Row r has n_list entries, a token
+ * indices[r][i] and the teacher's value teacher[r][i] (costs type).
+ *   tail = 1  teacher values are log-probabilities; every token that is not listed belongs to one more class:
+ *             D = sum q (ln q - ln p) over the listed tokens and that class (left out where no other token is finite)
+ *   tail = 0  the teacher's values are renormalised, q = softmax(teacher / tau) over the list; D = sum q (ln q - ln p)
+ *   weight    [n_rows] costs type or NULL (1): a row's factor; rows of weight 0 are not read
+ *   upstream, upstream_stride   costs type: the gradient of row r's weighted divergence is multiplied by
+ *             upstream[r * upstream_stride] (stride 0 or 1; NULL: 1)
+ *   scale     factor of the summed loss and of the gradient (1 / rows for a mean)
+ *   row_loss  [n_rows] costs type or NULL: weight * D
+ *   loss      1 element of the costs type or NULL: scale * sum(weight * D), added up in a fixed order
+ *   grad_x    [n_rows, V] or NULL, fully written: upstream * scale * weight * dD/dx
+ *   workspace cwrnnt_distill_workspace_bytes(p) bytes, 8-byte aligned; only needed for `loss`
+ */
+CWRNNT_API int64_t cwrnnt_distill_workspace_bytes(const cwrnnt_rows *p);
+CWRNNT_API int cwrnnt_distill(const cwrnnt_rows *p, int32_t tail, const void *x, const void *teacher,
+                              const int32_t *indices, const void *weight, const void *upstream,
+                              int32_t upstream_stride, double scale, void *workspace, int64_t workspace_bytes,
+                              void *row_loss, void *loss, void *grad_x, cwrnnt_stream_t stream);
+
+/*
  * Costs (and the reduced loss) without any caller workspace and without any allocation: for hosts that cannot call
  * cudaMalloc - a plug-in in a serving process whose framework owns all device memory, a foreign-language binding with
  * no device allocator to size a workspace with, a scoring loop that cannot afford the synchronisation an allocation

@@ -1,0 +1,91 @@
+"""CPU-side checks of the operators on rows of logits: the C ABI refuses bad descriptions, null pointers and workspaces
+before any launch, and the Python entry points refuse what they cannot take."""
+import ctypes
+
+import pytest
+import torch
+
+from compactwarprnntloss_b200 import capi, distill_loss, token_scores
+
+
+def _rows(**kw):
+    d = dict(n_rows=10, x_stride=64, grad_stride=64, temperature=1.0, V=64, dtype=capi.F32, n_list=2, top_k=0)
+    d.update(kw)
+    return ctypes.byref(capi.Rows(**d))
+
+
+BAD = [dict(n_rows=-1), dict(n_rows=2 ** 31), dict(V=0), dict(V=-3), dict(x_stride=63), dict(dtype=4), dict(dtype=-1),
+       dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")),
+       dict(n_list=-1), dict(n_list=33), dict(top_k=-1), dict(top_k=33), dict(V=8, top_k=9)]
+
+
+@pytest.mark.parametrize("bad", BAD)
+def test_bad_descriptions_are_refused(bad):
+    L = capi.lib()
+    one = ctypes.c_void_p(256)  # never followed: the description is refused first
+    assert L.cwrnnt_token_scores(_rows(**bad), one, one, one, one, one, one, one, None) == 1
+    assert L.cwrnnt_token_scores_backward(_rows(**bad), one, one, one, one, one, one, one, one, one, None) == 1
+    assert L.cwrnnt_distill(_rows(**bad), 1, one, one, one, None, None, 0, 1.0, one, 1 << 20, one, one, one, None) == 1
+    assert L.cwrnnt_distill_workspace_bytes(_rows(**bad)) < 0
+
+
+def test_missing_pointers_and_workspaces_are_refused():
+    L = capi.lib()
+    one = ctypes.c_void_p(256)
+    assert L.cwrnnt_token_scores(None, one, one, one, one, one, one, one, None) == 1
+    assert L.cwrnnt_token_scores(_rows(), None, one, one, None, None, None, None, None) == 1       # x
+    assert L.cwrnnt_token_scores(_rows(), one, None, one, None, None, None, None, None) == 1       # targets
+    assert L.cwrnnt_token_scores(_rows(), one, one, None, None, None, None, None, None) == 1       # log_probs
+    assert L.cwrnnt_token_scores(_rows(n_list=0, top_k=3), one, None, None, None, one, None, None, None) == 1
+    assert L.cwrnnt_token_scores(_rows(n_list=0, top_k=3), one, None, None, None, None, one, None, None) == 1
+    back = L.cwrnnt_token_scores_backward
+    assert back(_rows(), one, one, None, None, None, one, None, None, one, None) == 1              # lse
+    assert back(_rows(), one, one, None, one, None, one, None, None, None, None) == 1              # grad_x
+    assert back(_rows(), one, None, None, one, None, one, None, None, one, None) == 1              # targets
+    assert back(_rows(), one, one, None, one, None, None, one, None, one, None) == 1               # entropy
+    assert back(_rows(grad_stride=63), one, one, None, one, None, one, None, None, one, None) == 1
+    assert back(_rows(n_list=0, top_k=2), one, None, None, one, None, None, None, one, one, None) == 1
+    d = L.cwrnnt_distill
+    assert d(_rows(), 1, None, one, one, None, None, 0, 1.0, one, 1 << 20, one, one, one, None) == 1
+    assert d(_rows(), 1, one, None, one, None, None, 0, 1.0, one, 1 << 20, one, one, one, None) == 1
+    assert d(_rows(), 1, one, one, None, None, None, 0, 1.0, one, 1 << 20, one, one, one, None) == 1
+    assert d(_rows(), 2, one, one, one, None, None, 0, 1.0, one, 1 << 20, one, one, one, None) == 1
+    assert d(_rows(), 1, one, one, one, None, None, 2, 1.0, one, 1 << 20, one, one, one, None) == 1
+    assert d(_rows(n_list=0), 1, one, one, one, None, None, 0, 1.0, one, 1 << 20, one, one, one, None) == 1
+    assert d(_rows(grad_stride=1), 1, one, one, one, None, None, 0, 1.0, one, 1 << 20, one, one, one, None) == 1
+    n = L.cwrnnt_distill_workspace_bytes(_rows())
+    assert n >= 8 * 10
+    assert d(_rows(), 1, one, one, one, None, None, 0, 1.0, None, n, one, one, one, None) == 2
+    assert d(_rows(), 1, one, one, one, None, None, 0, 1.0, one, n - 1, one, one, one, None) == 2
+    assert d(_rows(), 1, one, one, one, None, None, 0, 1.0, ctypes.c_void_p(260), n, one, one, one, None) == 2
+
+
+def test_no_rows_is_no_work():
+    L = capi.lib()
+    assert L.cwrnnt_token_scores(_rows(n_rows=0), None, None, None, None, None, None, None, None) == 0
+    assert L.cwrnnt_token_scores_backward(_rows(n_rows=0), None, None, None, None, None, None, None, None, None, None) == 0
+    assert L.cwrnnt_distill(_rows(n_rows=0), 1, None, None, None, None, None, 0, 1.0, None, 0, None, None, None, None) == 0
+
+
+def test_python_entry_points_refuse_what_they_cannot_take():
+    x = torch.zeros(4, 9)
+    t = torch.zeros(4, 2, dtype=torch.int32)
+    with pytest.raises(AssertionError):
+        token_scores(x)                                   # nothing asked for
+    with pytest.raises(AssertionError):
+        token_scores(x, t.long())                         # int64 targets
+    with pytest.raises(AssertionError):
+        token_scores(x, t[:3])                            # another number of rows
+    with pytest.raises(RuntimeError, match="CUDA"):
+        token_scores(x, t)                                # not on a GPU
+    v = torch.zeros(4, 2)
+    for bad in (dict(teacher=v.double()), dict(teacher=v[:, :1]), dict(indices=t.long()), dict(weight=torch.zeros(3)),
+                dict(weight=torch.zeros(4, dtype=torch.float64)), dict(reduction="max"),
+                dict(teacher=torch.zeros(4, 33), indices=torch.zeros(4, 33, dtype=torch.int32)),
+                dict(teacher=torch.zeros(4, 0), indices=torch.zeros(4, 0, dtype=torch.int32))):
+        kw = dict(teacher=v, indices=t)
+        kw.update(bad)
+        with pytest.raises(AssertionError):
+            distill_loss(x, kw.pop("teacher"), kw.pop("indices"), **kw)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        distill_loss(x, v, t)
