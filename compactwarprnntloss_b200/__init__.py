@@ -6,6 +6,7 @@ Sub-modules:
   sharding  sequence sharding across GPUs and the cost-vector exchange
   synth     seeded synthetic workloads of the benchmark configurations
   joint     `compact_joint` - the joint network's broadcast-add written directly as compact rows
+  linear    `fused_linear` - the joint's linear layers: bias, activation and residual in the product's epilogue
   graphs    `GraphedStep` - a whole training step of the loss as one replayed CUDA graph per shape bucket
   scores    `token_scores` - log-probabilities of given tokens, entropy and best alternatives of logits rows
   distill   `distill_loss` - distillation from a teacher's top entries, loss and gradient in one pass
@@ -34,6 +35,9 @@ def __getattr__(name):
     if name in ("token_scores", "TokenScores"):
         from . import scores
         return getattr(scores, name)
+    if name == "fused_linear":
+        from . import linear
+        return linear.fused_linear
     if name == "distill_loss":
         from . import distill
         return distill.distill_loss

@@ -32,6 +32,7 @@ EXPORTS = [
     "cwrnnt_pipe_wait_costs", "cwrnnt_validate", "cwrnnt_validate_async", "cwrnnt_static_status", "cwrnnt_fill_costs", "cwrnnt_recursion", "cwrnnt_alignment_scratch_bytes", "cwrnnt_export_alignment",
     "cwrnnt_export_posteriors", "cwrnnt_pipe_create_traced", "cwrnnt_pipe_timeline",
     "cwrnnt_token_scores", "cwrnnt_token_scores_backward", "cwrnnt_distill_workspace_bytes", "cwrnnt_distill",
+    "cwrnnt_linear_workspace_bytes", "cwrnnt_linear_forward", "cwrnnt_linear_backward",
 ]
 
 
@@ -46,6 +47,13 @@ class Rows(ctypes.Structure):
     _fields_ = [("n_rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("grad_stride", ctypes.c_int64),
                 ("temperature", ctypes.c_double), ("V", ctypes.c_int32), ("dtype", ctypes.c_int32),
                 ("n_list", ctypes.c_int32), ("top_k", ctypes.c_int32)]
+
+
+class Linear(ctypes.Structure):
+    """cwrnnt_linear: shape, strides, type and activation of a linear layer."""
+    _fields_ = [("n_rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64),
+                ("g_stride", ctypes.c_int64), ("n_in", ctypes.c_int32), ("n_out", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32)]
 
 
 class CwrnntError(RuntimeError):
@@ -115,6 +123,11 @@ def lib():
         L.cwrnnt_distill_workspace_bytes.restype = i64
         L.cwrnnt_distill_workspace_bytes.argtypes = [rp]
         L.cwrnnt_distill.argtypes = [rp, i32, vp, vp, vp, vp, vp, i32, ctypes.c_double, vp, i64, vp, vp, vp, vp]
+        lp = ctypes.POINTER(Linear)
+        L.cwrnnt_linear_workspace_bytes.restype = i64
+        L.cwrnnt_linear_workspace_bytes.argtypes = [lp, i32]
+        L.cwrnnt_linear_forward.argtypes = [lp, vp, vp, vp, vp, vp, i64, vp, vp]
+        L.cwrnnt_linear_backward.argtypes = [lp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp]
         _lib = L
     return _lib
 

@@ -93,6 +93,26 @@ int check_rows(const cwrnnt_rows *p)
     return CWRNNT_OK;
 }
 
+int check_linear(const cwrnnt_linear *p)
+{
+    if (!p) return CWRNNT_ERR_ARGUMENT;
+    if (p->n_rows < 0 || p->n_rows > INT32_MAX - 1023) return CWRNNT_ERR_ARGUMENT;
+    if (p->n_in < 1 || p->n_out < 1 || p->n_in > (1 << 24) || p->n_out > (1 << 24)) return CWRNNT_ERR_ARGUMENT;
+    if (p->dtype != CWRNNT_F16 && p->dtype != CWRNNT_BF16) return CWRNNT_ERR_ARGUMENT;
+    if (p->activation < CWRNNT_ACT_NONE || p->activation > CWRNNT_ACT_SILU) return CWRNNT_ERR_ARGUMENT;
+    // rows of 2^38 elements apart and more are beyond a tensor map's strides
+    const int64_t most = int64_t(1) << 38;
+    if (p->x_stride < p->n_in || p->w_stride < p->n_in || p->x_stride > most || p->w_stride > most)
+        return CWRNNT_ERR_ARGUMENT;
+    return CWRNNT_OK;
+}
+
+// A matrix that TMA reads where it lies must start on a 16-byte boundary.
+bool linear_base(const void *m, int64_t stride)
+{
+    return m && (stride % 8 != 0 || reinterpret_cast<uintptr_t>(m) % 16 == 0);
+}
+
 }  // namespace
 
 void cwrnnt::set_last_error(const char *text) { std::snprintf(g_last_error, sizeof g_last_error, "%s", text); }
@@ -657,6 +677,49 @@ int cwrnnt_distill(const cwrnnt_rows *p, int32_t tail, const void *x, const void
     e = launch_distill(*p, tail != 0, x, teacher, indices, weight, upstream, upstream_stride, scale,
                        static_cast<double *>(workspace), row_loss, loss, grad_x, s);
     return e == cudaSuccess ? CWRNNT_OK : fail_launch("distill", e);
+}
+
+int64_t cwrnnt_linear_workspace_bytes(const cwrnnt_linear *p, int32_t backward)
+{
+    if (check_linear(p) != CWRNNT_OK || (backward && p->g_stride < p->n_out)) return -1;
+    return linear_workspace(*p, backward != 0);
+}
+
+int cwrnnt_linear_forward(const cwrnnt_linear *p, const void *x, const void *weight, const void *bias,
+                          const void *residual, void *workspace, int64_t workspace_bytes, void *y,
+                          cwrnnt_stream_t stream)
+{
+    int st = check_linear(p);
+    if (st) return st;
+    if (p->n_rows == 0) return CWRNNT_OK;
+    if (!linear_base(x, p->x_stride) || !linear_base(weight, p->w_stride) || !y) return CWRNNT_ERR_ARGUMENT;
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
+        workspace_bytes < linear_workspace(*p, false))
+        return CWRNNT_ERR_WORKSPACE;
+    cudaError_t e = launch_linear(*p, x, weight, bias, residual, workspace, y, reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? CWRNNT_OK : fail_launch("linear_forward", e);
+}
+
+int cwrnnt_linear_backward(const cwrnnt_linear *p, const void *x, const void *weight, const void *bias,
+                           const void *grad_y, void *workspace, int64_t workspace_bytes, void *grad_x,
+                           void *grad_weight, void *grad_bias, cwrnnt_stream_t stream)
+{
+    int st = check_linear(p);
+    if (st) return st;
+    if (p->g_stride < p->n_out || p->g_stride > (int64_t(1) << 38)) return CWRNNT_ERR_ARGUMENT;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaSuccess;
+    if (p->n_rows == 0) {  // sums over no rows
+        if (grad_weight) e = cudaMemsetAsync(grad_weight, 0, size_t(p->n_out) * p->n_in * 2, s);
+        if (e == cudaSuccess && grad_bias) e = cudaMemsetAsync(grad_bias, 0, size_t(p->n_out) * 2, s);
+        return e == cudaSuccess ? CWRNNT_OK : fail_launch("linear_backward", e);
+    }
+    if (!linear_base(x, p->x_stride) || !linear_base(weight, p->w_stride) || !linear_base(grad_y, p->g_stride))
+        return CWRNNT_ERR_ARGUMENT;
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < linear_workspace(*p, true))
+        return CWRNNT_ERR_WORKSPACE;
+    e = launch_linear_grad(*p, x, weight, bias, grad_y, workspace, grad_x, grad_weight, grad_bias, s);
+    return e == cudaSuccess ? CWRNNT_OK : fail_launch("linear_backward", e);
 }
 
 }  // extern "C"

@@ -164,6 +164,7 @@ template <>
 struct Elt<__half> {
     using acc = float;
     using cost = float;
+    static constexpr bool kBf16 = false;
     static constexpr int VE = 8;
     static __device__ __forceinline__ void unpack(const uint4 &v, float (&e)[8])
     {
@@ -202,6 +203,7 @@ template <>
 struct Elt<__nv_bfloat16> {
     using acc = float;
     using cost = float;
+    static constexpr bool kBf16 = true;
     static constexpr int VE = 8;
     static __device__ __forceinline__ void unpack(const uint4 &v, float (&e)[8])
     {

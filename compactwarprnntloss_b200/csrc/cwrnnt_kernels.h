@@ -98,4 +98,11 @@ cudaError_t launch_distill(const cwrnnt_rows &p, bool tail, const void *x, const
                            const void *weight, const void *upstream, int32_t upstream_stride, double scale,
                            double *partial, void *row_loss, void *loss, void *grad_x, cudaStream_t s);
 
+// Linear layers on the tensor cores: forward, gradients, and the workspace of either.
+int64_t linear_workspace(const cwrnnt_linear &p, bool backward);
+cudaError_t launch_linear(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *residual,
+                          void *workspace, void *y, cudaStream_t s);
+cudaError_t launch_linear_grad(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *g,
+                               void *workspace, void *grad_x, void *grad_w, void *grad_b, cudaStream_t s);
+
 }  // namespace cwrnnt

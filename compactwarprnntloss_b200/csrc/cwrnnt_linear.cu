@@ -1,0 +1,689 @@
+// The joint's linear layers on the tensor cores: y = act(x W^T + b) + r with everything but the product in its epilogue,
+// and its gradients. With z = x W^T + b and dz = dy * act'(z):
+//     dx = dz W,   dW = dz^T x,   db = sum over rows of dz,   dr = dy.
+// Nothing but the inputs is kept for the gradients: z is multiplied out again, and the epilogue of that product writes
+// dz at once (reading dy). Storing z in float instead costs more traffic than the product takes, storing it in 16 bits
+// costs digits of act'(z).
+//
+// One kernel for the four products: tiles of 128 x BN outputs, 64 elements of the sum a step. Operands come by tiled TMA
+// into a ring of 128-byte-swizzled stages; tcgen05.mma sums in TMEM in float. The forward product takes both operands
+// along the sum (K-major), dx takes W and dW takes both operands across it (MN-major): no operand is ever transposed in
+// memory. Warp 0 issues the loads, warp 1 the products, warps 2-5 carry the previous tile out of the second half of
+// TMEM meanwhile. CTAs are persistent; output columns run fastest, so that concurrent CTAs share their rows of x in L2.
+// Products with few tiles and long sums (dW) are split along the sum; the parts are float in the workspace, added in
+// a fixed order by a second kernel that carries the same epilogue.
+// TMA wants rows at multiples of 16 bytes: matrices of other strides are copied to such a stride first.
+#include "cwrnnt_kernels.h"
+#include "cwrnnt_tc.cuh"
+
+namespace cwrnnt {
+
+namespace {
+
+constexpr int kBM = 128, kBK = 64;
+constexpr int kLinearThreads = 192;
+constexpr int kMaxStages = 8;
+
+enum { kStore = 0, kSlope = 1, kPart = 2 };
+
+// ------------------------------------------------------------------------------------------------------- activations
+__device__ __forceinline__ float rcp(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// tanh to about 2^-22 relative: 1 - 2 / (1 + e^2z), and its series where that would cancel.
+__device__ __forceinline__ float tanh_full(float z)
+{
+    const float e = ex2_approx(fabsf(z) * 2.8853900817779268f);
+    const float t = copysignf(1.0f - 2.0f * rcp(1.0f + e), z);
+    const float s = z * z;
+    const float p = z * (1.0f + s * (-0.33333333333f + s * (0.13333333333f - 0.05396825397f * s)));
+    return fabsf(z) < 0.15f ? p : t;
+}
+__device__ __forceinline__ float activate(int act, float z)
+{
+    if (act == CWRNNT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
+    if (act == CWRNNT_ACT_TANH) return tanh_full(z);
+    if (act == CWRNNT_ACT_SILU) return z == -INFINITY ? 0.0f : z * rcp(1.0f + ex2_approx(-1.4426950408889634f * z));
+    return z;
+}
+__device__ __forceinline__ float slope(int act, float z)
+{
+    if (act == CWRNNT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+    if (act == CWRNNT_ACT_TANH) {  // 4 e / (1 + e)^2, e = exp(-2 |z|): no cancellation far out
+        const float e = ex2_approx(fabsf(z) * -2.8853900817779268f), r = rcp(1.0f + e);
+        return 4.0f * e * r * r;
+    }
+    if (act == CWRNNT_ACT_SILU) {  // s (1 + z (1 - s)), s the logistic function
+        if (fabsf(z) == INFINITY) return z > 0.0f ? 1.0f : 0.0f;
+        const float e = ex2_approx(-1.4426950408889634f * fabsf(z)), r = rcp(1.0f + e);
+        const float big = r, small = e * r;  // the larger and the smaller of s and 1 - s
+        return z >= 0.0f ? big * (1.0f + z * small) : small * (1.0f + z * big);
+    }
+    return 1.0f;
+}
+
+// ---------------------------------------------------------------------------------------------------------- epilogue
+struct Epilogue {
+    int mode;           // kStore, kSlope, kPart
+    int act;
+    const void *bias;   // [N] or null
+    const void *side;   // kStore: residual [M, side_ld] or null; kSlope: dy [M, side_ld]
+    void *out;          // [M, out_ld]
+    float *part;        // kPart: [splits, M, N]
+    int64_t side_ld, out_ld;
+    bool vec;           // rows of out and side allow 16-byte accesses; the columns come in whole groups of 8
+};
+
+// Columns [col, col + 8) of one row, `n` of them inside the matrix.
+template <typename T>
+__device__ __forceinline__ void finish8(const Epilogue &ep, float (&v)[8], int64_t row, int col, int n)
+{
+    using E = Elt<T>;
+    if (ep.bias) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c < n) v[c] += E::to_acc(__ldg(static_cast<const T *>(ep.bias) + col + c));
+    }
+    float s[8];
+    if (ep.side) {
+        const T *side = static_cast<const T *>(ep.side) + row * ep.side_ld + col;
+        if (ep.vec) {
+            E::unpack(__ldg(reinterpret_cast<const uint4 *>(side)), s);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) s[c] = c < n ? E::to_acc(__ldg(side + c)) : 0.0f;
+        }
+    }
+    if (ep.mode == kSlope) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = s[c] * slope(ep.act, v[c]);
+    } else {
+        if (ep.act != CWRNNT_ACT_NONE) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] = activate(ep.act, v[c]);
+        }
+        if (ep.side) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] += s[c];
+        }
+    }
+    T *out = static_cast<T *>(ep.out) + row * ep.out_ld + col;
+    if (ep.vec) {
+        *reinterpret_cast<uint4 *>(out) = E::pack(v);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c < n) out[c] = E::from_acc(v[c]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------- kernel
+struct Shape {
+    int64_t M;
+    int N;
+    int steps;             // steps of kBK along the sum, in all
+    int steps_per_split, splits;
+    int64_t tiles_m;
+    int tiles_n;
+    __device__ __forceinline__ int64_t tiles() const { return tiles_m * tiles_n * splits; }
+    // columns fastest, then rows, then parts of the sum
+    __device__ __forceinline__ void tile(int64_t t, int64_t &m, int &n, int &split) const
+    {
+        n = int(t % tiles_n);
+        t /= tiles_n;
+        m = t % tiles_m;
+        split = int(t / tiles_m);
+    }
+    __device__ __forceinline__ int first_step(int split) const { return split * steps_per_split; }
+    __device__ __forceinline__ int count_steps(int split) const
+    {
+        const int left = steps - first_step(split);
+        return left < steps_per_split ? left : steps_per_split;
+    }
+};
+
+template <int BN>
+struct Layout {
+    static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
+    static constexpr int kStages = 196608 / kStage < kMaxStages ? 196608 / kStage : kMaxStages;
+    static constexpr int kBytes = kStages * kStage + 1024;  // stages start on a 1024-byte boundary
+    static constexpr uint32_t kColumns = 2 * BN;            // two sums in TMEM
+};
+
+template <typename T, int BN, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kLinearThreads, 1)
+linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Shape sh,
+              const Epilogue ep)
+{
+    using L = Layout<BN>;
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full[L::kStages], empty[L::kStages], sum_full[2], sum_empty[2], drained;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int gave_up;
+    unsigned char *stages = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (warp == 0 && lane == 0) {
+        for (int i = 0; i < L::kStages; ++i) {
+            tc::mbar_init(&full[i], 1);
+            tc::mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&sum_full[i], 1);
+            tc::mbar_init(&sum_empty[i], 4);
+        }
+        tc::mbar_init(&drained, 1);
+        gave_up = 0;
+        tc::mbar_init_fence();
+        tc::prefetch_map(&map_a);
+        tc::prefetch_map(&map_b);
+    }
+    if (warp == 1) tc::tmem_alloc(&tmem_slot, L::kColumns);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int64_t total = sh.tiles();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int at = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            uint32_t started = 0;  // stages loaded at least once
+            for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                int64_t m;
+                int n, split;
+                sh.tile(t, m, n, split);
+                const int k0 = sh.first_step(split), k1 = k0 + sh.count_steps(split);
+                for (int k = k0; ok && k < k1; ++k) {
+                    ok = tc::mbar_wait(&empty[at], phase ^ 1, &gave_up);
+                    if (!ok) break;
+                    unsigned char *a = stages + at * L::kStage, *b = a + L::kA;
+                    tc::mbar_expect(&full[at], L::kStage);
+                    if (A_MN) {
+#pragma unroll
+                        for (int i = 0; i < kBM / 64; ++i)
+                            tc::load_2d(a + i * 8192, &map_a, &full[at], int(m) * kBM + i * 64, k * kBK);
+                    } else {
+                        tc::load_2d(a, &map_a, &full[at], k * kBK, int(m) * kBM);
+                    }
+                    if (B_MN) {
+#pragma unroll
+                        for (int i = 0; i < BN / 64; ++i)
+                            tc::load_2d(b + i * 8192, &map_b, &full[at], n * BN + i * 64, k * kBK);
+                    } else {
+                        tc::load_2d(b, &map_b, &full[at], k * kBK, n * BN);
+                    }
+                    started |= 1u << at;
+                    if (++at == L::kStages) at = 0, phase ^= 1;
+                }
+            }
+            // every load has landed before the CTA's memory goes: the last fill of each stage
+            for (int i = 0; i < L::kStages; ++i) {
+                if (!(started >> i & 1)) continue;
+                const uint32_t last = i < at ? phase : phase ^ 1;
+                const uint64_t since = tc::now_ns();
+                while (!tc::mbar_try(&full[i], last) && tc::now_ns() - since < 2000000000ull) {
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc =
+                tc::instruction(Elt<T>::kBf16 ? 1 : 0, A_MN, B_MN, kBM, BN);
+            int at = 0, half = 0;
+            uint32_t phase = 0, half_phase = 0;
+            bool ok = true;
+            for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                int64_t m;
+                int n, split;
+                sh.tile(t, m, n, split);
+                ok = tc::mbar_wait(&sum_empty[half], half_phase ^ 1, &gave_up);
+                if (!ok) break;
+                tc::fence_after();
+                const uint32_t d = tmem + uint32_t(half * BN);
+                const int steps = sh.count_steps(split);
+                for (int k = 0; ok && k < steps; ++k) {
+                    ok = tc::mbar_wait(&full[at], phase, &gave_up);
+                    if (!ok) break;
+                    tc::fence_after();
+                    const uint32_t a = tc::smem_addr(stages + at * L::kStage), b = a + L::kA;
+#pragma unroll
+                    for (int i = 0; i < kBK / 16; ++i) {
+                        // 16 elements of the sum: 32 bytes along a K-major row, 16 rows of an MN-major operand
+                        const uint64_t da = tc::operand(a + i * (A_MN ? 2048 : 32), A_MN ? 8192 : 16, 1024);
+                        const uint64_t db = tc::operand(b + i * (B_MN ? 2048 : 32), B_MN ? 8192 : 16, 1024);
+                        tc::mma_f16(d, da, db, idesc, k > 0 || i > 0);
+                    }
+                    tc::commit(&empty[at]);
+                    if (++at == L::kStages) at = 0, phase ^= 1;
+                }
+                if (ok) tc::commit(&sum_full[half]);
+                if (++half == 2) half = 0, half_phase ^= 1;
+            }
+            // every product has left the tensor core before the CTA's memory goes
+            tc::commit(&drained);
+            const uint64_t since = tc::now_ns();
+            while (!tc::mbar_try(&drained, 0) && tc::now_ns() - since < 2000000000ull) {
+            }
+        }
+    } else {
+        const int quarter = warp & 3;  // the TMEM lanes that this warp may read
+        int half = 0;
+        uint32_t half_phase = 0;
+        for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
+            int64_t m;
+            int n, split;
+            sh.tile(t, m, n, split);
+            const bool ok = tc::mbar_wait(&sum_full[half], half_phase, &gave_up);
+            tc::fence_after();
+            const int64_t row = m * kBM + quarter * 32 + lane;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 32) {
+                uint32_t r[32];
+                const int col = n * BN + c;
+                if (col >= sh.N) break;
+                __syncwarp();
+                tc::tmem_load32(tmem + uint32_t(half * BN + c) + (uint32_t(quarter * 32) << 16), r);
+                tc::tmem_load_wait();
+                // a wait that ran out leaves NaN
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int left = sh.N - (col + g * 8);
+                    if (left <= 0 || row >= sh.M) break;
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = ok ? __uint_as_float(r[g * 8 + i]) : NAN;
+                    if (ep.mode == kPart) {
+                        float *out = ep.part + (int64_t(split) * sh.M + row) * sh.N + col + g * 8;
+                        if (ep.vec) {
+                            *reinterpret_cast<float4 *>(out) = make_float4(v[0], v[1], v[2], v[3]);
+                            *reinterpret_cast<float4 *>(out + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (i < left) out[i] = v[i];
+                        }
+                    } else {
+                        finish8<T>(ep, v, row, col + g * 8, left < 8 ? left : 8);
+                    }
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&sum_empty[half]);
+            if (++half == 2) half = 0, half_phase ^= 1;
+        }
+    }
+    __syncwarp();
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc::fence_after();
+        tc::tmem_free(tmem, L::kColumns);
+    }
+}
+
+// The parts of a split sum, added in their order, and the epilogue.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const float *__restrict__ part, int splits, int64_t M, int N, const Epilogue ep)
+{
+    const int groups = (N + 7) / 8;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < M * groups; i += int64_t(gridDim.x) * 256) {
+        const int64_t row = i / groups;
+        const int col = int(i % groups) * 8, n = N - col < 8 ? N - col : 8;
+        float v[8] = {};
+        for (int s = 0; s < splits; ++s) {
+            const float *p = part + (int64_t(s) * M + row) * N + col;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (c < n) v[c] += __ldg(p + c);
+        }
+        finish8<T>(ep, v, row, col, n);
+    }
+}
+
+// [rows, cols] of any stride to rows at multiples of 16 bytes.
+template <typename T>
+__global__ void __launch_bounds__(256) restride_kernel(const T *__restrict__ src, int64_t src_ld, T *__restrict__ dst, int64_t dst_ld,
+                                int64_t rows, int cols)
+{
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * dst_ld; i += int64_t(gridDim.x) * 256) {
+        const int64_t r = i / dst_ld;
+        const int c = int(i % dst_ld);
+        dst[i] = c < cols ? src[r * src_ld + c] : Elt<T>::from_acc(0.0f);
+    }
+}
+
+// Column sums: each CTA adds up a run of rows of 256 columns in float; the runs' sums are added in order afterwards.
+constexpr int kSumRows = 8;
+template <typename T>
+__global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ g, int64_t ld, int64_t rows, int cols,
+                                                          int64_t run, float *__restrict__ part)
+{
+    using E = Elt<T>;
+    __shared__ float sums[kSumRows][256 + 8];
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    const int col = blockIdx.x * 256 + tx * 8;
+    float acc[8] = {};
+    const int64_t first = int64_t(blockIdx.y) * run, end = first + run < rows ? first + run : rows;
+    if (col < cols) {
+        for (int64_t r = first + ty; r < end; r += kSumRows) {
+            float v[8];
+            if (col + 8 <= cols) {
+                E::unpack(__ldg(reinterpret_cast<const uint4 *>(g + r * ld + col)), v);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] = col + c < cols ? E::to_acc(__ldg(g + r * ld + col + c)) : 0.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[c] += v[c];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) sums[ty][tx * 8 + c] = acc[c];
+    __syncthreads();
+    const int mine = blockIdx.x * 256 + threadIdx.x;
+    if (mine < cols) {
+        float s = 0.0f;
+        for (int y = 0; y < kSumRows; ++y) s += sums[y][threadIdx.x];
+        part[int64_t(blockIdx.y) * cols + mine] = s;
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) column_join_kernel(const float *__restrict__ part, int runs, int cols, T *__restrict__ out)
+{
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float s = 0.0f;
+    for (int i = 0; i < runs; ++i) s += __ldg(part + int64_t(i) * cols + c);
+    out[c] = Elt<T>::from_acc(s);
+}
+
+// --------------------------------------------------------------------------------------------------------- host side
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder()
+{
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) !=
+                cudaSuccess || found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// A [rows, cols] matrix in memory, 16-byte rows, read in boxes of 64 columns x `box_rows` rows.
+template <typename T>
+bool make_map(CUtensorMap *map, const void *p, int64_t rows, int64_t cols, int64_t ld, int box_rows)
+{
+    const EncodeFn encode = encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, strides[1] = {cuuint64_t(ld) * 2};
+    const cuuint32_t box[2] = {64, cuuint32_t(box_rows)}, one[2] = {1, 1};
+    return encode(map, Elt<T>::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                  const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How a product of M x N outputs and a sum of `len` is cut: the width of its tiles and the parts of its sum.
+struct Cut {
+    int bn, splits, steps_per_split;
+};
+Cut cut_product(int64_t M, int N, int64_t len, bool b_mn)
+{
+    const int64_t tiles_m = (M + kBM - 1) / kBM;
+    const int steps = int((len + kBK - 1) / kBK);
+    Cut c{256, 1, steps};
+    const int least = b_mn ? 64 : 32;
+    // narrower tiles until every SM has one
+    while (c.bn > least && (c.bn / 2 >= N || tiles_m * ((N + c.bn - 1) / c.bn) < kNumSMs)) c.bn /= 2;
+    // split long sums of few tiles, at least eight steps a part
+    const int64_t tiles = tiles_m * ((N + c.bn - 1) / c.bn);
+    if (tiles * 2 <= kNumSMs && steps >= 32) {
+        // wide tiles again: parts give the SMs their work
+        c.bn = N > 128 ? 256 : (N > 64 ? 128 : 64);
+        const int64_t wide = tiles_m * ((N + c.bn - 1) / c.bn);
+        int64_t parts = kNumSMs / wide;
+        if (parts > steps / 8) parts = steps / 8;
+        if (parts < 1) parts = 1;
+        c.steps_per_split = int((steps + parts - 1) / parts);
+        c.splits = (steps + c.steps_per_split - 1) / c.steps_per_split;
+    }
+    return c;
+}
+int64_t part_bytes(int64_t M, int N, const Cut &c) { return c.splits > 1 ? align_up(4 * c.splits * M * N, 256) : 0; }
+
+struct Matrix {  // [rows, cols], `mn`: its columns are the output's and its rows the sum's
+    const void *p;
+    int64_t rows, cols, ld;
+    bool mn;
+};
+
+template <typename T, int BN, bool A_MN, bool B_MN>
+cudaError_t run_product(const Matrix &a, const Matrix &b, const Shape &sh, const Epilogue &ep, cudaStream_t s)
+{
+    using L = Layout<BN>;
+    CUtensorMap ma, mb;
+    if (!make_map<T>(&ma, a.p, a.rows, a.cols, a.ld, A_MN ? kBK : kBM) ||
+        !make_map<T>(&mb, b.p, b.rows, b.cols, b.ld, B_MN ? kBK : BN))
+        return cudaErrorInvalidValue;
+    auto kernel = linear_kernel<T, BN, A_MN, B_MN>;
+    // the attribute belongs to the device that is current
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    if (e != cudaSuccess) return e;
+    const int64_t total = sh.tiles_m * sh.tiles_n * sh.splits;
+    kernel<<<unsigned(total < kNumSMs ? total : kNumSMs), kLinearThreads, L::kBytes, s>>>(ma, mb, sh, ep);
+    return cudaGetLastError();
+}
+
+template <typename T, bool A_MN, bool B_MN>
+cudaError_t run_product_bn(int bn, const Matrix &a, const Matrix &b, const Shape &sh, const Epilogue &ep, cudaStream_t s)
+{
+    switch (bn) {
+    case 256: return run_product<T, 256, A_MN, B_MN>(a, b, sh, ep, s);
+    case 128: return run_product<T, 128, A_MN, B_MN>(a, b, sh, ep, s);
+    case 64: return run_product<T, 64, A_MN, B_MN>(a, b, sh, ep, s);
+    }
+    if constexpr (!B_MN) return run_product<T, 32, A_MN, B_MN>(a, b, sh, ep, s);
+    return cudaErrorInvalidValue;
+}
+
+// out[M, N] = epilogue(sum over `len` of a * b); `part`: part_bytes() of workspace.
+template <typename T>
+cudaError_t product(const Matrix &a, const Matrix &b, int64_t M, int N, int64_t len, Epilogue ep, float *part, cudaStream_t s)
+{
+    if (M == 0) return cudaSuccess;
+    const Cut c = cut_product(M, N, len, b.mn);
+    Shape sh{};
+    sh.M = M, sh.N = N;
+    sh.steps = int((len + kBK - 1) / kBK);
+    sh.steps_per_split = c.steps_per_split, sh.splits = c.splits;
+    sh.tiles_m = (M + kBM - 1) / kBM, sh.tiles_n = (N + c.bn - 1) / c.bn;
+    auto on16 = [](const void *p, int64_t ld) { return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0); };
+    ep.vec = N % 8 == 0 && on16(ep.out, ep.out_ld) && on16(ep.side, ep.side_ld);
+    Epilogue here = ep;
+    if (c.splits > 1) {
+        here = Epilogue{};
+        here.mode = kPart, here.part = part, here.vec = N % 4 == 0 && N % 8 == 0;
+    }
+    cudaError_t e;
+    if (a.mn)
+        e = run_product_bn<T, true, true>(c.bn, a, b, sh, here, s);
+    else if (b.mn)
+        e = run_product_bn<T, false, true>(c.bn, a, b, sh, here, s);
+    else
+        e = run_product_bn<T, false, false>(c.bn, a, b, sh, here, s);
+    if (e != cudaSuccess || c.splits == 1) return e;
+    const int64_t items = M * ((N + 7) / 8), blocks = (items + 255) / 256;
+    join_kernel<T><<<unsigned(blocks < kNumSMs * 16 ? blocks : kNumSMs * 16), 256, 0, s>>>(part, c.splits, M, N, ep);
+    return cudaGetLastError();
+}
+
+// Workspace: copies of matrices whose rows TMA cannot take, dz, parts of split sums, column sums.
+int64_t padded(int64_t cols) { return align_up(cols, 8); }
+int64_t copy_bytes(int64_t rows, int64_t cols, int64_t ld)
+{
+    return ld % 8 ? align_up(rows * padded(cols) * 2, 256) : 0;
+}
+constexpr int kMostRuns = 256;
+
+struct LinearPlan {
+    int64_t x, w, g, dz, part, sums, total;  // offsets
+};
+LinearPlan plan_linear(const cwrnnt_linear &p, bool backward)
+{
+    LinearPlan q{};
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += align_up(bytes, 256);
+        return here;
+    };
+    q.x = take(copy_bytes(p.n_rows, p.n_in, p.x_stride));
+    q.w = take(copy_bytes(p.n_out, p.n_in, p.w_stride));
+    auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
+    int64_t parts = 0;
+    if (!backward || p.activation != CWRNNT_ACT_NONE)
+        parts = part_bytes(p.n_rows, p.n_out, cut_product(p.n_rows, p.n_out, p.n_in, false));
+    if (backward) {
+        if (p.activation != CWRNNT_ACT_NONE)
+            q.dz = take(p.n_rows * padded(p.n_out) * 2);
+        else
+            q.g = take(copy_bytes(p.n_rows, p.n_out, p.g_stride));
+        parts = most(parts, part_bytes(p.n_rows, p.n_in, cut_product(p.n_rows, p.n_in, p.n_out, true)));
+        parts = most(parts, part_bytes(p.n_out, p.n_in, cut_product(p.n_out, p.n_in, p.n_rows, true)));
+        q.sums = take(4 * int64_t(kMostRuns) * p.n_out);
+    }
+    q.part = take(parts);
+    q.total = at > 0 ? at : 256;
+    return q;
+}
+
+template <typename T>
+cudaError_t restride(const void *src, int64_t ld, int64_t rows, int64_t cols, void *dst, cudaStream_t s)
+{
+    const int64_t items = rows * padded(cols), blocks = (items + 255) / 256;
+    if (items == 0) return cudaSuccess;
+    restride_kernel<T><<<unsigned(blocks < kNumSMs * 32 ? blocks : kNumSMs * 32), 256, 0, s>>>(
+        static_cast<const T *>(src), ld, static_cast<T *>(dst), padded(cols), rows, int(cols));
+    return cudaGetLastError();
+}
+
+// `m` as TMA can take it, copied to `room` if need be.
+template <typename T>
+cudaError_t readable(Matrix &m, char *room, cudaStream_t s)
+{
+    if (m.ld % 8 == 0) return cudaSuccess;
+    const cudaError_t e = restride<T>(m.p, m.ld, m.rows, m.cols, room, s);
+    m.p = room, m.ld = padded(m.cols);
+    return e;
+}
+
+#define CWRNNT_TRY(call)                                   \
+    do {                                                   \
+        const cudaError_t e_ = (call);                     \
+        if (e_ != cudaSuccess) return e_;                  \
+    } while (0)
+
+template <typename T>
+cudaError_t linear_forward(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *residual,
+                           char *ws, void *y, cudaStream_t s)
+{
+    const LinearPlan q = plan_linear(p, false);
+    Matrix a{x, p.n_rows, p.n_in, p.x_stride, false}, b{w, p.n_out, p.n_in, p.w_stride, false};
+    CWRNNT_TRY(readable<T>(a, ws + q.x, s));
+    CWRNNT_TRY(readable<T>(b, ws + q.w, s));
+    Epilogue ep{};
+    ep.mode = kStore, ep.act = p.activation, ep.bias = bias;
+    ep.side = residual, ep.side_ld = p.n_out;
+    ep.out = y, ep.out_ld = p.n_out;
+    return product<T>(a, b, p.n_rows, p.n_out, p.n_in, ep, reinterpret_cast<float *>(ws + q.part), s);
+}
+
+template <typename T>
+cudaError_t linear_backward(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *g,
+                            char *ws, void *grad_x, void *grad_w, void *grad_b, cudaStream_t s)
+{
+    const LinearPlan q = plan_linear(p, true);
+    float *part = reinterpret_cast<float *>(ws + q.part);
+    Matrix mx{x, p.n_rows, p.n_in, p.x_stride, false}, mw{w, p.n_out, p.n_in, p.w_stride, false};
+    Matrix dz{g, p.n_rows, p.n_out, p.g_stride, false};
+    const bool act = p.activation != CWRNNT_ACT_NONE;
+    if (act || grad_w) CWRNNT_TRY(readable<T>(mx, ws + q.x, s));
+    if (act || grad_x) CWRNNT_TRY(readable<T>(mw, ws + q.w, s));
+    if (act) {
+        Epilogue ep{};
+        ep.mode = kSlope, ep.act = p.activation, ep.bias = bias;
+        ep.side = g, ep.side_ld = p.g_stride;
+        ep.out = ws + q.dz, ep.out_ld = padded(p.n_out);
+        CWRNNT_TRY(product<T>(mx, mw, p.n_rows, p.n_out, p.n_in, ep, part, s));
+        dz.p = ws + q.dz, dz.ld = padded(p.n_out);
+    } else {
+        CWRNNT_TRY(readable<T>(dz, ws + q.g, s));
+    }
+    if (grad_b) {
+        // runs of rows: enough of them to fill the GPU with CTAs of 256 columns
+        const int64_t across = (p.n_out + 255) / 256;
+        int64_t runs = (kNumSMs * 4 + across - 1) / across;
+        const int64_t most = (p.n_rows + 63) / 64;
+        if (runs > most) runs = most;
+        if (runs > kMostRuns) runs = kMostRuns;
+        if (runs < 1) runs = 1;
+        const int64_t run = (p.n_rows + runs - 1) / runs;
+        float *sums = reinterpret_cast<float *>(ws + q.sums);
+        column_sums_kernel<T><<<dim3(unsigned(across), unsigned(runs)), 256, 0, s>>>(
+            static_cast<const T *>(dz.p), dz.ld, p.n_rows, p.n_out, run, sums);
+        CWRNNT_TRY(cudaGetLastError());
+        column_join_kernel<T><<<unsigned(across), 256, 0, s>>>(sums, int(runs), p.n_out, static_cast<T *>(grad_b));
+        CWRNNT_TRY(cudaGetLastError());
+    }
+    if (grad_x) {
+        Epilogue ep{};
+        ep.out = grad_x, ep.out_ld = p.n_in;
+        Matrix b = mw;
+        b.mn = true;
+        CWRNNT_TRY(product<T>(dz, b, p.n_rows, p.n_in, p.n_out, ep, part, s));
+    }
+    if (grad_w) {
+        Epilogue ep{};
+        ep.out = grad_w, ep.out_ld = p.n_in;
+        Matrix a = dz, b = mx;
+        a.mn = b.mn = true;
+        CWRNNT_TRY(product<T>(a, b, p.n_out, p.n_in, p.n_rows, ep, part, s));
+    }
+    return cudaSuccess;
+}
+
+}  // namespace
+
+int64_t linear_workspace(const cwrnnt_linear &p, bool backward) { return plan_linear(p, backward).total; }
+
+cudaError_t launch_linear(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *residual,
+                          void *workspace, void *y, cudaStream_t s)
+{
+    if (p.dtype == CWRNNT_F16)
+        return linear_forward<__half>(p, x, w, bias, residual, static_cast<char *>(workspace), y, s);
+    return linear_forward<__nv_bfloat16>(p, x, w, bias, residual, static_cast<char *>(workspace), y, s);
+}
+
+cudaError_t launch_linear_grad(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *g,
+                               void *workspace, void *grad_x, void *grad_w, void *grad_b, cudaStream_t s)
+{
+    char *ws = static_cast<char *>(workspace);
+    if (p.dtype == CWRNNT_F16) return linear_backward<__half>(p, x, w, bias, g, ws, grad_x, grad_w, grad_b, s);
+    return linear_backward<__nv_bfloat16>(p, x, w, bias, g, ws, grad_x, grad_w, grad_b, s);
+}
+
+}  // namespace cwrnnt

@@ -399,6 +399,101 @@ std::tuple<OptTensor, OptTensor, OptTensor> distill(const torch::Tensor &x, cons
     return {rows, loss, gx};
 }
 
+// ------------------------------------------------------------------------------------------------- linear layers
+
+// A matrix with unit column stride as the C ABI reads it where it lies; copied where its rows overlap, or where TMA would
+// have to start off a 16-byte boundary.
+torch::Tensor readable(const torch::Tensor &m)
+{
+    const bool rows_ok = m.size(0) < 2 || m.stride(0) >= m.size(1);
+    const bool columns_ok = m.size(1) < 2 || m.stride(1) == 1;
+    const int64_t ld = m.size(0) < 2 ? m.size(1) : m.stride(0);
+    if (!rows_ok || !columns_ok) return m.clone(torch::MemoryFormat::Contiguous);
+    if (ld % 8 == 0 && reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 != 0)
+        return m.clone(torch::MemoryFormat::Contiguous);
+    return m;
+}
+int64_t leading(const torch::Tensor &m) { return m.size(0) < 2 ? m.size(1) : m.stride(0); }
+
+cwrnnt_linear describe_linear(const torch::Tensor &x, const torch::Tensor &weight, const OptTensor &bias,
+                              int64_t activation)
+{
+    CHECK_CUDA(x);
+    TORCH_CHECK(x.dim() == 2 && weight.dim() == 2 && x.size(1) == weight.size(1) && x.size(1) > 0 && weight.size(0) > 0,
+                "x must be [rows, n_in] and weight [n_out, n_in]");
+    TORCH_CHECK(x.scalar_type() == torch::ScalarType::Half || x.scalar_type() == torch::ScalarType::BFloat16,
+                "x must be float16 or bfloat16, got ", x.scalar_type());
+    TORCH_CHECK(weight.scalar_type() == x.scalar_type() && weight.device() == x.device(),
+                "weight must have the type and device of x");
+    TORCH_CHECK(x.size(1) <= (1 << 24) && weight.size(0) <= (1 << 24) && x.size(0) <= INT32_MAX - 1023,
+                "a side of the product is too long");
+    if (bias)
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == weight.size(0) && bias->scalar_type() == x.scalar_type() &&
+                        bias->device() == x.device() && bias->is_contiguous(),
+                    "bias must be [n_out], contiguous, of the type and device of x");
+    cwrnnt_linear p{};
+    p.n_rows = x.size(0);
+    p.n_in = static_cast<int32_t>(x.size(1));
+    p.n_out = static_cast<int32_t>(weight.size(0));
+    p.x_stride = leading(x);
+    p.w_stride = leading(weight);
+    p.g_stride = weight.size(0);
+    p.dtype = dtype_code(x);
+    p.activation = static_cast<int32_t>(activation);
+    return p;
+}
+
+torch::Tensor linear_forward(const torch::Tensor &x_, const torch::Tensor &weight_, const OptTensor &bias,
+                             const OptTensor &residual, int64_t activation)
+{
+    CHECK_CUDA(x_);
+    CHECK_CUDA(weight_);
+    TORCH_CHECK(x_.dim() == 2 && weight_.dim() == 2, "x must be [rows, n_in] and weight [n_out, n_in]");
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const auto x = readable(x_), weight = readable(weight_);
+    const cwrnnt_linear p = describe_linear(x, weight, bias, activation);
+    if (residual)
+        TORCH_CHECK(residual->dim() == 2 && residual->size(0) == p.n_rows && residual->size(1) == p.n_out &&
+                        residual->scalar_type() == x.scalar_type() && residual->device() == x.device() &&
+                        residual->is_contiguous(),
+                    "residual must be [rows, n_out], contiguous, of the type and device of x");
+    const int64_t bytes = cwrnnt_linear_workspace_bytes(&p, 0);
+    TORCH_CHECK(bytes >= 0, "invalid linear layer");
+    auto ws = torch::empty({bytes}, x.options().dtype(torch::kUInt8));
+    auto y = torch::empty({x.size(0), weight.size(0)}, x.options());
+    check_status(cwrnnt_linear_forward(&p, x.data_ptr(), weight.data_ptr(), ptr(bias), ptr(residual), ws.data_ptr(),
+                                       bytes, y.data_ptr(), current_stream()),
+                 "cwrnnt_linear_forward");
+    return y;
+}
+
+// Returns (grad_x?, grad_weight?, grad_bias?).
+std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(const torch::Tensor &x_, const torch::Tensor &weight_,
+                                                            const OptTensor &bias, const torch::Tensor &grad_y,
+                                                            int64_t activation, bool want_x, bool want_weight,
+                                                            bool want_bias)
+{
+    CHECK_CUDA(x_);
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const auto x = readable(x_), weight = readable(weight_), g = readable(grad_y);
+    cwrnnt_linear p = describe_linear(x, weight, bias, activation);
+    TORCH_CHECK(g.dim() == 2 && g.size(0) == p.n_rows && g.size(1) == p.n_out && g.scalar_type() == x.scalar_type() &&
+                    g.device() == x.device(),
+                "the upstream gradient must be [rows, n_out], of the type and device of x");
+    p.g_stride = leading(g);
+    const int64_t bytes = cwrnnt_linear_workspace_bytes(&p, 1);
+    TORCH_CHECK(bytes >= 0, "invalid linear layer");
+    auto ws = torch::empty({bytes}, x.options().dtype(torch::kUInt8));
+    OptTensor gx, gw, gb;
+    if (want_x) gx = torch::empty({x.size(0), x.size(1)}, x.options());
+    if (want_weight) gw = torch::empty({weight.size(0), weight.size(1)}, x.options());
+    if (want_bias) gb = torch::empty({weight.size(0)}, x.options());
+    check_status(cwrnnt_linear_backward(&p, x.data_ptr(), weight.data_ptr(), ptr(bias), g.data_ptr(), ws.data_ptr(),
+                                        bytes, ptr(gx), ptr(gw), ptr(gb), current_stream()),
+                 "cwrnnt_linear_backward");
+    return {gx, gw, gb};
+}
+
 // ------------------------------------------------------------------- the reference module's functions, same shapes
 
 // cwarp_cuda.cpp:84-108. xs are log-probabilities. Returns (costs [N], grads [STU,2], alphas, betas [N,Tmax,Umax+1]).
@@ -505,6 +600,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("_token_scores", &token_scores, "Scores of logits rows: (log_probs, entropy, top_log_probs, top_indices, stats).");
     m.def("_token_scores_backward", &token_scores_backward, "Gradient of the scores w.r.t. the rows.");
     m.def("_distill", &distill, "Distillation from a teacher's top entries: (row_loss, loss, grad_x).");
+    m.def("_linear_forward", &linear_forward, "act(x W^T + bias) + residual on the tensor cores.");
+    m.def("_linear_backward", &linear_backward, "Gradients of a linear layer: (grad_x, grad_weight, grad_bias).");
     m.attr("MAX_LIST") = static_cast<int>(CWRNNT_MAX_LIST);
     m.attr("FUSED_LOG_SOFTMAX") = static_cast<int>(CWRNNT_FUSED_LOG_SOFTMAX);
     m.attr("COSTS_ONLY") = static_cast<int>(CWRNNT_COSTS_ONLY);

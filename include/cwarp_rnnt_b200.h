@@ -413,6 +413,37 @@ CWRNNT_API int cwrnnt_distill(const cwrnnt_rows *p, int32_t tail, const void *x,
                               void *row_loss, void *loss, void *grad_x, cwrnnt_stream_t stream);
 
 /*
+ * The joint's linear layers on the tensor cores, everything but the product in its epilogue:
+ *     y = act(x W^T + bias) + residual        x [n_rows, n_in], weight [n_out, n_in], y [n_rows, n_out]
+ * with float sums; x, weight, bias, residual, y and all gradients are of p->dtype, CWRNNT_F16 or CWRNNT_BF16 (other
+ * types are refused: the tensor cores have no product of theirs). cwrnnt_linear_backward writes, for the upstream
+ * gradient grad_y, whichever of grad_x, grad_weight and grad_bias are not NULL (the residual's is grad_y itself);
+ * nothing but the inputs is kept for it, and dz = grad_y * act'(z) is rounded to the type before its products, as the
+ * tensor cores take it. x, weight and grad_y may have rows further apart than their length; where such a stride is a
+ * multiple of 8 elements the matrix must start on a 16-byte boundary, other strides are copied first (into the
+ * workspace). bias, residual and all outputs are contiguous. Sums are split and joined in a fixed order: results
+ * repeat bit for bit. Every wait inside the kernels is bounded (two seconds); a tile whose wait runs out is NaN.
+ * workspace: cwrnnt_linear_workspace_bytes(p, backward) bytes, 256-byte aligned; not shared by calls that may overlap.
+ */
+#define CWRNNT_ACT_SILU 3 /* z / (1 + exp(-z)); cwrnnt_linear_* only */
+typedef struct {
+    int64_t n_rows;   /* rows of x, y and grad_y (at most 2^31 - 1024)               */
+    int64_t x_stride; /* elements from one row of x to the next, >= n_in             */
+    int64_t w_stride; /* of weight, >= n_in                                          */
+    int64_t g_stride; /* of grad_y, >= n_out; not read by the forward                */
+    int32_t n_in, n_out;
+    int32_t dtype;      /* CWRNNT_F16 or CWRNNT_BF16                                 */
+    int32_t activation; /* CWRNNT_ACT_*                                              */
+} cwrnnt_linear;
+CWRNNT_API int64_t cwrnnt_linear_workspace_bytes(const cwrnnt_linear *p, int32_t backward);
+CWRNNT_API int cwrnnt_linear_forward(const cwrnnt_linear *p, const void *x, const void *weight, const void *bias,
+                                     const void *residual, void *workspace, int64_t workspace_bytes, void *y,
+                                     cwrnnt_stream_t stream);
+CWRNNT_API int cwrnnt_linear_backward(const cwrnnt_linear *p, const void *x, const void *weight, const void *bias,
+                                      const void *grad_y, void *workspace, int64_t workspace_bytes, void *grad_x,
+                                      void *grad_weight, void *grad_bias, cwrnnt_stream_t stream);
+
+/*
  * Costs (and the reduced loss) without any caller workspace and without any allocation: for hosts that cannot call
  * cudaMalloc - a plug-in in a serving process whose framework owns all device memory, a foreign-language binding with
  * no device allocator to size a workspace with, a scoring loop that cannot afford the synchronisation an allocation

@@ -89,3 +89,58 @@ def test_python_entry_points_refuse_what_they_cannot_take():
             distill_loss(x, kw.pop("teacher"), kw.pop("indices"), **kw)
     with pytest.raises(RuntimeError, match="CUDA"):
         distill_loss(x, v, t)
+
+
+def _linear(**kw):
+    d = dict(n_rows=64, x_stride=32, w_stride=32, g_stride=48, n_in=32, n_out=48, dtype=capi.BF16, activation=0)
+    d.update(kw)
+    return ctypes.byref(capi.Linear(**d))
+
+
+LINEAR_BAD = [dict(n_rows=-1), dict(n_rows=2 ** 31), dict(n_in=0), dict(n_out=0), dict(n_in=2 ** 25), dict(x_stride=31),
+              dict(w_stride=31), dict(x_stride=2 ** 39), dict(dtype=capi.F32), dict(dtype=capi.F64), dict(dtype=9),
+              dict(activation=-1), dict(activation=4)]
+
+
+@pytest.mark.parametrize("bad", LINEAR_BAD)
+def test_bad_linear_layers_are_refused(bad):
+    L = capi.lib()
+    one = ctypes.c_void_p(256)
+    assert L.cwrnnt_linear_workspace_bytes(_linear(**bad), 0) < 0
+    assert L.cwrnnt_linear_forward(_linear(**bad), one, one, one, one, one, 1 << 40, one, None) == 1
+    assert L.cwrnnt_linear_backward(_linear(**bad), one, one, one, one, one, 1 << 40, one, one, one, None) == 1
+
+
+def test_linear_pointers_and_workspaces():
+    L = capi.lib()
+    one, odd = ctypes.c_void_p(256), ctypes.c_void_p(264)
+    n, m = L.cwrnnt_linear_workspace_bytes(_linear(), 0), L.cwrnnt_linear_workspace_bytes(_linear(), 1)
+    assert n >= 256 and m >= 256
+    assert L.cwrnnt_linear_workspace_bytes(_linear(x_stride=33), 0) >= 64 * 32 * 2  # a copy of x
+    f, b = L.cwrnnt_linear_forward, L.cwrnnt_linear_backward
+    assert f(None, one, one, None, None, one, n, one, None) == 1
+    assert f(_linear(), None, one, None, None, one, n, one, None) == 1
+    assert f(_linear(), one, None, None, None, one, n, one, None) == 1
+    assert f(_linear(), one, one, None, None, one, n, None, None) == 1
+    assert f(_linear(), odd, one, None, None, one, n, one, None) == 1      # off a 16-byte boundary
+    assert f(_linear(), one, odd, None, None, one, n, one, None) == 1
+    assert f(_linear(), one, one, None, None, None, n, one, None) == 2
+    assert f(_linear(), one, one, None, None, odd, n, one, None) == 2
+    assert f(_linear(), one, one, None, None, one, n - 1, one, None) == 2
+    assert b(_linear(g_stride=47), one, one, None, one, one, m, one, one, one, None) == 1
+    assert b(_linear(), one, one, None, None, one, m, one, one, one, None) == 1
+    assert b(_linear(), one, one, None, odd, one, m, one, one, one, None) == 1
+    assert b(_linear(), one, one, None, one, one, m - 1, one, one, one, None) == 2
+    assert f(_linear(n_rows=0), None, None, None, None, None, 0, None, None) == 0
+    assert b(_linear(n_rows=0), None, None, None, None, None, 0, None, None, None, None) == 0
+
+
+def test_fused_linear_refuses_what_it_cannot_take():
+    from compactwarprnntloss_b200 import fused_linear
+    x, w = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(6, 8, dtype=torch.bfloat16)
+    for args, kw in (((x.float(), w.float()), {}), ((x.double(), w.double()), {}), ((x, w[:, :7]), {}),
+                     ((x, w, torch.zeros(5)), {}), ((x, w, None, torch.zeros(4, 5)), {}), ((x, w), dict(activation="gelu"))):
+        with pytest.raises(AssertionError):
+            fused_linear(*args, **kw)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fused_linear(x, w)
