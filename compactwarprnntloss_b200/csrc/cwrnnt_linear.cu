@@ -8,8 +8,8 @@
 // One kernel for the four products: tiles of 128 x BN outputs, 64 elements of the sum a step. Operands come by tiled TMA
 // into a ring of 128-byte-swizzled stages; tcgen05.mma sums in TMEM in float. The forward product takes both operands
 // along the sum (K-major), dx takes W and dW takes both operands across it (MN-major): no operand is ever transposed in
-// memory. Warp 0 issues the loads, warp 1 the products, warps 2-5 carry the previous tile out of the second half of
-// TMEM meanwhile. CTAs are persistent; output columns run fastest, so that concurrent CTAs share their rows of x in L2.
+// memory. Warp 0 issues the loads, warp 1 the products; four or eight more warps carry the previous tile out of the other half
+// of TMEM meanwhile, through swizzled shared memory and TMA stores (residual and dy come the same way). CTAs are persistent; output columns run fastest, so that concurrent CTAs share their rows of x in L2.
 // Products with few tiles and long sums (dW) are split along the sum; the parts are float in the workspace, added in
 // a fixed order by a second kernel that carries the same epilogue.
 // TMA wants rows at multiples of 16 bytes: matrices of other strides are copied to such a stride first.
@@ -21,7 +21,6 @@ namespace cwrnnt {
 namespace {
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kLinearThreads = 192;
 constexpr int kMaxStages = 8;
 
 enum { kStore = 0, kSlope = 1, kPart = 2 };
@@ -71,23 +70,49 @@ struct Epilogue {
     int act;
     const void *bias;   // [N] or null
     const void *side;   // kStore: residual [M, side_ld] or null; kSlope: dy [M, side_ld]
-    void *out;          // [M, out_ld]
-    float *part;        // kPart: [splits, M, N]
+    void *out;          // [M, out_ld]; kPart: float [splits * rows of tiles, out_ld]
     int64_t side_ld, out_ld;
-    bool vec;           // rows of out and side allow 16-byte accesses; the columns come in whole groups of 8
+    bool tma_out, tma_side;  // rows of out / side lie on 16-byte boundaries: they go by TMA
+    bool vec;                // all 16-byte accesses allowed, columns in whole groups of 8
 };
 
-// Columns [col, col + 8) of one row, `n` of them inside the matrix.
+// Eight consecutive elements of the product become eight of the output: bias, then the activation (plus the residual) or
+// the upstream gradient times the activation's slope.
 template <typename T>
-__device__ __forceinline__ void finish8(const Epilogue &ep, float (&v)[8], int64_t row, int col, int n)
+__device__ __forceinline__ void finish(const Epilogue &ep, float (&v)[8], const float (&side)[8])
+{
+    if (ep.mode == kSlope) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = side[c] * slope(ep.act, v[c]);
+        return;
+    }
+    if (ep.act == CWRNNT_ACT_RELU) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = activate(CWRNNT_ACT_RELU, v[c]);
+    } else if (ep.act == CWRNNT_ACT_TANH) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = activate(CWRNNT_ACT_TANH, v[c]);
+    } else if (ep.act == CWRNNT_ACT_SILU) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = activate(CWRNNT_ACT_SILU, v[c]);
+    }
+    if (ep.side) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] += side[c];
+    }
+}
+
+// Columns [col, col + 8) of one row straight from and to global memory, `n` of them inside the matrix.
+template <typename T>
+__device__ __forceinline__ void finish_in_place(const Epilogue &ep, float (&v)[8], int64_t row, int col, int n)
 {
     using E = Elt<T>;
+    float s[8] = {};
     if (ep.bias) {
 #pragma unroll
         for (int c = 0; c < 8; ++c)
             if (c < n) v[c] += E::to_acc(__ldg(static_cast<const T *>(ep.bias) + col + c));
     }
-    float s[8];
     if (ep.side) {
         const T *side = static_cast<const T *>(ep.side) + row * ep.side_ld + col;
         if (ep.vec) {
@@ -97,19 +122,7 @@ __device__ __forceinline__ void finish8(const Epilogue &ep, float (&v)[8], int64
             for (int c = 0; c < 8; ++c) s[c] = c < n ? E::to_acc(__ldg(side + c)) : 0.0f;
         }
     }
-    if (ep.mode == kSlope) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = s[c] * slope(ep.act, v[c]);
-    } else {
-        if (ep.act != CWRNNT_ACT_NONE) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) v[c] = activate(ep.act, v[c]);
-        }
-        if (ep.side) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) v[c] += s[c];
-        }
-    }
+    finish<T>(ep, v, s);
     T *out = static_cast<T *>(ep.out) + row * ep.out_ld + col;
     if (ep.vec) {
         *reinterpret_cast<uint4 *>(out) = E::pack(v);
@@ -124,10 +137,11 @@ __device__ __forceinline__ void finish8(const Epilogue &ep, float (&v)[8], int64
 struct Shape {
     int64_t M;
     int N;
-    int steps;             // steps of kBK along the sum, in all
+    int steps;  // steps of kBK along the sum, in all
     int steps_per_split, splits;
     int64_t tiles_m;
     int tiles_n;
+    int stages;
     __device__ __forceinline__ int64_t tiles() const { return tiles_m * tiles_n * splits; }
     // columns fastest, then rows, then parts of the sum
     __device__ __forceinline__ void tile(int64_t t, int64_t &m, int &n, int &split) const
@@ -145,36 +159,164 @@ struct Shape {
     }
 };
 
+// A warp of the epilogue carries 32 rows by pieces of 128 bytes (64 columns of 16 bits, 32 of a part's floats) through a
+// buffer of its own, in the swizzle of the TMA copies: 16-byte group j of row r lies at group j ^ (r & 7), so that neither
+// a thread's row nor a row of the warp meets bank conflicts.
+constexpr int kPiece = 32 * 128;
 template <int BN>
 struct Layout {
     static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
-    static constexpr int kStages = 196608 / kStage < kMaxStages ? 196608 / kStage : kMaxStages;
-    static constexpr int kBytes = kStages * kStage + 1024;  // stages start on a 1024-byte boundary
-    static constexpr uint32_t kColumns = 2 * BN;            // two sums in TMEM
+    static constexpr int kCarriers = BN >= 128 ? 8 : 4;  // warps of the epilogue
+    static constexpr int kThreads = 64 + 32 * kCarriers;
+    static constexpr uint32_t kColumns = 2 * BN;         // two sums in TMEM
+    static constexpr int kRoom = 227 * 1024 - 4096 - 1024;  // shared memory but for the static part and the alignment
+    static constexpr int stages(bool side)
+    {
+        const int n = (kRoom - kCarriers * kPiece * (side ? 2 : 1)) / kStage;
+        return n < kMaxStages ? n : kMaxStages;
+    }
+    static constexpr int bytes(bool side) { return 1024 + stages(side) * kStage + kCarriers * kPiece * (side ? 2 : 1); }
+};
+
+__device__ __forceinline__ uint4 *piece_group(unsigned char *piece, int row, int group)
+{
+    return reinterpret_cast<uint4 *>(piece + row * 128 + ((group ^ (row & 7)) << 4));
+}
+
+// One warp's share of one tile. `d`: TMEM address of the sum's first column in this warp's lanes.
+template <typename T, int BN>
+struct Carrier {
+    using E = Elt<T>;
+    const Epilogue &ep;
+    const Shape &sh;
+    const CUtensorMap *map_out, *map_side;
+    unsigned char *out_piece, *side_piece;
+    float *bias;  // 64 floats
+    uint64_t *side_bar;
+    volatile int *gave_up;
+    uint32_t side_phase;
+    int lane;
+
+    __device__ __forceinline__ void ask_side(int64_t row0, int col)
+    {
+        if (lane == 0) {
+            tc::mbar_expect(side_bar, kPiece);
+            tc::load_2d(side_piece, map_side, side_bar, col, int(row0));
+        }
+    }
+    // 64 columns from `col` on (32 of a part)
+    __device__ __forceinline__ void piece(uint32_t d, int64_t row0, int64_t out_row0, int col, int n0, bool ok,
+                                          int next_col, int64_t next_row0)
+    {
+        const bool part = ep.mode == kPart;
+        if (!part && ep.bias) {
+            const T *b = static_cast<const T *>(ep.bias);
+            bias[lane] = col + lane < sh.N ? E::to_acc(__ldg(b + col + lane)) : 0.0f;
+            bias[32 + lane] = col + 32 + lane < sh.N ? E::to_acc(__ldg(b + col + 32 + lane)) : 0.0f;
+        }
+        uint4 side[8];
+        if (ep.side) {
+            if (ep.tma_side) {
+                ok = tc::mbar_wait(side_bar, side_phase, gave_up) && ok;
+                side_phase ^= 1;
+            } else {
+                // rows off the boundaries: each row of the piece as 64 consecutive elements
+                T *s = reinterpret_cast<T *>(side_piece);
+                for (int r = 0; r < 32; ++r)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int c = h * 32 + lane;
+                        T v = E::from_acc(0.0f);
+                        if (row0 + r < sh.M && col + c < sh.N)
+                            v = __ldg(static_cast<const T *>(ep.side) + (row0 + r) * ep.side_ld + col + c);
+                        s[r * 64 + (((c >> 3) ^ (r & 7)) << 3) + (c & 7)] = v;
+                    }
+                __syncwarp();
+            }
+#pragma unroll
+            for (int g = 0; g < 8; ++g) side[g] = *piece_group(side_piece, lane, g);
+            __syncwarp();
+            if (ep.tma_side && next_col >= 0) ask_side(next_row0, next_col);
+        }
+        if (lane == 0) tc::stores_read();
+        __syncwarp();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (part && half) break;
+            uint32_t r[32];
+            tc::tmem_load32(d + uint32_t(col - n0 + half * 32), r);
+            tc::tmem_load_wait();
+            if (part) {
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    uint4 w = make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
+                    if (!ok) w = make_uint4(0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u);
+                    *piece_group(out_piece, lane, g) = w;
+                }
+                continue;
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float v[8], s[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = ok ? __uint_as_float(r[g * 8 + i]) : NAN;
+                if (ep.bias) {
+                    const float4 b0 = *reinterpret_cast<const float4 *>(bias + half * 32 + g * 8);
+                    const float4 b1 = *reinterpret_cast<const float4 *>(bias + half * 32 + g * 8 + 4);
+                    v[0] += b0.x, v[1] += b0.y, v[2] += b0.z, v[3] += b0.w;
+                    v[4] += b1.x, v[5] += b1.y, v[6] += b1.z, v[7] += b1.w;
+                }
+                if (ep.side) E::unpack(side[half * 4 + g], s);
+                finish<T>(ep, v, s);
+                *piece_group(out_piece, lane, half * 4 + g) = E::pack(v);
+            }
+        }
+        if (ep.tma_out) {
+            tc::fence_async();
+            __syncwarp();
+            if (lane == 0) tc::store_2d(map_out, out_piece, col, int(out_row0));
+        } else {
+            __syncwarp();
+            const T *o = reinterpret_cast<const T *>(out_piece);
+            for (int k = 0; k < 32; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c = h * 32 + lane;
+                    if (row0 + k < sh.M && col + c < sh.N)
+                        static_cast<T *>(ep.out)[(row0 + k) * ep.out_ld + col + c] =
+                            o[k * 64 + (((c >> 3) ^ (k & 7)) << 3) + (c & 7)];
+                }
+            __syncwarp();
+        }
+    }
 };
 
 template <typename T, int BN, bool A_MN, bool B_MN>
-__global__ void __launch_bounds__(kLinearThreads, 1)
-linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Shape sh,
+__global__ void __launch_bounds__(Layout<BN>::kThreads, 1)
+linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+              const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_side, const Shape sh,
               const Epilogue ep)
 {
     using L = Layout<BN>;
     extern __shared__ unsigned char raw[];
-    __shared__ uint64_t full[L::kStages], empty[L::kStages], sum_full[2], sum_empty[2], drained;
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], sum_full[2], sum_empty[2], drained;
+    __shared__ uint64_t side_full[L::kCarriers];
+    __shared__ __align__(16) float bias[L::kCarriers][64];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     unsigned char *stages = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (warp == 0 && lane == 0) {
-        for (int i = 0; i < L::kStages; ++i) {
+        for (int i = 0; i < sh.stages; ++i) {
             tc::mbar_init(&full[i], 1);
             tc::mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&sum_full[i], 1);
-            tc::mbar_init(&sum_empty[i], 4);
+            tc::mbar_init(&sum_empty[i], L::kCarriers);
         }
+        for (int i = 0; i < L::kCarriers; ++i) tc::mbar_init(&side_full[i], 1);
         tc::mbar_init(&drained, 1);
         gave_up = 0;
         tc::mbar_init_fence();
@@ -219,11 +361,11 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         tc::load_2d(b, &map_b, &full[at], k * kBK, n * BN);
                     }
                     started |= 1u << at;
-                    if (++at == L::kStages) at = 0, phase ^= 1;
+                    if (++at == sh.stages) at = 0, phase ^= 1;
                 }
             }
             // every load has landed before the CTA's memory goes: the last fill of each stage
-            for (int i = 0; i < L::kStages; ++i) {
+            for (int i = 0; i < sh.stages; ++i) {
                 if (!(started >> i & 1)) continue;
                 const uint32_t last = i < at ? phase : phase ^ 1;
                 const uint64_t since = tc::now_ns();
@@ -233,8 +375,6 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr uint32_t idesc =
-                tc::instruction(Elt<T>::kBf16 ? 1 : 0, A_MN, B_MN, kBM, BN);
             int at = 0, half = 0;
             uint32_t phase = 0, half_phase = 0;
             bool ok = true;
@@ -242,6 +382,10 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 int64_t m;
                 int n, split;
                 sh.tile(t, m, n, split);
+                // the last tile of a row is as wide as the matrix needs it
+                const int left = (sh.N - n * BN + 15) / 16 * 16;
+                const uint32_t idesc =
+                    tc::instruction(Elt<T>::kBf16 ? 1 : 0, A_MN, B_MN, kBM, left < BN ? left : BN);
                 ok = tc::mbar_wait(&sum_empty[half], half_phase ^ 1, &gave_up);
                 if (!ok) break;
                 tc::fence_after();
@@ -260,7 +404,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         tc::mma_f16(d, da, db, idesc, k > 0 || i > 0);
                     }
                     tc::commit(&empty[at]);
-                    if (++at == L::kStages) at = 0, phase ^= 1;
+                    if (++at == sh.stages) at = 0, phase ^= 1;
                 }
                 if (ok) tc::commit(&sum_full[half]);
                 if (++half == 2) half = 0, half_phase ^= 1;
@@ -273,43 +417,52 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         }
     } else {
         const int quarter = warp & 3;  // the TMEM lanes that this warp may read
+        const int carrier = warp - 2, share = carrier / 4;
+        constexpr int kShares = L::kCarriers / 4;
         int half = 0;
         uint32_t half_phase = 0;
+        unsigned char *pieces = stages + sh.stages * L::kStage;
+        Carrier<T, BN> c{ep, sh, &map_out, &map_side, pieces + carrier * kPiece,
+                         pieces + (L::kCarriers + carrier) * kPiece, bias[carrier], &side_full[carrier], &gave_up, 0,
+                         lane};
+        const int step = ep.mode == kPart ? 32 : 64;
+        const bool ask = BN >= 64 && ep.side && ep.tma_side;
+        bool asked = false;
         for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
             int64_t m;
             int n, split;
             sh.tile(t, m, n, split);
+            const int64_t row0 = m * kBM + quarter * 32;
+            const int n0 = n * BN;
+            const int end = n0 + BN < sh.N ? n0 + BN : sh.N;
+            int col = n0 + share * step;
+            if (ask && !asked && col < end && row0 < sh.M) c.ask_side(row0, col);
+            asked = false;
             const bool ok = tc::mbar_wait(&sum_full[half], half_phase, &gave_up);
             tc::fence_after();
-            const int64_t row = m * kBM + quarter * 32 + lane;
-#pragma unroll 1
-            for (int c = 0; c < BN; c += 32) {
+            __syncwarp();
+            const uint32_t d = tmem + uint32_t(half * BN) + (uint32_t(quarter * 32) << 16);
+            if constexpr (BN >= 64) {
+                if (row0 < sh.M) {
+                    for (; col < end; col += kShares * step) {
+                        const int next = col + kShares * step;
+                        c.piece(d, row0, split * sh.tiles_m * kBM + row0, col, n0, ok, next < end ? next : -1, row0);
+                    }
+                }
+            } else {
+                const int64_t row = row0 + lane;
                 uint32_t r[32];
-                const int col = n * BN + c;
-                if (col >= sh.N) break;
-                __syncwarp();
-                tc::tmem_load32(tmem + uint32_t(half * BN + c) + (uint32_t(quarter * 32) << 16), r);
+                tc::tmem_load32(d, r);
                 tc::tmem_load_wait();
-                // a wait that ran out leaves NaN
+                if (row < sh.M) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int left = sh.N - (col + g * 8);
-                    if (left <= 0 || row >= sh.M) break;
-                    float v[8];
+                    for (int g = 0; g < 4; ++g) {
+                        const int left = sh.N - (n0 + g * 8);
+                        if (left <= 0) break;
+                        float v[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = ok ? __uint_as_float(r[g * 8 + i]) : NAN;
-                    if (ep.mode == kPart) {
-                        float *out = ep.part + (int64_t(split) * sh.M + row) * sh.N + col + g * 8;
-                        if (ep.vec) {
-                            *reinterpret_cast<float4 *>(out) = make_float4(v[0], v[1], v[2], v[3]);
-                            *reinterpret_cast<float4 *>(out + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (i < left) out[i] = v[i];
-                        }
-                    } else {
-                        finish8<T>(ep, v, row, col + g * 8, left < 8 ? left : 8);
+                        for (int i = 0; i < 8; ++i) v[i] = ok ? __uint_as_float(r[g * 8 + i]) : NAN;
+                        finish_in_place<T>(ep, v, row, n0 + g * 8, left < 8 ? left : 8);
                     }
                 }
             }
@@ -318,6 +471,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             if (lane == 0) tc::mbar_arrive(&sum_empty[half]);
             if (++half == 2) half = 0, half_phase ^= 1;
         }
+        if (lane == 0) tc::stores_done();
     }
     __syncwarp();
     tc::fence_before();
@@ -330,20 +484,21 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 
 // The parts of a split sum, added in their order, and the epilogue.
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const float *__restrict__ part, int splits, int64_t M, int N, const Epilogue ep)
+__global__ void __launch_bounds__(256)
+join_kernel(const float *__restrict__ part, int splits, int64_t part_rows, int64_t M, int N, const Epilogue ep)
 {
-    const int groups = (N + 7) / 8;
+    const int groups = (N + 7) / 8, ld = groups * 8;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < M * groups; i += int64_t(gridDim.x) * 256) {
         const int64_t row = i / groups;
         const int col = int(i % groups) * 8, n = N - col < 8 ? N - col : 8;
         float v[8] = {};
         for (int s = 0; s < splits; ++s) {
-            const float *p = part + (int64_t(s) * M + row) * N + col;
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if (c < n) v[c] += __ldg(p + c);
+            const float4 *p = reinterpret_cast<const float4 *>(part + (s * part_rows + row) * ld + col);
+            const float4 a = __ldg(p), b = __ldg(p + 1);
+            v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+            v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
         }
-        finish8<T>(ep, v, row, col, n);
+        finish_in_place<T>(ep, v, row, col, n);
     }
 }
 
@@ -394,14 +549,24 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ 
         part[int64_t(blockIdx.y) * cols + mine] = s;
     }
 }
+// 32 columns a CTA, eight threads each, whose sums are added in order.
 template <typename T>
-__global__ void __launch_bounds__(256) column_join_kernel(const float *__restrict__ part, int runs, int cols, T *__restrict__ out)
+__global__ void __launch_bounds__(256)
+column_join_kernel(const float *__restrict__ part, int runs, int cols, T *__restrict__ out)
 {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+    __shared__ float sums[8][33];
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32, c = blockIdx.x * 32 + tx;
     float s = 0.0f;
-    for (int i = 0; i < runs; ++i) s += __ldg(part + int64_t(i) * cols + c);
-    out[c] = Elt<T>::from_acc(s);
+    if (c < cols) {
+#pragma unroll 4
+        for (int i = ty; i < runs; i += 8) s += __ldg(part + int64_t(i) * cols + c);
+    }
+    sums[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < cols) {
+        for (int y = 1; y < 8; ++y) s += sums[y][tx];
+        out[c] = Elt<T>::from_acc(s);
+    }
 }
 
 // --------------------------------------------------------------------------------------------------------- host side
@@ -423,16 +588,18 @@ EncodeFn encoder()
     return fn;
 }
 
-// A [rows, cols] matrix in memory, 16-byte rows, read in boxes of 64 columns x `box_rows` rows.
+// A [rows, cols] matrix in memory, 16-byte rows, copied in boxes of 128 bytes x `box_rows` rows.
 template <typename T>
 bool make_map(CUtensorMap *map, const void *p, int64_t rows, int64_t cols, int64_t ld, int box_rows)
 {
     const EncodeFn encode = encoder();
     if (!encode) return false;
-    const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, strides[1] = {cuuint64_t(ld) * 2};
-    const cuuint32_t box[2] = {64, cuuint32_t(box_rows)}, one[2] = {1, 1};
-    return encode(map, Elt<T>::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                  const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, strides[1] = {cuuint64_t(ld) * sizeof(T)};
+    const cuuint32_t box[2] = {128 / sizeof(T), cuuint32_t(box_rows)}, one[2] = {1, 1};
+    CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    if constexpr (sizeof(T) == 2)
+        type = Elt<T>::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return encode(map, type, 2, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -463,7 +630,12 @@ Cut cut_product(int64_t M, int N, int64_t len, bool b_mn)
     }
     return c;
 }
-int64_t part_bytes(int64_t M, int N, const Cut &c) { return c.splits > 1 ? align_up(4 * c.splits * M * N, 256) : 0; }
+// Parts are [splits * rows of whole tiles, N up to a multiple of 8] floats.
+int64_t part_rows(int64_t M) { return align_up(M, kBM); }
+int64_t part_bytes(int64_t M, int N, const Cut &c)
+{
+    return c.splits > 1 ? 4 * c.splits * part_rows(M) * align_up(N, 8) : 0;
+}
 
 struct Matrix {  // [rows, cols], `mn`: its columns are the output's and its rows the sum's
     const void *p;
@@ -472,19 +644,26 @@ struct Matrix {  // [rows, cols], `mn`: its columns are the output's and its row
 };
 
 template <typename T, int BN, bool A_MN, bool B_MN>
-cudaError_t run_product(const Matrix &a, const Matrix &b, const Shape &sh, const Epilogue &ep, cudaStream_t s)
+cudaError_t run_product(const Matrix &a, const Matrix &b, Shape sh, const Epilogue &ep, cudaStream_t s)
 {
     using L = Layout<BN>;
-    CUtensorMap ma, mb;
-    if (!make_map<T>(&ma, a.p, a.rows, a.cols, a.ld, A_MN ? kBK : kBM) ||
-        !make_map<T>(&mb, b.p, b.rows, b.cols, b.ld, B_MN ? kBK : BN))
-        return cudaErrorInvalidValue;
+    CUtensorMap ma, mb, mo{}, ms{};
+    bool good = make_map<T>(&ma, a.p, a.rows, a.cols, a.ld, A_MN ? kBK : kBM) &&
+                make_map<T>(&mb, b.p, b.rows, b.cols, b.ld, B_MN ? kBK : BN);
+    if (ep.mode == kPart)
+        good = good && make_map<float>(&mo, ep.out, sh.splits * part_rows(sh.M), sh.N, ep.out_ld, 32);
+    else if (ep.tma_out)
+        good = good && make_map<T>(&mo, ep.out, sh.M, sh.N, ep.out_ld, 32);
+    if (ep.side && ep.tma_side) good = good && make_map<T>(&ms, ep.side, sh.M, sh.N, ep.side_ld, 32);
+    if (!good) return cudaErrorInvalidValue;
+    const bool side = ep.side != nullptr;
+    sh.stages = L::stages(side);
     auto kernel = linear_kernel<T, BN, A_MN, B_MN>;
     // the attribute belongs to the device that is current
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes(false) > L::bytes(true) ? L::bytes(false) : L::bytes(true));
     if (e != cudaSuccess) return e;
     const int64_t total = sh.tiles_m * sh.tiles_n * sh.splits;
-    kernel<<<unsigned(total < kNumSMs ? total : kNumSMs), kLinearThreads, L::kBytes, s>>>(ma, mb, sh, ep);
+    kernel<<<unsigned(total < kNumSMs ? total : kNumSMs), L::kThreads, L::bytes(side), s>>>(ma, mb, mo, ms, sh, ep);
     return cudaGetLastError();
 }
 
@@ -511,12 +690,15 @@ cudaError_t product(const Matrix &a, const Matrix &b, int64_t M, int N, int64_t 
     sh.steps = int((len + kBK - 1) / kBK);
     sh.steps_per_split = c.steps_per_split, sh.splits = c.splits;
     sh.tiles_m = (M + kBM - 1) / kBM, sh.tiles_n = (N + c.bn - 1) / c.bn;
-    auto on16 = [](const void *p, int64_t ld) { return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0); };
-    ep.vec = N % 8 == 0 && on16(ep.out, ep.out_ld) && on16(ep.side, ep.side_ld);
+    auto on16 = [](const void *p, int64_t ld) {
+        return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0);
+    };
+    ep.tma_out = on16(ep.out, ep.out_ld), ep.tma_side = on16(ep.side, ep.side_ld);
+    ep.vec = N % 8 == 0 && ep.tma_out && ep.tma_side;
     Epilogue here = ep;
     if (c.splits > 1) {
         here = Epilogue{};
-        here.mode = kPart, here.part = part, here.vec = N % 4 == 0 && N % 8 == 0;
+        here.mode = kPart, here.out = part, here.out_ld = align_up(N, 8), here.tma_out = true;
     }
     cudaError_t e;
     if (a.mn)
@@ -527,7 +709,7 @@ cudaError_t product(const Matrix &a, const Matrix &b, int64_t M, int N, int64_t 
         e = run_product_bn<T, false, false>(c.bn, a, b, sh, here, s);
     if (e != cudaSuccess || c.splits == 1) return e;
     const int64_t items = M * ((N + 7) / 8), blocks = (items + 255) / 256;
-    join_kernel<T><<<unsigned(blocks < kNumSMs * 16 ? blocks : kNumSMs * 16), 256, 0, s>>>(part, c.splits, M, N, ep);
+    join_kernel<T><<<unsigned(blocks < kNumSMs * 16 ? blocks : kNumSMs * 16), 256, 0, s>>>(part, c.splits, part_rows(M), M, N, ep);
     return cudaGetLastError();
 }
 
@@ -646,7 +828,7 @@ cudaError_t linear_backward(const cwrnnt_linear &p, const void *x, const void *w
         column_sums_kernel<T><<<dim3(unsigned(across), unsigned(runs)), 256, 0, s>>>(
             static_cast<const T *>(dz.p), dz.ld, p.n_rows, p.n_out, run, sums);
         CWRNNT_TRY(cudaGetLastError());
-        column_join_kernel<T><<<unsigned(across), 256, 0, s>>>(sums, int(runs), p.n_out, static_cast<T *>(grad_b));
+        column_join_kernel<T><<<unsigned((p.n_out + 31) / 32), 256, 0, s>>>(sums, int(runs), p.n_out, static_cast<T *>(grad_b));
         CWRNNT_TRY(cudaGetLastError());
     }
     if (grad_x) {
