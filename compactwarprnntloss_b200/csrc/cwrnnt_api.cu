@@ -619,7 +619,7 @@ int cwrnnt_read_status(const void *workspace, int32_t out[4], cwrnnt_stream_t st
 }
 
 int cwrnnt_token_scores(const cwrnnt_rows *p, const void *x, const int32_t *targets, void *log_probs, void *entropy,
-                        void *top_log_probs, int32_t *top_indices, double *stats, cwrnnt_stream_t stream)
+                        void *top_log_probs, int32_t *top_indices, void *stats, cwrnnt_stream_t stream)
 {
     int st = check_rows(p);
     if (st) return st;
@@ -632,7 +632,7 @@ int cwrnnt_token_scores(const cwrnnt_rows *p, const void *x, const int32_t *targ
 }
 
 int cwrnnt_token_scores_backward(const cwrnnt_rows *p, const void *x, const int32_t *targets,
-                                 const int32_t *top_indices, const double *stats, const void *entropy,
+                                 const int32_t *top_indices, const void *stats, const void *entropy,
                                  const void *g_log_probs, const void *g_entropy, const void *g_top, void *grad_x,
                                  cwrnnt_stream_t stream)
 {

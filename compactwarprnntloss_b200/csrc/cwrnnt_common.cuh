@@ -165,6 +165,8 @@ struct Elt<__half> {
     using acc = float;
     using cost = float;
     static constexpr bool kBf16 = false;
+    using pair = __half2;
+    static __device__ __forceinline__ pair both(float v) { return __float2half2_rn(v); }
     static constexpr int VE = 8;
     static __device__ __forceinline__ void unpack(const uint4 &v, float (&e)[8])
     {
@@ -204,6 +206,8 @@ struct Elt<__nv_bfloat16> {
     using acc = float;
     using cost = float;
     static constexpr bool kBf16 = true;
+    using pair = __nv_bfloat162;
+    static __device__ __forceinline__ pair both(float v) { return __float2bfloat162_rn(v); }
     static constexpr int VE = 8;
     static __device__ __forceinline__ void unpack(const uint4 &v, float (&e)[8])
     {

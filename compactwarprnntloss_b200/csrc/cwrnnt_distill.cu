@@ -29,10 +29,10 @@ struct DistillArgs {
     const T *x;
     T *gx;  // null: loss only
     int64_t n_rows, x_stride, g_stride;
-    int V, K;
-    A kappa;         // log2(e) / tau
-    double inv_tau;  // 1 / tau
-    double scale;    // of the summed loss and of the gradient
+    int V, K, KP;  // KP: K up to a power of two
+    A kappa;       // log2(e) / tau
+    A inv_tau;     // 1 / tau
+    double scale;  // of the summed loss and of the gradient
     const C *teacher, *weight, *upstream;
     int upstream_stride;
     const int32_t *index;
@@ -40,55 +40,94 @@ struct DistillArgs {
     double *partial;  // one sum per CTA
 };
 
+// e^a to 2^-33 relative, for a <= 0 and a little above, in a dozen double operations: 2^n times the series of e^r,
+// |r| <= ln2 / 2 (its first omitted term: 0.347^9 / 9! = 2e-10). What the teacher leaves for the rest is one minus a sum
+// of these, and a float's digits would not do for that.
+__device__ __forceinline__ double exp_mid(double a)
+{
+    if (!(a > -700.0)) return a != a ? a : 0.0;
+    if (a > 700.0) return INFINITY;
+    const double n = rint(a * kLog2e), r = fma(n, -kLn2, a);
+    double p = 1.0 / 40320.0;
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return p * __hiloint2double((int(n) + 1023) << 20, 0);
+}
+__device__ __forceinline__ double teacher_exp(double a, float) { return exp_mid(a); }
+__device__ __forceinline__ double teacher_exp(double a, double) { return exp(a); }
+
+// Sums and maxima over the lanes of a row that hold its entries: lanes 0 .. KP-1 (a power of two, the others hold the
+// neutral element), the result in every lane of the row. All lanes of a warp call these together.
+template <int LPR, typename V>
+__device__ __forceinline__ V entry_sum(V v, int KP)
+{
+    for (int o = KP >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return __shfl_sync(0xffffffffu, v, 0, LPR);
+}
+template <int LPR, typename V>
+__device__ __forceinline__ V entry_max(V v, int KP)
+{
+    for (int o = KP >> 1; o > 0; o >>= 1) v = Base2<V>::max_of(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return __shfl_sync(0xffffffffu, v, 0, LPR);
+}
+
 // One row's teacher entry, held by lane e of the row's lanes, and what follows from all of them.
+template <typename A>
 struct Entries {
-    int c;           // token, -1: none
-    bool first;      // no earlier entry names the same token
-    double q, lq;    // teacher's probability and its logarithm
-    double sum_q;    // over the row
-    bool bad;        // some token of the row lies outside it
+    int c;       // token, -1: none
+    bool first;  // no earlier entry names the same token
+    bool bad;    // some token of the row lies outside it
+    A q, lq;     // teacher's probability and its logarithm
+    A sum_q;     // over the row
+    A left;      // one minus that, at least 0
+    A dup_q;     // q of all entries with this token, added up in their order
 };
 
-// All lanes of a warp call this together; LPR lanes belong to a row, lane `gl` of them holds entry gl.
-template <int LPR, bool TAIL, typename C>
-__device__ __forceinline__ Entries load_entries(const C *teacher, const int32_t *index, int V, int K, double inv_tau,
-                                                int64_t r, int gl, bool active)
+// All lanes of a warp call this together; LPR lanes belong to a row, lane `gl` of them holds entry gl: token `c`, value
+// `a` (-1, -inf: none).
+template <int LPR, bool TAIL, typename A>
+__device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, int KP, A inv_tau, int gl)
 {
     constexpr unsigned kAll = 0xffffffffu;
-    Entries en;
-    en.c = -1;
-    double a = -INFINITY;
-    if (active && gl < K) {
-        en.c = __ldg(index + r * K + gl);
-        a = double(__ldg(teacher + r * K + gl));
-    }
-    const unsigned outside = __ballot_sync(kAll, en.c >= V);
+    using M = Base2<A>;
+    Entries<A> en;
+    const unsigned outside = __ballot_sync(kAll, c >= V);
     en.bad = ((outside >> ((threadIdx.x & 31) / LPR * LPR)) & (LPR == 32 ? kAll : (1u << (LPR & 31)) - 1u)) != 0;
-    if (en.c >= V || en.c < 0) en.c = -1;
-    en.first = en.c >= 0;
-    for (int o = 0; o < K; ++o) {
-        const int other = __shfl_sync(kAll, en.c, o, LPR);
-        if (o < gl && other == en.c) en.first = false;
-    }
-    if (en.c < 0) a = -INFINITY;
+    en.c = c < 0 || c >= V ? -1 : c;
+    if (en.c < 0) a = A(-INFINITY);
     if (TAIL) {
         en.lq = a;
-        en.q = exp(a);
+        const double q = teacher_exp(double(a), A(0));
+        const double sum = entry_sum<LPR>(q, KP);
+        en.q = A(q);
+        en.sum_q = A(sum);
+        en.left = A(fmax(0.0, 1.0 - sum));
     } else {
-        const double z = a * inv_tau;
-        double m = z;
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(kAll, m, o));
-        const double w = m == -INFINITY ? 0.0 : exp(z - m);
-        double s = w;
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
-        en.lq = s == 0.0 ? -INFINITY : z - m - log(s);
-        en.q = s == 0.0 ? 0.0 : w / s;
+        const A z = a * inv_tau;
+        const A m = entry_max<LPR>(z, KP);
+        const A w = m == A(-INFINITY) ? A(0) : M::exp2_of((z - m) * A(kLog2e));
+        const A s = entry_sum<LPR>(w, KP);
+        en.lq = s == A(0) ? A(-INFINITY) : z - m - M::ln_of(s);
+        en.q = s == A(0) ? A(0) : w / s;
+        en.sum_q = s == A(0) ? A(0) : s / s;
+        en.left = A(0);
     }
-    en.sum_q = en.q;
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) en.sum_q += __shfl_xor_sync(kAll, en.sum_q, o);
+    en.first = en.c >= 0;
+    en.dup_q = A(0);
+    for (int o = 0; o < K; ++o) {
+        const int other = __shfl_sync(kAll, en.c, o, LPR);
+        const A oq = __shfl_sync(kAll, en.q, o, LPR);
+        if (other == en.c) {
+            en.dup_q += oq;
+            if (o < gl) en.first = false;
+        }
+    }
     return en;
 }
 
@@ -96,107 +135,95 @@ __device__ __forceinline__ Entries load_entries(const C *teacher, const int32_t 
 template <typename T>
 __device__ __forceinline__ void blank_element(uint4 &v, int c)
 {
-    using E = Elt<T>;
-    typename E::acc e[E::VE];
-    E::unpack(v, e);
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t ninf = Elt<T>::kBf16 ? 0xff80ff80u : 0xfc00fc00u, mask = c & 1 ? 0xffff0000u : 0x0000ffffu;
 #pragma unroll
-    for (int k = 0; k < E::VE; ++k)
-        if (k == c) e[k] = typename E::acc(-INFINITY);
-    v = E::pack(e);
+        for (int k = 0; k < 4; ++k)
+            if (k == c >> 1) w[k] = (w[k] & ~mask) | (ninf & mask);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k == c) w[k] = 0xff800000u;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (k == c) w[2 * k] = 0u, w[2 * k + 1] = 0xfff00000u;
+    }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // What the row's statistics and entries give: its divergence, and its gradient's factors. The gradient is
-//     2^((x - top) * kappa - low) * factor                                    where no entry names the token
-//     2^((x - all_top) * kappa - all_low) * all_factor - q_factor * its q     where one does
+//     2^((x - top) * kappa) * factor                                   where no entry names the token
+//     2^((x - all_top) * kappa) * all_factor - q_factor * dup_q        where one does
 template <typename A>
 struct RowResult {
-    double loss;  // weighted
-    A top, low, factor;
-    A all_top, all_low, all_factor;
-    double q_factor;
+    A loss;  // weighted
+    A top, factor;
+    A all_top, all_factor;
+    A q_factor;
 };
 
-// `st`: statistics of the entries that are not listed (with a tail) or of the whole row (without). `xc`: the student's
-// logit at this lane's entry (-inf: none). All lanes of a warp call this together; LPR lanes belong to a row.
+// `st`: maximum and sum 2^((x - max) * kappa) of the entries that are not listed (with a tail) or of the whole row
+// (without). `xc`: the student's logit at this lane's entry (-inf: none). All lanes of a warp call this together; LPR lanes belong to a row.
 template <int LPR, bool TAIL, typename A>
-__device__ __forceinline__ RowResult<A> solve_row(const RowStats<A> &st, const Entries &en, A xc, A kappa,
-                                                  double inv_tau, double weight, double gain)
+__device__ __forceinline__ RowResult<A> solve_row(const RowStats<A> &st, const Entries<A> &en, A xc, A kappa, A inv_tau,
+                                                  A weight, A gain, int KP)
 {
-    constexpr unsigned kAll = 0xffffffffu;
     using M = Base2<A>;
-    RowStats<A> all = st;
+    const A rest_sum = st.s;
+    A all_max = st.max, all_sum = rest_sum;
     if (TAIL) {
-        RowStats<A> mine;  // a listed token counts once, however often it is named
-        mine.clear();
-        if (en.first && xc != A(-INFINITY)) {
-            const A shift = RowStats<A>::shift_of(xc, kappa);
-            mine.max = xc == xc ? xc : A(-INFINITY);  // (no maximum takes up a NaN; the sum does)
-            mine.s = RowStats<A>::extreme(shift) ? xc - xc + A(1) : M::exp2_of(M::fma_of(xc, kappa, -shift));
-        }
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) {
-            RowStats<A> other;
-            other.max = __shfl_xor_sync(kAll, mine.max, o);
-            other.s = __shfl_xor_sync(kAll, mine.s, o);
-            other.t = A(0);
-            mine.template join<false>(other, kappa);
-        }
-        all.template join<false>(mine, kappa);
+        // a listed token counts once, however often it is named (no maximum takes up a NaN; the sum does)
+        const A mine = en.first ? xc : A(-INFINITY);
+        all_max = M::max_of(st.max, entry_max<LPR>(mine, KP));
+        const A base = all_max == A(-INFINITY) ? A(0) : all_max;
+        const A listed = entry_sum<LPR>(M::exp2_of((mine - base) * kappa), KP);
+        all_sum = listed + (st.max == A(-INFINITY) ? rest_sum : rest_sum * M::exp2_of((st.max - base) * kappa));
     }
-    const bool nothing = all.nothing();  // the student's row has no finite entry: nothing to learn
-    const double log2_s = nothing ? 0.0 : all.log2_sum(kappa);
-    const double ln_s = kLn2 * log2_s, max = double(all.max);
-    double each = 0.0;
-    if (en.q > 0.0) each = en.q * (en.lq - log_prob_of(xc, max, inv_tau, ln_s));
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) each += __shfl_xor_sync(kAll, each, o);
-    double q_all = en.sum_q, q_rest = 0.0, p_rest = 1.0, rest2_s = log2_s;
+    const bool nothing = all_max == A(-INFINITY) && all_sum == all_sum;  // no finite entry: nothing to learn
+    const A ln_s = nothing ? A(0) : M::ln_of(all_sum);
+    A each = A(0);
+    if (en.q > A(0)) each = en.q * (en.lq - log_prob_of(xc, all_max, inv_tau, ln_s));
+    each = entry_sum<LPR>(each, KP);
+    A q_all = en.sum_q, q_rest = A(0), p_rest = A(1);
     if (TAIL && !st.nothing()) {
-        rest2_s = st.log2_sum(kappa);
-        const double ln_rest = (double(st.max) - max) * inv_tau + kLn2 * rest2_s - ln_s;
-        q_rest = fmax(0.0, 1.0 - en.sum_q);
-        q_all += q_rest;
-        p_rest = exp(ln_rest);
-        if (q_rest > 0.0) each += q_rest * (log(q_rest) - ln_rest);
+        const A ln_rest = (st.max - all_max) * inv_tau + (M::ln_of(rest_sum) - ln_s);
+        q_rest = en.left;
+        q_all = en.sum_q + q_rest;
+        p_rest = rest_sum * M::exp2_of((st.max - all_max) * kappa) / all_sum;
+        if (q_rest > A(0)) each += q_rest * (M::ln_of(q_rest) - ln_rest);
     }
-    double up = gain * weight * inv_tau;
-    if (nothing) each = up = 0.0;
-    if (en.bad) each = up = NAN;
-    if (ln_s != ln_s) each = NAN;  // (with no entry at all, a NaN logit would go unseen)
+    A up = gain * weight * inv_tau;
+    if (nothing) each = up = A(0);
+    if (en.bad) each = up = A(NAN);
+    if (ln_s != ln_s) each = A(NAN);  // (with no entry at all, a NaN logit would go unseen)
     RowResult<A> res;
-    res.loss = weight == 0.0 ? 0.0 : weight * each;
-    // the logarithms are rounded to the arithmetic type; the factors undo that
-    res.all_top = nothing ? A(0) : all.max;
-    res.all_low = A(log2_s);
-    res.all_factor = A(up * q_all * exp2(double(res.all_low) - log2_s));
+    res.loss = weight == A(0) ? A(0) : weight * each;
+    res.all_top = nothing ? A(0) : all_max;
+    res.all_factor = nothing && !en.bad ? A(0) : up * q_all / all_sum;
     res.q_factor = up;
     if (TAIL) {
-        res.top = st.nothing() ? A(0) : st.max;
-        res.low = A(rest2_s);
-        res.factor = A(up * (q_all * p_rest - q_rest) * exp2(double(res.low) - rest2_s));
+        // (Q p_rest - q_rest) / p_rest p_j, with p_j / p_rest taken from the rest's own sum
+        res.top = st.max == A(-INFINITY) ? A(0) : st.max;
+        res.factor = st.nothing() ? (en.bad ? A(NAN) : A(0)) : up * (q_all * p_rest - q_rest) / rest_sum;
     } else {
-        res.top = res.all_top, res.low = res.all_low, res.factor = res.all_factor;
+        res.top = res.all_top, res.factor = res.all_factor;
     }
     return res;
 }
 
-// The gradient at this lane's entry, if no earlier one names the same token: `q` of all entries that do, added up.
-template <int LPR, typename T>
-__device__ __forceinline__ void write_entry(T *out, const Entries &en, typename Elt<T>::acc xc,
+// The gradient at this lane's entry, if no earlier one names the same token.
+template <typename T>
+__device__ __forceinline__ void write_entry(T *out, const Entries<typename Elt<T>::acc> &en, typename Elt<T>::acc xc,
                                             const RowResult<typename Elt<T>::acc> &res, typename Elt<T>::acc kappa,
-                                            int K, bool wanted)
+                                            bool wanted)
 {
     using A = typename Elt<T>::acc;
     using M = Base2<A>;
-    double q = 0.0;
-    for (int o = 0; o < K; ++o) {
-        const int other = __shfl_sync(0xffffffffu, en.c, o, LPR);
-        const double oq = __shfl_sync(0xffffffffu, en.q, o, LPR);
-        if (other == en.c) q += oq;
-    }
     if (wanted && en.first)
-        out[en.c] = Elt<T>::from_acc(A(double(M::exp2_of(M::fma_of(xc - res.all_top, kappa, -res.all_low))) *
-                                           double(res.all_factor) - res.q_factor * q));
+        out[en.c] = Elt<T>::from_acc(
+            M::fma_of(M::exp2_of((xc - res.all_top) * kappa), res.all_factor, -res.q_factor * en.dup_q));
 }
 
 // Sum over the CTA of one double per thread, in a fixed order, in thread 0.
@@ -213,14 +240,17 @@ __device__ __forceinline__ double sum_cta(double v)
 }
 
 // Rows of at most LPR * NV vectors and at most LPR entries. Group g of a CTA takes the rows first + g, + GPC, ..
+// The terms of the sum are kept in registers for the gradient where the row has at most 64 elements a lane; longer rows
+// keep their vectors and take the terms again.
 template <typename T, int LPR, int NV, bool ALIGNED, bool TAIL>
 __global__ void __launch_bounds__(kRowThreads)
-distill_rows_kernel(const DistillArgs<T> a, int run_len)
+distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
 {
     using E = Elt<T>;
     using A = typename E::acc;
     using M = Base2<A>;
-    constexpr int GPC = kRowThreads / LPR;
+    constexpr int GPC = kRowThreads / LPR, VE = E::VE;
+    constexpr bool kKeep = NV * VE * sizeof(A) <= 256;
     constexpr unsigned kAll = 0xffffffffu;
     const int gl = threadIdx.x % LPR, group = threadIdx.x / LPR;
     const int64_t first = int64_t(blockIdx.x) * GPC * run_len + group;
@@ -230,26 +260,31 @@ distill_rows_kernel(const DistillArgs<T> a, int run_len)
         const bool active = r < a.n_rows;
         if (!__any_sync(kAll, active)) break;
         const int64_t rr = active ? r : 0;
-        const double weight = active ? (a.weight ? double(__ldg(a.weight + r)) : 1.0) : 0.0;
-        const bool seen = active && weight != 0.0;  // a row without weight is not read
+        const A weight = active ? (a.weight ? A(__ldg(a.weight + r)) : A(1)) : A(0);
+        const bool seen = active && weight != A(0);  // a row without weight is not read
         const T *row = a.x + rr * a.x_stride;
         const RowVectors<T, ALIGNED> rv(row, a.V);
+        int c = -1;
+        A value = A(-INFINITY);
+        if (seen && gl < a.K) {
+            c = __ldg(a.index + r * a.K + gl);
+            value = A(__ldg(a.teacher + r * a.K + gl));
+        }
         uint4 v[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             v[j] = vector_of_nothing<T>();
             if (seen && j * LPR + gl < rv.count) v[j] = rv.load(j * LPR + gl);
         }
-        const Entries en = load_entries<LPR, TAIL>(a.teacher, a.index, a.V, a.K, a.inv_tau, rr, gl, seen);
-        const A xc = en.c >= 0 ? E::to_acc(__ldg(row + en.c)) : A(-INFINITY);
+        const A xc = c >= 0 && c < a.V ? E::to_acc(__ldg(row + c)) : A(-INFINITY);
+        const Entries<A> en = weigh_entries<LPR, TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, gl);
         if (TAIL) {
             for (int e = 0; e < a.K; ++e) {
-                const int c = __shfl_sync(kAll, en.c, e, LPR);
-                const int at = c + rv.head, i = at / E::VE;
-                if (c >= 0 && i % LPR == gl) {
+                const int at = __shfl_sync(kAll, en.c, e, LPR) + rv.head, i = at / VE;
+                if (at >= rv.head && i % LPR == gl) {
 #pragma unroll
                     for (int j = 0; j < NV; ++j)
-                        if (i == j * LPR + gl) blank_element<T>(v[j], at % E::VE);
+                        if (i == j * LPR + gl) blank_element<T>(v[j], at % VE);
                 }
             }
         }
@@ -259,16 +294,32 @@ distill_rows_kernel(const DistillArgs<T> a, int run_len)
         for (int j = 0; j < NV; ++j) st.max = M::max_of(st.max, E::vec_max(v[j]));
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) st.max = M::max_of(st.max, __shfl_xor_sync(kAll, st.max, o));
-        const A shift = RowStats<A>::shift_of(st.max, a.kappa);
+        A term[kKeep ? NV : 1][VE];
+        if constexpr (kKeep) {
+            // the difference from the maximum first: no shift to be rounded, and no row too extreme
+            const A base = st.max == A(-INFINITY) ? A(0) : st.max;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) add_terms<T, false>(v[j], a.kappa, st.max, shift, st.s, st.t);
+            for (int j = 0; j < NV; ++j) {
+                E::unpack(v[j], term[j]);
+#pragma unroll
+                for (int k = 0; k < VE; ++k) {
+                    term[j][k] = M::exp2_of((term[j][k] - base) * a.kappa);
+                    st.s += term[j][k];
+                }
+            }
+        } else {
+            const A shift = RowStats<A>::shift_of(st.max, a.kappa);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) add_terms<T, false>(v[j], a.kappa, st.max, shift, st.s, st.t);
+            st.s = st.sum(a.kappa);
+        }
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) st.s += __shfl_xor_sync(kAll, st.s, o);
-        const double up = a.upstream && active ? double(__ldg(a.upstream + r * a.upstream_stride)) : 1.0;
-        const RowResult<A> res = solve_row<LPR, TAIL>(st, en, xc, a.kappa, a.inv_tau, weight, up * a.scale);
+        const A up = a.upstream && active ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
+        const RowResult<A> res = solve_row<LPR, TAIL>(st, en, xc, a.kappa, a.inv_tau, weight, up * A(a.scale), a.KP);
         if (active && gl == 0) {
-            if (a.row_loss) a.row_loss[r] = typename E::cost(res.loss);
-            sum += res.loss;
+            if (a.row_loss) a.row_loss[r] = res.loss;
+            sum += double(res.loss);
         }
         if (a.gx) {
             T *out = a.gx + rr * a.g_stride;
@@ -277,16 +328,20 @@ distill_rows_kernel(const DistillArgs<T> a, int run_len)
             for (int j = 0; j < NV; ++j) {
                 const int i = j * LPR + gl;
                 if (active && i < rv.count) {
-                    A e[E::VE];
-                    E::unpack(v[j], e);
+                    A e[VE];
+                    if constexpr (!kKeep) E::unpack(v[j], e);
 #pragma unroll
-                    for (int c = 0; c < E::VE; ++c)
-                        e[c] = M::exp2_of(M::fma_of(e[c] - res.top, a.kappa, -res.low)) * res.factor;
+                    for (int k = 0; k < VE; ++k) {
+                        if constexpr (kKeep)
+                            e[k] = term[j][k] * res.factor;
+                        else
+                            e[k] = M::exp2_of((e[k] - res.top) * a.kappa) * res.factor;
+                    }
                     store_vector(out, rv, i, same, e);
                 }
             }
             __syncwarp();
-            write_entry<LPR, T>(out, en, xc, res, a.kappa, a.K, seen);
+            write_entry<T>(out, en, xc, res, a.kappa, seen);
         }
     }
     if (a.partial) {
@@ -308,14 +363,20 @@ distill_long_kernel(const DistillArgs<T> a)
     __shared__ int listed[32];  // positions of the listed tokens, counted from the first vector's start; -1: none
     const int tid = threadIdx.x, lane = tid & 31;
     const int64_t r = blockIdx.x;
-    const double weight = a.weight ? double(__ldg(a.weight + r)) : 1.0;
+    const A weight = a.weight ? A(__ldg(a.weight + r)) : A(1);
     const T *row = a.x + r * a.x_stride;
     T *out = a.gx ? a.gx + r * a.g_stride : nullptr;
     const RowVectors<T, ALIGNED> rv(row, a.V);
     const bool same = ALIGNED || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    const bool seen = weight != 0.0;  // a row without weight is not read
-    const Entries en = load_entries<32, TAIL>(a.teacher, a.index, a.V, a.K, a.inv_tau, r, lane, seen);
-    const A xc = en.c >= 0 ? E::to_acc(__ldg(row + en.c)) : A(-INFINITY);
+    const bool seen = weight != A(0);  // a row without weight is not read
+    int c = -1;
+    A value = A(-INFINITY);
+    if (seen && lane < a.K) {
+        c = __ldg(a.index + r * a.K + lane);
+        value = A(__ldg(a.teacher + r * a.K + lane));
+    }
+    const A xc = c >= 0 && c < a.V ? E::to_acc(__ldg(row + c)) : A(-INFINITY);
+    const Entries<A> en = weigh_entries<32, TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, lane);
     if (tid < 32) listed[tid] = en.c >= 0 ? en.c + rv.head : -1;
     __syncthreads();
 
@@ -370,11 +431,12 @@ distill_long_kernel(const DistillArgs<T> a)
     st = parts[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) st.template join<false>(parts[w], a.kappa);
-    const double up = a.upstream ? double(__ldg(a.upstream + r * a.upstream_stride)) : 1.0;
-    const RowResult<A> res = solve_row<32, TAIL>(st, en, xc, a.kappa, a.inv_tau, weight, up * a.scale);
+    st.s = st.sum(a.kappa);
+    const A up = a.upstream ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
+    const RowResult<A> res = solve_row<32, TAIL>(st, en, xc, a.kappa, a.inv_tau, weight, up * A(a.scale), a.KP);
     if (tid == 0) {
-        if (a.row_loss) a.row_loss[r] = typename E::cost(res.loss);
-        if (a.partial) a.partial[r] = res.loss * a.scale;
+        if (a.row_loss) a.row_loss[r] = res.loss;
+        if (a.partial) a.partial[r] = double(res.loss) * a.scale;
     }
     if (!out) return;
     for (int at = 0; at < rv.count; at += kRowThreads * NV) {
@@ -391,13 +453,13 @@ distill_long_kernel(const DistillArgs<T> a)
                 A e[E::VE];
                 E::unpack(v[j], e);
 #pragma unroll
-                for (int c = 0; c < E::VE; ++c) e[c] = M::exp2_of(M::fma_of(e[c] - res.top, a.kappa, -res.low)) * res.factor;
+                for (int k = 0; k < E::VE; ++k) e[k] = M::exp2_of((e[k] - res.top) * a.kappa) * res.factor;
                 store_vector(out, rv, i, same, e);
             }
         }
     }
     __syncthreads();
-    if (tid < 32) write_entry<32, T>(out, en, xc, res, a.kappa, a.K, seen);
+    if (tid < 32) write_entry<T>(out, en, xc, res, a.kappa, seen);
 }
 
 // The CTAs' sums, added up in a fixed order.
@@ -422,7 +484,7 @@ template <typename T, int LPR, int NV, bool ALIGNED>
 int64_t launch_distill_rows(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 {
     constexpr int GPC = kRowThreads / LPR;
-    const int run_len = 1;
+    const int run_len = a.n_rows > int64_t(GPC) * kNumSMs * 32 ? 4 : 1;
     const int64_t grid = (a.n_rows + int64_t(GPC) * run_len - 1) / (int64_t(GPC) * run_len);
     if (tail)
         distill_rows_kernel<T, LPR, NV, ALIGNED, true><<<unsigned(grid), kRowThreads, 0, s>>>(a, run_len);
@@ -437,9 +499,11 @@ int64_t launch_distill_t(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 {
     constexpr int VE = Elt<T>::VE;
     const int nv = ALIGNED ? a.V / VE : (a.V + 2 * VE - 2) / VE;
-    if (nv <= 16 && a.K <= 4) return launch_distill_rows<T, 4, 4, ALIGNED>(a, tail, s);
-    if (nv <= 32 && a.K <= 8) return launch_distill_rows<T, 8, 4, ALIGNED>(a, tail, s);
-    if (nv <= 64 && a.K <= 16) return launch_distill_rows<T, 16, 4, ALIGNED>(a, tail, s);
+    if constexpr (sizeof(T) <= 4) {
+        if (nv <= 16 && a.K <= 4) return launch_distill_rows<T, 4, 4, ALIGNED>(a, tail, s);
+        if (nv <= 32 && a.K <= 8) return launch_distill_rows<T, 8, 4, ALIGNED>(a, tail, s);
+        if (nv <= 64 && a.K <= 16) return launch_distill_rows<T, 16, 4, ALIGNED>(a, tail, s);
+    }
     if (nv <= 128) return launch_distill_rows<T, 32, 4, ALIGNED>(a, tail, s);
     if (nv <= 256) return launch_distill_rows<T, 32, 8, ALIGNED>(a, tail, s);
     if (nv <= 512) return launch_distill_rows<T, 32, 16, ALIGNED>(a, tail, s);
@@ -461,7 +525,8 @@ cudaError_t launch_distill_of(const cwrnnt_rows &p, bool tail, const void *x, co
     a.x = static_cast<const T *>(x), a.gx = static_cast<T *>(gx);
     a.n_rows = p.n_rows, a.x_stride = p.x_stride, a.g_stride = p.grad_stride;
     a.V = p.V, a.K = p.n_list;
-    a.inv_tau = 1.0 / p.temperature;
+    for (a.KP = 1; a.KP < a.K;) a.KP *= 2;
+    a.inv_tau = typename Elt<T>::acc(1.0 / p.temperature);
     a.kappa = typename Elt<T>::acc(kLog2e / p.temperature);
     a.scale = scale;
     a.teacher = static_cast<const C *>(teacher), a.weight = static_cast<const C *>(weight);

@@ -86,10 +86,10 @@ cudaError_t launch_joint(const cwrnnt_problem &p, int activation, bool backward,
 
 // Scores of logits rows and their gradient (arguments as in the C ABI).
 cudaError_t launch_token_scores(const cwrnnt_rows &p, const void *x, const int32_t *targets, void *log_probs,
-                                void *entropy, void *top_log_probs, int32_t *top_indices, double *stats,
+                                void *entropy, void *top_log_probs, int32_t *top_indices, void *stats,
                                 cudaStream_t s);
 cudaError_t launch_token_scores_grad(const cwrnnt_rows &p, const void *x, const int32_t *targets,
-                                     const int32_t *top_indices, const double *stats, const void *entropy,
+                                     const int32_t *top_indices, const void *stats, const void *entropy,
                                      const void *g_log_probs, const void *g_entropy, const void *g_top, void *grad_x,
                                      cudaStream_t s);
 

@@ -81,13 +81,7 @@ struct Base2;
 template <>
 struct Base2<float> {
     static __device__ __forceinline__ float exp2_of(float d) { return ex2_approx(d); }
-    // log2(s): the binary exponent is split off exactly, so the absolute error stays near 2^-24 for large sums
-    static __device__ __forceinline__ double log2_of(float s)
-    {
-        int e;
-        const float f = frexpf(s, &e);
-        return double(e) + double(logf(f)) * 1.4426950408889634;
-    }
+    static __device__ __forceinline__ float ln_of(float s) { return logf(s); }
     static __device__ __forceinline__ float fma_of(float a, float b, float c) { return fmaf(a, b, c); }
     static __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
     // below this exponent a term is zero; it keeps 0 * (-inf) out of sum p log p
@@ -98,7 +92,7 @@ struct Base2<float> {
 template <>
 struct Base2<double> {
     static __device__ __forceinline__ double exp2_of(double d) { return exp2(d); }
-    static __device__ __forceinline__ double log2_of(double s) { return log2(s); }
+    static __device__ __forceinline__ double ln_of(double s) { return log(s); }
     static __device__ __forceinline__ double fma_of(double a, double b, double c) { return fma(a, b, c); }
     static __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
     static constexpr double kFloor = -5000.0;
@@ -148,28 +142,27 @@ struct RowStats {
     }
     // no finite entry (and no NaN either)
     __device__ __forceinline__ bool nothing() const { return max == A(-INFINITY) && s == s; }
-    // log2 of sum 2^((x - max) * kappa), the rounding of the shift undone
-    __device__ __forceinline__ double log2_sum(A kappa) const
+    // sum 2^((x - max) * kappa), the rounding of the shift undone
+    __device__ __forceinline__ A sum(A kappa) const
     {
         const A shift = shift_of(max, kappa);
-        const double excess = extreme(shift) || max == A(-INFINITY)
-                                  ? 0.0 : double(Base2<A>::fma_of(max, kappa, -shift));
-        return Base2<A>::log2_of(s) - excess;
+        if (extreme(shift) || max == A(-INFINITY)) return s;
+        return s * Base2<A>::exp2_of(-Base2<A>::fma_of(max, kappa, -shift));
     }
     // entropy of the row's softmax: ln s - ln2 * t / s
-    __device__ __forceinline__ double entropy() const
+    __device__ __forceinline__ A entropy() const
     {
-        if (s == A(0)) return 0.0;
-        return kLn2 * (Base2<A>::log2_of(s) - double(t) / double(s));
+        if (s == A(0)) return A(0);
+        return Base2<A>::ln_of(s) - A(kLn2) * (t / s);
     }
 };
 
-// ln of an entry's probability, (x - max) / tau - ln s, in double: log-probabilities near zero keep their digits, and
-// so do those of rows of the type's lowest value.
+// ln of an entry's probability, (x - max) / tau - ln s: log-probabilities near zero keep their digits, and so do those
+// of rows of the type's lowest value.
 template <typename A>
-__device__ __forceinline__ double log_prob_of(A x, double max, double inv_tau, double ln_s)
+__device__ __forceinline__ A log_prob_of(A x, A max, A inv_tau, A ln_s)
 {
-    return x == A(-INFINITY) ? (ln_s == ln_s ? -INFINITY : NAN) : (double(x) - max) * inv_tau - ln_s;
+    return x == A(-INFINITY) ? (ln_s == ln_s ? A(-INFINITY) : A(NAN)) : Base2<A>::fma_of(x - max, inv_tau, -ln_s);
 }
 
 // Adds one vector's terms at a fixed maximum and its shift.
@@ -241,6 +234,47 @@ __device__ __forceinline__ TopKey<float> shfl_xor_key(unsigned mask, const TopKe
 __device__ __forceinline__ TopKey<double> shfl_xor_key(unsigned mask, const TopKey<double> &k, int by)
 {
     return TopKey<double>{__shfl_xor_sync(mask, k.o, by), __shfl_xor_sync(mask, k.i, by)};
+}
+
+// The same order in 32 bits for the 16-bit types' rows of at most 65 535 entries; 0 comes after every entry.
+template <typename T>
+__device__ __forceinline__ uint32_t short_key(T v, int index)
+{
+    const float f = Elt<T>::to_acc(v) + 0.0f;  // -0 -> +0
+    const uint32_t b = __float_as_uint(f);
+    uint32_t o;
+    if constexpr (Elt<T>::kBf16) {
+        o = b >> 16;
+    } else {
+        o = uint32_t(__half_as_ushort(__float2half_rn(f)));
+    }
+    o = o & 0x8000u ? ~o & 0xffffu : o | 0x8000u;
+    return (o << 16) | (0xffffu - uint32_t(index));
+}
+
+// Which elements of a vector are at least `bar` (no NaN among them): bit c for element c.
+template <typename T>
+__device__ __forceinline__ uint32_t at_least(const uint4 &v, typename Elt<T>::acc bar)
+{
+    using E = Elt<T>;
+    uint32_t bits = 0;
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        using T2 = typename E::pair;
+        const T2 b2 = E::both(bar);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t m = __hge2_mask(*reinterpret_cast<const T2 *>(&w[i]), b2);
+            bits |= m & ((1u << (2 * i)) | (1u << (2 * i + 1 + 16)));
+        }
+        bits = (bits | (bits >> 16)) & 0xffu;
+    } else {
+        typename E::acc e[E::VE];
+        E::unpack(v, e);
+#pragma unroll
+        for (int c = 0; c < E::VE; ++c) bits |= e[c] >= bar ? 1u << c : 0u;
+    }
+    return bits;
 }
 
 // The best key of vector `i` of a row that comes after `last` in the order.

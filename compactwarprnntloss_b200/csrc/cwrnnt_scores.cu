@@ -12,10 +12,10 @@
 // stay in registers, a row of up to 512 vectors (8 KB) does too, so that the selection of the largest entries reads
 // nothing again. Longer rows go through a CTA each; their selection reads them a second time, from L2.
 //
-// Selection: the k-th largest of the lanes' own maxima is a lower bound of the row's k-th largest entry. The entries at
-// or above it - about as many as k, since each lane's maximum is one of them - are collected in shared memory and
-// ranked by counting how many come before each. Rows with too many equal entries for that, and rows with NaN, are
-// picked one entry at a time instead.
+// Selection: of the lanes' own maxima, the largest value that at least k of them reach is a lower bound of the row's
+// k-th largest entry. The entries at or above it - about as many as k - are collected in shared memory and ranked by
+// counting how many come before each. Rows with too many equal entries for that, and rows with NaN, are picked one
+// entry at a time instead.
 #include "cwrnnt_kernels.h"
 #include "cwrnnt_rowops.cuh"
 
@@ -30,59 +30,110 @@ struct ScoresArgs {
     const T *x;
     int64_t n_rows, x_stride;
     int V, n_targets, top_k;
-    A kappa;         // log2(e) / tau
-    double inv_tau;  // 1 / tau
+    A kappa;    // log2(e) / tau
+    A inv_tau;  // 1 / tau
     const int32_t *targets;
     C *log_probs, *entropy, *top_log_probs;
     int32_t *top_indices;
-    double *stats;
+    C *stats;
 };
 
 // What a row's log-probabilities are taken from.
+template <typename A>
 struct RowLog {
-    double max, ln_s;
+    A max, ln_s;
 };
 
 template <typename T>
-__device__ __forceinline__ void emit_top(const ScoresArgs<T> &a, const T *row, int64_t r, const RowLog &log,
-                                         int rank, int index)
+__device__ __forceinline__ void emit_top(const ScoresArgs<T> &a, const T *row, int64_t r,
+                                         const RowLog<typename Elt<T>::acc> &log, int rank, int index)
 {
     a.top_indices[r * a.top_k + rank] = index;
     a.top_log_probs[r * a.top_k + rank] =
-        typename Elt<T>::cost(log_prob_of(Elt<T>::to_acc(__ldg(row + index)), log.max, a.inv_tau, log.ln_s));
+        log_prob_of(Elt<T>::to_acc(__ldg(row + index)), log.max, a.inv_tau, log.ln_s);
 }
 
 // One target's log-probability: 0 where there is none (negative), NaN where it lies outside the row.
 template <typename T>
-__device__ __forceinline__ void emit_target(const ScoresArgs<T> &a, const T *row, int64_t r, const RowLog &log,
-                                            int i)
+__device__ __forceinline__ void emit_target(const ScoresArgs<T> &a, const T *row, int64_t r,
+                                            const RowLog<typename Elt<T>::acc> &log, int t, int i)
 {
-    const int t = __ldg(a.targets + r * a.n_targets + i);
-    double lp = 0.0;
+    using A = typename Elt<T>::acc;
+    A lp = A(0);
     if (t >= a.V)
-        lp = NAN;
+        lp = A(NAN);
     else if (t >= 0)
         lp = log_prob_of(Elt<T>::to_acc(__ldg(row + t)), log.max, a.inv_tau, log.ln_s);
-    a.log_probs[r * a.n_targets + i] = typename Elt<T>::cost(lp);
+    a.log_probs[r * a.n_targets + i] = lp;
+}
+
+// Candidate keys of rows held in registers: 16-bit rows fit 32 bits (at most 32 * 16 * 8 entries).
+template <typename T>
+struct Candidate {
+    using Key = TopKey<typename Elt<T>::acc>;
+    using Word = Key;
+    static __device__ __forceinline__ Key of(T v, int index) { return Key::of(Elt<T>::to_acc(v), index); }
+    static __device__ __forceinline__ bool before(const Key &a, const Key &b) { return a.before(b); }
+    static __device__ __forceinline__ int index(const Key &k) { return k.index(); }
+};
+template <typename T>
+struct ShortCandidate {
+    using Word = uint32_t;
+    static __device__ __forceinline__ uint32_t of(T v, int index) { return short_key<T>(v, index); }
+    static __device__ __forceinline__ bool before(uint32_t a, uint32_t b) { return a > b; }
+    static __device__ __forceinline__ int index(uint32_t k) { return int(0xffffu - (k & 0xffffu)); }
+};
+template <>
+struct Candidate<__half> : ShortCandidate<__half> {};
+template <>
+struct Candidate<__nv_bfloat16> : ShortCandidate<__nv_bfloat16> {};
+
+__host__ __device__ constexpr int candidates_of(int lpr) { return 4 * lpr; }
+
+// The largest entries one after the other, each by a pass over the row (from L1 or L2): for the rows of `slow` groups. Kept
+// out of line, or its keys would take the registers of the usual path.
+template <typename T, int LPR, bool ALIGNED>
+__device__ __noinline__ void pick_one_by_one(const ScoresArgs<T> &a, const T *row, int64_t r,
+                                             RowLog<typename Elt<T>::acc> log, bool slow)
+{
+    using Key = TopKey<typename Elt<T>::acc>;
+    const int gl = threadIdx.x % LPR;
+    const RowVectors<T, ALIGNED> rv(row, a.V);
+    Key last = Key::all();
+    for (int round = 0; round < a.top_k; ++round) {
+        Key best = Key::none();
+        if (slow) {
+#pragma unroll 1
+            for (int i = gl; i < rv.count; i += LPR) best_after(rv, i, rv.load(i), last, best);
+        }
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) {
+            const Key other = shfl_xor_key(0xffffffffu, best, o);
+            if (other.before(best)) best = other;
+        }
+        last = best;
+        if (slow && gl == 0) emit_top(a, row, r, log, round, best.index());
+    }
 }
 
 // Rows of at most LPR * NV vectors: LPR lanes hold a row in NV vectors each. All lanes of a warp take every collective
 // step together, whichever of their groups has a row left. Group g of a CTA takes the rows first + g, + GPC, ..
 template <typename T, int LPR, int NV, bool ALIGNED, bool ENT>
 __global__ void __launch_bounds__(kRowThreads)
-scores_rows_kernel(const ScoresArgs<T> a, int run_len)
+scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
 {
     using E = Elt<T>;
     using A = typename E::acc;
     using M = Base2<A>;
-    using Key = TopKey<A>;
+    using Cand = Candidate<T>;
+    using Word = typename Cand::Word;
     constexpr int GPC = kRowThreads / LPR;
-    constexpr int kCap = 4 * LPR;  // candidates of a group
+    constexpr int kCap = candidates_of(LPR);
     constexpr unsigned kAll = 0xffffffffu;
-    extern __shared__ __align__(16) unsigned char scratch[];  // kCap keys and one counter per group, when top_k > 0
-    const int gl = threadIdx.x % LPR, group = threadIdx.x / LPR;
-    Key *keys = reinterpret_cast<Key *>(scratch) + group * kCap;
-    int *counter = reinterpret_cast<int *>(reinterpret_cast<Key *>(scratch) + GPC * kCap) + group;
+    extern __shared__ __align__(16) unsigned char scratch[];  // kCap candidates per group, when top_k > 0
+    const int gl = threadIdx.x % LPR, group = threadIdx.x / LPR, lane = threadIdx.x & 31;
+    const unsigned group_bits = (LPR == 32 ? kAll : (1u << (LPR & 31)) - 1u) << (lane / LPR * LPR);
+    Word *cands = reinterpret_cast<Word *>(scratch) + group * kCap;
 
     const int64_t first = int64_t(blockIdx.x) * GPC * run_len + group;
     for (int step = 0; step < run_len; ++step) {
@@ -97,6 +148,7 @@ scores_rows_kernel(const ScoresArgs<T> a, int run_len)
             v[j] = vector_of_nothing<T>();
             if (active && j * LPR + gl < rv.count) v[j] = rv.load(j * LPR + gl);
         }
+        const int target = active && gl < a.n_targets ? __ldg(a.targets + r * a.n_targets + gl) : -1;
         A own = A(-INFINITY);
 #pragma unroll
         for (int j = 0; j < NV; ++j) own = M::max_of(own, E::vec_max(v[j]));
@@ -113,70 +165,71 @@ scores_rows_kernel(const ScoresArgs<T> a, int run_len)
             st.s += __shfl_xor_sync(kAll, st.s, o);
             if (ENT) st.t += __shfl_xor_sync(kAll, st.t, o);
         }
-        const RowLog log{double(st.max), st.nothing() ? 0.0 : kLn2 * st.log2_sum(a.kappa)};
+        const A sum = st.sum(a.kappa);
+        const RowLog<A> log{st.max, st.nothing() ? A(0) : M::ln_of(sum)};
         if (active) {
             if (gl == 0) {
-                if (ENT) a.entropy[r] = typename E::cost(st.entropy());
-                if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = log.ln_s;
+                if (ENT) a.entropy[r] = st.entropy();
+                if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = sum;
             }
-            for (int i = gl; i < a.n_targets; i += LPR) emit_target(a, row, r, log, i);
+            if (gl < a.n_targets) emit_target(a, row, r, log, target, gl);
+            for (int i = gl + LPR; i < a.n_targets; i += LPR)
+                emit_target(a, row, r, log, __ldg(a.targets + r * a.n_targets + i), i);
         }
         if (a.top_k > 0) {
-            int rank = 0;
-            for (int j = 0; j < LPR; ++j) {
-                const A other = __shfl_sync(kAll, own, j, LPR);
-                rank += other > own || (other == own && j < gl);
-            }
-            const unsigned hit = __ballot_sync(kAll, rank == a.top_k - 1) >> ((threadIdx.x & 31) / LPR * LPR);
-            const A bar = __shfl_sync(kAll, own, (__ffs(hit) - 1) & (LPR - 1), LPR);
-            if (gl == 0) *counter = 0;
-            __syncwarp();
-            if (active) {
+            // the bar: a lane whose maximum fewer than k lanes exceed is at or below it
+            int above = 0;
+#pragma unroll 8
+            for (int j = 0; j < LPR; ++j) above += __shfl_sync(kAll, own, j, LPR) > own;
+            A bar = above < a.top_k ? own : A(INFINITY);
 #pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int i = j * LPR + gl;
-                    if (i < rv.count && E::vec_max(v[j]) >= bar) {
-                        A e[E::VE];
-                        E::unpack(v[j], e);
-#pragma unroll
-                        for (int c = 0; c < E::VE; ++c) {
-                            const int k = rv.first(i) + c;
-                            if (e[c] >= bar && (ALIGNED || (k >= 0 && k < a.V))) {
-                                const int at = atomicAdd(counter, 1);
-                                if (at < kCap) keys[at] = Key::of(e[c], k);
-                            }
-                        }
+            for (int o = LPR / 2; o > 0; o >>= 1) bar = fmin(bar, __shfl_xor_sync(kAll, bar, o));
+            int n = 0;
+            auto collect = [&](uint32_t bits, int j0) {
+                // one candidate of every lane at a time; their places follow from the ballot
+                for (;;) {
+                    const unsigned have = __ballot_sync(kAll, bits != 0) & group_bits;
+                    if (!__any_sync(kAll, bits != 0)) break;
+                    if (bits) {
+                        const int b = __ffs(bits) - 1;
+                        bits &= bits - 1;
+                        const int k = rv.first((j0 + b / E::VE) * LPR + gl) + b % E::VE;
+                        const int at = n + __popc(have & ((1u << lane) - 1u));
+                        if (at < kCap) cands[at] = Cand::of(__ldg(row + k), k);
                     }
+                    n += __popc(have);
                 }
+            };
+            constexpr int kPer = 32 / E::VE;  // vectors whose elements fit a word of bits
+#pragma unroll
+            for (int j0 = 0; j0 < NV; j0 += kPer) {
+                uint32_t bits = 0;
+#pragma unroll
+                for (int j = j0; j < NV && j < j0 + kPer; ++j) {
+                    const int i = j * LPR + gl;
+                    uint32_t hit = at_least<T>(v[j], bar);
+                    if (!ALIGNED) {  // elements before and behind the row
+                        const int f = rv.first(i);
+                        if (f < 0) hit &= ~0u << (-f);
+                        if (a.V - f < E::VE) hit &= a.V > f ? (1u << (a.V - f)) - 1u : 0u;
+                    }
+                    if (!active || i >= rv.count) hit = 0;
+                    bits |= hit << ((j - j0) * E::VE);
+                }
+                collect(bits, j0);
             }
             __syncwarp();
-            const int n = *counter;
             const bool slow = active && (n > kCap || n < a.top_k || st.s != st.s);
             if (active && !slow) {
                 for (int i = gl; i < n; i += LPR) {
-                    const Key mine = keys[i];
+                    const Word mine = cands[i];
                     int before = 0;
-                    for (int j = 0; j < n; ++j) before += keys[j].before(mine);
-                    if (before < a.top_k) emit_top(a, row, r, log, before, mine.index());
+                    for (int j = 0; j < n; ++j) before += Cand::before(cands[j], mine);
+                    if (before < a.top_k) emit_top(a, row, r, log, before, Cand::index(mine));
                 }
             }
-            if (__any_sync(kAll, slow)) {
-                Key last = Key::all();
-                for (int round = 0; round < a.top_k; ++round) {
-                    Key best = Key::none();
-#pragma unroll
-                    for (int j = 0; j < NV; ++j)
-                        if (active && j * LPR + gl < rv.count) best_after(rv, j * LPR + gl, v[j], last, best);
-#pragma unroll
-                    for (int o = LPR / 2; o > 0; o >>= 1) {
-                        const Key other = shfl_xor_key(kAll, best, o);
-                        if (other.before(best)) best = other;
-                    }
-                    last = best;
-                    if (slow && gl == 0) emit_top(a, row, r, log, round, best.index());
-                }
-            }
-            __syncwarp();  // the next row fills the same buffers
+            if (__any_sync(kAll, slow)) pick_one_by_one<T, LPR, ALIGNED>(a, row, r, log, slow);
+            __syncwarp();  // the next row fills the same buffer
         }
     }
 }
@@ -242,12 +295,13 @@ scores_long_kernel(const ScoresArgs<T> a)
     }
     const A own = st.max;
     st = join_cta<A, ENT>(st, a.kappa, parts);
-    const RowLog log{double(st.max), st.nothing() ? 0.0 : kLn2 * st.log2_sum(a.kappa)};
+    const A sum = st.sum(a.kappa);
+    const RowLog<A> log{st.max, st.nothing() ? A(0) : M::ln_of(sum)};
     if (tid == 0) {
-        if (ENT) a.entropy[r] = typename E::cost(st.entropy());
-        if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = log.ln_s;
+        if (ENT) a.entropy[r] = st.entropy();
+        if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = sum;
     }
-    if (tid < a.n_targets) emit_target(a, row, r, log, tid);
+    if (tid < a.n_targets) emit_target(a, row, r, log, __ldg(a.targets + r * a.n_targets + tid), tid);
     if (a.top_k == 0) return;
 
     // the bar: the k-th largest of the maxima of 64 groups of four threads
@@ -328,8 +382,7 @@ struct ScoresGradArgs {
     A kappa;
     double inv_tau;
     const int32_t *targets, *top_indices;
-    const double *stats;
-    const C *entropy, *g_log_probs, *g_entropy, *g_top;
+    const C *stats, *entropy, *g_log_probs, *g_entropy, *g_top;
 
     __device__ __forceinline__ int entries() const { return n_targets + top_k; }
     __device__ __forceinline__ int index(int64_t r, int e) const
@@ -338,17 +391,15 @@ struct ScoresGradArgs {
                                     : __ldg(top_indices + r * top_k + (e - n_targets));
         return t < V ? t : -1;
     }
-    __device__ __forceinline__ double upstream(int64_t r, int e) const
+    __device__ __forceinline__ C upstream(int64_t r, int e) const
     {
-        const bool t = e < n_targets;
-        const C *g = t ? g_log_probs : g_top;
-        return g ? double(__ldg(g + (t ? r * n_targets + e : r * top_k + (e - n_targets)))) : 0.0;
+        return e < n_targets ? __ldg(g_log_probs + r * n_targets + e) : __ldg(g_top + r * top_k + (e - n_targets));
     }
 };
 
-// Element-wise once the row's log-sum-exp is known: LPR threads a row (a part of a warp, a warp, or a CTA), four vectors
-// of each in flight. The entries that were picked are written a second time behind a barrier, by the first entry that
-// names them, which adds up all that do.
+// Element-wise once the row's maximum and sum are known: LPR threads a row (a part of a warp, a warp, or a CTA), four
+// vectors of each in flight. The entries that were picked are written a second time behind a barrier, by the first entry
+// that names them, which adds up all that do (in their order: the sum does not depend on timing).
 template <typename T, int LPR, bool ALIGNED>
 __global__ void __launch_bounds__(kRowThreads)
 scores_grad_kernel(const ScoresGradArgs<T> a)
@@ -369,39 +420,42 @@ scores_grad_kernel(const ScoresGradArgs<T> a)
     const RowVectors<T, ALIGNED> rv(row, a.V);
     const bool same = ALIGNED || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
 
+    uint4 v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+        if (active && j * LPR + gl < rv.count) v[j] = rv.load(j * LPR + gl);
     const int n = active ? a.entries() : 0;
-    double total = 0.0;
+    A total = A(0);
     for (int e = gl % kSum; e < n; e += kSum)
         if (a.index(rr, e) >= 0) total += a.upstream(rr, e);
 #pragma unroll
     for (int o = kSum / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const double max = active ? __ldg(a.stats + 2 * rr) : 0.0;
-    const double log2_s = active ? __ldg(a.stats + 2 * rr + 1) * kLog2e : 0.0;
-    const bool nothing = max == -INFINITY && log2_s == log2_s;  // no finite entry: no gradient
-    // p = 2^((x - top) * kappa - low), the rounding of `low` put into the row's factors
-    const A top = nothing ? A(0) : A(max), low = A(log2_s);
-    const double undo = exp2(double(low) - log2_s);
-    const double gh = a.g_entropy && active ? double(__ldg(a.g_entropy + rr)) : 0.0;
-    const double h = a.g_entropy && active ? double(__ldg(a.entropy + rr)) : 0.0;
-    const double scale = nothing ? 0.0 : a.inv_tau;
-    const A c0 = A(-(total + gh * h) * scale * undo), c1 = A(-gh * kLn2 * scale * undo);
+    const A max = active ? __ldg(a.stats + 2 * rr) : A(0);
+    const A sum = active ? __ldg(a.stats + 2 * rr + 1) : A(1);
+    const bool nothing = max == A(-INFINITY) && sum == sum;  // no finite entry: no gradient
+    // p = 2^((x - top) * kappa) / sum; the row's factors carry 1 / (sum * tau)
+    const A top = nothing ? A(0) : max;
+    const A scale = nothing ? A(0) : A(a.inv_tau) / sum;
+    A c0 = -total, c1 = A(0);
+    if (a.g_entropy && active) {
+        const A gh = __ldg(a.g_entropy + rr);
+        c0 -= gh * (__ldg(a.entropy + rr) - (nothing ? A(0) : M::ln_of(sum)));
+        c1 = -gh * A(kLn2);
+    }
+    c0 *= scale, c1 *= scale;
     if (active) {
         for (int at = 0; at < rv.count; at += LPR * NV) {
-            uint4 v[NV];
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int i = at + j * LPR + gl;
-                if (i < rv.count) v[j] = rv.load(i);
-            }
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int i = at + j * LPR + gl;
                 if (i < rv.count) {
                     A e[E::VE];
                     E::unpack(v[j], e);
+                    const int ahead = i + LPR * NV;
+                    if (ahead < rv.count) v[j] = rv.load(ahead);
 #pragma unroll
                     for (int c = 0; c < E::VE; ++c) {
-                        const A d = M::fma_of(e[c] - top, a.kappa, -low);
+                        const A d = (e[c] - top) * a.kappa;
                         e[c] = M::exp2_of(d) * M::fma_of(c1, M::max_of(d, M::kFloor), c0);
                     }
                     store_vector(out, rv, i, same, e);
@@ -417,16 +471,20 @@ scores_grad_kernel(const ScoresGradArgs<T> a)
     for (int e = gl; e < n; e += LPR) {
         const int t = a.index(rr, e);
         if (t < 0) continue;
-        double g = 0.0;
+        A g = a.upstream(rr, e);
         bool first = true;
-        for (int o = 0; o < n; ++o)
-            if (a.index(rr, o) == t) {
-                g += a.upstream(rr, o);
-                first = first && o >= e;
-            }
+        if (a.n_targets > 0) {  // (the best entries differ from one another)
+            g = A(0);
+            for (int o = 0; o < n; ++o)
+                if (a.index(rr, o) == t) {
+                    g += a.upstream(rr, o);
+                    first = first && o >= e;
+                }
+        }
         if (first) {
-            const A d = M::fma_of(E::to_acc(__ldg(row + t)) - top, a.kappa, -low);
-            out[t] = E::from_acc(A(g * scale) + M::exp2_of(d) * M::fma_of(c1, M::max_of(d, M::kFloor), c0));
+            const A d = (E::to_acc(__ldg(row + t)) - top) * a.kappa;
+            const A own = nothing ? A(0) : g * A(a.inv_tau);
+            out[t] = E::from_acc(own + M::exp2_of(d) * M::fma_of(c1, M::max_of(d, M::kFloor), c0));
         }
     }
 }
@@ -452,7 +510,7 @@ cudaError_t launch_scores_rows(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
     constexpr int GPC = kRowThreads / LPR;
     const int run_len = 1;
     const int64_t grid = (a.n_rows + int64_t(GPC) * run_len - 1) / (int64_t(GPC) * run_len);
-    const size_t smem = a.top_k > 0 ? GPC * (4 * LPR * sizeof(TopKey<typename Elt<T>::acc>) + sizeof(int)) : 0;
+    const size_t smem = a.top_k > 0 ? GPC * candidates_of(LPR) * sizeof(typename Candidate<T>::Word) : 0;
     if (ent)
         scores_rows_kernel<T, LPR, NV, ALIGNED, true><<<unsigned(grid), kRowThreads, smem, s>>>(a, run_len);
     else
@@ -466,9 +524,14 @@ cudaError_t launch_scores_t(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
     const int nv = vectors_of<T>(a.V, ALIGNED);
     // the bar of the selection is taken among the lanes' maxima: at least twice as many lanes as entries, up to a warp
     const int lanes = 2 * a.top_k;
-    if (nv <= 16 && lanes <= 4) return launch_scores_rows<T, 4, 4, ALIGNED>(a, ent, s);
-    if (nv <= 32 && lanes <= 8) return launch_scores_rows<T, 8, 4, ALIGNED>(a, ent, s);
-    if (nv <= 64 && lanes <= 16) return launch_scores_rows<T, 16, 4, ALIGNED>(a, ent, s);
+    if constexpr (sizeof(T) <= 4) {
+        if (nv <= 16 && lanes <= 4) return launch_scores_rows<T, 4, 4, ALIGNED>(a, ent, s);
+        if (nv <= 16 && lanes <= 8) return launch_scores_rows<T, 8, 2, ALIGNED>(a, ent, s);
+        if (nv <= 32 && lanes <= 8) return launch_scores_rows<T, 8, 4, ALIGNED>(a, ent, s);
+        if (nv <= 32 && lanes <= 16) return launch_scores_rows<T, 16, 2, ALIGNED>(a, ent, s);
+        if (nv <= 64 && lanes <= 16) return launch_scores_rows<T, 16, 4, ALIGNED>(a, ent, s);
+        if (nv <= 64) return launch_scores_rows<T, 32, 2, ALIGNED>(a, ent, s);
+    }
     if (nv <= 128) return launch_scores_rows<T, 32, 4, ALIGNED>(a, ent, s);
     if (nv <= 256) return launch_scores_rows<T, 32, 8, ALIGNED>(a, ent, s);
     if (nv <= 512) return launch_scores_rows<T, 32, 16, ALIGNED>(a, ent, s);
@@ -481,19 +544,19 @@ cudaError_t launch_scores_t(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
 
 template <typename T>
 cudaError_t launch_scores_of(const cwrnnt_rows &p, const void *x, const int32_t *targets, void *log_probs,
-                             void *entropy, void *top_log_probs, int32_t *top_indices, double *stats, cudaStream_t s)
+                             void *entropy, void *top_log_probs, int32_t *top_indices, void *stats, cudaStream_t s)
 {
     using C = typename Elt<T>::cost;
     ScoresArgs<T> a{};
     a.x = static_cast<const T *>(x);
     a.n_rows = p.n_rows, a.x_stride = p.x_stride;
     a.V = p.V, a.n_targets = p.n_list, a.top_k = p.top_k;
-    a.inv_tau = 1.0 / p.temperature;
+    a.inv_tau = typename Elt<T>::acc(1.0 / p.temperature);
     a.kappa = typename Elt<T>::acc(kLog2e / p.temperature);
     a.targets = targets;
     a.log_probs = static_cast<C *>(log_probs), a.entropy = static_cast<C *>(entropy);
     a.top_log_probs = static_cast<C *>(top_log_probs);
-    a.top_indices = top_indices, a.stats = stats;
+    a.top_indices = top_indices, a.stats = static_cast<C *>(stats);
     return rows_aligned<T>(x, p.x_stride, p.V) ? launch_scores_t<T, true>(a, entropy != nullptr, s)
                                                : launch_scores_t<T, false>(a, entropy != nullptr, s);
 }
@@ -514,7 +577,7 @@ cudaError_t launch_scores_grad_t(const ScoresGradArgs<T> &a, cudaStream_t s)
 
 template <typename T>
 cudaError_t launch_scores_grad_of(const cwrnnt_rows &p, const void *x, const int32_t *targets,
-                                  const int32_t *top_indices, const double *stats, const void *entropy,
+                                  const int32_t *top_indices, const void *stats, const void *entropy,
                                   const void *g_log_probs, const void *g_entropy, const void *g_top, void *gx,
                                   cudaStream_t s)
 {
@@ -527,7 +590,7 @@ cudaError_t launch_scores_grad_of(const cwrnnt_rows &p, const void *x, const int
     a.inv_tau = 1.0 / p.temperature;
     a.kappa = typename Elt<T>::acc(kLog2e / p.temperature);
     a.targets = targets, a.top_indices = top_indices;
-    a.stats = stats, a.entropy = static_cast<const C *>(entropy);
+    a.stats = static_cast<const C *>(stats), a.entropy = static_cast<const C *>(entropy);
     a.g_log_probs = static_cast<const C *>(g_log_probs), a.g_entropy = static_cast<const C *>(g_entropy);
     a.g_top = static_cast<const C *>(g_top);
     const bool aligned = rows_aligned<T>(x, p.x_stride, p.V) && rows_aligned<T>(gx, p.grad_stride, p.V);
@@ -537,7 +600,7 @@ cudaError_t launch_scores_grad_of(const cwrnnt_rows &p, const void *x, const int
 }  // namespace
 
 cudaError_t launch_token_scores(const cwrnnt_rows &p, const void *x, const int32_t *targets, void *log_probs,
-                                void *entropy, void *top_log_probs, int32_t *top_indices, double *stats, cudaStream_t s)
+                                void *entropy, void *top_log_probs, int32_t *top_indices, void *stats, cudaStream_t s)
 {
     switch (p.dtype) {
     case CWRNNT_F32:
@@ -553,7 +616,7 @@ cudaError_t launch_token_scores(const cwrnnt_rows &p, const void *x, const int32
 }
 
 cudaError_t launch_token_scores_grad(const cwrnnt_rows &p, const void *x, const int32_t *targets,
-                                     const int32_t *top_indices, const double *stats, const void *entropy,
+                                     const int32_t *top_indices, const void *stats, const void *entropy,
                                      const void *g_log_probs, const void *g_entropy, const void *g_top, void *grad_x,
                                      cudaStream_t s)
 {

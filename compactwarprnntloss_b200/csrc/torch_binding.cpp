@@ -339,9 +339,9 @@ token_scores(const torch::Tensor &x, const OptTensor &targets, int64_t top_k, bo
         top = torch::empty({p.n_rows, p.top_k}, costs);
         index = torch::empty({p.n_rows, p.top_k}, x.options().dtype(torch::kInt32));
     }
-    if (keep) stats = torch::empty({p.n_rows, 2}, x.options().dtype(torch::kDouble));
+    if (keep) stats = torch::empty({p.n_rows, 2}, costs);
     check_status(cwrnnt_token_scores(&p, x.data_ptr(), static_cast<const int32_t *>(ptr(targets)), ptr(lp), ptr(ent),
-                                     ptr(top), static_cast<int32_t *>(ptr(index)), static_cast<double *>(ptr(stats)),
+                                     ptr(top), static_cast<int32_t *>(ptr(index)), ptr(stats),
                                      current_stream()),
                  "cwrnnt_token_scores");
     return {lp, ent, top, index, stats};
@@ -358,7 +358,7 @@ torch::Tensor token_scores_backward(const torch::Tensor &x, const OptTensor &tar
         if (*t) check_companion(**t, x, type, "an upstream gradient");
     auto gx = torch::empty({x.size(0), x.size(1)}, x.options());
     check_status(cwrnnt_token_scores_backward(&p, x.data_ptr(), static_cast<const int32_t *>(ptr(targets)),
-                                              static_cast<const int32_t *>(ptr(index)), stats.data_ptr<double>(),
+                                              static_cast<const int32_t *>(ptr(index)), stats.data_ptr(),
                                               ptr(entropy), ptr(g_lp), ptr(g_ent), ptr(g_top), gx.data_ptr(),
                                               current_stream()),
                  "cwrnnt_token_scores_backward");

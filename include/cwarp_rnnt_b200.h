@@ -374,12 +374,12 @@ typedef struct {
  *   log_probs       [n_rows, n_list] ln softmax(x/tau) at targets [n_rows, n_list]; 0 where the target is negative
  *   entropy         [n_rows] or NULL (not wanted)
  *   top_log_probs, top_indices  [n_rows, top_k] the largest entries, lowest index first among equal ones
- *   stats           [n_rows, 2] double or NULL: the row's largest logit and ln sum exp((x - largest) / tau), what
+ *   stats           [n_rows, 2] costs type or NULL: the row's largest logit and sum exp((x - largest) / tau), what
  *                   cwrnnt_token_scores_backward needs
  * log_probs, entropy and top_log_probs are of the costs type.
  */
 CWRNNT_API int cwrnnt_token_scores(const cwrnnt_rows *p, const void *x, const int32_t *targets, void *log_probs,
-                                   void *entropy, void *top_log_probs, int32_t *top_indices, double *stats,
+                                   void *entropy, void *top_log_probs, int32_t *top_indices, void *stats,
                                    cwrnnt_stream_t stream);
 /*
  * grad_x [n_rows, V], fully written, from the upstream gradients of log_probs, entropy and top_log_probs (costs type;
@@ -387,7 +387,7 @@ CWRNNT_API int cwrnnt_token_scores(const cwrnnt_rows *p, const void *x, const in
  * top entries is not differentiated. A target outside the row gets no gradient.
  */
 CWRNNT_API int cwrnnt_token_scores_backward(const cwrnnt_rows *p, const void *x, const int32_t *targets,
-                                            const int32_t *top_indices, const double *stats, const void *entropy,
+                                            const int32_t *top_indices, const void *stats, const void *entropy,
                                             const void *g_log_probs, const void *g_entropy, const void *g_top,
                                             void *grad_x, cwrnnt_stream_t stream);
 
