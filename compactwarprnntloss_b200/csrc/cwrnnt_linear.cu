@@ -74,6 +74,7 @@ struct Epilogue {
     int64_t side_ld, out_ld;
     bool tma_out, tma_side;  // rows of out / side lie on 16-byte boundaries: they go by TMA
     bool vec;                // all 16-byte accesses allowed, columns in whole groups of 8
+    float *sums;             // kSlope: sums over each 32 rows of dz, [rows / 32, N], or null
 };
 
 // Eight consecutive elements of the product become eight of the output: bias, then the activation (plus the residual) or
@@ -142,6 +143,13 @@ struct Shape {
     int64_t tiles_m;
     int tiles_n;
     int stages;
+    int64_t part_rows;
+    // columns that tile n multiplies out: the last tile of a row is as wide as the matrix needs it
+    __device__ __forceinline__ int width(int n, int bn, int ctas) const
+    {
+        const int unit = 16 * ctas, left = (N - n * bn + unit - 1) / unit * unit;
+        return left < bn ? left : bn;
+    }
     __device__ __forceinline__ int64_t tiles() const { return tiles_m * tiles_n * splits; }
     // columns fastest, then rows, then parts of the sum
     __device__ __forceinline__ void tile(int64_t t, int64_t &m, int &n, int &split) const
@@ -165,7 +173,10 @@ struct Shape {
 constexpr int kPiece = 32 * 128;
 template <int BN>
 struct Layout {
-    static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
+    // the widest tiles are shared by two CTAs: 256 rows, half of them and half of the columns' operand in each
+    static constexpr bool kPair = BN == 256;
+    static constexpr int kRowsB = kPair ? BN / 2 : BN;
+    static constexpr int kA = kBM * kBK * 2, kB = kRowsB * kBK * 2, kStage = kA + kB;
     static constexpr int kCarriers = BN >= 128 ? 8 : 4;  // warps of the epilogue
     static constexpr int kThreads = 64 + 32 * kCarriers;
     static constexpr uint32_t kColumns = 2 * BN;         // two sums in TMEM
@@ -271,12 +282,24 @@ struct Carrier {
                 *piece_group(out_piece, lane, half * 4 + g) = E::pack(v);
             }
         }
-        if (ep.tma_out) {
-            tc::fence_async();
-            __syncwarp();
-            if (lane == 0) tc::store_2d(map_out, out_piece, col, int(out_row0));
-        } else {
-            __syncwarp();
+        if (ep.tma_out) tc::fence_async();
+        __syncwarp();
+        if (ep.tma_out && lane == 0) tc::store_2d(map_out, out_piece, col, int(out_row0));
+        if (ep.sums) {
+            // rows behind the matrix are zero here: their upstream gradient is
+            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll 8
+            for (int k = 0; k < 32; ++k) {
+                const uint32_t w = reinterpret_cast<const uint32_t *>(piece_group(out_piece, k, lane >> 2))[lane & 3];
+                float v[8];
+                E::unpack(make_uint4(w, 0u, 0u, 0u), v);
+                s0 += v[0], s1 += v[1];
+            }
+            float *to = ep.sums + (row0 / 32) * sh.N + col + 2 * lane;
+            if (col + 2 * lane < sh.N) to[0] = s0;
+            if (col + 2 * lane + 1 < sh.N) to[1] = s1;
+        }
+        if (!ep.tma_out) {
             const T *o = reinterpret_cast<const T *>(out_piece);
             for (int k = 0; k < 32; ++k)
 #pragma unroll
@@ -306,6 +329,10 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     __shared__ int gave_up;
     unsigned char *stages = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr bool kPair = L::kPair;
+    constexpr int kCtas = kPair ? 2 : 1;
+    const int rank = kPair ? int(tc::cluster_rank()) : 0;
+    const int64_t t0 = blockIdx.x / kCtas, dt = gridDim.x / kCtas;
 
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < sh.stages; ++i) {
@@ -314,7 +341,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&sum_full[i], 1);
-            tc::mbar_init(&sum_empty[i], L::kCarriers);
+            tc::mbar_init(&sum_empty[i], L::kCarriers * kCtas);
         }
         for (int i = 0; i < L::kCarriers; ++i) tc::mbar_init(&side_full[i], 1);
         tc::mbar_init(&drained, 1);
@@ -323,9 +350,13 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         tc::prefetch_map(&map_a);
         tc::prefetch_map(&map_b);
     }
-    if (warp == 1) tc::tmem_alloc(&tmem_slot, L::kColumns);
+    if (warp == 1) tc::tmem_alloc<kPair>(&tmem_slot, L::kColumns);
+    __syncwarp();
     tc::fence_before();
-    __syncthreads();
+    if (kPair)
+        tc::cluster_sync();
+    else
+        __syncthreads();
     tc::fence_after();
     const uint32_t tmem = tmem_slot;
     const int64_t total = sh.tiles();
@@ -336,36 +367,44 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             uint32_t phase = 0;
             bool ok = true;
             uint32_t started = 0;  // stages loaded at least once
-            for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+            for (int64_t t = t0; ok && t < total; t += dt) {
                 int64_t m;
                 int n, split;
                 sh.tile(t, m, n, split);
                 const int k0 = sh.first_step(split), k1 = k0 + sh.count_steps(split);
+                const int row = (int(m) * kCtas + rank) * kBM;
+                const int col = n * BN + rank * (sh.width(n, BN, kCtas) / 2);
                 for (int k = k0; ok && k < k1; ++k) {
                     ok = tc::mbar_wait(&empty[at], phase ^ 1, &gave_up);
                     if (!ok) break;
                     unsigned char *a = stages + at * L::kStage, *b = a + L::kA;
-                    tc::mbar_expect(&full[at], L::kStage);
+                    if (rank == 0) tc::mbar_expect(&full[at], L::kStage * kCtas);
+                    const uint32_t bar = kPair ? tc::peer_addr(&full[at], 0) : 0;
+                    auto load = [&](unsigned char *dst, const CUtensorMap *map, int x, int y) {
+                        if (kPair)
+                            tc::load_2d_pair(dst, map, bar, x, y);
+                        else
+                            tc::load_2d(dst, map, &full[at], x, y);
+                    };
                     if (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < kBM / 64; ++i)
-                            tc::load_2d(a + i * 8192, &map_a, &full[at], int(m) * kBM + i * 64, k * kBK);
+                        for (int i = 0; i < kBM / 64; ++i) load(a + i * 8192, &map_a, row + i * 64, k * kBK);
                     } else {
-                        tc::load_2d(a, &map_a, &full[at], k * kBK, int(m) * kBM);
+                        load(a, &map_a, k * kBK, row);
                     }
                     if (B_MN) {
 #pragma unroll
-                        for (int i = 0; i < BN / 64; ++i)
-                            tc::load_2d(b + i * 8192, &map_b, &full[at], n * BN + i * 64, k * kBK);
+                        for (int i = 0; i < L::kRowsB / 64; ++i) load(b + i * 8192, &map_b, col + i * 64, k * kBK);
                     } else {
-                        tc::load_2d(b, &map_b, &full[at], k * kBK, n * BN);
+                        load(b, &map_b, k * kBK, col);
                     }
                     started |= 1u << at;
                     if (++at == sh.stages) at = 0, phase ^= 1;
                 }
             }
-            // every load has landed before the CTA's memory goes: the last fill of each stage
-            for (int i = 0; i < sh.stages; ++i) {
+            // every load has landed before the CTA's memory goes: the last fill of each stage (of a pair, the first CTA's
+            // barriers count both CTAs' loads, and the other waits for it at the end)
+            for (int i = 0; rank == 0 && i < sh.stages; ++i) {
                 if (!(started >> i & 1)) continue;
                 const uint32_t last = i < at ? phase : phase ^ 1;
                 const uint64_t since = tc::now_ns();
@@ -374,18 +413,16 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             int at = 0, half = 0;
             uint32_t phase = 0, half_phase = 0;
             bool ok = true;
-            for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+            for (int64_t t = t0; ok && t < total; t += dt) {
                 int64_t m;
                 int n, split;
                 sh.tile(t, m, n, split);
-                // the last tile of a row is as wide as the matrix needs it
-                const int left = (sh.N - n * BN + 15) / 16 * 16;
-                const uint32_t idesc =
-                    tc::instruction(Elt<T>::kBf16 ? 1 : 0, A_MN, B_MN, kBM, left < BN ? left : BN);
+                const uint32_t idesc = tc::instruction(Elt<T>::kBf16 ? 1 : 0, A_MN, B_MN, kBM * kCtas,
+                                                       sh.width(n, BN, kCtas));
                 ok = tc::mbar_wait(&sum_empty[half], half_phase ^ 1, &gave_up);
                 if (!ok) break;
                 tc::fence_after();
@@ -401,16 +438,16 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         // 16 elements of the sum: 32 bytes along a K-major row, 16 rows of an MN-major operand
                         const uint64_t da = tc::operand(a + i * (A_MN ? 2048 : 32), A_MN ? 8192 : 16, 1024);
                         const uint64_t db = tc::operand(b + i * (B_MN ? 2048 : 32), B_MN ? 8192 : 16, 1024);
-                        tc::mma_f16(d, da, db, idesc, k > 0 || i > 0);
+                        tc::mma_f16<kPair>(d, da, db, idesc, k > 0 || i > 0);
                     }
-                    tc::commit(&empty[at]);
+                    tc::commit<kPair>(&empty[at]);
                     if (++at == sh.stages) at = 0, phase ^= 1;
                 }
-                if (ok) tc::commit(&sum_full[half]);
+                if (ok) tc::commit<kPair>(&sum_full[half]);
                 if (++half == 2) half = 0, half_phase ^= 1;
             }
             // every product has left the tensor core before the CTA's memory goes
-            tc::commit(&drained);
+            tc::commit<kPair>(&drained);
             const uint64_t since = tc::now_ns();
             while (!tc::mbar_try(&drained, 0) && tc::now_ns() - since < 2000000000ull) {
             }
@@ -428,11 +465,11 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         const int step = ep.mode == kPart ? 32 : 64;
         const bool ask = BN >= 64 && ep.side && ep.tma_side;
         bool asked = false;
-        for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
+        for (int64_t t = t0; t < total; t += dt) {
             int64_t m;
             int n, split;
             sh.tile(t, m, n, split);
-            const int64_t row0 = m * kBM + quarter * 32;
+            const int64_t row0 = (m * kCtas + rank) * kBM + quarter * 32;
             const int n0 = n * BN;
             const int end = n0 + BN < sh.N ? n0 + BN : sh.N;
             int col = n0 + share * step;
@@ -446,7 +483,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 if (row0 < sh.M) {
                     for (; col < end; col += kShares * step) {
                         const int next = col + kShares * step;
-                        c.piece(d, row0, split * sh.tiles_m * kBM + row0, col, n0, ok, next < end ? next : -1, row0);
+                        c.piece(d, row0, split * sh.part_rows + row0, col, n0, ok, next < end ? next : -1, row0);
                     }
                 }
             } else {
@@ -468,17 +505,25 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             }
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&sum_empty[half]);
+            if (lane == 0) {
+                if (kPair)
+                    tc::mbar_arrive_peer(tc::peer_addr(&sum_empty[half], 0));
+                else
+                    tc::mbar_arrive(&sum_empty[half]);
+            }
             if (++half == 2) half = 0, half_phase ^= 1;
         }
         if (lane == 0) tc::stores_done();
     }
     __syncwarp();
     tc::fence_before();
-    __syncthreads();
+    if (kPair)
+        tc::cluster_sync();
+    else
+        __syncthreads();
     if (warp == 1) {
         tc::fence_after();
-        tc::tmem_free(tmem, L::kColumns);
+        tc::tmem_free<kPair>(tmem, L::kColumns);
     }
 }
 
@@ -549,6 +594,18 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ 
         part[int64_t(blockIdx.y) * cols + mine] = s;
     }
 }
+// Sums of `each` runs at a time.
+__global__ void __launch_bounds__(256)
+column_fold_kernel(const float *__restrict__ part, int64_t runs, int64_t each, int cols, float *__restrict__ out)
+{
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    const int64_t first = blockIdx.y * each, end = first + each < runs ? first + each : runs;
+    if (c >= cols) return;
+    float s = 0.0f;
+#pragma unroll 8
+    for (int64_t i = first; i < end; ++i) s += __ldg(part + i * cols + c);
+    out[int64_t(blockIdx.y) * cols + c] = s;
+}
 // 32 columns a CTA, eight threads each, whose sums are added in order.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -607,22 +664,22 @@ bool make_map(CUtensorMap *map, const void *p, int64_t rows, int64_t cols, int64
 // How a product of M x N outputs and a sum of `len` is cut: the width of its tiles and the parts of its sum.
 struct Cut {
     int bn, splits, steps_per_split;
+    int rows() const { return bn == 256 ? 2 * kBM : kBM; }  // of a tile (of both CTAs of a pair)
+    int64_t tiles(int64_t M, int N) const { return ((M + rows() - 1) / rows()) * ((N + bn - 1) / bn); }
+    int at_once() const { return bn == 256 ? kNumSMs / 2 : kNumSMs; }
 };
 Cut cut_product(int64_t M, int N, int64_t len, bool b_mn)
 {
-    const int64_t tiles_m = (M + kBM - 1) / kBM;
     const int steps = int((len + kBK - 1) / kBK);
     Cut c{256, 1, steps};
     const int least = b_mn ? 64 : 32;
     // narrower tiles until every SM has one
-    while (c.bn > least && (c.bn / 2 >= N || tiles_m * ((N + c.bn - 1) / c.bn) < kNumSMs)) c.bn /= 2;
+    while (c.bn > least && (c.bn / 2 >= N || c.tiles(M, N) < c.at_once())) c.bn /= 2;
     // split long sums of few tiles, at least eight steps a part
-    const int64_t tiles = tiles_m * ((N + c.bn - 1) / c.bn);
-    if (tiles * 2 <= kNumSMs && steps >= 32) {
+    if (c.tiles(M, N) * 2 <= kNumSMs && steps >= 32) {
         // wide tiles again: parts give the SMs their work
-        c.bn = N > 128 ? 256 : (N > 64 ? 128 : 64);
-        const int64_t wide = tiles_m * ((N + c.bn - 1) / c.bn);
-        int64_t parts = kNumSMs / wide;
+        c.bn = N > 128 && M > 128 ? 256 : (N > 64 ? 128 : 64);
+        int64_t parts = c.at_once() / c.tiles(M, N);
         if (parts > steps / 8) parts = steps / 8;
         if (parts < 1) parts = 1;
         c.steps_per_split = int((steps + parts - 1) / parts);
@@ -631,7 +688,7 @@ Cut cut_product(int64_t M, int N, int64_t len, bool b_mn)
     return c;
 }
 // Parts are [splits * rows of whole tiles, N up to a multiple of 8] floats.
-int64_t part_rows(int64_t M) { return align_up(M, kBM); }
+int64_t part_rows(int64_t M) { return align_up(M, 2 * kBM); }
 int64_t part_bytes(int64_t M, int N, const Cut &c)
 {
     return c.splits > 1 ? 4 * c.splits * part_rows(M) * align_up(N, 8) : 0;
@@ -649,7 +706,7 @@ cudaError_t run_product(const Matrix &a, const Matrix &b, Shape sh, const Epilog
     using L = Layout<BN>;
     CUtensorMap ma, mb, mo{}, ms{};
     bool good = make_map<T>(&ma, a.p, a.rows, a.cols, a.ld, A_MN ? kBK : kBM) &&
-                make_map<T>(&mb, b.p, b.rows, b.cols, b.ld, B_MN ? kBK : BN);
+                make_map<T>(&mb, b.p, b.rows, b.cols, b.ld, B_MN ? kBK : L::kRowsB);
     if (ep.mode == kPart)
         good = good && make_map<float>(&mo, ep.out, sh.splits * part_rows(sh.M), sh.N, ep.out_ld, 32);
     else if (ep.tma_out)
@@ -662,9 +719,19 @@ cudaError_t run_product(const Matrix &a, const Matrix &b, Shape sh, const Epilog
     // the attribute belongs to the device that is current
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes(false) > L::bytes(true) ? L::bytes(false) : L::bytes(true));
     if (e != cudaSuccess) return e;
-    const int64_t total = sh.tiles_m * sh.tiles_n * sh.splits;
-    kernel<<<unsigned(total < kNumSMs ? total : kNumSMs), L::kThreads, L::bytes(side), s>>>(ma, mb, mo, ms, sh, ep);
-    return cudaGetLastError();
+    const int ctas = L::kPair ? 2 : 1;
+    const int64_t total = sh.tiles_m * sh.tiles_n * sh.splits * ctas;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(total < kNumSMs ? total : kNumSMs));
+    cfg.blockDim = dim3(L::kThreads);
+    cfg.dynamicSmemBytes = L::bytes(side);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = L::kPair ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, ms, sh, ep);
 }
 
 template <typename T, bool A_MN, bool B_MN>
@@ -683,13 +750,13 @@ cudaError_t run_product_bn(int bn, const Matrix &a, const Matrix &b, const Shape
 template <typename T>
 cudaError_t product(const Matrix &a, const Matrix &b, int64_t M, int N, int64_t len, Epilogue ep, float *part, cudaStream_t s)
 {
-    if (M == 0) return cudaSuccess;
     const Cut c = cut_product(M, N, len, b.mn);
     Shape sh{};
     sh.M = M, sh.N = N;
     sh.steps = int((len + kBK - 1) / kBK);
     sh.steps_per_split = c.steps_per_split, sh.splits = c.splits;
-    sh.tiles_m = (M + kBM - 1) / kBM, sh.tiles_n = (N + c.bn - 1) / c.bn;
+    sh.tiles_m = (M + c.rows() - 1) / c.rows(), sh.tiles_n = (N + c.bn - 1) / c.bn;
+    sh.part_rows = part_rows(M);
     auto on16 = [](const void *p, int64_t ld) {
         return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0);
     };
@@ -746,7 +813,7 @@ LinearPlan plan_linear(const cwrnnt_linear &p, bool backward)
             q.g = take(copy_bytes(p.n_rows, p.n_out, p.g_stride));
         parts = most(parts, part_bytes(p.n_rows, p.n_in, cut_product(p.n_rows, p.n_in, p.n_out, true)));
         parts = most(parts, part_bytes(p.n_out, p.n_in, cut_product(p.n_out, p.n_in, p.n_rows, true)));
-        q.sums = take(4 * int64_t(kMostRuns) * p.n_out);
+        q.sums = take(4 * (kMostRuns + (p.n_rows + 31) / 32) * int64_t(p.n_out));
     }
     q.part = take(parts);
     q.total = at > 0 ? at : 256;
@@ -805,30 +872,42 @@ cudaError_t linear_backward(const cwrnnt_linear &p, const void *x, const void *w
     const bool act = p.activation != CWRNNT_ACT_NONE;
     if (act || grad_w) CWRNNT_TRY(readable<T>(mx, ws + q.x, s));
     if (act || grad_x) CWRNNT_TRY(readable<T>(mw, ws + q.w, s));
+    // column sums: of the epilogue's pieces of 32 rows where it forms dz, else of runs of rows of the matrix
+    float *sums = reinterpret_cast<float *>(ws + q.sums), *folded = sums + (p.n_rows + 31) / 32 * int64_t(p.n_out);
+    int64_t runs = 0;
     if (act) {
         Epilogue ep{};
         ep.mode = kSlope, ep.act = p.activation, ep.bias = bias;
         ep.side = g, ep.side_ld = p.g_stride;
         ep.out = ws + q.dz, ep.out_ld = padded(p.n_out);
+        const Cut c = cut_product(p.n_rows, p.n_out, p.n_in, false);
+        if (grad_b && c.splits == 1 && c.bn >= 64) ep.sums = sums, runs = (p.n_rows + 31) / 32;
         CWRNNT_TRY(product<T>(mx, mw, p.n_rows, p.n_out, p.n_in, ep, part, s));
         dz.p = ws + q.dz, dz.ld = padded(p.n_out);
     } else {
         CWRNNT_TRY(readable<T>(dz, ws + q.g, s));
     }
     if (grad_b) {
-        // runs of rows: enough of them to fill the GPU with CTAs of 256 columns
         const int64_t across = (p.n_out + 255) / 256;
-        int64_t runs = (kNumSMs * 4 + across - 1) / across;
-        const int64_t most = (p.n_rows + 63) / 64;
-        if (runs > most) runs = most;
-        if (runs > kMostRuns) runs = kMostRuns;
-        if (runs < 1) runs = 1;
-        const int64_t run = (p.n_rows + runs - 1) / runs;
-        float *sums = reinterpret_cast<float *>(ws + q.sums);
-        column_sums_kernel<T><<<dim3(unsigned(across), unsigned(runs)), 256, 0, s>>>(
-            static_cast<const T *>(dz.p), dz.ld, p.n_rows, p.n_out, run, sums);
-        CWRNNT_TRY(cudaGetLastError());
-        column_join_kernel<T><<<unsigned((p.n_out + 31) / 32), 256, 0, s>>>(sums, int(runs), p.n_out, static_cast<T *>(grad_b));
+        if (runs == 0) {
+            // enough runs to fill the GPU with CTAs of 256 columns
+            runs = (kNumSMs * 4 + across - 1) / across;
+            const int64_t most = (p.n_rows + 63) / 64;
+            if (runs > most) runs = most;
+            if (runs > kMostRuns) runs = kMostRuns;
+            const int64_t run = (p.n_rows + runs - 1) / runs;
+            column_sums_kernel<T><<<dim3(unsigned(across), unsigned(runs)), 256, 0, s>>>(
+                static_cast<const T *>(dz.p), dz.ld, p.n_rows, p.n_out, run, sums);
+            CWRNNT_TRY(cudaGetLastError());
+        }
+        if (runs > kMostRuns) {
+            const int64_t each = (runs + kMostRuns / 2 - 1) / (kMostRuns / 2), groups = (runs + each - 1) / each;
+            column_fold_kernel<<<dim3(unsigned(across), unsigned(groups)), 256, 0, s>>>(sums, runs, each, p.n_out, folded);
+            CWRNNT_TRY(cudaGetLastError());
+            sums = folded, runs = groups;
+        }
+        column_join_kernel<T><<<unsigned((p.n_out + 31) / 32), 256, 0, s>>>(sums, int(runs), p.n_out,
+                                                                              static_cast<T *>(grad_b));
         CWRNNT_TRY(cudaGetLastError());
     }
     if (grad_x) {

@@ -4,6 +4,8 @@
 // Exports the reference module's three functions with the reference's argument order and result shapes
 // (cwarp_cuda.cpp:138-153) for callers of `cwarp_rnnt._C`, plus the fused entry points the autograd function uses.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -494,6 +496,161 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(const torch::Tensor 
     return {gx, gw, gb};
 }
 
+// ----------------------------------------------------------------------- the operators above as autograd functions
+// (In C++, so that a small step does not spend its time in the interpreter.) None of them is differentiable twice: a
+// gradient that was computed with create_graph raises when it is differentiated.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+variable_list once_differentiable(variable_list grads, const char *name)
+{
+    if (!at::GradMode::is_enabled()) return grads;
+    auto refuse = std::make_shared<torch::autograd::DelayedError>(
+        std::string(name) + " is not differentiable twice", static_cast<int64_t>(grads.size()));
+    for (auto &g : grads)
+        if (g.defined()) g = g.detach().requires_grad_(true);
+    return (*refuse)(std::move(grads));
+}
+OptTensor some(const torch::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+class TokenScoresFn : public torch::autograd::Function<TokenScoresFn> {
+public:
+    // outputs: those of (log_probs, entropy, top_log_probs, top_indices) that were asked for
+    static variable_list forward(AutogradContext *ctx, const torch::Tensor &x, const OptTensor &targets, int64_t top_k,
+                                 bool entropy, double temperature)
+    {
+        auto [lp, ent, top, index, stats] = token_scores(x, targets, top_k, entropy, temperature, true);
+        ctx->save_for_backward({x, targets.value_or(torch::Tensor()), index.value_or(torch::Tensor()), *stats,
+                                ent.value_or(torch::Tensor())});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->set_materialize_grads(false);
+        if (index) ctx->mark_non_differentiable({*index});
+        variable_list out;
+        for (const OptTensor *t : {&lp, &ent, &top, &index})
+            if (*t) out.push_back(**t);
+        return out;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const auto saved = ctx->get_saved_variables();
+        OptTensor up[3];  // in the order of the outputs
+        size_t at = 0;
+        const bool have[3] = {saved[1].defined(), saved[4].defined(), saved[2].defined()};
+        bool any = false;
+        for (int i = 0; i < 3; ++i) {
+            if (!have[i]) continue;
+            if (grads[at].defined()) up[i] = grads[at].detach().contiguous(), any = true;
+            ++at;
+        }
+        variable_list out(5);
+        if (any)
+            out[0] = token_scores_backward(saved[0].detach(), some(saved[1]), some(saved[2]), saved[3], some(saved[4]),
+                                           up[0], up[1], up[2], ctx->saved_data["temperature"].toDouble());
+        return once_differentiable(std::move(out), "token_scores");
+    }
+};
+
+std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> token_scores_ad(const torch::Tensor &x, const OptTensor &targets,
+                                                                       int64_t top_k, bool entropy, double temperature)
+{
+    if (!(at::GradMode::is_enabled() && x.requires_grad())) {
+        auto [lp, ent, top, index, stats] = token_scores(x, targets, top_k, entropy, temperature, false);
+        return {lp, ent, top, index};
+    }
+    auto out = TokenScoresFn::apply(x, targets, top_k, entropy, temperature);
+    size_t at = 0;
+    auto next = [&](bool wanted) { return wanted ? OptTensor(out[at++]) : OptTensor(); };
+    auto lp = next(targets.has_value()), ent = next(entropy), top = next(top_k > 0), index = next(top_k > 0);
+    return {lp, ent, top, index};
+}
+
+class DistillFn : public torch::autograd::Function<DistillFn> {
+public:
+    static torch::Tensor forward(AutogradContext *ctx, const torch::Tensor &x, const torch::Tensor &teacher,
+                                 const torch::Tensor &indices, const OptTensor &weight, bool tail, double temperature,
+                                 double scale, bool reduced, bool eager)
+    {
+        auto [rows, loss, grad] =
+            distill(x, teacher, indices, weight, {}, tail, temperature, scale, !reduced, reduced, reduced && eager);
+        ctx->save_for_backward({x, teacher, indices, weight.value_or(torch::Tensor())});
+        ctx->saved_data["tail"] = tail;
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["scale"] = scale;
+        if (grad) ctx->saved_data["grad"] = *grad;
+        return reduced ? *loss : *rows;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        variable_list out(9);
+        const auto g = grads[0].detach();
+        const auto eager = ctx->saved_data.find("grad");
+        if (eager != ctx->saved_data.end()) {
+            // computed during forward for an upstream gradient of 1; handed over once (a second backward over a
+            // retained graph recomputes it below)
+            out[0] = eager->second.toTensor();
+            ctx->saved_data.erase(eager);
+            if (out[0].numel()) rnnt_scale_grad(out[0], g);
+        } else {
+            const auto saved = ctx->get_saved_variables();
+            out[0] = *std::get<2>(distill(saved[0].detach(), saved[1], saved[2], some(saved[3]), g.contiguous(),
+                                          ctx->saved_data["tail"].toBool(), ctx->saved_data["temperature"].toDouble(),
+                                          ctx->saved_data["scale"].toDouble(), false, false, true));
+        }
+        return once_differentiable(std::move(out), "distill_loss");
+    }
+};
+
+torch::Tensor distill_ad(const torch::Tensor &x, const torch::Tensor &teacher, const torch::Tensor &indices,
+                         const OptTensor &weight, bool tail, double temperature, double scale, bool reduced, bool eager)
+{
+    if (at::GradMode::is_enabled() && x.requires_grad())
+        return DistillFn::apply(x, teacher, indices, weight, tail, temperature, scale, reduced, eager);
+    auto [rows, loss, grad] =
+        distill(x, teacher, indices, weight, {}, tail, temperature, scale, !reduced, reduced, false);
+    return reduced ? *loss : *rows;
+}
+
+class LinearFn : public torch::autograd::Function<LinearFn> {
+public:
+    static torch::Tensor forward(AutogradContext *ctx, const torch::Tensor &x, const torch::Tensor &weight,
+                                 const OptTensor &bias, const OptTensor &residual, int64_t activation)
+    {
+        ctx->save_for_backward({x, weight, bias.value_or(torch::Tensor())});
+        ctx->saved_data["activation"] = activation;
+        ctx->saved_data["residual"] = residual.has_value();
+        return linear_forward(x, weight, bias, residual, activation);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        variable_list out(5);
+        const auto saved = ctx->get_saved_variables();
+        const auto g = grads[0].detach();
+        // (edges are counted over the tensors that were given: the bias is the third if there is one)
+        const bool want[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                              saved[2].defined() && ctx->needs_input_grad(2)};
+        if (want[0] || want[1] || want[2]) {
+            const OptTensor bias = saved[2].defined() ? OptTensor(saved[2].detach()) : OptTensor();
+            auto [gx, gw, gb] = linear_backward(saved[0].detach(), saved[1].detach(), bias, g,
+                                                ctx->saved_data["activation"].toInt(), want[0], want[1], want[2]);
+            if (gx) out[0] = *gx;
+            if (gw) out[1] = *gw;
+            if (gb) out[2] = *gb;
+        }
+        if (ctx->saved_data["residual"].toBool()) out[3] = g;
+        return once_differentiable(std::move(out), "fused_linear");
+    }
+};
+
+torch::Tensor linear_ad(const torch::Tensor &x, const torch::Tensor &weight, const OptTensor &bias,
+                        const OptTensor &residual, int64_t activation)
+{
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) ||
+                                       (residual && residual->requires_grad())))
+        return LinearFn::apply(x, weight, bias, residual, activation);
+    return linear_forward(x, weight, bias, residual, activation);
+}
+
 // ------------------------------------------------------------------- the reference module's functions, same shapes
 
 // cwarp_cuda.cpp:84-108. xs are log-probabilities. Returns (costs [N], grads [STU,2], alphas, betas [N,Tmax,Umax+1]).
@@ -597,11 +754,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("_rnnt_status", &rnnt_status, "Status words of a workspace (synchronises).");
     m.def("_pack_padded", &pack_padded, "Padded [N,T,U+1,V] -> compact [n_rows,V].");
     m.def("_unpack_padded", &unpack_padded, "Compact [n_rows,V] -> zero-padded [N,T,U+1,V].");
-    m.def("_token_scores", &token_scores, "Scores of logits rows: (log_probs, entropy, top_log_probs, top_indices, stats).");
-    m.def("_token_scores_backward", &token_scores_backward, "Gradient of the scores w.r.t. the rows.");
-    m.def("_distill", &distill, "Distillation from a teacher's top entries: (row_loss, loss, grad_x).");
-    m.def("_linear_forward", &linear_forward, "act(x W^T + bias) + residual on the tensor cores.");
-    m.def("_linear_backward", &linear_backward, "Gradients of a linear layer: (grad_x, grad_weight, grad_bias).");
+    m.def("_token_scores", &token_scores_ad,
+          "Scores of logits rows: (log_probs, entropy, top_log_probs, top_indices), differentiable.");
+    m.def("_distill", &distill_ad, "Distillation from a teacher's top entries: the loss, or one per row; differentiable.");
+    m.def("_linear", &linear_ad, "act(x W^T + bias) + residual on the tensor cores, differentiable.");
     m.attr("MAX_LIST") = static_cast<int>(CWRNNT_MAX_LIST);
     m.attr("FUSED_LOG_SOFTMAX") = static_cast<int>(CWRNNT_FUSED_LOG_SOFTMAX);
     m.attr("COSTS_ONLY") = static_cast<int>(CWRNNT_COSTS_ONLY);

@@ -7,42 +7,13 @@ A transducer is distilled the same way with two entries per lattice node: the bl
 else being the rest, weighted by the node posteriors that `analyse` returns. The reference project has no counterpart.
 The CUDA library is mandatory (no CPU or PyTorch fallback).
 """
-from typing import Any, Literal, Optional
+from typing import Literal, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .scores import as_rows, core
 
 __all__ = ["distill_loss"]
-
-
-class _DistillLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, x, teacher, indices, weight, tail, temperature, scale, reduced, eager):
-        ctx.grad_x = None
-        rows, loss, grad = core._distill(x, teacher, indices, weight, None, tail, temperature, scale, not reduced,
-                                         reduced, reduced and eager)
-        ctx.grad_x = grad
-        ctx.save_for_backward(x, teacher, indices, weight)
-        ctx.args = (tail, temperature, scale)
-        return loss if reduced else rows
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, g):
-        if ctx.grad_x is not None:
-            # computed during forward for an upstream gradient of 1; handed over once (a second backward over a
-            # retained graph recomputes it below)
-            grad, ctx.grad_x = ctx.grad_x, None
-            if grad.numel():
-                core._rnnt_scale_grad(grad, g)
-        else:
-            x, teacher, indices, weight = ctx.saved_tensors
-            tail, temperature, scale = ctx.args
-            _, _, grad = core._distill(x, teacher, indices, weight, g.contiguous(), tail, temperature, scale, False,
-                                       False, True)
-        return grad, None, None, None, None, None, None, None, None
 
 
 def distill_loss(x: torch.Tensor, teacher: torch.Tensor, indices: torch.Tensor, *,
@@ -83,10 +54,5 @@ def distill_loss(x: torch.Tensor, teacher: torch.Tensor, indices: torch.Tensor, 
         weight = weight.detach().reshape(n).contiguous()
     reduced = reduction in ("mean", "sum")
     scale = 1.0 / float(mean_denominator or max(n, 1)) if reduction == "mean" else 1.0
-    if rows.requires_grad and torch.is_grad_enabled():
-        out = _DistillLoss.apply(rows, teacher, indices, weight, tail, float(temperature), scale, reduced, eager_grad)
-    else:
-        per_row, loss, _ = core._distill(rows, teacher, indices, weight, None, tail, float(temperature), scale,
-                                         not reduced, reduced, False)
-        out = loss if reduced else per_row
-    return out if reduced else out.reshape(lead)
+    out = core._distill(rows, teacher, indices, weight, tail, temperature, scale, reduced, eager_grad)
+    return out if reduced or len(lead) == 1 else out.reshape(lead)

@@ -9,34 +9,15 @@ refused, `torch.nn.functional.linear` has them). The backward pass keeps nothing
 pre-activations out again and differentiates the activation in that product's epilogue. The reference project leaves
 the layer to its callers. The CUDA library is mandatory (no CPU or PyTorch fallback).
 """
-from typing import Any, Optional
+from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .scores import core
 
 __all__ = ["fused_linear", "LINEAR_ACTIVATIONS"]
 
 LINEAR_ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "tanh": 2, "silu": 3}
-
-
-class _FusedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, x, weight, bias, residual, activation):
-        ctx.save_for_backward(x, weight, bias)
-        ctx.activation = activation
-        return core._linear_forward(x, weight, bias, residual, activation)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, g):
-        x, weight, bias = ctx.saved_tensors
-        want = ctx.needs_input_grad
-        gx = gw = gb = None
-        if want[0] or want[1] or want[2]:
-            gx, gw, gb = core._linear_backward(x, weight, bias, g, ctx.activation, want[0], want[1], want[2])
-        return gx, gw, gb, (g if want[3] else None), None
 
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -55,9 +36,5 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     if residual is not None:
         assert residual.shape == lead + (weight.size(0),)
         residual = residual.reshape(-1, weight.size(0)).contiguous()
-    code = LINEAR_ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rows, weight, bias, residual)):
-        y = _FusedLinear.apply(rows, weight, bias, residual, code)
-    else:
-        y = core._linear_forward(rows, weight, bias, residual, code)
+    y = core._linear(rows, weight, bias, residual, LINEAR_ACTIVATIONS[activation])
     return y if len(lead) == 1 else y.reshape(lead + (weight.size(0),))

@@ -9,10 +9,9 @@ step, and the entries that `distill_loss` takes from a teacher are calls of this
 no counterpart; its callers go through `log_softmax` (test/test.py:19-20). The CUDA library is mandatory (no CPU or
 PyTorch fallback).
 """
-from typing import Any, NamedTuple, Optional
+from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 try:
     from . import _C as core
@@ -33,32 +32,12 @@ class TokenScores(NamedTuple):
 
 def as_rows(x: torch.Tensor) -> torch.Tensor:
     """[..., V] -> [rows, V] with unit column stride, without a copy where the rows lie evenly spaced in memory."""
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     rows = x.reshape(-1, x.size(-1))
     if (rows.size(1) > 1 and rows.stride(1) != 1) or (rows.size(0) > 1 and rows.stride(0) < rows.size(1)):
         rows = rows.contiguous()
     return rows
-
-
-class _TokenScores(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, x, targets, top_k, entropy, temperature):
-        lp, ent, top, index, stats = core._token_scores(x, targets, top_k, entropy, temperature, True)
-        ctx.save_for_backward(x, targets, index, stats, ent)
-        ctx.temperature = temperature
-        ctx.set_materialize_grads(False)
-        if index is not None:
-            ctx.mark_non_differentiable(index)
-        return lp, ent, top, index
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, g_lp, g_ent, g_top, _):
-        x, targets, index, stats, ent = ctx.saved_tensors
-        g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
-        if g_lp is None and g_ent is None and g_top is None:
-            return None, None, None, None, None
-        gx = core._token_scores_backward(x, targets, index, stats, ent, g_lp, g_ent, g_top, ctx.temperature)
-        return gx, None, None, None, None
 
 
 def token_scores(x: torch.Tensor, targets: Optional[torch.Tensor] = None, *, top_k: int = 0, entropy: bool = False,
@@ -81,10 +60,7 @@ def token_scores(x: torch.Tensor, targets: Optional[torch.Tensor] = None, *, top
         assert targets.shape == lead or targets.shape[:-1] == lead, "targets must match the rows of x"
         per_row = targets.size(-1) if targets.dim() > len(lead) else 1
         wanted = targets.reshape(rows.size(0), per_row).contiguous()
-    if rows.requires_grad and torch.is_grad_enabled():
-        lp, ent, top, index = _TokenScores.apply(rows, wanted, top_k, entropy, float(temperature))
-    else:
-        lp, ent, top, index, _ = core._token_scores(rows, wanted, top_k, entropy, float(temperature), False)
+    lp, ent, top, index = core._token_scores(rows, wanted, top_k, entropy, temperature)
     if len(lead) != 1:
         ent = None if ent is None else ent.reshape(lead)
         top, index = (None if t is None else t.reshape(lead + (top_k,)) for t in (top, index))

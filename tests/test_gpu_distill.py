@@ -277,3 +277,14 @@ def test_transducer_distilled_through_the_lattice():
     _, dense = o.fused(case["x"], case["lx"], case["ly"], case["y"], 0, weights=np.full(3, 1.0 / 3))
     # the lattice's own gradient is good to 1e-5 (the parity tests' bound)
     assert (np.abs(x.grad.double().cpu().numpy() - (grad + dense)) <= 1e-5 + 2 * ro.SUM32 * gmag).all()
+
+
+def test_not_differentiable_twice():
+    x, val, idx = _case(14, 6, 50, 2, torch.float32)
+    for reduction in ("mean", "none"):
+        xd = x.to(DEV).requires_grad_(True)
+        loss = distill_loss(xd, val.to(DEV), idx.to(DEV), reduction=reduction)
+        g, = torch.autograd.grad(loss.sum(), [xd], create_graph=True)
+        assert torch.isfinite(g).all()
+        with pytest.raises(RuntimeError, match="twice"):
+            g.sum().backward()

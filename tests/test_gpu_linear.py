@@ -296,3 +296,12 @@ def test_joint_linear_loss_chain(oracle):
     _check(h2.cpu(), W2.cpu(), b2.cpu(), None, logits.grad.cpu(), None, "bf16", logits, (h2.grad, W2.grad, b2.grad, None))
     costs, _ = oracle.fused(_np(logits), case["lx"], case["ly"], case["y"], 0, weights=np.full(3, 1.0 / 3))
     assert abs(float(loss.detach()) - costs.mean()) <= 1e-5 * abs(costs.mean())
+
+
+def test_not_differentiable_twice():
+    x, w, b, r, _ = (t.to(DEV) for t in _case(13, 20, 16, 24, "bf16"))
+    xl = x.requires_grad_(True)
+    g, = torch.autograd.grad(fused_linear(xl, w, b, r, activation="tanh").float().sum(), [xl], create_graph=True)
+    assert torch.isfinite(g).all()
+    with pytest.raises(RuntimeError, match="twice"):
+        g.float().sum().backward()

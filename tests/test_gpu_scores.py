@@ -277,3 +277,11 @@ def test_rows_beyond_32_bit_offsets():
     last = type(got)(*(None if v is None else v[-4:] for v in got))
     _check(tail, None, 3, 1.0, last)
     assert got.top_indices[:-4].cpu().tolist() == [[0, 1, 2]] * (R - 4)
+
+
+def test_not_differentiable_twice():
+    x = _logits(9, 4, 60, torch.float32).to(DEV).requires_grad_(True)
+    g, = torch.autograd.grad(token_scores(x, entropy=True).entropy.sum(), [x], create_graph=True)
+    assert torch.isfinite(g).all()
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
