@@ -16,6 +16,8 @@
 #include "cwrnnt_kernels.h"
 #include "cwrnnt_tc.cuh"
 
+#include <cstddef>
+
 namespace cwrnnt {
 
 namespace {
@@ -77,30 +79,20 @@ struct Epilogue {
     float *sums;             // kSlope: sums over each 32 rows of dz, [rows / 32, N], or null
 };
 
-// Eight consecutive elements of the product become eight of the output: bias, then the activation (plus the residual) or
-// the upstream gradient times the activation's slope.
-template <typename T>
-__device__ __forceinline__ void finish(const Epilogue &ep, float (&v)[8], const float (&side)[8])
+// What becomes of an element of the product once the bias is added: an activation, or (kSlopeOf + activation) the upstream
+// gradient times the activation's slope.
+constexpr int kSlopeOf = 8;
+template <int KIND, bool SIDE>
+__device__ __forceinline__ float finish(float v, float side)
 {
-    if (ep.mode == kSlope) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = side[c] * slope(ep.act, v[c]);
-        return;
-    }
-    if (ep.act == CWRNNT_ACT_RELU) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = activate(CWRNNT_ACT_RELU, v[c]);
-    } else if (ep.act == CWRNNT_ACT_TANH) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = activate(CWRNNT_ACT_TANH, v[c]);
-    } else if (ep.act == CWRNNT_ACT_SILU) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = activate(CWRNNT_ACT_SILU, v[c]);
-    }
-    if (ep.side) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] += side[c];
-    }
+    if (KIND >= kSlopeOf) return side * slope(KIND - kSlopeOf, v);
+    v = activate(KIND, v);
+    return SIDE ? v + side : v;
+}
+__device__ __forceinline__ float finish_as(const Epilogue &ep, float v, float side)
+{
+    if (ep.mode == kSlope) return side * slope(ep.act, v);
+    return activate(ep.act, v) + side;
 }
 
 // Columns [col, col + 8) of one row straight from and to global memory, `n` of them inside the matrix.
@@ -123,7 +115,8 @@ __device__ __forceinline__ void finish_in_place(const Epilogue &ep, float (&v)[8
             for (int c = 0; c < 8; ++c) s[c] = c < n ? E::to_acc(__ldg(side + c)) : 0.0f;
         }
     }
-    finish<T>(ep, v, s);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = finish_as(ep, v[c], s[c]);
     T *out = static_cast<T *>(ep.out) + row * ep.out_ld + col;
     if (ep.vec) {
         *reinterpret_cast<uint4 *>(out) = E::pack(v);
@@ -171,6 +164,16 @@ struct Shape {
 // buffer of its own, in the swizzle of the TMA copies: 16-byte group j of row r lies at group j ^ (r & 7), so that neither
 // a thread's row nor a row of the warp meets bank conflicts.
 constexpr int kPiece = 32 * 128;
+constexpr int kMostCarriers = 8;
+
+// The kernel's shared memory behind the stages and the pieces.
+struct Control {
+    uint64_t full[kMaxStages], empty[kMaxStages], sum_full[2], sum_empty[2], drained, side_full[kMostCarriers];
+    uint32_t tmem_slot;
+    int gave_up;
+    float bias[kMostCarriers][64];
+};
+static_assert(offsetof(Control, bias) % 16 == 0, "read in vectors");
 template <int BN>
 struct Layout {
     // the widest tiles are shared by two CTAs: 256 rows, half of them and half of the columns' operand in each
@@ -180,13 +183,15 @@ struct Layout {
     static constexpr int kCarriers = BN >= 128 ? 8 : 4;  // warps of the epilogue
     static constexpr int kThreads = 64 + 32 * kCarriers;
     static constexpr uint32_t kColumns = 2 * BN;         // two sums in TMEM
-    static constexpr int kRoom = 227 * 1024 - 4096 - 1024;  // shared memory but for the static part and the alignment
     static constexpr int stages(bool side)
     {
-        const int n = (kRoom - kCarriers * kPiece * (side ? 2 : 1)) / kStage;
+        const int n = (227 * 1024 - int(sizeof(Control)) - kCarriers * kPiece * (side ? 2 : 1)) / kStage;
         return n < kMaxStages ? n : kMaxStages;
     }
-    static constexpr int bytes(bool side) { return 1024 + stages(side) * kStage + kCarriers * kPiece * (side ? 2 : 1); }
+    static constexpr int bytes(bool side)
+    {
+        return stages(side) * kStage + kCarriers * kPiece * (side ? 2 : 1) + int(sizeof(Control));
+    }
 };
 
 __device__ __forceinline__ uint4 *piece_group(unsigned char *piece, int row, int group)
@@ -194,94 +199,144 @@ __device__ __forceinline__ uint4 *piece_group(unsigned char *piece, int row, int
     return reinterpret_cast<uint4 *>(piece + row * 128 + ((group ^ (row & 7)) << 4));
 }
 
-// One warp's share of one tile. `d`: TMEM address of the sum's first column in this warp's lanes.
-template <typename T, int BN>
+// One warp's share of the tiles: 32 rows, by pieces of 64 columns (32 of a part). What a piece needs from global memory
+// (upstream gradient or residual by TMA, the bias in registers) is asked for one piece ahead, and the sums are given
+// back to the products as soon as they are read. The piece's arithmetic is compiled for each kind of epilogue: with
+// branches between its eight-column groups two warps per scheduler could not hide its latencies (measured on the
+// Conformer logits: 0.40 ms that way).
+template <typename T>
 struct Carrier {
     using E = Elt<T>;
     const Epilogue &ep;
-    const Shape &sh;
+    const int64_t M;
+    const int N;
     const CUtensorMap *map_out, *map_side;
     unsigned char *out_piece, *side_piece;
-    float *bias;  // 64 floats
+    float *bias;  // 64 of them
     uint64_t *side_bar;
     volatile int *gave_up;
     uint32_t side_phase;
     int lane;
+    float next_bias[2];
 
-    __device__ __forceinline__ void ask_side(int64_t row0, int col)
+    // what the piece at (row0, col) needs
+    __device__ __forceinline__ void ask(int row0, int col)
     {
-        if (lane == 0) {
+        if (ep.side && ep.tma_side && lane == 0) {
             tc::mbar_expect(side_bar, kPiece);
-            tc::load_2d(side_piece, map_side, side_bar, col, int(row0));
+            tc::load_2d(side_piece, map_side, side_bar, col, row0);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = col + h * 32 + lane;
+            next_bias[h] = ep.bias && c < N ? E::to_acc(__ldg(static_cast<const T *>(ep.bias) + c)) : 0.0f;
         }
     }
-    // 64 columns from `col` on (32 of a part)
-    __device__ __forceinline__ void piece(uint32_t d, int64_t row0, int64_t out_row0, int col, int n0, bool ok,
-                                          int next_col, int64_t next_row0)
+    template <int KIND, bool SIDE, typename Release>
+    __device__ __forceinline__ void columns(uint32_t d, int row0, int next_col, bool ok, Release &release)
     {
-        const bool part = ep.mode == kPart;
-        if (!part && ep.bias) {
-            const T *b = static_cast<const T *>(ep.bias);
-            bias[lane] = col + lane < sh.N ? E::to_acc(__ldg(b + col + lane)) : 0.0f;
-            bias[32 + lane] = col + 32 + lane < sh.N ? E::to_acc(__ldg(b + col + 32 + lane)) : 0.0f;
-        }
+        uint32_t r[2][32];
+        tc::tmem_load32(d, r[0]);
+        tc::tmem_load32(d + 32, r[1]);
         uint4 side[8];
-        if (ep.side) {
-            if (ep.tma_side) {
-                ok = tc::mbar_wait(side_bar, side_phase, gave_up) && ok;
-                side_phase ^= 1;
-            } else {
-                // rows off the boundaries: each row of the piece as 64 consecutive elements
-                T *s = reinterpret_cast<T *>(side_piece);
-                for (int r = 0; r < 32; ++r)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int c = h * 32 + lane;
-                        T v = E::from_acc(0.0f);
-                        if (row0 + r < sh.M && col + c < sh.N)
-                            v = __ldg(static_cast<const T *>(ep.side) + (row0 + r) * ep.side_ld + col + c);
-                        s[r * 64 + (((c >> 3) ^ (r & 7)) << 3) + (c & 7)] = v;
-                    }
-                __syncwarp();
-            }
+        if (SIDE) {
 #pragma unroll
             for (int g = 0; g < 8; ++g) side[g] = *piece_group(side_piece, lane, g);
-            __syncwarp();
-            if (ep.tma_side && next_col >= 0) ask_side(next_row0, next_col);
         }
-        if (lane == 0) tc::stores_read();
+        tc::tmem_load_wait();
         __syncwarp();
+        if (next_col >= 0)
+            ask(row0, next_col);
+        else
+            release();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            if (part && half) break;
-            uint32_t r[32];
-            tc::tmem_load32(d + uint32_t(col - n0 + half * 32), r);
-            tc::tmem_load_wait();
-            if (part) {
+        for (int g = 0; g < 8; ++g) {
+            float v[8], s[8] = {};
+            const float4 b0 = *reinterpret_cast<const float4 *>(bias + g * 8);
+            const float4 b1 = *reinterpret_cast<const float4 *>(bias + g * 8 + 4);
+            const float b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+            if (SIDE) E::unpack(side[g], s);
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    uint4 w = make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
-                    if (!ok) w = make_uint4(0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u);
-                    *piece_group(out_piece, lane, g) = w;
+            for (int i = 0; i < 8; ++i)
+                v[i] = finish<KIND, SIDE>(__uint_as_float(r[g / 4][g % 4 * 8 + i]) + b[i], s[i]);
+            uint4 w = E::pack(v);
+            if (!ok) w = make_uint4(~0u, ~0u, ~0u, ~0u);  // a wait that ran out leaves NaN
+            *piece_group(out_piece, lane, g) = w;
+        }
+    }
+    template <typename Release>
+    __device__ __forceinline__ void columns_of_part(uint32_t d, int row0, int next_col, bool ok, Release &release)
+    {
+        uint32_t r[32];
+        tc::tmem_load32(d, r);
+        tc::tmem_load_wait();
+        __syncwarp();
+        if (next_col < 0) release();
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+            uint4 w = make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
+            if (!ok) w = make_uint4(~0u, ~0u, ~0u, ~0u);
+            *piece_group(out_piece, lane, g) = w;
+        }
+    }
+    // `d`: TMEM address of the piece's first column in this warp's lanes; `release`: gives the tile's sums back
+    template <typename Release>
+    __device__ __forceinline__ void piece(uint32_t d, int row0, int64_t out_row0, int col, bool ok, int next_col,
+                                          Release &release)
+    {
+        if (ep.mode != kPart) {
+            bias[lane] = next_bias[0], bias[32 + lane] = next_bias[1];
+            if (ep.side) {
+                if (ep.tma_side) {
+                    ok = tc::mbar_wait(side_bar, side_phase, gave_up) && ok;
+                    side_phase ^= 1;
+                } else {
+                    // rows off the boundaries: each row of the piece as 64 consecutive elements
+                    T *s = reinterpret_cast<T *>(side_piece);
+                    for (int r = 0; r < 32; ++r)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int c = h * 32 + lane;
+                            T v = E::from_acc(0.0f);
+                            if (row0 + r < M && col + c < N)
+                                v = __ldg(static_cast<const T *>(ep.side) + int64_t(row0 + r) * ep.side_ld + col + c);
+                            s[r * 64 + (((c >> 3) ^ (r & 7)) << 3) + (c & 7)] = v;
+                        }
                 }
-                continue;
-            }
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float v[8], s[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = ok ? __uint_as_float(r[g * 8 + i]) : NAN;
-                if (ep.bias) {
-                    const float4 b0 = *reinterpret_cast<const float4 *>(bias + half * 32 + g * 8);
-                    const float4 b1 = *reinterpret_cast<const float4 *>(bias + half * 32 + g * 8 + 4);
-                    v[0] += b0.x, v[1] += b0.y, v[2] += b0.z, v[3] += b0.w;
-                    v[4] += b1.x, v[5] += b1.y, v[6] += b1.z, v[7] += b1.w;
-                }
-                if (ep.side) E::unpack(side[half * 4 + g], s);
-                finish<T>(ep, v, s);
-                *piece_group(out_piece, lane, half * 4 + g) = E::pack(v);
             }
         }
+        if (lane == 0) tc::stores_read();  // the last piece has left the buffer
+        __syncwarp();
+#define CWRNNT_KIND(KIND, SIDE) columns<KIND, SIDE>(d, row0, next_col, ok, release)
+        if (ep.mode == kPart) {
+            columns_of_part(d, row0, next_col, ok, release);
+        } else if (ep.mode == kSlope) {
+            if (ep.act == CWRNNT_ACT_RELU)
+                CWRNNT_KIND(kSlopeOf + CWRNNT_ACT_RELU, true);
+            else if (ep.act == CWRNNT_ACT_TANH)
+                CWRNNT_KIND(kSlopeOf + CWRNNT_ACT_TANH, true);
+            else
+                CWRNNT_KIND(kSlopeOf + CWRNNT_ACT_SILU, true);
+        } else if (ep.side) {
+            if (ep.act == CWRNNT_ACT_NONE)
+                CWRNNT_KIND(CWRNNT_ACT_NONE, true);
+            else if (ep.act == CWRNNT_ACT_RELU)
+                CWRNNT_KIND(CWRNNT_ACT_RELU, true);
+            else if (ep.act == CWRNNT_ACT_TANH)
+                CWRNNT_KIND(CWRNNT_ACT_TANH, true);
+            else
+                CWRNNT_KIND(CWRNNT_ACT_SILU, true);
+        } else {
+            if (ep.act == CWRNNT_ACT_NONE)
+                CWRNNT_KIND(CWRNNT_ACT_NONE, false);
+            else if (ep.act == CWRNNT_ACT_RELU)
+                CWRNNT_KIND(CWRNNT_ACT_RELU, false);
+            else if (ep.act == CWRNNT_ACT_TANH)
+                CWRNNT_KIND(CWRNNT_ACT_TANH, false);
+            else
+                CWRNNT_KIND(CWRNNT_ACT_SILU, false);
+        }
+#undef CWRNNT_KIND
         if (ep.tma_out) tc::fence_async();
         __syncwarp();
         if (ep.tma_out && lane == 0) tc::store_2d(map_out, out_piece, col, int(out_row0));
@@ -295,9 +350,9 @@ struct Carrier {
                 E::unpack(make_uint4(w, 0u, 0u, 0u), v);
                 s0 += v[0], s1 += v[1];
             }
-            float *to = ep.sums + (row0 / 32) * sh.N + col + 2 * lane;
-            if (col + 2 * lane < sh.N) to[0] = s0;
-            if (col + 2 * lane + 1 < sh.N) to[1] = s1;
+            float *to = ep.sums + int64_t(row0 / 32) * N + col + 2 * lane;
+            if (col + 2 * lane < N) to[0] = s0;
+            if (col + 2 * lane + 1 < N) to[1] = s1;
         }
         if (!ep.tma_out) {
             const T *o = reinterpret_cast<const T *>(out_piece);
@@ -305,29 +360,29 @@ struct Carrier {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int c = h * 32 + lane;
-                    if (row0 + k < sh.M && col + c < sh.N)
-                        static_cast<T *>(ep.out)[(row0 + k) * ep.out_ld + col + c] =
+                    if (row0 + k < M && col + c < N)
+                        static_cast<T *>(ep.out)[int64_t(row0 + k) * ep.out_ld + col + c] =
                             o[k * 64 + (((c >> 3) ^ (k & 7)) << 3) + (c & 7)];
                 }
-            __syncwarp();
         }
+        __syncwarp();
     }
 };
 
 template <typename T, int BN, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(Layout<BN>::kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-              const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_side, const Shape sh,
-              const Epilogue ep)
+              const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_side,
+              const __grid_constant__ Shape sh, const __grid_constant__ Epilogue ep)
 {
     using L = Layout<BN>;
-    extern __shared__ unsigned char raw[];
-    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], sum_full[2], sum_empty[2], drained;
-    __shared__ uint64_t side_full[L::kCarriers];
-    __shared__ __align__(16) float bias[L::kCarriers][64];
-    __shared__ uint32_t tmem_slot;
-    __shared__ int gave_up;
-    unsigned char *stages = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    // stages, pieces, control: the stages start on a 1024-byte boundary, as the swizzle wants it
+    extern __shared__ __align__(1024) unsigned char stages[];
+    unsigned char *const pieces = stages + sh.stages * L::kStage;
+    Control &ctl = *reinterpret_cast<Control *>(pieces + L::kCarriers * kPiece * (ep.side ? 2 : 1));
+    uint64_t *const full = ctl.full, *const empty = ctl.empty;
+    uint64_t *const sum_full = ctl.sum_full, *const sum_empty = ctl.sum_empty;
+    const bool placed = (tc::smem_addr(stages) & 1023) == 0;  // else every role gives up at once
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr bool kPair = L::kPair;
     constexpr int kCtas = kPair ? 2 : 1;
@@ -343,14 +398,14 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             tc::mbar_init(&sum_full[i], 1);
             tc::mbar_init(&sum_empty[i], L::kCarriers * kCtas);
         }
-        for (int i = 0; i < L::kCarriers; ++i) tc::mbar_init(&side_full[i], 1);
-        tc::mbar_init(&drained, 1);
-        gave_up = 0;
+        for (int i = 0; i < L::kCarriers; ++i) tc::mbar_init(&ctl.side_full[i], 1);
+        tc::mbar_init(&ctl.drained, 1);
+        ctl.gave_up = !placed;
         tc::mbar_init_fence();
         tc::prefetch_map(&map_a);
         tc::prefetch_map(&map_b);
     }
-    if (warp == 1) tc::tmem_alloc<kPair>(&tmem_slot, L::kColumns);
+    if (warp == 1) tc::tmem_alloc<kPair>(&ctl.tmem_slot, L::kColumns);
     __syncwarp();
     tc::fence_before();
     if (kPair)
@@ -358,14 +413,14 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     else
         __syncthreads();
     tc::fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = ctl.tmem_slot;
     const int64_t total = sh.tiles();
 
     if (warp == 0) {
         if (lane == 0) {
             int at = 0;
             uint32_t phase = 0;
-            bool ok = true;
+            bool ok = placed;
             uint32_t started = 0;  // stages loaded at least once
             for (int64_t t = t0; ok && t < total; t += dt) {
                 int64_t m;
@@ -375,7 +430,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 const int row = (int(m) * kCtas + rank) * kBM;
                 const int col = n * BN + rank * (sh.width(n, BN, kCtas) / 2);
                 for (int k = k0; ok && k < k1; ++k) {
-                    ok = tc::mbar_wait(&empty[at], phase ^ 1, &gave_up);
+                    ok = tc::mbar_wait(&empty[at], phase ^ 1, &ctl.gave_up);
                     if (!ok) break;
                     unsigned char *a = stages + at * L::kStage, *b = a + L::kA;
                     if (rank == 0) tc::mbar_expect(&full[at], L::kStage * kCtas);
@@ -416,20 +471,20 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         if (lane == 0 && rank == 0) {
             int at = 0, half = 0;
             uint32_t phase = 0, half_phase = 0;
-            bool ok = true;
+            bool ok = placed;
             for (int64_t t = t0; ok && t < total; t += dt) {
                 int64_t m;
                 int n, split;
                 sh.tile(t, m, n, split);
                 const uint32_t idesc = tc::instruction(Elt<T>::kBf16 ? 1 : 0, A_MN, B_MN, kBM * kCtas,
                                                        sh.width(n, BN, kCtas));
-                ok = tc::mbar_wait(&sum_empty[half], half_phase ^ 1, &gave_up);
+                ok = tc::mbar_wait(&sum_empty[half], half_phase ^ 1, &ctl.gave_up);
                 if (!ok) break;
                 tc::fence_after();
                 const uint32_t d = tmem + uint32_t(half * BN);
                 const int steps = sh.count_steps(split);
                 for (int k = 0; ok && k < steps; ++k) {
-                    ok = tc::mbar_wait(&full[at], phase, &gave_up);
+                    ok = tc::mbar_wait(&full[at], phase, &ctl.gave_up);
                     if (!ok) break;
                     tc::fence_after();
                     const uint32_t a = tc::smem_addr(stages + at * L::kStage), b = a + L::kA;
@@ -447,9 +502,9 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 if (++half == 2) half = 0, half_phase ^= 1;
             }
             // every product has left the tensor core before the CTA's memory goes
-            tc::commit<kPair>(&drained);
+            tc::commit<kPair>(&ctl.drained);
             const uint64_t since = tc::now_ns();
-            while (!tc::mbar_try(&drained, 0) && tc::now_ns() - since < 2000000000ull) {
+            while (!tc::mbar_try(&ctl.drained, 0) && tc::now_ns() - since < 2000000000ull) {
             }
         }
     } else {
@@ -458,39 +513,47 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         constexpr int kShares = L::kCarriers / 4;
         int half = 0;
         uint32_t half_phase = 0;
-        unsigned char *pieces = stages + sh.stages * L::kStage;
-        Carrier<T, BN> c{ep, sh, &map_out, &map_side, pieces + carrier * kPiece,
-                         pieces + (L::kCarriers + carrier) * kPiece, bias[carrier], &side_full[carrier], &gave_up, 0,
-                         lane};
+        Carrier<T> c{ep, sh.M, sh.N, &map_out, &map_side, pieces + carrier * kPiece,
+                     pieces + (L::kCarriers + carrier) * kPiece, ctl.bias[carrier], &ctl.side_full[carrier], &ctl.gave_up,
+                     0, lane, {}};
         const int step = ep.mode == kPart ? 32 : 64;
-        const bool ask = BN >= 64 && ep.side && ep.tma_side;
-        bool asked = false;
         for (int64_t t = t0; t < total; t += dt) {
             int64_t m;
             int n, split;
             sh.tile(t, m, n, split);
-            const int64_t row0 = (m * kCtas + rank) * kBM + quarter * 32;
+            const int row0 = int(m * kCtas + rank) * kBM + quarter * 32;
             const int n0 = n * BN;
             const int end = n0 + BN < sh.N ? n0 + BN : sh.N;
             int col = n0 + share * step;
-            if (ask && !asked && col < end && row0 < sh.M) c.ask_side(row0, col);
-            asked = false;
-            const bool ok = tc::mbar_wait(&sum_full[half], half_phase, &gave_up);
+            const bool mine = row0 < sh.M && col < end;
+            if (BN >= 64 && mine) c.ask(row0, col);
+            const bool ok = tc::mbar_wait(&sum_full[half], half_phase, &ctl.gave_up);
             tc::fence_after();
             __syncwarp();
             const uint32_t d = tmem + uint32_t(half * BN) + (uint32_t(quarter * 32) << 16);
+            auto release = [&] {  // this half of TMEM is free for another tile's sums
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (kPair)
+                        tc::mbar_arrive_peer(tc::peer_addr(&sum_empty[half], 0));
+                    else
+                        tc::mbar_arrive(&sum_empty[half]);
+                }
+            };
             if constexpr (BN >= 64) {
-                if (row0 < sh.M) {
-                    for (; col < end; col += kShares * step) {
-                        const int next = col + kShares * step;
-                        c.piece(d, row0, split * sh.part_rows + row0, col, n0, ok, next < end ? next : -1, row0);
-                    }
+                if (!mine) release();
+                for (; mine && col < end; col += kShares * step) {
+                    const int next = col + kShares * step;
+                    c.piece(d + uint32_t(col - n0), row0, split * sh.part_rows + row0, col, ok, next < end ? next : -1,
+                            release);
                 }
             } else {
                 const int64_t row = row0 + lane;
                 uint32_t r[32];
                 tc::tmem_load32(d, r);
                 tc::tmem_load_wait();
+                release();
                 if (row < sh.M) {
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
@@ -502,14 +565,6 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         finish_in_place<T>(ep, v, row, n0 + g * 8, left < 8 ? left : 8);
                     }
                 }
-            }
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (kPair)
-                    tc::mbar_arrive_peer(tc::peer_addr(&sum_empty[half], 0));
-                else
-                    tc::mbar_arrive(&sum_empty[half]);
             }
             if (++half == 2) half = 0, half_phase ^= 1;
         }
