@@ -114,7 +114,7 @@ __device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, in
         const A w = m == A(-INFINITY) ? A(0) : M::exp2_of((z - m) * A(kLog2e));
         const A s = entry_sum<LPR>(w, KP);
         en.lq = s == A(0) ? A(-INFINITY) : z - m - M::ln_of(s);
-        en.q = s == A(0) ? A(0) : w / s;
+        en.q = s == A(0) ? A(0) : M::ratio(w, s);
         en.sum_q = s == A(0) ? A(0) : s / s;
         en.left = A(0);
     }
@@ -191,7 +191,7 @@ __device__ __forceinline__ RowResult<A> solve_row(const RowStats<A> &st, const E
         const A ln_rest = (st.max - all_max) * inv_tau + (M::ln_of(rest_sum) - ln_s);
         q_rest = en.left;
         q_all = en.sum_q + q_rest;
-        p_rest = rest_sum * M::exp2_of((st.max - all_max) * kappa) / all_sum;
+        p_rest = rest_sum * M::exp2_of((st.max - all_max) * kappa) * M::ratio(A(1), all_sum);
         if (q_rest > A(0)) each += q_rest * (M::ln_of(q_rest) - ln_rest);
     }
     A up = gain * weight * inv_tau;
@@ -201,12 +201,12 @@ __device__ __forceinline__ RowResult<A> solve_row(const RowStats<A> &st, const E
     RowResult<A> res;
     res.loss = weight == A(0) ? A(0) : weight * each;
     res.all_top = nothing ? A(0) : all_max;
-    res.all_factor = nothing && !en.bad ? A(0) : up * q_all / all_sum;
+    res.all_factor = nothing && !en.bad ? A(0) : M::ratio(up * q_all, all_sum);
     res.q_factor = up;
     if (TAIL) {
         // (Q p_rest - q_rest) / p_rest p_j, with p_j / p_rest taken from the rest's own sum
         res.top = st.max == A(-INFINITY) ? A(0) : st.max;
-        res.factor = st.nothing() ? (en.bad ? A(NAN) : A(0)) : up * (q_all * p_rest - q_rest) / rest_sum;
+        res.factor = st.nothing() ? (en.bad ? A(NAN) : A(0)) : M::ratio(up * (q_all * p_rest - q_rest), rest_sum);
     } else {
         res.top = res.all_top, res.factor = res.all_factor;
     }
@@ -499,10 +499,14 @@ int64_t launch_distill_t(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 {
     constexpr int VE = Elt<T>::VE;
     const int nv = ALIGNED ? a.V / VE : (a.V + 2 * VE - 2) / VE;
+    // Few lanes a row, many elements a lane: what a row costs beside its elements (about 600 instructions of a warp) is
+    // shared by the rows of a warp. 64 elements a lane is what registers hold; every entry has a lane.
     if constexpr (sizeof(T) <= 4) {
-        if (nv <= 16 && a.K <= 4) return launch_distill_rows<T, 4, 4, ALIGNED>(a, tail, s);
-        if (nv <= 32 && a.K <= 8) return launch_distill_rows<T, 8, 4, ALIGNED>(a, tail, s);
-        if (nv <= 64 && a.K <= 16) return launch_distill_rows<T, 16, 4, ALIGNED>(a, tail, s);
+        constexpr int NV = 64 / VE;
+        if (nv <= 4 * NV && a.K <= 4) return launch_distill_rows<T, 4, NV, ALIGNED>(a, tail, s);
+        if (nv <= 8 * NV && a.K <= 8) return launch_distill_rows<T, 8, NV, ALIGNED>(a, tail, s);
+        if (nv <= 16 * NV && a.K <= 16) return launch_distill_rows<T, 16, NV, ALIGNED>(a, tail, s);
+        if (nv <= 64) return launch_distill_rows<T, 32, 2, ALIGNED>(a, tail, s);
     }
     if (nv <= 128) return launch_distill_rows<T, 32, 4, ALIGNED>(a, tail, s);
     if (nv <= 256) return launch_distill_rows<T, 32, 8, ALIGNED>(a, tail, s);

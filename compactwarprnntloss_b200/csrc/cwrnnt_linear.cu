@@ -582,6 +582,80 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     }
 }
 
+// A few rows of x (a decoding step): one warp per COLS output columns, all rows at once, the weights read once and straight
+// from memory. Tiles of 128 rows would multiply zeros, and their set-up takes longer than this product
+// (8 x 1024 x 640 bf16: 5.2 against 8.4 us). kFewRows rows are the most that one pass carries; a second dimension of
+// CTAs carries more. Four columns a warp read x a quarter as often, where there are columns enough for all SMs.
+constexpr int kFewRows = 8;
+constexpr int kRowsAtMost = 16;  // products of more rows take tiles
+template <typename T, bool VEC, int COLS>
+__global__ void __launch_bounds__(256)
+few_rows_kernel(const T *__restrict__ x, int64_t x_ld, const T *__restrict__ w, int64_t w_ld, int M, int N, int K,
+                const __grid_constant__ Epilogue ep)
+{
+    using E = Elt<T>;
+    const int lane = threadIdx.x & 31, n0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * COLS, m0 = blockIdx.y * kFewRows;
+    if (n0 >= N) return;
+    const int rows = M - m0 < kFewRows ? M - m0 : kFewRows;
+    const T *wn[COLS], *xm = x + int64_t(m0) * x_ld;
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) wn[j] = w + int64_t(n0 + j < N ? n0 + j : n0) * w_ld;
+    float sum[COLS][kFewRows] = {};
+    constexpr int kStep = VEC ? 8 : 1;
+#pragma unroll 2
+    for (int k = lane * kStep; k < K; k += 32 * kStep) {
+        float a[COLS][kStep], b[kStep];
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) {
+            if constexpr (VEC)
+                E::unpack(__ldg(reinterpret_cast<const uint4 *>(wn[j] + k)), a[j]);
+            else
+                a[j][0] = E::to_acc(__ldg(wn[j] + k));
+        }
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r) {
+            if (r < rows) {
+                if constexpr (VEC)
+                    E::unpack(__ldg(reinterpret_cast<const uint4 *>(xm + r * x_ld + k)), b);
+                else
+                    b[0] = E::to_acc(__ldg(xm + r * x_ld + k));
+#pragma unroll
+                for (int j = 0; j < COLS; ++j)
+#pragma unroll
+                    for (int i = 0; i < kStep; ++i) sum[j][r] = fmaf(a[j][i], b[i], sum[j][r]);
+            }
+        }
+    }
+    float mine = 0.0f;  // lane j * kFewRows + r keeps column j of row r
+#pragma unroll
+    for (int j = 0; j < COLS; ++j)
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum[j][r] += __shfl_xor_sync(0xffffffffu, sum[j][r], o);
+            if (lane == j * kFewRows + r) mine = sum[j][r];
+        }
+    const int n = n0 + lane / kFewRows, r = lane % kFewRows;
+    if (lane < COLS * kFewRows && r < rows && n < N) {
+        const int64_t row = m0 + r;
+        if (ep.bias) mine += E::to_acc(__ldg(static_cast<const T *>(ep.bias) + n));
+        const float side = ep.side ? E::to_acc(__ldg(static_cast<const T *>(ep.side) + row * ep.side_ld + n)) : 0.0f;
+        static_cast<T *>(ep.out)[row * ep.out_ld + n] = E::from_acc(finish_as(ep, mine, side));
+    }
+}
+template <typename T, int COLS>
+cudaError_t run_few_rows(const T *x, int64_t x_ld, const T *w, int64_t w_ld, int M, int N, int K, const Epilogue &ep,
+                         cudaStream_t s)
+{
+    const dim3 grid(unsigned((N + 8 * COLS - 1) / (8 * COLS)), unsigned((M + kFewRows - 1) / kFewRows));
+    auto even = [](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
+    if (K % 8 == 0 && even(x, x_ld) && even(w, w_ld))
+        few_rows_kernel<T, true, COLS><<<grid, 256, 0, s>>>(x, x_ld, w, w_ld, M, N, K, ep);
+    else
+        few_rows_kernel<T, false, COLS><<<grid, 256, 0, s>>>(x, x_ld, w, w_ld, M, N, K, ep);
+    return cudaGetLastError();
+}
+
 // The parts of a split sum, added in their order, and the epilogue.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -716,6 +790,9 @@ bool make_map(CUtensorMap *map, const void *p, int64_t rows, int64_t cols, int64
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Products of a few rows need no tiles (and no copies for TMA).
+bool takes_few_rows(int64_t M, bool across) { return !across && M <= kRowsAtMost; }
+
 // How a product of M x N outputs and a sum of `len` is cut: the width of its tiles and the parts of its sum.
 struct Cut {
     int bn, splits, steps_per_split;
@@ -726,10 +803,21 @@ struct Cut {
 Cut cut_product(int64_t M, int N, int64_t len, bool b_mn)
 {
     const int steps = int((len + kBK - 1) / kBK);
-    Cut c{256, 1, steps};
+    // Widths by what the waves of tiles cost, in clocks: a step takes what its operands take from L2 (about 60 bytes a
+    // clock and SM), or its product; a tile takes its set-up and its epilogue, which hides behind the next tile's steps
+    // only. Measured at 1000 x 1024 x 640 (width 64: one wave) and 40009 x 640 x 512 (pairs: 37 us, width 128: 52 us).
     const int least = b_mn ? 64 : 32;
-    // narrower tiles until every SM has one
-    while (c.bn > least && (c.bn / 2 >= N || c.tiles(M, N) < c.at_once())) c.bn /= 2;
+    Cut c{0, 1, steps};
+    int64_t best = 0;
+    for (const int bn : {256, 128, 64, 32}) {
+        if (bn < least || (bn > least && bn / 2 >= N)) continue;
+        const Cut t{bn, 1, steps};
+        const int64_t waves = (t.tiles(M, N) + t.at_once() - 1) / t.at_once();
+        const int loads = (kBM + (bn == 256 ? 128 : bn)) * kBK * 2 / 60, product = bn == 256 ? 512 : 2 * bn * 2;
+        const int64_t epilogue = bn * 18, main = steps * int64_t(loads > product ? loads : product);
+        const int64_t cost = waves * (main > epilogue ? main : epilogue) + epilogue;
+        if (c.bn == 0 || cost < best) c = t, best = cost;
+    }
     // split long sums of few tiles, at least eight steps a part
     if (c.tiles(M, N) * 2 <= kNumSMs && steps >= 32) {
         // wide tiles again: parts give the SMs their work
@@ -805,6 +893,11 @@ cudaError_t run_product_bn(int bn, const Matrix &a, const Matrix &b, const Shape
 template <typename T>
 cudaError_t product(const Matrix &a, const Matrix &b, int64_t M, int N, int64_t len, Epilogue ep, float *part, cudaStream_t s)
 {
+    if (takes_few_rows(M, a.mn || b.mn)) {
+        const T *x = static_cast<const T *>(a.p), *w = static_cast<const T *>(b.p);
+        if (N >= 2048) return run_few_rows<T, 4>(x, a.ld, w, b.ld, int(M), N, int(len), ep, s);
+        return run_few_rows<T, 1>(x, a.ld, w, b.ld, int(M), N, int(len), ep, s);
+    }
     const Cut c = cut_product(M, N, len, b.mn);
     Shape sh{};
     sh.M = M, sh.N = N;
@@ -855,8 +948,9 @@ LinearPlan plan_linear(const cwrnnt_linear &p, bool backward)
         at += align_up(bytes, 256);
         return here;
     };
-    q.x = take(copy_bytes(p.n_rows, p.n_in, p.x_stride));
-    q.w = take(copy_bytes(p.n_out, p.n_in, p.w_stride));
+    const bool copies = backward || !takes_few_rows(p.n_rows, false);
+    q.x = take(copies ? copy_bytes(p.n_rows, p.n_in, p.x_stride) : 0);
+    q.w = take(copies ? copy_bytes(p.n_out, p.n_in, p.w_stride) : 0);
     auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
     int64_t parts = 0;
     if (!backward || p.activation != CWRNNT_ACT_NONE)
@@ -907,8 +1001,10 @@ cudaError_t linear_forward(const cwrnnt_linear &p, const void *x, const void *w,
 {
     const LinearPlan q = plan_linear(p, false);
     Matrix a{x, p.n_rows, p.n_in, p.x_stride, false}, b{w, p.n_out, p.n_in, p.w_stride, false};
-    CWRNNT_TRY(readable<T>(a, ws + q.x, s));
-    CWRNNT_TRY(readable<T>(b, ws + q.w, s));
+    if (!takes_few_rows(p.n_rows, false)) {
+        CWRNNT_TRY(readable<T>(a, ws + q.x, s));
+        CWRNNT_TRY(readable<T>(b, ws + q.w, s));
+    }
     Epilogue ep{};
     ep.mode = kStore, ep.act = p.activation, ep.bias = bias;
     ep.side = residual, ep.side_ld = p.n_out;
@@ -936,7 +1032,7 @@ cudaError_t linear_backward(const cwrnnt_linear &p, const void *x, const void *w
         ep.side = g, ep.side_ld = p.g_stride;
         ep.out = ws + q.dz, ep.out_ld = padded(p.n_out);
         const Cut c = cut_product(p.n_rows, p.n_out, p.n_in, false);
-        if (grad_b && c.splits == 1 && c.bn >= 64) ep.sums = sums, runs = (p.n_rows + 31) / 32;
+        if (grad_b && c.splits == 1 && c.bn >= 64 && !takes_few_rows(p.n_rows, false)) ep.sums = sums, runs = (p.n_rows + 31) / 32;
         CWRNNT_TRY(product<T>(mx, mw, p.n_rows, p.n_out, p.n_in, ep, part, s));
         dz.p = ws + q.dz, dz.ld = padded(p.n_out);
     } else {

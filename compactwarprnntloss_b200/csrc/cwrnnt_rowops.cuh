@@ -84,6 +84,7 @@ struct Base2<float> {
     static __device__ __forceinline__ float ln_of(float s) { return logf(s); }
     static __device__ __forceinline__ float fma_of(float a, float b, float c) { return fmaf(a, b, c); }
     static __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+    static __device__ __forceinline__ float ratio(float a, float b) { return __fdividef(a, b); }  // b in [2^-126, 2^126]
     // below this exponent a term is zero; it keeps 0 * (-inf) out of sum p log p
     static constexpr float kFloor = -1000.0f;
     // largest shift that x*kappa - shift is formed with; beyond it (rows of the type's lowest value) x*kappa overflows
@@ -95,6 +96,7 @@ struct Base2<double> {
     static __device__ __forceinline__ double ln_of(double s) { return log(s); }
     static __device__ __forceinline__ double fma_of(double a, double b, double c) { return fma(a, b, c); }
     static __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
+    static __device__ __forceinline__ double ratio(double a, double b) { return a / b; }
     static constexpr double kFloor = -5000.0;
     static constexpr double kMostShift = 1e307;
 };

@@ -144,3 +144,16 @@ def test_fused_linear_refuses_what_it_cannot_take():
             fused_linear(*args, **kw)
     with pytest.raises(RuntimeError, match="CUDA"):
         fused_linear(x, w)
+
+
+def test_every_linear_layer_has_a_workspace():
+    """The plans of all sizes are host arithmetic: both passes, widths and lengths around every tile and split."""
+    L = capi.lib()
+    sizes = (1, 7, 8, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 640, 1000, 1024, 4096, 20000)
+    for m in (1, 16, 17, 128, 129, 256, 1000, 9001, 40009, 314340, 2 ** 31 - 1024):
+        for n in sizes:
+            for k in sizes:
+                for act in (0, 2):
+                    p = ctypes.byref(capi.Linear(m, k, k, n, k, n, capi.BF16, act))
+                    f, b = L.cwrnnt_linear_workspace_bytes(p, 0), L.cwrnnt_linear_workspace_bytes(p, 1)
+                    assert f >= 256 and b >= 256 and f % 256 == 0 and b % 256 == 0
