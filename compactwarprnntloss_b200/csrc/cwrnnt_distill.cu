@@ -255,28 +255,49 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
     const int gl = threadIdx.x % LPR, group = threadIdx.x / LPR;
     const int64_t first = int64_t(blockIdx.x) * GPC * run_len + group;
     double sum = 0.0;
+    // A row's weight decides whether it is read, its tokens what is read of it: both are asked for two rows ahead, the
+    // logits at the tokens one row ahead, so that no load of a row waits for another.
+    struct Ahead {
+        A weight, value;
+        int c;
+    };
+    auto look = [&](int step) {
+        const int64_t r = first + int64_t(step) * GPC;
+        Ahead h{A(0), A(-INFINITY), -1};
+        if (step < run_len && r < a.n_rows) {
+            h.weight = a.weight ? A(__ldg(a.weight + r)) : A(1);
+            if (gl < a.K) {
+                h.c = __ldg(a.index + r * a.K + gl);
+                h.value = A(__ldg(a.teacher + r * a.K + gl));
+            }
+        }
+        return h;
+    };
+    auto pick = [&](int step, const Ahead &h) {
+        const int64_t r = first + int64_t(step) * GPC;
+        return h.weight != A(0) && h.c >= 0 && h.c < a.V ? E::to_acc(__ldg(a.x + r * a.x_stride + h.c)) : A(-INFINITY);
+    };
+    Ahead now = look(0), next = look(1);
+    A xc = pick(0, now);
     for (int step = 0; step < run_len; ++step) {
         const int64_t r = first + int64_t(step) * GPC;
         const bool active = r < a.n_rows;
         if (!__any_sync(kAll, active)) break;
         const int64_t rr = active ? r : 0;
-        const A weight = active ? (a.weight ? A(__ldg(a.weight + r)) : A(1)) : A(0);
-        const bool seen = active && weight != A(0);  // a row without weight is not read
+        const A weight = now.weight;
+        const bool seen = weight != A(0);  // a row without weight is not read
         const T *row = a.x + rr * a.x_stride;
         const RowVectors<T, ALIGNED> rv(row, a.V);
-        int c = -1;
-        A value = A(-INFINITY);
-        if (seen && gl < a.K) {
-            c = __ldg(a.index + r * a.K + gl);
-            value = A(__ldg(a.teacher + r * a.K + gl));
-        }
         uint4 v[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             v[j] = vector_of_nothing<T>();
             if (seen && j * LPR + gl < rv.count) v[j] = rv.load(j * LPR + gl);
         }
-        const A xc = c >= 0 && c < a.V ? E::to_acc(__ldg(row + c)) : A(-INFINITY);
+        const A next_xc = pick(step + 1, next);
+        const Ahead after = look(step + 2);
+        const int c = seen ? now.c : -1;
+        const A value = now.value;
         const Entries<A> en = weigh_entries<LPR, TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, gl);
         if (TAIL) {
             for (int e = 0; e < a.K; ++e) {
@@ -343,6 +364,7 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
             __syncwarp();
             write_entry<T>(out, en, xc, res, a.kappa, seen);
         }
+        now = next, next = after, xc = next_xc;
     }
     if (a.partial) {
         sum = sum_cta(sum);
@@ -484,7 +506,8 @@ template <typename T, int LPR, int NV, bool ALIGNED>
 int64_t launch_distill_rows(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 {
     constexpr int GPC = kRowThreads / LPR;
-    const int run_len = a.n_rows > int64_t(GPC) * kNumSMs * 32 ? 4 : 1;
+    // runs of rows where there are enough for every SM: the first row of a run has nothing asked for ahead
+    const int run_len = a.n_rows > int64_t(GPC) * kNumSMs * 32 ? 8 : 1;
     const int64_t grid = (a.n_rows + int64_t(GPC) * run_len - 1) / (int64_t(GPC) * run_len);
     if (tail)
         distill_rows_kernel<T, LPR, NV, ALIGNED, true><<<unsigned(grid), kRowThreads, 0, s>>>(a, run_len);
