@@ -136,6 +136,7 @@ struct Elt;
 
 template <>
 struct Elt<float> {
+    static __device__ __forceinline__ float floor() { return -INFINITY; }
     using acc = float;    // arithmetic type of the streaming kernels
     using cost = float;   // type of costs / loss / grad_costs
     static constexpr int VE = 4;  // elements per 16-byte vector
@@ -167,6 +168,16 @@ struct Elt<__half> {
     static constexpr bool kBf16 = false;
     using pair = __half2;
     static __device__ __forceinline__ pair both(float v) { return __float2half2_rn(v); }
+    // every element at least the lowest finite value (NaN stays)
+    static __device__ __forceinline__ float floor() { return -65504.0f; }
+    static __device__ __forceinline__ uint4 at_least_floor(uint4 v)
+    {
+        const __half2 f = __float2half2_rn(floor());
+        __half2 *h = reinterpret_cast<__half2 *>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], f);
+        return v;
+    }
     static constexpr int VE = 8;
     static __device__ __forceinline__ void unpack(const uint4 &v, float (&e)[8])
     {
@@ -208,6 +219,16 @@ struct Elt<__nv_bfloat16> {
     static constexpr bool kBf16 = true;
     using pair = __nv_bfloat162;
     static __device__ __forceinline__ pair both(float v) { return __float2bfloat162_rn(v); }
+    // every element at least -1e30 (NaN stays)
+    static __device__ __forceinline__ float floor() { return -1e30f; }
+    static __device__ __forceinline__ uint4 at_least_floor(uint4 v)
+    {
+        const __nv_bfloat162 f = __float2bfloat162_rn(floor());
+        __nv_bfloat162 *h = reinterpret_cast<__nv_bfloat162 *>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], f);
+        return v;
+    }
     static constexpr int VE = 8;
     static __device__ __forceinline__ void unpack(const uint4 &v, float (&e)[8])
     {
@@ -245,6 +266,7 @@ struct Elt<__nv_bfloat16> {
 
 template <>
 struct Elt<double> {
+    static __device__ __forceinline__ double floor() { return -INFINITY; }
     using acc = double;
     using cost = double;
     static constexpr int VE = 2;

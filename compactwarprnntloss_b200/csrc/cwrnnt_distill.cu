@@ -182,17 +182,24 @@ __device__ __forceinline__ RowResult<A> solve_row(const RowStats<A> &st, const E
         all_sum = listed + (st.max == A(-INFINITY) ? rest_sum : rest_sum * M::exp2_of((st.max - base) * kappa));
     }
     const bool nothing = all_max == A(-INFINITY) && all_sum == all_sum;  // no finite entry: nothing to learn
-    const A ln_s = nothing ? A(0) : M::ln_of(all_sum);
+    // the three logarithms at once, each in a lane of its own
+    const int gl = threadIdx.x % LPR;
+    const A of = gl == 0 ? (nothing ? A(1) : all_sum) : gl == 1 ? rest_sum : en.left;
+    const A ln = M::ln_of(of);
+    const A ln_s = __shfl_sync(0xffffffffu, ln, 0, LPR);
     A each = A(0);
     if (en.q > A(0)) each = en.q * (en.lq - log_prob_of(xc, all_max, inv_tau, ln_s));
     each = entry_sum<LPR>(each, KP);
     A q_all = en.sum_q, q_rest = A(0), p_rest = A(1);
-    if (TAIL && !st.nothing()) {
-        const A ln_rest = (st.max - all_max) * inv_tau + (M::ln_of(rest_sum) - ln_s);
-        q_rest = en.left;
-        q_all = en.sum_q + q_rest;
-        p_rest = rest_sum * M::exp2_of((st.max - all_max) * kappa) * M::ratio(A(1), all_sum);
-        if (q_rest > A(0)) each += q_rest * (M::ln_of(q_rest) - ln_rest);
+    if (TAIL) {
+        const A ln_rest = (st.max - all_max) * inv_tau + (__shfl_sync(0xffffffffu, ln, 1, LPR) - ln_s);
+        const A ln_left = __shfl_sync(0xffffffffu, ln, 2, LPR);
+        if (!st.nothing()) {
+            q_rest = en.left;
+            q_all = en.sum_q + q_rest;
+            p_rest = rest_sum * M::exp2_of((st.max - all_max) * kappa) * M::ratio(A(1), all_sum);
+            if (q_rest > A(0)) each += q_rest * (ln_left - ln_rest);
+        }
     }
     A up = gain * weight * inv_tau;
     if (nothing) each = up = A(0);
@@ -240,9 +247,8 @@ __device__ __forceinline__ double sum_cta(double v)
 }
 
 // Rows of at most LPR * NV vectors and at most LPR entries. Group g of a CTA takes the rows first + g, + GPC, ..
-// The terms of the sum are kept in registers for the gradient where the row has at most 64 elements a lane; longer rows
-// keep their vectors and take the terms again.
-template <typename T, int LPR, int NV, bool ALIGNED, bool TAIL>
+// The terms of the sum stay in registers for the gradient.
+template <typename T, int LPR, int NV, int MODE, bool TAIL>
 __global__ void __launch_bounds__(kRowThreads)
 distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
 {
@@ -250,7 +256,6 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
     using A = typename E::acc;
     using M = Base2<A>;
     constexpr int GPC = kRowThreads / LPR, VE = E::VE;
-    constexpr bool kKeep = NV * VE * sizeof(A) <= 256;
     constexpr unsigned kAll = 0xffffffffu;
     const int gl = threadIdx.x % LPR, group = threadIdx.x / LPR;
     const int64_t first = int64_t(blockIdx.x) * GPC * run_len + group;
@@ -287,13 +292,9 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
         const A weight = now.weight;
         const bool seen = weight != A(0);  // a row without weight is not read
         const T *row = a.x + rr * a.x_stride;
-        const RowVectors<T, ALIGNED> rv(row, a.V);
+        const RowVectors<T, MODE> rv(row, a.V);
         uint4 v[NV];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            v[j] = vector_of_nothing<T>();
-            if (seen && j * LPR + gl < rv.count) v[j] = rv.load(j * LPR + gl);
-        }
+        rv.template load_all<LPR>(v, gl, seen);
         const A next_xc = pick(step + 1, next);
         const Ahead after = look(step + 2);
         const int c = seen ? now.c : -1;
@@ -315,27 +316,30 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
         for (int j = 0; j < NV; ++j) st.max = M::max_of(st.max, E::vec_max(v[j]));
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) st.max = M::max_of(st.max, __shfl_xor_sync(kAll, st.max, o));
-        A term[kKeep ? NV : 1][VE];
-        if constexpr (kKeep) {
-            // the difference from the maximum first: no shift to be rounded, and no row too extreme
-            const A base = st.max == A(-INFINITY) ? A(0) : st.max;
+        // A term is the same number in the sum and in the gradient, so the rounding of the shift leaves their ratio; it
+        // is undone where the sum's logarithm is taken.
+        const TermsAt<T> at(st.max, a.kappa);
+        A term[NV][VE];
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                E::unpack(v[j], term[j]);
+        for (int j = 0; j < NV; ++j) {
+            E::unpack(v[j], term[j]);
+            if (at.plain) {
 #pragma unroll
-                for (int k = 0; k < VE; ++k) {
-                    term[j][k] = M::exp2_of((term[j][k] - base) * a.kappa);
-                    st.s += term[j][k];
-                }
+                for (int k = 0; k < VE; ++k) term[j][k] = M::fma_of(term[j][k], a.kappa, -at.shift);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VE; ++k) term[j][k] = at.exponent(term[j][k], a.kappa);
             }
-        } else {
-            const A shift = RowStats<A>::shift_of(st.max, a.kappa);
 #pragma unroll
-            for (int j = 0; j < NV; ++j) add_terms<T, false>(v[j], a.kappa, st.max, shift, st.s, st.t);
-            st.s = st.sum(a.kappa);
+            for (int k = 0; k < VE; ++k) {
+                term[j][k] = M::exp2_of(term[j][k]);
+                st.s += term[j][k];
+            }
         }
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) st.s += __shfl_xor_sync(kAll, st.s, o);
+        const A undo = at.plain ? M::exp2_of(-M::fma_of(at.max, a.kappa, -at.shift)) : A(1);
+        st.s *= undo;
         const A up = a.upstream && active ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
         const RowResult<A> res = solve_row<LPR, TAIL>(st, en, xc, a.kappa, a.inv_tau, weight, up * A(a.scale), a.KP);
         if (active && gl == 0) {
@@ -344,21 +348,15 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
         }
         if (a.gx) {
             T *out = a.gx + rr * a.g_stride;
-            const bool same = ALIGNED || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+            const bool same = MODE != kAny || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+            const A factor = res.factor * undo;
+            if (active) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int i = j * LPR + gl;
-                if (active && i < rv.count) {
-                    A e[VE];
-                    if constexpr (!kKeep) E::unpack(v[j], e);
+                for (int j = 0; j < NV; ++j) {
+                    const int i = j * LPR + gl;
 #pragma unroll
-                    for (int k = 0; k < VE; ++k) {
-                        if constexpr (kKeep)
-                            e[k] = term[j][k] * res.factor;
-                        else
-                            e[k] = M::exp2_of((e[k] - res.top) * a.kappa) * res.factor;
-                    }
-                    store_vector(out, rv, i, same, e);
+                    for (int k = 0; k < VE; ++k) term[j][k] *= factor;
+                    if (MODE == kFull || i < rv.count) rv.store(out, i, same, term[j]);
                 }
             }
             __syncwarp();
@@ -372,116 +370,146 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
     }
 }
 
-// Any row: one CTA each. Every warp holds the row's entries in its lanes.
-template <typename T, bool ALIGNED, bool TAIL>
+// Rows that registers do not hold: a warp each (LANES = 32) or a CTA each (LANES = 256). Every warp holds the row's
+// entries in its lanes. The sums run along the row, then the gradient does, reading the row a second time from L2.
+template <typename T, int LANES, int MODE, bool TAIL>
 __global__ void __launch_bounds__(kRowThreads)
-distill_long_kernel(const DistillArgs<T> a)
+distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
 {
     using E = Elt<T>;
     using A = typename E::acc;
     using M = Base2<A>;
     constexpr int NV = 4, kWarps = kRowThreads / 32;
-    __shared__ RowStats<A> parts[kWarps];
-    __shared__ int listed[32];  // positions of the listed tokens, counted from the first vector's start; -1: none
-    const int tid = threadIdx.x, lane = tid & 31;
-    const int64_t r = blockIdx.x;
-    const A weight = a.weight ? A(__ldg(a.weight + r)) : A(1);
-    const T *row = a.x + r * a.x_stride;
-    T *out = a.gx ? a.gx + r * a.g_stride : nullptr;
-    const RowVectors<T, ALIGNED> rv(row, a.V);
-    const bool same = ALIGNED || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    const bool seen = weight != A(0);  // a row without weight is not read
-    int c = -1;
-    A value = A(-INFINITY);
-    if (seen && lane < a.K) {
-        c = __ldg(a.index + r * a.K + lane);
-        value = A(__ldg(a.teacher + r * a.K + lane));
-    }
-    const A xc = c >= 0 && c < a.V ? E::to_acc(__ldg(row + c)) : A(-INFINITY);
-    const Entries<A> en = weigh_entries<32, TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, lane);
-    if (tid < 32) listed[tid] = en.c >= 0 ? en.c + rv.head : -1;
-    __syncthreads();
-
-    // the next of this thread's vectors, from vector `from` on, that holds a listed token
-    auto next_listed = [&](int from) {
-        int next = 0x7fffffff;
-        for (int e = 0; e < a.K; ++e) {
-            const int i = listed[e] / E::VE;
-            if (listed[e] >= 0 && i % kRowThreads == tid && i >= from && i < next) next = i;
+    constexpr unsigned kAll = 0xffffffffu;
+    __shared__ RowStats<A> parts[LANES == 32 ? 1 : kWarps];
+    __shared__ int listed_of[LANES == 32 ? kWarps : 1][32];  // positions of the listed tokens, counted from the first
+                                                             // vector's start; -1: none
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int me = LANES == 32 ? lane : threadIdx.x;
+    const int64_t r = LANES == 32 ? int64_t(blockIdx.x) * kWarps + warp : int64_t(blockIdx.x);
+    const bool active = r < a.n_rows;
+    A loss = A(0);
+    if (active) {
+        const A weight = a.weight ? A(__ldg(a.weight + r)) : A(1);
+        const T *row = a.x + r * a.x_stride;
+        T *out = a.gx ? a.gx + r * a.g_stride : nullptr;
+        const RowVectors<T, MODE> rv(row, a.V);
+        const bool same = MODE != kAny || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+        const bool seen = weight != A(0);  // a row without weight is not read
+        int c = -1;
+        A value = A(-INFINITY);
+        if (seen && lane < a.K) {
+            c = __ldg(a.index + r * a.K + lane);
+            value = A(__ldg(a.teacher + r * a.K + lane));
         }
-        return next;
-    };
-    RowStats<A> st;
-    st.clear();
-    if (seen) {
-        int next = TAIL ? next_listed(0) : 0x7fffffff;
-        for (int at = 0; at < rv.count; at += kRowThreads * NV) {
-            uint4 v[NV];
+        // f(first vector, four vectors LANES apart) over the row
+        auto sweep = [&](auto &&f) {
+            uint4 v[NV], ahead[NV];
+            auto load = [&](uint4(&to)[NV], int at) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int i = at + j * kRowThreads + tid;
-                v[j] = i < rv.count ? rv.load(i) : vector_of_nothing<T>();
-            }
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int i = at + j * kRowThreads + tid;
-                if (TAIL && i == next) {
-                    for (int e = 0; e < a.K; ++e)
-                        if (listed[e] >= 0 && listed[e] / E::VE == i) blank_element<T>(v[j], listed[e] % E::VE);
-                    next = next_listed(i + 1);
+                for (int j = 0; j < NV; ++j) {
+                    const int i = at + j * LANES;
+                    to[j] = vector_of_nothing<T>();
+                    if (seen && i < rv.count) to[j] = rv.load(i);
                 }
+            };
+            load(v, me);
+#pragma unroll 1
+            for (int at = me; at - me < rv.count; at += NV * LANES) {
+                if (at - me + NV * LANES < rv.count) load(ahead, at + NV * LANES);
+                f(at, v);
+#pragma unroll
+                for (int j = 0; j < NV; ++j) v[j] = ahead[j];
             }
-            A m = st.max;
-#pragma unroll
-            for (int j = 0; j < NV; ++j) m = M::max_of(m, E::vec_max(v[j]));
-            if (m > st.max) st.template raise<false>(m, a.kappa);
-            const A shift = RowStats<A>::shift_of(st.max, a.kappa);
-#pragma unroll
-            for (int j = 0; j < NV; ++j) add_terms<T, false>(v[j], a.kappa, st.max, shift, st.s, st.t);
-        }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        RowStats<A> other;
-        other.max = __shfl_xor_sync(0xffffffffu, st.max, o);
-        other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        other.t = A(0);
-        st.template join<false>(other, a.kappa);
-    }
-    if (lane == 0) parts[tid >> 5] = st;
-    __syncthreads();
-    st = parts[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) st.template join<false>(parts[w], a.kappa);
-    st.s = st.sum(a.kappa);
-    const A up = a.upstream ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
-    const RowResult<A> res = solve_row<32, TAIL>(st, en, xc, a.kappa, a.inv_tau, weight, up * A(a.scale), a.KP);
-    if (tid == 0) {
-        if (a.row_loss) a.row_loss[r] = res.loss;
-        if (a.partial) a.partial[r] = double(res.loss) * a.scale;
-    }
-    if (!out) return;
-    for (int at = 0; at < rv.count; at += kRowThreads * NV) {
-        uint4 v[NV];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = at + j * kRowThreads + tid;
-            v[j] = seen && i < rv.count ? rv.load(i) : vector_of_nothing<T>();
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = at + j * kRowThreads + tid;
-            if (i < rv.count) {
-                A e[E::VE];
-                E::unpack(v[j], e);
-#pragma unroll
-                for (int k = 0; k < E::VE; ++k) e[k] = M::exp2_of((e[k] - res.top) * a.kappa) * res.factor;
-                store_vector(out, rv, i, same, e);
+        };
+        int *const listed = listed_of[LANES == 32 ? warp : 0];
+        const A xc = c >= 0 && c < a.V ? E::to_acc(__ldg(row + c)) : A(-INFINITY);
+        const Entries<A> en = weigh_entries<32, TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, lane);
+        if (me < 32) listed[lane] = en.c >= 0 ? en.c + rv.head : -1;
+        if (LANES == 32)
+            __syncwarp();
+        else
+            __syncthreads();
+
+        // the next of this lane's vectors, from vector `from` on, that holds a listed token
+        auto next_listed = [&](int from) {
+            int next = 0x7fffffff;
+            for (int e = 0; e < a.K; ++e) {
+                const int i = listed[e] / E::VE;
+                if (listed[e] >= 0 && i % LANES == me && i >= from && i < next) next = i;
             }
+            return next;
+        };
+        RowStats<A> st;
+        st.clear();
+        if (seen) {
+            int next = TAIL ? next_listed(0) : 0x7fffffff;
+            sweep([&](int at, uint4(&v)[NV]) {
+                if (TAIL && next < at + NV * LANES) {
+                    const int past = at + NV * LANES;
+                    for (int e = 0; e < a.K; ++e) {
+                        const int i = listed[e] / E::VE;
+                        if (listed[e] < 0 || i % LANES != me || i < at || i >= past) continue;
+#pragma unroll
+                        for (int j = 0; j < NV; ++j)
+                            if (i == at + j * LANES) blank_element<T>(v[j], listed[e] % E::VE);
+                    }
+                    next = next_listed(past);
+                }
+                A m = st.max;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) m = M::max_of(m, E::vec_max(v[j]));
+                if (m > st.max) st.template raise<false>(m, a.kappa);
+                const TermsAt<T> terms(st.max, a.kappa);
+#pragma unroll
+                for (int j = 0; j < NV; ++j) add_terms<T, false>(v[j], a.kappa, terms, st.s, st.t);
+            });
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            RowStats<A> other;
+            other.max = __shfl_xor_sync(kAll, st.max, o);
+            other.s = __shfl_xor_sync(kAll, st.s, o);
+            other.t = A(0);
+            st.template join<false>(other, a.kappa);
+        }
+        if (LANES > 32) {  // the warps' parts, joined in their order: the same bits in every thread
+            if (lane == 0) parts[warp] = st;
+            __syncthreads();
+            st = parts[0];
+#pragma unroll 1
+            for (int w = 1; w < kWarps; ++w) st.template join<false>(parts[w], a.kappa);
+        }
+        st.s = st.sum(a.kappa);
+        const A up = a.upstream ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
+        const RowResult<A> res = solve_row<32, TAIL>(st, en, xc, a.kappa, a.inv_tau, weight, up * A(a.scale), a.KP);
+        loss = res.loss;
+        if (me == 0 && a.row_loss) a.row_loss[r] = loss;
+        if (out) {
+            sweep([&](int at, uint4(&v)[NV]) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int i = at + j * LANES;
+                    if (i < rv.count) {
+                        A e[E::VE];
+                        E::unpack(v[j], e);
+#pragma unroll
+                        for (int k = 0; k < E::VE; ++k) e[k] = M::exp2_of((e[k] - res.top) * a.kappa) * res.factor;
+                        rv.store(out, i, same, e);
+                    }
+                }
+            });
+            if (LANES == 32)
+                __syncwarp();
+            else
+                __syncthreads();
+            if (me < 32) write_entry<T>(out, en, xc, res, a.kappa, seen);
         }
     }
-    __syncthreads();
-    if (tid < 32) write_entry<T>(out, en, xc, res, a.kappa, seen);
+    if (a.partial) {
+        const double sum = sum_cta(me == 0 ? double(loss) : 0.0);
+        if (threadIdx.x == 0) a.partial[blockIdx.x] = sum * a.scale;
+    }
 }
 
 // The CTAs' sums, added up in a fixed order.
@@ -509,10 +537,28 @@ int64_t launch_distill_rows(const DistillArgs<T> &a, bool tail, cudaStream_t s)
     // runs of rows where there are enough for every SM: the first row of a run has nothing asked for ahead
     const int run_len = a.n_rows > int64_t(GPC) * kNumSMs * 32 ? 8 : 1;
     const int64_t grid = (a.n_rows + int64_t(GPC) * run_len - 1) / (int64_t(GPC) * run_len);
+    auto go = [&](auto kernel) { kernel<<<unsigned(grid), kRowThreads, 0, s>>>(a, run_len); };
+    if constexpr (ALIGNED) {
+        if (a.V == LPR * NV * Elt<T>::VE)
+            tail ? go(distill_rows_kernel<T, LPR, NV, kFull, true>) : go(distill_rows_kernel<T, LPR, NV, kFull, false>);
+        else
+            tail ? go(distill_rows_kernel<T, LPR, NV, kAligned, true>)
+                 : go(distill_rows_kernel<T, LPR, NV, kAligned, false>);
+    } else {
+        tail ? go(distill_rows_kernel<T, LPR, NV, kAny, true>) : go(distill_rows_kernel<T, LPR, NV, kAny, false>);
+    }
+    return grid;
+}
+
+template <typename T, int LANES, bool ALIGNED>
+int64_t launch_distill_stream(const DistillArgs<T> &a, bool tail, cudaStream_t s)
+{
+    constexpr int rows = kRowThreads / LANES, MODE = ALIGNED ? kAligned : kAny;
+    const int64_t grid = (a.n_rows + rows - 1) / rows;
     if (tail)
-        distill_rows_kernel<T, LPR, NV, ALIGNED, true><<<unsigned(grid), kRowThreads, 0, s>>>(a, run_len);
+        distill_stream_kernel<T, LANES, MODE, true><<<unsigned(grid), kRowThreads, 0, s>>>(a);
     else
-        distill_rows_kernel<T, LPR, NV, ALIGNED, false><<<unsigned(grid), kRowThreads, 0, s>>>(a, run_len);
+        distill_stream_kernel<T, LANES, MODE, false><<<unsigned(grid), kRowThreads, 0, s>>>(a);
     return grid;
 }
 
@@ -520,25 +566,21 @@ int64_t launch_distill_rows(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 template <typename T, bool ALIGNED>
 int64_t launch_distill_t(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 {
-    constexpr int VE = Elt<T>::VE;
+    constexpr int VE = Elt<T>::VE, NV = 64 / VE < 16 ? 64 / VE : 16;
     const int nv = ALIGNED ? a.V / VE : (a.V + 2 * VE - 2) / VE;
-    // Few lanes a row, many elements a lane: what a row costs beside its elements (about 600 instructions of a warp) is
+    // Few lanes a row, many elements a lane: what a row costs beside its elements (about 400 instructions of a warp) is
     // shared by the rows of a warp. 64 elements a lane is what registers hold; every entry has a lane.
     if constexpr (sizeof(T) <= 4) {
-        constexpr int NV = 64 / VE;
         if (nv <= 4 * NV && a.K <= 4) return launch_distill_rows<T, 4, NV, ALIGNED>(a, tail, s);
         if (nv <= 8 * NV && a.K <= 8) return launch_distill_rows<T, 8, NV, ALIGNED>(a, tail, s);
         if (nv <= 16 * NV && a.K <= 16) return launch_distill_rows<T, 16, NV, ALIGNED>(a, tail, s);
         if (nv <= 64) return launch_distill_rows<T, 32, 2, ALIGNED>(a, tail, s);
+        if (nv <= 128) return launch_distill_rows<T, 32, 4, ALIGNED>(a, tail, s);
     }
-    if (nv <= 128) return launch_distill_rows<T, 32, 4, ALIGNED>(a, tail, s);
-    if (nv <= 256) return launch_distill_rows<T, 32, 8, ALIGNED>(a, tail, s);
-    if (nv <= 512) return launch_distill_rows<T, 32, 16, ALIGNED>(a, tail, s);
-    if (tail)
-        distill_long_kernel<T, ALIGNED, true><<<unsigned(a.n_rows), kRowThreads, 0, s>>>(a);
-    else
-        distill_long_kernel<T, ALIGNED, false><<<unsigned(a.n_rows), kRowThreads, 0, s>>>(a);
-    return a.n_rows;
+    if (nv <= 32 * NV) return launch_distill_rows<T, 32, NV, ALIGNED>(a, tail, s);
+    // a warp carries a longer row where there are rows enough for the SMs' warps
+    if (nv <= 2048 && a.n_rows >= kNumSMs * 32) return launch_distill_stream<T, 32, ALIGNED>(a, tail, s);
+    return launch_distill_stream<T, kRowThreads, ALIGNED>(a, tail, s);
 }
 
 template <typename T>

@@ -11,66 +11,88 @@ constexpr int kRowThreads = 256;  // threads of a CTA in the row operators
 // Vector i of a row covers the elements [i*VE - head, i*VE - head + VE), where `head` elements lie between the last
 // 16-byte boundary at or below the row's start and that start: vectors are always aligned, whatever V and the row
 // stride. The first and the last vector can reach over the row's ends; they are put together element by element, with
-// `fill` outside, so nothing outside the row is read. ALIGNED: every row starts on a boundary and ends on one.
-template <typename T, bool ALIGNED>
-struct RowVectors {
-    const T *row;
-    int V, head, count;
-    __device__ __forceinline__ RowVectors(const T *row_, int V_) : row(row_), V(V_)
-    {
-        constexpr int VE = Elt<T>::VE;
-        head = ALIGNED ? 0 : int((reinterpret_cast<uintptr_t>(row_) & 15) / sizeof(T));
-        count = (V_ + head + VE - 1) / VE;
-    }
-    __device__ __forceinline__ int first(int i) const { return i * Elt<T>::VE - head; }
-    __device__ __forceinline__ bool whole(int i) const
-    {
-        return ALIGNED || (first(i) >= 0 && first(i) + Elt<T>::VE <= V);
-    }
-    __device__ __forceinline__ uint4 load(int i) const
-    {
-        if (whole(i)) return __ldg(reinterpret_cast<const uint4 *>(row + first(i)));
-        return edge(i);
-    }
-    __device__ __noinline__ uint4 edge(int i) const
-    {
-        using E = Elt<T>;
-        typename E::acc e[E::VE];
+// -inf outside, so nothing outside the row is read. What a launch knows of its rows:
+//   kAny      nothing
+//   kAligned  every row starts and ends on a 16-byte boundary
+//   kFull     the same, and a row is exactly the vectors that its lanes hold in registers
+enum { kAny = 0, kAligned = 1, kFull = 2 };
+
+// The edges, out of line: they would fill the instruction cache from within every unrolled loop.
+template <typename T>
+__device__ __noinline__ uint4 load_edge(const T *row, int first, int V)
+{
+    using E = Elt<T>;
+    typename E::acc e[E::VE];
 #pragma unroll
-        for (int c = 0; c < E::VE; ++c) {
-            const int k = first(i) + c;
-            e[c] = k >= 0 && k < V ? E::to_acc(__ldg(row + k)) : typename E::acc(-INFINITY);
-        }
-        return E::pack(e);
+    for (int c = 0; c < E::VE; ++c) {
+        const int k = first + c;
+        e[c] = k >= 0 && k < V ? E::to_acc(__ldg(row + k)) : typename E::acc(-INFINITY);
     }
-};
+    return E::pack(e);
+}
+template <typename T>
+__device__ __noinline__ void store_edge(T *out, int first, int V, uint4 v)
+{
+    const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+    for (int c = 0; c < Elt<T>::VE; ++c)
+        if (first + c >= 0 && first + c < V) out[first + c] = e[c];
+}
 
 template <typename T>
 __device__ __forceinline__ uint4 vector_of_nothing()
 {
-    typename Elt<T>::acc e[Elt<T>::VE];
-#pragma unroll
-    for (int c = 0; c < Elt<T>::VE; ++c) e[c] = typename Elt<T>::acc(-INFINITY);
-    return Elt<T>::pack(e);
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t w = Elt<T>::kBf16 ? 0xff80ff80u : 0xfc00fc00u;
+        return make_uint4(w, w, w, w);
+    } else if constexpr (sizeof(T) == 4) {
+        return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+    } else {
+        return make_uint4(0u, 0xfff00000u, 0u, 0xfff00000u);
+    }
 }
 
-// Stores vector i of a row of gradients. `same`: the output row has the input row's alignment, so that vector i is one
-// 16-byte store; else element by element.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void store_vector(T *out, const RowVectors<T, ALIGNED> &rv, int i, bool same,
-                                             const typename Elt<T>::acc (&e)[Elt<T>::VE])
-{
-    using E = Elt<T>;
-    if (same && rv.whole(i)) {
-        *reinterpret_cast<uint4 *>(out + rv.first(i)) = E::pack(e);
-        return;
+template <typename T, int MODE>
+struct RowVectors {
+    static constexpr int VE = Elt<T>::VE;
+    const T *row;
+    int V, head, count;
+    __device__ __forceinline__ RowVectors(const T *row_, int V_) : row(row_), V(V_)
+    {
+        head = MODE != kAny ? 0 : int((reinterpret_cast<uintptr_t>(row_) & 15) / sizeof(T));
+        count = MODE != kAny ? V_ / VE : (V_ + head + VE - 1) / VE;
     }
+    __device__ __forceinline__ int first(int i) const { return i * VE - head; }
+    __device__ __forceinline__ bool whole(int i) const
+    {
+        return MODE != kAny || (first(i) >= 0 && first(i) + VE <= V);
+    }
+    __device__ __forceinline__ uint4 load(int i) const
+    {
+        if (whole(i)) return __ldg(reinterpret_cast<const uint4 *>(row + first(i)));
+        return load_edge(row, first(i), V);
+    }
+    // vectors lane, lane + LANES, .. of the row into registers
+    template <int LANES, int NV>
+    __device__ __forceinline__ void load_all(uint4 (&v)[NV], int lane, bool active) const
+    {
 #pragma unroll
-    for (int c = 0; c < E::VE; ++c) {
-        const int k = rv.first(i) + c;
-        if (k >= 0 && k < rv.V) out[k] = E::from_acc(e[c]);
+        for (int j = 0; j < NV; ++j) {
+            v[j] = vector_of_nothing<T>();
+            if (MODE == kFull ? active : active && j * LANES + lane < count) v[j] = load(j * LANES + lane);
+        }
     }
-}
+    // Stores vector i of a row of gradients. `same`: the output row has the input row's alignment, so that vector i is
+    // one 16-byte store; else element by element.
+    __device__ __forceinline__ void store(T *out, int i, bool same, const typename Elt<T>::acc (&e)[VE]) const
+    {
+        const uint4 v = Elt<T>::pack(e);
+        if (MODE != kAny || (same && whole(i)))
+            *reinterpret_cast<uint4 *>(out + first(i)) = v;
+        else
+            store_edge(out, first(i), V, v);
+    }
+};
 
 // ---------------------------------------------------------------------------------------------- softmax of a row
 // With temperature tau and kappa = log2(e)/tau, a term of the row's softmax is 2^(x*kappa - shift): one FFMA and one
@@ -167,29 +189,53 @@ __device__ __forceinline__ A log_prob_of(A x, A max, A inv_tau, A ln_s)
     return x == A(-INFINITY) ? (ln_s == ln_s ? A(-INFINITY) : A(NAN)) : Base2<A>::fma_of(x - max, inv_tau, -ln_s);
 }
 
-// Adds one vector's terms at a fixed maximum and its shift.
+// How a row's (or a thread's) terms are formed at a fixed maximum: as x*kappa - shift, or from the difference to the
+// maximum where that product overflows (rows of the type's lowest value). `floored`: a floor under x is far below any term
+// that counts, so it may keep 0 * (-inf) out of sum p log p.
+template <typename T>
+struct TermsAt {
+    using A = typename Elt<T>::acc;
+    A max, shift;
+    bool plain, floored;
+    __device__ __forceinline__ TermsAt(A max_, A kappa)
+        : max(max_ == A(-INFINITY) ? A(0) : max_), shift(RowStats<A>::shift_of(max_, kappa))
+    {
+        plain = !RowStats<A>::extreme(shift);
+        floored = sizeof(T) == 2 && plain && (Elt<T>::floor() - max) * kappa < A(-200);
+    }
+    __device__ __forceinline__ A exponent(A x, A kappa) const
+    {
+        return plain ? Base2<A>::fma_of(x, kappa, -shift) : (x - max) * kappa;
+    }
+};
+
+// Adds one vector's terms to s = sum 2^d and, ENT, t = sum 2^d d.
 template <typename T, bool ENT>
-__device__ __forceinline__ void add_terms(const uint4 &v, typename Elt<T>::acc kappa, typename Elt<T>::acc max,
-                                          typename Elt<T>::acc shift, typename Elt<T>::acc &s,
-                                          typename Elt<T>::acc &t)
+__device__ __forceinline__ void add_terms(uint4 v, typename Elt<T>::acc kappa, const TermsAt<T> &at,
+                                          typename Elt<T>::acc &s, typename Elt<T>::acc &t)
 {
     using E = Elt<T>;
     using A = typename E::acc;
     using M = Base2<A>;
+    constexpr bool kFloors = ENT && sizeof(T) == 2;
     A e[E::VE];
-    E::unpack(v, e);
-    if (RowStats<A>::extreme(shift)) {
+    if (kFloors ? at.floored : at.plain) {
+        if constexpr (kFloors) v = E::at_least_floor(v);
+        E::unpack(v, e);
 #pragma unroll
-        for (int c = 0; c < E::VE; ++c) e[c] = (e[c] - max) * kappa;
+        for (int c = 0; c < E::VE; ++c) {
+            const A d = M::fma_of(e[c], kappa, -at.shift), w = M::exp2_of(d);
+            s += w;
+            if (ENT) t = M::fma_of(w, kFloors ? d : M::max_of(d, M::kFloor), t);
+        }
     } else {
+        E::unpack(v, e);
 #pragma unroll
-        for (int c = 0; c < E::VE; ++c) e[c] = M::fma_of(e[c], kappa, -shift);
-    }
-#pragma unroll
-    for (int c = 0; c < E::VE; ++c) {
-        const A w = M::exp2_of(e[c]);
-        s += w;
-        if (ENT) t = M::fma_of(w, M::max_of(e[c], M::kFloor), t);
+        for (int c = 0; c < E::VE; ++c) {
+            const A d = at.exponent(e[c], kappa), w = M::exp2_of(d);
+            s += w;
+            if (ENT) t = M::fma_of(w, M::max_of(d, M::kFloor), t);
+        }
     }
 }
 
@@ -279,9 +325,23 @@ __device__ __forceinline__ uint32_t at_least(const uint4 &v, typename Elt<T>::ac
     return bits;
 }
 
+// The same for vector i of a row, without the elements before and behind the row.
+template <typename T, int MODE>
+__device__ __forceinline__ uint32_t at_least(const RowVectors<T, MODE> &rv, int i, const uint4 &v,
+                                             typename Elt<T>::acc bar)
+{
+    uint32_t hit = at_least<T>(v, bar);
+    if (MODE == kAny && !rv.whole(i)) {
+        const int f = rv.first(i);
+        if (f < 0) hit &= ~0u << (-f);
+        if (rv.V - f < Elt<T>::VE) hit &= rv.V > f ? (1u << (rv.V - f)) - 1u : 0u;
+    }
+    return hit;
+}
+
 // The best key of vector `i` of a row that comes after `last` in the order.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void best_after(const RowVectors<T, ALIGNED> &rv, int i, const uint4 &v,
+template <typename T, int MODE>
+__device__ __forceinline__ void best_after(const RowVectors<T, MODE> &rv, int i, const uint4 &v,
                                            const TopKey<typename Elt<T>::acc> &last,
                                            TopKey<typename Elt<T>::acc> &best)
 {
@@ -292,7 +352,7 @@ __device__ __forceinline__ void best_after(const RowVectors<T, ALIGNED> &rv, int
 #pragma unroll
     for (int c = 0; c < E::VE; ++c) {
         const int k = rv.first(i) + c;
-        if (!ALIGNED && (k < 0 || k >= rv.V)) continue;
+        if (MODE == kAny && (k < 0 || k >= rv.V)) continue;
         const Key key = Key::of(e[c], k);
         if (last.before(key) && key.before(best)) best = key;
     }

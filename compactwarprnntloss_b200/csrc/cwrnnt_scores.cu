@@ -8,9 +8,9 @@
 // The lattice's own gather (blank and label of every node) is the special case of two targets; here the columns are
 // free, any V and any alignment is taken, and the entropy and the best alternatives come out of the same pass.
 //
-// Bound: HBM. Forward reads V * sizeof(element) per row, backward reads and writes that much; the statistics of a row
-// stay in registers, a row of up to 512 vectors (8 KB) does too, so that the selection of the largest entries reads
-// nothing again. Longer rows go through a CTA each; their selection reads them a second time, from L2.
+// Bound: HBM. Forward reads V * sizeof(element) per row, backward reads and writes that much. Rows of up to 256 vectors
+// (4 KB) stay in the registers of the lanes that share them, longer ones run through a warp or a CTA each with their
+// statistics alongside; the selection of the largest entries reads those again, from L1 or L2.
 //
 // Selection: of the lanes' own maxima, the largest value that at least k of them reach is a lower bound of the row's
 // k-th largest entry. The entries at or above it - about as many as k - are collected in shared memory and ranked by
@@ -90,15 +90,44 @@ struct Candidate<__nv_bfloat16> : ShortCandidate<__nv_bfloat16> {};
 
 __host__ __device__ constexpr int candidates_of(int lpr) { return 4 * lpr; }
 
+// A lower bound of a row's k-th largest entry that about k entries reach: of the maxima of its lanes (of their two halves,
+// where k is more than half the lanes), the smallest that fewer than k exceed. All lanes of a warp call this together.
+template <int LPR, typename A>
+__device__ __forceinline__ A bar_of(A early, A late, int k)
+{
+    constexpr unsigned kAll = 0xffffffffu;
+    A bar = A(INFINITY);
+    if (2 * k <= LPR) {
+        const A own = Base2<A>::max_of(early, late);
+        int above = 0;
+#pragma unroll 8
+        for (int j = 0; j < LPR; ++j) above += __shfl_sync(kAll, own, j, LPR) > own;
+        if (above < k) bar = own;
+    } else {
+        int above0 = 0, above1 = 0;
+#pragma unroll 4
+        for (int j = 0; j < LPR; ++j) {
+            const A o0 = __shfl_sync(kAll, early, j, LPR), o1 = __shfl_sync(kAll, late, j, LPR);
+            above0 += (o0 > early) + (o1 > early);
+            above1 += (o0 > late) + (o1 > late);
+        }
+        if (above0 < k) bar = early;
+        if (above1 < k) bar = fmin(bar, late);
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) bar = fmin(bar, __shfl_xor_sync(kAll, bar, o));
+    return bar;
+}
+
 // The largest entries one after the other, each by a pass over the row (from L1 or L2): for the rows of `slow` groups. Kept
 // out of line, or its keys would take the registers of the usual path.
-template <typename T, int LPR, bool ALIGNED>
+template <typename T, int LPR, int MODE>
 __device__ __noinline__ void pick_one_by_one(const ScoresArgs<T> &a, const T *row, int64_t r,
                                              RowLog<typename Elt<T>::acc> log, bool slow)
 {
     using Key = TopKey<typename Elt<T>::acc>;
     const int gl = threadIdx.x % LPR;
-    const RowVectors<T, ALIGNED> rv(row, a.V);
+    const RowVectors<T, MODE> rv(row, a.V);
     Key last = Key::all();
     for (int round = 0; round < a.top_k; ++round) {
         Key best = Key::none();
@@ -118,7 +147,7 @@ __device__ __noinline__ void pick_one_by_one(const ScoresArgs<T> &a, const T *ro
 
 // Rows of at most LPR * NV vectors: LPR lanes hold a row in NV vectors each. All lanes of a warp take every collective
 // step together, whichever of their groups has a row left. Group g of a CTA takes the rows first + g, + GPC, ..
-template <typename T, int LPR, int NV, bool ALIGNED, bool ENT>
+template <typename T, int LPR, int NV, int MODE, bool ENT>
 __global__ void __launch_bounds__(kRowThreads)
 scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
 {
@@ -141,25 +170,26 @@ scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
         const bool active = r < a.n_rows;
         if (!__any_sync(kAll, active)) break;
         const T *row = a.x + (active ? r : 0) * a.x_stride;
-        const RowVectors<T, ALIGNED> rv(row, a.V);
+        const RowVectors<T, MODE> rv(row, a.V);
         uint4 v[NV];
+        rv.template load_all<LPR>(v, gl, active);
+        const int target = active && gl < a.n_targets ? __ldg(a.targets + r * a.n_targets + gl) : -1;
+        A own = A(-INFINITY), own_late = A(-INFINITY);  // over the first and the second half of the lane's vectors
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            v[j] = vector_of_nothing<T>();
-            if (active && j * LPR + gl < rv.count) v[j] = rv.load(j * LPR + gl);
+            if (j < NV / 2)
+                own = M::max_of(own, E::vec_max(v[j]));
+            else
+                own_late = M::max_of(own_late, E::vec_max(v[j]));
         }
-        const int target = active && gl < a.n_targets ? __ldg(a.targets + r * a.n_targets + gl) : -1;
-        A own = A(-INFINITY);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) own = M::max_of(own, E::vec_max(v[j]));
         RowStats<A> st;
         st.clear();
-        st.max = own;
+        st.max = M::max_of(own, own_late);
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) st.max = M::max_of(st.max, __shfl_xor_sync(kAll, st.max, o));
-        const A shift = RowStats<A>::shift_of(st.max, a.kappa);
+        const TermsAt<T> terms(st.max, a.kappa);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) add_terms<T, ENT>(v[j], a.kappa, st.max, shift, st.s, st.t);
+        for (int j = 0; j < NV; ++j) add_terms<T, ENT>(v[j], a.kappa, terms, st.s, st.t);
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) {
             st.s += __shfl_xor_sync(kAll, st.s, o);
@@ -177,13 +207,7 @@ scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
                 emit_target(a, row, r, log, __ldg(a.targets + r * a.n_targets + i), i);
         }
         if (a.top_k > 0) {
-            // the bar: a lane whose maximum fewer than k lanes exceed is at or below it
-            int above = 0;
-#pragma unroll 8
-            for (int j = 0; j < LPR; ++j) above += __shfl_sync(kAll, own, j, LPR) > own;
-            A bar = above < a.top_k ? own : A(INFINITY);
-#pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) bar = fmin(bar, __shfl_xor_sync(kAll, bar, o));
+            A bar = bar_of<LPR>(own, own_late, a.top_k);
             int n = 0;
             auto collect = [&](uint32_t bits, int j0) {
                 // one candidate of every lane at a time; their places follow from the ballot
@@ -207,13 +231,9 @@ scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
 #pragma unroll
                 for (int j = j0; j < NV && j < j0 + kPer; ++j) {
                     const int i = j * LPR + gl;
-                    uint32_t hit = at_least<T>(v[j], bar);
-                    if (!ALIGNED) {  // elements before and behind the row
-                        const int f = rv.first(i);
-                        if (f < 0) hit &= ~0u << (-f);
-                        if (a.V - f < E::VE) hit &= a.V > f ? (1u << (a.V - f)) - 1u : 0u;
-                    }
-                    if (!active || i >= rv.count) hit = 0;
+                    uint32_t hit = at_least(rv, i, v[j], bar);
+                    if (MODE != kFull && i >= rv.count) hit = 0;
+                    if (!active) hit = 0;
                     bits |= hit << ((j - j0) * E::VE);
                 }
                 collect(bits, j0);
@@ -228,147 +248,158 @@ scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
                     if (before < a.top_k) emit_top(a, row, r, log, before, Cand::index(mine));
                 }
             }
-            if (__any_sync(kAll, slow)) pick_one_by_one<T, LPR, ALIGNED>(a, row, r, log, slow);
+            if (__any_sync(kAll, slow)) pick_one_by_one<T, LPR, MODE>(a, row, r, log, slow);
             __syncwarp();  // the next row fills the same buffer
         }
     }
 }
 
-// Statistics of a row over the CTA, the same bits in every thread: the warps' parts are joined in warp order.
-template <typename A, bool ENT>
-__device__ __forceinline__ RowStats<A> join_cta(RowStats<A> st, A kappa, RowStats<A> *parts)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        RowStats<A> other;
-        other.max = __shfl_xor_sync(0xffffffffu, st.max, o);
-        other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        other.t = ENT ? __shfl_xor_sync(0xffffffffu, st.t, o) : A(0);
-        st.template join<ENT>(other, kappa);
-    }
-    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = st;
-    __syncthreads();
-    st = parts[0];
-#pragma unroll
-    for (int w = 1; w < kRowThreads / 32; ++w) st.template join<ENT>(parts[w], kappa);
-    return st;
-}
-
-// Any row: one CTA each, four vectors of every thread in flight, running statistics.
-template <typename T, bool ALIGNED, bool ENT>
+// Rows that registers do not hold: a warp each (LANES = 32) or a CTA each (LANES = 256). The statistics run along; four
+// vectors of every lane are in flight while four are added up. The selection reads the row again, from L1 or L2.
+template <typename T, int LANES, int MODE, bool ENT>
 __global__ void __launch_bounds__(kRowThreads)
-scores_long_kernel(const ScoresArgs<T> a)
+scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
 {
     using E = Elt<T>;
     using A = typename E::acc;
     using M = Base2<A>;
     using Key = TopKey<A>;
-    constexpr int NV = 4, kCap = 512, kBars = 64, kWarps = kRowThreads / 32;
-    __shared__ RowStats<A> parts[kWarps];
-    __shared__ Key keys[kCap];
-    __shared__ Key best_of[kWarps];
-    __shared__ A bars[kBars];
-    __shared__ A bar_shared;
+    constexpr int NV = 4, kWarps = kRowThreads / 32, kCap = LANES == 32 ? 96 : 512, kBars = 64;
+    constexpr unsigned kAll = 0xffffffffu;
+    extern __shared__ __align__(16) unsigned char scratch[];  // kCap keys per row of the CTA, when top_k > 0
+    __shared__ RowStats<A> parts[LANES == 32 ? 1 : kWarps];
+    __shared__ A bars[LANES == 32 ? 1 : kBars];
     __shared__ int counter;
-    const int tid = threadIdx.x;
-    const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int me = LANES == 32 ? lane : threadIdx.x;
+    const int64_t r = LANES == 32 ? int64_t(blockIdx.x) * kWarps + warp : int64_t(blockIdx.x);
+    if (r >= a.n_rows) return;  // whole warps (or the CTA) leave together
+    Key *const keys = reinterpret_cast<Key *>(scratch) + (LANES == 32 ? warp * kCap : 0);
     const T *row = a.x + r * a.x_stride;
-    const RowVectors<T, ALIGNED> rv(row, a.V);
-    if (tid == 0) counter = 0;
+    const RowVectors<T, MODE> rv(row, a.V);
+    if (LANES > 32 && threadIdx.x == 0) counter = 0;
+
+    // f(first vector, four vectors LANES apart) over the row
+    auto sweep = [&](auto &&f) {
+        uint4 v[NV], ahead[NV];
+        auto load = [&](uint4(&to)[NV], int at) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int i = at + j * LANES;
+                to[j] = vector_of_nothing<T>();
+                if (i < rv.count) to[j] = rv.load(i);
+            }
+        };
+        load(v, me);
+#pragma unroll 1
+        for (int at = me; at - me < rv.count; at += NV * LANES) {
+            if (at - me + NV * LANES < rv.count) load(ahead, at + NV * LANES);
+            f(at, v);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) v[j] = ahead[j];
+        }
+    };
 
     RowStats<A> st;
     st.clear();
-    for (int at = 0; at < rv.count; at += kRowThreads * NV) {
-        uint4 v[NV];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = at + j * kRowThreads + tid;
-            v[j] = i < rv.count ? rv.load(i) : vector_of_nothing<T>();
-        }
-        A m = st.max;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) m = M::max_of(m, E::vec_max(v[j]));
+    A early = A(-INFINITY), late = A(-INFINITY);  // maxima over the first and the second two vectors of each four
+    sweep([&](int, const uint4(&v)[NV]) {
+        early = M::max_of(early, M::max_of(E::vec_max(v[0]), E::vec_max(v[1])));
+        late = M::max_of(late, M::max_of(E::vec_max(v[2]), E::vec_max(v[3])));
+        const A m = M::max_of(early, late);
         if (m > st.max) st.template raise<ENT>(m, a.kappa);
-        const A shift = RowStats<A>::shift_of(st.max, a.kappa);
+        const TermsAt<T> terms(st.max, a.kappa);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) add_terms<T, ENT>(v[j], a.kappa, st.max, shift, st.s, st.t);
-    }
+        for (int j = 0; j < NV; ++j) add_terms<T, ENT>(v[j], a.kappa, terms, st.s, st.t);
+    });
     const A own = st.max;
-    st = join_cta<A, ENT>(st, a.kappa, parts);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        RowStats<A> other;
+        other.max = __shfl_xor_sync(kAll, st.max, o);
+        other.s = __shfl_xor_sync(kAll, st.s, o);
+        other.t = ENT ? __shfl_xor_sync(kAll, st.t, o) : A(0);
+        st.template join<ENT>(other, a.kappa);
+    }
+    if (LANES > 32) {  // the warps' parts, joined in their order: the same bits in every thread
+        A four = M::max_of(own, __shfl_xor_sync(kAll, own, 1));
+        four = M::max_of(four, __shfl_xor_sync(kAll, four, 2));
+        if (lane == 0) parts[warp] = st;
+        if (lane % 4 == 0) bars[threadIdx.x / 4] = four;
+        __syncthreads();
+        st = parts[0];
+#pragma unroll 1
+        for (int w = 1; w < kWarps; ++w) st.template join<ENT>(parts[w], a.kappa);
+    }
     const A sum = st.sum(a.kappa);
     const RowLog<A> log{st.max, st.nothing() ? A(0) : M::ln_of(sum)};
-    if (tid == 0) {
+    if (me == 0) {
         if (ENT) a.entropy[r] = st.entropy();
         if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = sum;
     }
-    if (tid < a.n_targets) emit_target(a, row, r, log, __ldg(a.targets + r * a.n_targets + tid), tid);
+    if (me < a.n_targets) emit_target(a, row, r, log, __ldg(a.targets + r * a.n_targets + me), me);
     if (a.top_k == 0) return;
 
-    // the bar: the k-th largest of the maxima of 64 groups of four threads
-    A four = M::max_of(own, __shfl_xor_sync(0xffffffffu, own, 1));
-    four = M::max_of(four, __shfl_xor_sync(0xffffffffu, four, 2));
-    if (tid % 4 == 0) bars[tid / 4] = four;
-    __syncthreads();
-    if (tid < kBars) {
-        const A mine = bars[tid];
-        int rank = 0;
-        for (int j = 0; j < kBars; ++j) rank += bars[j] > mine || (bars[j] == mine && j < tid);
-        if (rank == a.top_k - 1) bar_shared = mine;
-    }
-    __syncthreads();
-    const A bar = bar_shared;
-    for (int at = 0; at < rv.count; at += kRowThreads * NV) {
-        uint4 v[NV];
+    A bar = A(INFINITY);
+    if (LANES == 32) {
+        bar = bar_of<32>(early, late, a.top_k);
+    } else {  // of 64 groups of four lanes
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = at + j * kRowThreads + tid;
-            v[j] = i < rv.count ? rv.load(i) : vector_of_nothing<T>();
+        for (int h = 0; h < 2; ++h) {
+            const A mine = bars[lane + 32 * h];
+            int above = 0;
+#pragma unroll 8
+            for (int j = 0; j < kBars; ++j) above += bars[j] > mine;
+            if (above < a.top_k) bar = fmin(bar, mine);
         }
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = at + j * kRowThreads + tid;
-            if (i < rv.count && E::vec_max(v[j]) >= bar) {
-                A e[E::VE];
-                E::unpack(v[j], e);
+        for (int o = 16; o > 0; o >>= 1) bar = fmin(bar, __shfl_xor_sync(kAll, bar, o));
+    }
+    int n = 0;
+    sweep([&](int at, const uint4(&v)[NV]) {
+        uint32_t bits = 0;
 #pragma unroll
-                for (int c = 0; c < E::VE; ++c) {
-                    const int k = rv.first(i) + c;
-                    if (e[c] >= bar && (ALIGNED || (k >= 0 && k < a.V))) {
-                        const int n = atomicAdd(&counter, 1);
-                        if (n < kCap) keys[n] = Key::of(e[c], k);
-                    }
-                }
+        for (int j = 0; j < NV; ++j) {
+            const int i = at + j * LANES;
+            if (i < rv.count) bits |= at_least(rv, i, v[j], bar) << (j * E::VE);
+        }
+        // one candidate of every lane at a time; their places follow from the ballot
+        for (;;) {
+            const unsigned have = __ballot_sync(kAll, bits != 0);
+            if (!have) break;
+            int base = n;
+            if (LANES > 32) {
+                if (lane == 0) base = atomicAdd(&counter, __popc(have));
+                base = __shfl_sync(kAll, base, 0);
             }
+            if (bits) {
+                const int b = __ffs(bits) - 1;
+                bits &= bits - 1;
+                const int k = rv.first(at + b / E::VE * LANES) + b % E::VE;
+                const int to = base + __popc(have & ((1u << lane) - 1u));
+                if (to < kCap) keys[to] = Key::of(E::to_acc(__ldg(row + k)), k);
+            }
+            n += __popc(have);
         }
+    });
+    if (LANES > 32) {
+        __syncthreads();
+        n = counter;
+    } else {
+        __syncwarp();
     }
-    __syncthreads();
-    const int n = counter;
     if (n <= kCap && n >= a.top_k && st.s == st.s) {
-        for (int i = tid; i < n; i += kRowThreads) {
+        for (int i = me; i < n; i += LANES) {
             const Key mine = keys[i];
             int before = 0;
+#pragma unroll 4
             for (int j = 0; j < n; ++j) before += keys[j].before(mine);
             if (before < a.top_k) emit_top(a, row, r, log, before, mine.index());
         }
         return;
     }
-    Key last = Key::all();
-    for (int round = 0; round < a.top_k; ++round) {
-        Key best = Key::none();
-        for (int i = tid; i < rv.count; i += kRowThreads) best_after(rv, i, rv.load(i), last, best);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const Key other = shfl_xor_key(0xffffffffu, best, o);
-            if (other.before(best)) best = other;
-        }
-        if ((tid & 31) == 0) best_of[tid >> 5] = best;
-        __syncthreads();
-        for (int w = 0; w < kWarps; ++w)
-            if (best_of[w].before(best)) best = best_of[w];
-        last = best;
-        if (tid == 0) emit_top(a, row, r, log, round, best.index());
-        __syncthreads();  // the next round fills best_of again
-    }
+    // (uniform over the row's lanes)
+    if (LANES == 32 || warp == 0) pick_one_by_one<T, 32, MODE>(a, row, r, log, true);
 }
 
 template <typename T>
@@ -400,7 +431,7 @@ struct ScoresGradArgs {
 // Element-wise once the row's maximum and sum are known: LPR threads a row (a part of a warp, a warp, or a CTA), four
 // vectors of each in flight. The entries that were picked are written a second time behind a barrier, by the first entry
 // that names them, which adds up all that do (in their order: the sum does not depend on timing).
-template <typename T, int LPR, bool ALIGNED>
+template <typename T, int LPR, int MODE>
 __global__ void __launch_bounds__(kRowThreads)
 scores_grad_kernel(const ScoresGradArgs<T> a)
 {
@@ -417,8 +448,8 @@ scores_grad_kernel(const ScoresGradArgs<T> a)
     const int64_t rr = active ? r : 0;
     const T *row = a.x + rr * a.x_stride;
     T *out = a.gx + rr * a.g_stride;
-    const RowVectors<T, ALIGNED> rv(row, a.V);
-    const bool same = ALIGNED || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    const RowVectors<T, MODE> rv(row, a.V);
+    const bool same = MODE != kAny || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
 
     uint4 v[NV];
 #pragma unroll
@@ -458,7 +489,7 @@ scores_grad_kernel(const ScoresGradArgs<T> a)
                         const A d = (e[c] - top) * a.kappa;
                         e[c] = M::exp2_of(d) * M::fma_of(c1, M::max_of(d, M::kFloor), c0);
                     }
-                    store_vector(out, rv, i, same, e);
+                    rv.store(out, i, same, e);
                 }
             }
         }
@@ -511,10 +542,29 @@ cudaError_t launch_scores_rows(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
     const int run_len = 1;
     const int64_t grid = (a.n_rows + int64_t(GPC) * run_len - 1) / (int64_t(GPC) * run_len);
     const size_t smem = a.top_k > 0 ? GPC * candidates_of(LPR) * sizeof(typename Candidate<T>::Word) : 0;
+    auto go = [&](auto kernel) {
+        kernel<<<unsigned(grid), kRowThreads, smem, s>>>(a, run_len);
+        return cudaGetLastError();
+    };
+    if constexpr (ALIGNED) {
+        if (a.V == LPR * NV * Elt<T>::VE)
+            return ent ? go(scores_rows_kernel<T, LPR, NV, kFull, true>) : go(scores_rows_kernel<T, LPR, NV, kFull, false>);
+        return ent ? go(scores_rows_kernel<T, LPR, NV, kAligned, true>)
+                   : go(scores_rows_kernel<T, LPR, NV, kAligned, false>);
+    }
+    return ent ? go(scores_rows_kernel<T, LPR, NV, kAny, true>) : go(scores_rows_kernel<T, LPR, NV, kAny, false>);
+}
+
+template <typename T, int LANES, bool ALIGNED>
+cudaError_t launch_scores_stream(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
+{
+    constexpr int rows = kRowThreads / LANES, MODE = ALIGNED ? kAligned : kAny;
+    const size_t smem = a.top_k > 0 ? (LANES == 32 ? rows * 96 : 512) * sizeof(TopKey<typename Elt<T>::acc>) : 0;
+    const unsigned grid = unsigned((a.n_rows + rows - 1) / rows);
     if (ent)
-        scores_rows_kernel<T, LPR, NV, ALIGNED, true><<<unsigned(grid), kRowThreads, smem, s>>>(a, run_len);
+        scores_stream_kernel<T, LANES, MODE, true><<<grid, kRowThreads, smem, s>>>(a);
     else
-        scores_rows_kernel<T, LPR, NV, ALIGNED, false><<<unsigned(grid), kRowThreads, smem, s>>>(a, run_len);
+        scores_stream_kernel<T, LANES, MODE, false><<<grid, kRowThreads, smem, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -534,12 +584,9 @@ cudaError_t launch_scores_t(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
     }
     if (nv <= 128) return launch_scores_rows<T, 32, 4, ALIGNED>(a, ent, s);
     if (nv <= 256) return launch_scores_rows<T, 32, 8, ALIGNED>(a, ent, s);
-    if (nv <= 512) return launch_scores_rows<T, 32, 16, ALIGNED>(a, ent, s);
-    if (ent)
-        scores_long_kernel<T, ALIGNED, true><<<unsigned(a.n_rows), kRowThreads, 0, s>>>(a);
-    else
-        scores_long_kernel<T, ALIGNED, false><<<unsigned(a.n_rows), kRowThreads, 0, s>>>(a);
-    return cudaGetLastError();
+    // a warp carries a longer row where there are rows enough for the SMs' warps
+    if (nv <= 2048 && a.n_rows >= kNumSMs * 32) return launch_scores_stream<T, 32, ALIGNED>(a, ent, s);
+    return launch_scores_stream<T, kRowThreads, ALIGNED>(a, ent, s);
 }
 
 template <typename T>
@@ -564,14 +611,15 @@ cudaError_t launch_scores_of(const cwrnnt_rows &p, const void *x, const int32_t 
 template <typename T, bool ALIGNED>
 cudaError_t launch_scores_grad_t(const ScoresGradArgs<T> &a, cudaStream_t s)
 {
+    constexpr int kMode = ALIGNED ? kAligned : kAny;
     const int nv = vectors_of<T>(a.V, ALIGNED);
     auto grid = [&](int lpr) { return unsigned((a.n_rows + kRowThreads / lpr - 1) / (kRowThreads / lpr)); };
     if (nv <= 32)
-        scores_grad_kernel<T, 8, ALIGNED><<<grid(8), kRowThreads, 0, s>>>(a);
+        scores_grad_kernel<T, 8, kMode><<<grid(8), kRowThreads, 0, s>>>(a);
     else if (nv <= 1024)
-        scores_grad_kernel<T, 32, ALIGNED><<<grid(32), kRowThreads, 0, s>>>(a);
+        scores_grad_kernel<T, 32, kMode><<<grid(32), kRowThreads, 0, s>>>(a);
     else
-        scores_grad_kernel<T, kRowThreads, ALIGNED><<<grid(kRowThreads), kRowThreads, 0, s>>>(a);
+        scores_grad_kernel<T, kRowThreads, kMode><<<grid(kRowThreads), kRowThreads, 0, s>>>(a);
     return cudaGetLastError();
 }
 
