@@ -123,10 +123,9 @@ __device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, in
     for (int o = 0; o < K; ++o) {
         const int other = __shfl_sync(kAll, en.c, o, LPR);
         const A oq = __shfl_sync(kAll, en.q, o, LPR);
-        if (other == en.c) {
-            en.dup_q += oq;
-            if (o < gl) en.first = false;
-        }
+        const bool mine = other == en.c;
+        en.dup_q += mine ? oq : A(0);
+        en.first = en.first && !(mine && o < gl);
     }
     return en;
 }
@@ -302,8 +301,9 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
         const Entries<A> en = weigh_entries<LPR, TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, gl);
         if (TAIL) {
             for (int e = 0; e < a.K; ++e) {
-                const int at = __shfl_sync(kAll, en.c, e, LPR) + rv.head, i = at / VE;
-                if (at >= rv.head && i % LPR == gl) {
+                const int token = __shfl_sync(kAll, en.c, e, LPR);
+                const int at = rv.place(token < 0 ? 0 : token), i = at / VE;
+                if (token >= 0 && i % LPR == gl) {
 #pragma unroll
                     for (int j = 0; j < NV; ++j)
                         if (i == j * LPR + gl) blank_element<T>(v[j], at % VE);
@@ -380,10 +380,8 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
     using A = typename E::acc;
     using M = Base2<A>;
     constexpr int NV = 4, kWarps = kRowThreads / 32;
-    constexpr unsigned kAll = 0xffffffffu;
     __shared__ RowStats<A> parts[LANES == 32 ? 1 : kWarps];
-    __shared__ int listed_of[LANES == 32 ? kWarps : 1][32];  // positions of the listed tokens, counted from the first
-                                                             // vector's start; -1: none
+    __shared__ int listed_of[LANES == 32 ? kWarps : 1][32];  // places of the listed tokens; -1: none
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int me = LANES == 32 ? lane : threadIdx.x;
     const int64_t r = LANES == 32 ? int64_t(blockIdx.x) * kWarps + warp : int64_t(blockIdx.x);
@@ -402,30 +400,10 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
             c = __ldg(a.index + r * a.K + lane);
             value = A(__ldg(a.teacher + r * a.K + lane));
         }
-        // f(first vector, four vectors LANES apart) over the row
-        auto sweep = [&](auto &&f) {
-            uint4 v[NV], ahead[NV];
-            auto load = [&](uint4(&to)[NV], int at) {
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int i = at + j * LANES;
-                    to[j] = vector_of_nothing<T>();
-                    if (seen && i < rv.count) to[j] = rv.load(i);
-                }
-            };
-            load(v, me);
-#pragma unroll 1
-            for (int at = me; at - me < rv.count; at += NV * LANES) {
-                if (at - me + NV * LANES < rv.count) load(ahead, at + NV * LANES);
-                f(at, v);
-#pragma unroll
-                for (int j = 0; j < NV; ++j) v[j] = ahead[j];
-            }
-        };
         int *const listed = listed_of[LANES == 32 ? warp : 0];
         const A xc = c >= 0 && c < a.V ? E::to_acc(__ldg(row + c)) : A(-INFINITY);
         const Entries<A> en = weigh_entries<32, TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, lane);
-        if (me < 32) listed[lane] = en.c >= 0 ? en.c + rv.head : -1;
+        if (me < 32) listed[lane] = en.c >= 0 ? rv.place(en.c) : -1;
         if (LANES == 32)
             __syncwarp();
         else
@@ -444,7 +422,7 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
         st.clear();
         if (seen) {
             int next = TAIL ? next_listed(0) : 0x7fffffff;
-            sweep([&](int at, uint4(&v)[NV]) {
+            rv.template sweep<LANES>(me, true, [&](int at, uint4(&v)[NV]) {
                 if (TAIL && next < at + NV * LANES) {
                     const int past = at + NV * LANES;
                     for (int e = 0; e < a.K; ++e) {
@@ -465,14 +443,7 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
                 for (int j = 0; j < NV; ++j) add_terms<T, false>(v[j], a.kappa, terms, st.s, st.t);
             });
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            RowStats<A> other;
-            other.max = __shfl_xor_sync(kAll, st.max, o);
-            other.s = __shfl_xor_sync(kAll, st.s, o);
-            other.t = A(0);
-            st.template join<false>(other, a.kappa);
-        }
+        join_lanes<32, false>(st, a.kappa);
         if (LANES > 32) {  // the warps' parts, joined in their order: the same bits in every thread
             if (lane == 0) parts[warp] = st;
             __syncthreads();
@@ -486,7 +457,7 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
         loss = res.loss;
         if (me == 0 && a.row_loss) a.row_loss[r] = loss;
         if (out) {
-            sweep([&](int at, uint4(&v)[NV]) {
+            rv.template sweep<LANES>(me, seen, [&](int at, uint4(&v)[NV]) {
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
                     const int i = at + j * LANES;

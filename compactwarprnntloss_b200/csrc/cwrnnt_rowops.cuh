@@ -8,10 +8,9 @@ namespace cwrnnt {
 constexpr int kRowThreads = 256;  // threads of a CTA in the row operators
 
 // ------------------------------------------------------------------------------------------------ rows as vectors
-// Vector i of a row covers the elements [i*VE - head, i*VE - head + VE), where `head` elements lie between the last
-// 16-byte boundary at or below the row's start and that start: vectors are always aligned, whatever V and the row
-// stride. The first and the last vector can reach over the row's ends; they are put together element by element, with
-// -inf outside, so nothing outside the row is read. What a launch knows of its rows:
+// A row is read in 16-byte vectors that lie on 16-byte boundaries, whatever V and the row stride. What lies before the
+// first boundary and behind the last is put together element by element, with -inf outside the row, so nothing outside
+// it is read. What a launch knows of its rows:
 //   kAny      nothing
 //   kAligned  every row starts and ends on a 16-byte boundary
 //   kFull     the same, and a row is exactly the vectors that its lanes hold in registers
@@ -52,24 +51,48 @@ __device__ __forceinline__ uint4 vector_of_nothing()
     }
 }
 
+// The whole vectors come first (0 .. whole_count-1, one load each), then the edges, if there are any: the elements before
+// the first boundary, then those behind the last.
 template <typename T, int MODE>
 struct RowVectors {
     static constexpr int VE = Elt<T>::VE;
     const T *row;
-    int V, head, count;
+    int V, lead, whole_count, count;  // lead: elements before the first boundary
     __device__ __forceinline__ RowVectors(const T *row_, int V_) : row(row_), V(V_)
     {
-        head = MODE != kAny ? 0 : int((reinterpret_cast<uintptr_t>(row_) & 15) / sizeof(T));
-        count = MODE != kAny ? V_ / VE : (V_ + head + VE - 1) / VE;
+        if (MODE != kAny) {
+            lead = 0;
+            count = whole_count = V_ / VE;
+            return;
+        }
+        lead = int((16 - (reinterpret_cast<uintptr_t>(row_) & 15)) & 15) / int(sizeof(T));
+        if (lead > V_) {  // the row lies between two boundaries
+            whole_count = 0;
+            count = 1;
+        } else {
+            whole_count = (V_ - lead) / VE;
+            count = whole_count + (lead > 0) + (lead + whole_count * VE < V_);
+        }
     }
-    __device__ __forceinline__ int first(int i) const { return i * VE - head; }
-    __device__ __forceinline__ bool whole(int i) const
+    __device__ __forceinline__ bool whole(int i) const { return MODE != kAny || i < whole_count; }
+    // first element of vector i (before the row, if it is the leading edge)
+    __device__ __forceinline__ int first(int i) const
     {
-        return MODE != kAny || (first(i) >= 0 && first(i) + VE <= V);
+        if (MODE != kAny) return i * VE;
+        return i < whole_count ? lead + i * VE : (i == whole_count && lead > 0 ? lead - VE : lead + whole_count * VE);
+    }
+    // where element k lies: vector * VE + place in it
+    __device__ __forceinline__ int place(int k) const
+    {
+        if (MODE != kAny) return k;
+        const int behind = lead + whole_count * VE;
+        if (k < lead) return whole_count * VE + k - (lead - VE);
+        if (k >= behind) return (whole_count + (lead > 0)) * VE + k - behind;
+        return k - lead;
     }
     __device__ __forceinline__ uint4 load(int i) const
     {
-        if (whole(i)) return __ldg(reinterpret_cast<const uint4 *>(row + first(i)));
+        if (whole(i)) return __ldg(reinterpret_cast<const uint4 *>(row + lead) + i);
         return load_edge(row, first(i), V);
     }
     // vectors lane, lane + LANES, .. of the row into registers
@@ -82,13 +105,35 @@ struct RowVectors {
             if (MODE == kFull ? active : active && j * LANES + lane < count) v[j] = load(j * LANES + lane);
         }
     }
+    // f(i, v) for all vectors of the row, four a lane at a time (v[j] is vector i + j * LANES, nothing behind the last):
+    // straight loads but for the last of them
+    template <int LANES, typename F>
+    __device__ __forceinline__ void sweep(int lane, bool seen, F &&f) const
+    {
+#pragma unroll 1
+        for (int at = 0; at < count; at += 4 * LANES) {
+            uint4 v[4];
+            if (seen && at + 4 * LANES <= whole_count) {
+                const uint4 *p = reinterpret_cast<const uint4 *>(row + lead) + at + lane;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = __ldg(p + j * LANES);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = vector_of_nothing<T>();
+                    if (seen && at + j * LANES + lane < count) v[j] = load(at + j * LANES + lane);
+                }
+            }
+            f(at + lane, v);
+        }
+    }
     // Stores vector i of a row of gradients. `same`: the output row has the input row's alignment, so that vector i is
     // one 16-byte store; else element by element.
     __device__ __forceinline__ void store(T *out, int i, bool same, const typename Elt<T>::acc (&e)[VE]) const
     {
         const uint4 v = Elt<T>::pack(e);
         if (MODE != kAny || (same && whole(i)))
-            *reinterpret_cast<uint4 *>(out + first(i)) = v;
+            *(reinterpret_cast<uint4 *>(out + lead) + i) = v;
         else
             store_edge(out, first(i), V, v);
     }
@@ -166,18 +211,28 @@ struct RowStats {
     }
     // no finite entry (and no NaN either)
     __device__ __forceinline__ bool nothing() const { return max == A(-INFINITY) && s == s; }
-    // sum 2^((x - max) * kappa), the rounding of the shift undone
-    __device__ __forceinline__ A sum(A kappa) const
+    // log2 of the factor by which the rounding of the shift has made the sums too large
+    __device__ __forceinline__ A excess(A kappa) const
     {
         const A shift = shift_of(max, kappa);
-        if (extreme(shift) || max == A(-INFINITY)) return s;
-        return s * Base2<A>::exp2_of(-Base2<A>::fma_of(max, kappa, -shift));
+        if (extreme(shift) || max == A(-INFINITY)) return A(0);
+        return Base2<A>::fma_of(max, kappa, -shift);
     }
-    // entropy of the row's softmax: ln s - ln2 * t / s
-    __device__ __forceinline__ A entropy() const
+    // sum 2^((x - max) * kappa)
+    __device__ __forceinline__ A sum(A kappa) const { return s * Base2<A>::exp2_of(-excess(kappa)); }
+};
+
+// What a row's log-probabilities are taken from, and its entropy ln s - ln2 * t / s: of a row's joined statistics.
+template <typename A>
+struct RowLog {
+    A max, sum, ln_s, entropy;
+    __device__ __forceinline__ RowLog(const RowStats<A> &st, A kappa) : max(st.max)
     {
-        if (s == A(0)) return A(0);
-        return Base2<A>::ln_of(s) - A(kLn2) * (t / s);
+        using M = Base2<A>;
+        const A over = st.excess(kappa), ln = M::ln_of(st.s);
+        sum = st.s * M::exp2_of(-over);
+        ln_s = st.nothing() ? A(0) : ln - A(kLn2) * over;
+        entropy = st.s == A(0) ? A(0) : ln - A(kLn2) * M::ratio(st.t, st.s);
     }
 };
 
@@ -187,6 +242,21 @@ template <typename A>
 __device__ __forceinline__ A log_prob_of(A x, A max, A inv_tau, A ln_s)
 {
     return x == A(-INFINITY) ? (ln_s == ln_s ? A(-INFINITY) : A(NAN)) : Base2<A>::fma_of(x - max, inv_tau, -ln_s);
+}
+
+// The statistics of a row over the lanes of a warp that hold its parts: to the common maximum, then added up.
+template <int LANES, bool ENT, typename A>
+__device__ __forceinline__ void join_lanes(RowStats<A> &st, A kappa)
+{
+    A m = st.max;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = Base2<A>::max_of(m, __shfl_xor_sync(0xffffffffu, m, o));
+    st.template raise<ENT>(m, kappa);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+        if (ENT) st.t += __shfl_xor_sync(0xffffffffu, st.t, o);
+    }
 }
 
 // How a row's (or a thread's) terms are formed at a fixed maximum: as x*kappa - shift, or from the difference to the

@@ -38,12 +38,6 @@ struct ScoresArgs {
     C *stats;
 };
 
-// What a row's log-probabilities are taken from.
-template <typename A>
-struct RowLog {
-    A max, ln_s;
-};
-
 template <typename T>
 __device__ __forceinline__ void emit_top(const ScoresArgs<T> &a, const T *row, int64_t r,
                                          const RowLog<typename Elt<T>::acc> &log, int rank, int index)
@@ -195,12 +189,11 @@ scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
             st.s += __shfl_xor_sync(kAll, st.s, o);
             if (ENT) st.t += __shfl_xor_sync(kAll, st.t, o);
         }
-        const A sum = st.sum(a.kappa);
-        const RowLog<A> log{st.max, st.nothing() ? A(0) : M::ln_of(sum)};
+        const RowLog<A> log(st, a.kappa);
         if (active) {
             if (gl == 0) {
-                if (ENT) a.entropy[r] = st.entropy();
-                if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = sum;
+                if (ENT) a.entropy[r] = log.entropy;
+                if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = log.sum;
             }
             if (gl < a.n_targets) emit_target(a, row, r, log, target, gl);
             for (int i = gl + LPR; i < a.n_targets; i += LPR)
@@ -254,8 +247,10 @@ scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
     }
 }
 
-// Rows that registers do not hold: a warp each (LANES = 32) or a CTA each (LANES = 256). The statistics run along; four
-// vectors of every lane are in flight while four are added up. The selection reads the row again, from L1 or L2.
+__host__ __device__ constexpr int stream_candidates(int lanes) { return lanes == 32 ? 96 : 512; }
+
+// Rows that registers do not hold: a warp each (LANES = 32) or a CTA each (LANES = 256). The statistics run along, with
+// four vectors of every lane in flight. The selection reads the row again, from L1 or L2.
 template <typename T, int LANES, int MODE, bool ENT>
 __global__ void __launch_bounds__(kRowThreads)
 scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
@@ -264,7 +259,7 @@ scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
     using A = typename E::acc;
     using M = Base2<A>;
     using Key = TopKey<A>;
-    constexpr int NV = 4, kWarps = kRowThreads / 32, kCap = LANES == 32 ? 96 : 512, kBars = 64;
+    constexpr int NV = 4, kWarps = kRowThreads / 32, kCap = stream_candidates(LANES), kBars = 64;
     constexpr unsigned kAll = 0xffffffffu;
     extern __shared__ __align__(16) unsigned char scratch[];  // kCap keys per row of the CTA, when top_k > 0
     __shared__ RowStats<A> parts[LANES == 32 ? 1 : kWarps];
@@ -279,31 +274,10 @@ scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
     const RowVectors<T, MODE> rv(row, a.V);
     if (LANES > 32 && threadIdx.x == 0) counter = 0;
 
-    // f(first vector, four vectors LANES apart) over the row
-    auto sweep = [&](auto &&f) {
-        uint4 v[NV], ahead[NV];
-        auto load = [&](uint4(&to)[NV], int at) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int i = at + j * LANES;
-                to[j] = vector_of_nothing<T>();
-                if (i < rv.count) to[j] = rv.load(i);
-            }
-        };
-        load(v, me);
-#pragma unroll 1
-        for (int at = me; at - me < rv.count; at += NV * LANES) {
-            if (at - me + NV * LANES < rv.count) load(ahead, at + NV * LANES);
-            f(at, v);
-#pragma unroll
-            for (int j = 0; j < NV; ++j) v[j] = ahead[j];
-        }
-    };
-
     RowStats<A> st;
     st.clear();
     A early = A(-INFINITY), late = A(-INFINITY);  // maxima over the first and the second two vectors of each four
-    sweep([&](int, const uint4(&v)[NV]) {
+    rv.template sweep<LANES>(me, true, [&](int, const uint4(&v)[NV]) {
         early = M::max_of(early, M::max_of(E::vec_max(v[0]), E::vec_max(v[1])));
         late = M::max_of(late, M::max_of(E::vec_max(v[2]), E::vec_max(v[3])));
         const A m = M::max_of(early, late);
@@ -313,14 +287,7 @@ scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
         for (int j = 0; j < NV; ++j) add_terms<T, ENT>(v[j], a.kappa, terms, st.s, st.t);
     });
     const A own = st.max;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        RowStats<A> other;
-        other.max = __shfl_xor_sync(kAll, st.max, o);
-        other.s = __shfl_xor_sync(kAll, st.s, o);
-        other.t = ENT ? __shfl_xor_sync(kAll, st.t, o) : A(0);
-        st.template join<ENT>(other, a.kappa);
-    }
+    join_lanes<32, ENT>(st, a.kappa);
     if (LANES > 32) {  // the warps' parts, joined in their order: the same bits in every thread
         A four = M::max_of(own, __shfl_xor_sync(kAll, own, 1));
         four = M::max_of(four, __shfl_xor_sync(kAll, four, 2));
@@ -331,11 +298,10 @@ scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
 #pragma unroll 1
         for (int w = 1; w < kWarps; ++w) st.template join<ENT>(parts[w], a.kappa);
     }
-    const A sum = st.sum(a.kappa);
-    const RowLog<A> log{st.max, st.nothing() ? A(0) : M::ln_of(sum)};
+    const RowLog<A> log(st, a.kappa);
     if (me == 0) {
-        if (ENT) a.entropy[r] = st.entropy();
-        if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = sum;
+        if (ENT) a.entropy[r] = log.entropy;
+        if (a.stats) a.stats[2 * r] = log.max, a.stats[2 * r + 1] = log.sum;
     }
     if (me < a.n_targets) emit_target(a, row, r, log, __ldg(a.targets + r * a.n_targets + me), me);
     if (a.top_k == 0) return;
@@ -356,7 +322,7 @@ scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
         for (int o = 16; o > 0; o >>= 1) bar = fmin(bar, __shfl_xor_sync(kAll, bar, o));
     }
     int n = 0;
-    sweep([&](int at, const uint4(&v)[NV]) {
+    rv.template sweep<LANES>(me, true, [&](int at, const uint4(&v)[NV]) {
         uint32_t bits = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -539,7 +505,7 @@ template <typename T, int LPR, int NV, bool ALIGNED>
 cudaError_t launch_scores_rows(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
 {
     constexpr int GPC = kRowThreads / LPR;
-    const int run_len = 1;
+    const int run_len = a.n_rows > int64_t(GPC) * kNumSMs * 32 ? 4 : 1;
     const int64_t grid = (a.n_rows + int64_t(GPC) * run_len - 1) / (int64_t(GPC) * run_len);
     const size_t smem = a.top_k > 0 ? GPC * candidates_of(LPR) * sizeof(typename Candidate<T>::Word) : 0;
     auto go = [&](auto kernel) {
@@ -559,7 +525,7 @@ template <typename T, int LANES, bool ALIGNED>
 cudaError_t launch_scores_stream(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
 {
     constexpr int rows = kRowThreads / LANES, MODE = ALIGNED ? kAligned : kAny;
-    const size_t smem = a.top_k > 0 ? (LANES == 32 ? rows * 96 : 512) * sizeof(TopKey<typename Elt<T>::acc>) : 0;
+    const size_t smem = a.top_k > 0 ? rows * stream_candidates(LANES) * sizeof(TopKey<typename Elt<T>::acc>) : 0;
     const unsigned grid = unsigned((a.n_rows + rows - 1) / rows);
     if (ent)
         scores_stream_kernel<T, LANES, MODE, true><<<grid, kRowThreads, smem, s>>>(a);
