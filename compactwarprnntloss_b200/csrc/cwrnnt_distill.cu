@@ -62,22 +62,22 @@ __device__ __forceinline__ double exp_mid(double a)
 __device__ __forceinline__ double teacher_exp(double a, float) { return exp_mid(a); }
 __device__ __forceinline__ double teacher_exp(double a, double) { return exp(a); }
 
-// Sums and maxima over the lanes of a row that hold its entries: lanes 0 .. KP-1 (a power of two, the others hold the
-// neutral element), the result in every lane of the row. All lanes of a warp call these together.
-template <int LPR, typename V>
-__device__ __forceinline__ V entry_sum(V v, int KP)
+// Sums and maxima over the KP lanes (a power of two, at most `width`) that hold a row's entries, the first of the row's
+// `width` lanes; the result in all of them. All lanes of a warp call these together.
+template <typename V>
+__device__ __forceinline__ V entry_sum(V v, int KP, int width)
 {
     for (int o = KP >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return __shfl_sync(0xffffffffu, v, 0, LPR);
+    return __shfl_sync(0xffffffffu, v, 0, width);
 }
-template <int LPR, typename V>
-__device__ __forceinline__ V entry_max(V v, int KP)
+template <typename V>
+__device__ __forceinline__ V entry_max(V v, int KP, int width)
 {
     for (int o = KP >> 1; o > 0; o >>= 1) v = Base2<V>::max_of(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return __shfl_sync(0xffffffffu, v, 0, LPR);
+    return __shfl_sync(0xffffffffu, v, 0, width);
 }
 
-// One row's teacher entry, held by lane e of the row's lanes, and what follows from all of them.
+// One row's teacher entry, held by lane e of `width` lanes that belong to the row, and what follows from all of them.
 template <typename A>
 struct Entries {
     int c;       // token, -1: none
@@ -89,30 +89,29 @@ struct Entries {
     A dup_q;     // q of all entries with this token, added up in their order
 };
 
-// All lanes of a warp call this together; LPR lanes belong to a row, lane `gl` of them holds entry gl: token `c`, value
-// `a` (-1, -inf: none).
-template <int LPR, bool TAIL, typename A>
-__device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, int KP, A inv_tau, int gl)
+// All lanes of a warp call this together; lane `e` of a row's lanes holds entry e: token `c`, value `a` (-1, -inf: none).
+template <bool TAIL, typename A>
+__device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, int KP, A inv_tau, int e, int width)
 {
     constexpr unsigned kAll = 0xffffffffu;
     using M = Base2<A>;
     Entries<A> en;
-    const unsigned outside = __ballot_sync(kAll, c >= V);
-    en.bad = ((outside >> ((threadIdx.x & 31) / LPR * LPR)) & (LPR == 32 ? kAll : (1u << (LPR & 31)) - 1u)) != 0;
+    const unsigned outside = __ballot_sync(kAll, c >= V) >> ((threadIdx.x & 31) / width * width);
+    en.bad = (outside & (width == 32 ? kAll : (1u << width) - 1u)) != 0;
     en.c = c < 0 || c >= V ? -1 : c;
     if (en.c < 0) a = A(-INFINITY);
     if (TAIL) {
         en.lq = a;
         const double q = teacher_exp(double(a), A(0));
-        const double sum = entry_sum<LPR>(q, KP);
+        const double sum = entry_sum(q, KP, width);
         en.q = A(q);
         en.sum_q = A(sum);
         en.left = A(fmax(0.0, 1.0 - sum));
     } else {
         const A z = a * inv_tau;
-        const A m = entry_max<LPR>(z, KP);
+        const A m = entry_max(z, KP, width);
         const A w = m == A(-INFINITY) ? A(0) : M::exp2_of((z - m) * A(kLog2e));
-        const A s = entry_sum<LPR>(w, KP);
+        const A s = entry_sum(w, KP, width);
         en.lq = s == A(0) ? A(-INFINITY) : z - m - M::ln_of(s);
         en.q = s == A(0) ? A(0) : M::ratio(w, s);
         en.sum_q = s == A(0) ? A(0) : s / s;
@@ -121,11 +120,11 @@ __device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, in
     en.first = en.c >= 0;
     en.dup_q = A(0);
     for (int o = 0; o < K; ++o) {
-        const int other = __shfl_sync(kAll, en.c, o, LPR);
-        const A oq = __shfl_sync(kAll, en.q, o, LPR);
+        const int other = __shfl_sync(kAll, en.c, o, width);
+        const A oq = __shfl_sync(kAll, en.q, o, width);
         const bool mine = other == en.c;
         en.dup_q += mine ? oq : A(0);
-        en.first = en.first && !(mine && o < gl);
+        en.first = en.first && !(mine && o < e);
     }
     return en;
 }
@@ -152,84 +151,90 @@ __device__ __forceinline__ void blank_element(uint4 &v, int c)
     v = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// What the row's statistics and entries give: its divergence, and its gradient's factors. The gradient is
-//     2^((x - top) * kappa) * factor                                   where no entry names the token
-//     2^((x - all_top) * kappa) * all_factor - q_factor * dup_q        where one does
+// A row's maximum and sum 2^((x - max) * kappa): of the tokens that are not listed (rest) and of all. Without a tail the
+// two are the same.
 template <typename A>
-struct RowResult {
-    A loss;  // weighted
-    A top, factor;
-    A all_top, all_factor;
-    A q_factor;
+struct RowSums {
+    A rest_max, rest_sum, all_max, all_sum;
+    __device__ __forceinline__ bool nothing() const { return all_max == A(-INFINITY) && all_sum == all_sum; }
+    __device__ __forceinline__ bool no_rest() const { return rest_max == A(-INFINITY) && rest_sum == rest_sum; }
 };
 
-// `st`: maximum and sum 2^((x - max) * kappa) of the entries that are not listed (with a tail) or of the whole row
-// (without). `xc`: the student's logit at this lane's entry (-inf: none). All lanes of a warp call this together; LPR lanes belong to a row.
-template <int LPR, bool TAIL, typename A>
-__device__ __forceinline__ RowResult<A> solve_row(const RowStats<A> &st, const Entries<A> &en, A xc, A kappa, A inv_tau,
-                                                  A weight, A gain, int KP)
+// `mine`: the student's logit at this lane's entry if no earlier one names the token, else -inf: a listed token counts once,
+// however often it is named. (No maximum takes up a NaN; the sum does.)
+template <bool TAIL, typename A>
+__device__ __forceinline__ RowSums<A> all_sums(A max, A sum, A mine, A kappa, int KP, int width)
 {
     using M = Base2<A>;
-    const A rest_sum = st.s;
-    A all_max = st.max, all_sum = rest_sum;
+    RowSums<A> s{max, sum, max, sum};
     if (TAIL) {
-        // a listed token counts once, however often it is named (no maximum takes up a NaN; the sum does)
-        const A mine = en.first ? xc : A(-INFINITY);
-        all_max = M::max_of(st.max, entry_max<LPR>(mine, KP));
-        const A base = all_max == A(-INFINITY) ? A(0) : all_max;
-        const A listed = entry_sum<LPR>(M::exp2_of((mine - base) * kappa), KP);
-        all_sum = listed + (st.max == A(-INFINITY) ? rest_sum : rest_sum * M::exp2_of((st.max - base) * kappa));
+        s.all_max = M::max_of(max, entry_max(mine, KP, width));
+        const A base = s.all_max == A(-INFINITY) ? A(0) : s.all_max;
+        const A listed = entry_sum(M::exp2_of((mine - base) * kappa), KP, width);
+        s.all_sum = listed + (max == A(-INFINITY) ? sum : sum * M::exp2_of((max - base) * kappa));
     }
-    const bool nothing = all_max == A(-INFINITY) && all_sum == all_sum;  // no finite entry: nothing to learn
-    // the three logarithms at once, each in a lane of its own
-    const int gl = threadIdx.x % LPR;
-    const A of = gl == 0 ? (nothing ? A(1) : all_sum) : gl == 1 ? rest_sum : en.left;
-    const A ln = M::ln_of(of);
-    const A ln_s = __shfl_sync(0xffffffffu, ln, 0, LPR);
-    A each = A(0);
-    if (en.q > A(0)) each = en.q * (en.lq - log_prob_of(xc, all_max, inv_tau, ln_s));
-    each = entry_sum<LPR>(each, KP);
-    A q_all = en.sum_q, q_rest = A(0), p_rest = A(1);
-    if (TAIL) {
-        const A ln_rest = (st.max - all_max) * inv_tau + (__shfl_sync(0xffffffffu, ln, 1, LPR) - ln_s);
-        const A ln_left = __shfl_sync(0xffffffffu, ln, 2, LPR);
-        if (!st.nothing()) {
-            q_rest = en.left;
-            q_all = en.sum_q + q_rest;
-            p_rest = rest_sum * M::exp2_of((st.max - all_max) * kappa) * M::ratio(A(1), all_sum);
-            if (q_rest > A(0)) each += q_rest * (ln_left - ln_rest);
-        }
-    }
-    A up = gain * weight * inv_tau;
-    if (nothing) each = up = A(0);
-    if (en.bad) each = up = A(NAN);
-    if (ln_s != ln_s) each = A(NAN);  // (with no entry at all, a NaN logit would go unseen)
-    RowResult<A> res;
-    res.loss = weight == A(0) ? A(0) : weight * each;
-    res.all_top = nothing ? A(0) : all_max;
-    res.all_factor = nothing && !en.bad ? A(0) : M::ratio(up * q_all, all_sum);
-    res.q_factor = up;
-    if (TAIL) {
-        // (Q p_rest - q_rest) / p_rest p_j, with p_j / p_rest taken from the rest's own sum
-        res.top = st.max == A(-INFINITY) ? A(0) : st.max;
-        res.factor = st.nothing() ? (en.bad ? A(NAN) : A(0)) : M::ratio(up * (q_all * p_rest - q_rest), rest_sum);
-    } else {
-        res.top = res.all_top, res.factor = res.all_factor;
-    }
-    return res;
+    return s;
 }
 
-// The gradient at this lane's entry, if no earlier one names the same token.
-template <typename T>
-__device__ __forceinline__ void write_entry(T *out, const Entries<typename Elt<T>::acc> &en, typename Elt<T>::acc xc,
-                                            const RowResult<typename Elt<T>::acc> &res, typename Elt<T>::acc kappa,
-                                            bool wanted)
+// The factors of a row's gradient, which is
+//     2^((x - rest_max) * kappa) * factor                              where no entry names the token
+//     2^((x - all_max) * kappa) * all_factor - q_factor * dup_q        where one does
+template <typename A>
+struct RowFactors {
+    A rest_top, factor, all_top, all_factor, q_factor;
+};
+// `gain`: weight, upstream gradient, scale and 1 / tau together.
+template <bool TAIL, typename A>
+__device__ __forceinline__ RowFactors<A> gradient_factors(const RowSums<A> &s, A sum_q, A left, bool bad, A gain, A kappa)
 {
-    using A = typename Elt<T>::acc;
     using M = Base2<A>;
-    if (wanted && en.first)
-        out[en.c] = Elt<T>::from_acc(
-            M::fma_of(M::exp2_of((xc - res.all_top) * kappa), res.all_factor, -res.q_factor * en.dup_q));
+    const bool nothing = s.nothing(), no_rest = s.no_rest();
+    const A up = bad ? A(NAN) : nothing ? A(0) : gain;
+    RowFactors<A> f;
+    f.all_top = nothing ? A(0) : s.all_max;
+    f.q_factor = up;
+    const A share = nothing ? A(0) : M::ratio(A(1), s.all_sum);
+    if (TAIL) {
+        // (Q p_rest - q_rest) / p_rest p_j, with p_j / p_rest taken from the rest's own sum
+        const A q_rest = no_rest ? A(0) : left, q_all = sum_q + q_rest;
+        const A p_rest = s.rest_sum * M::exp2_of((s.rest_max - s.all_max) * kappa) * share;
+        f.all_factor = up * q_all * share;
+        f.rest_top = no_rest ? A(0) : s.rest_max;
+        f.factor = no_rest ? (bad ? A(NAN) : A(0)) : M::ratio(up * (q_all * p_rest - q_rest), s.rest_sum);
+    } else {
+        f.all_factor = f.factor = up * sum_q * share;
+        f.rest_top = f.all_top;
+    }
+    return f;
+}
+
+// A row's weighted divergence. Lane e of the row's `width` lanes holds entry e: its q, lq and the student's logit xc there.
+template <bool TAIL, typename A>
+__device__ __forceinline__ A divergence(const RowSums<A> &s, A q, A lq, A xc, A left, bool bad, A weight, A inv_tau, int KP,
+                                        int width)
+{
+    using M = Base2<A>;
+    const bool nothing = s.nothing();
+    const A ln_s = nothing ? A(0) : M::ln_of(s.all_sum);
+    A each = A(0);
+    if (q > A(0)) each = q * (lq - log_prob_of(xc, s.all_max, inv_tau, ln_s));
+    each = entry_sum(each, KP, width);
+    if (TAIL && !s.no_rest() && left > A(0)) {
+        const A ln_rest = (s.rest_max - s.all_max) * inv_tau + (M::ln_of(s.rest_sum) - ln_s);
+        each += left * (M::ln_of(left) - ln_rest);
+    }
+    if (nothing) each = A(0);
+    if (bad || ln_s != ln_s) each = A(NAN);  // (with no entry at all, a NaN logit would go unseen)
+    return weight == A(0) ? A(0) : weight * each;
+}
+
+// The gradient at an entry that no earlier one names the same token as.
+template <typename T>
+__device__ __forceinline__ void write_entry(T *out, int c, typename Elt<T>::acc dup_q, typename Elt<T>::acc xc,
+                                            const RowFactors<typename Elt<T>::acc> &f, typename Elt<T>::acc kappa)
+{
+    using M = Base2<typename Elt<T>::acc>;
+    out[c] = Elt<T>::from_acc(M::fma_of(M::exp2_of((xc - f.all_top) * kappa), f.all_factor, -f.q_factor * dup_q));
 }
 
 // Sum over the CTA of one double per thread, in a fixed order, in thread 0.
@@ -245,8 +250,24 @@ __device__ __forceinline__ double sum_cta(double v)
     return v;
 }
 
-// Rows of at most LPR * NV vectors and at most LPR entries. Group g of a CTA takes the rows first + g, + GPC, ..
-// The terms of the sum stay in registers for the gradient.
+// What a warp keeps in shared memory of the rows that it carries: their entries, and a record each.
+template <typename A>
+struct EntryRecord {
+    int c;    // token, -1: none
+    int own;  // no earlier entry of the row names it
+    A q, lq, dup_q, xc;
+};
+template <typename A>
+struct RowRecord {
+    A weight, gain, sum_q, left;
+    RowSums<A> sums;
+    int bad;
+};
+
+// Rows of at most LPR * NV vectors and at most LPR entries. Group g of a CTA takes the rows first + g, + GPC, .. run_len
+// times. What a row needs beside its elements would cost a warp more instructions than the elements do, so the warp does
+// that for all of its rows at once, before and after they pass: an entry to a lane. The terms of a row's sum stay in
+// registers for its gradient. (314340 x 1024 bf16, two entries a row: 0.30 ms with that work done row by row.)
 template <typename T, int LPR, int NV, int MODE, bool TAIL>
 __global__ void __launch_bounds__(kRowThreads)
 distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
@@ -254,54 +275,57 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
     using E = Elt<T>;
     using A = typename E::acc;
     using M = Base2<A>;
-    constexpr int GPC = kRowThreads / LPR, VE = E::VE;
+    constexpr int GPC = kRowThreads / LPR, VE = E::VE, kRows = 32 / LPR;  // kRows: of a warp at a time
     constexpr unsigned kAll = 0xffffffffu;
-    const int gl = threadIdx.x % LPR, group = threadIdx.x / LPR;
-    const int64_t first = int64_t(blockIdx.x) * GPC * run_len + group;
-    double sum = 0.0;
-    // A row's weight decides whether it is read, its tokens what is read of it: both are asked for two rows ahead, the
-    // logits at the tokens one row ahead, so that no load of a row waits for another.
-    struct Ahead {
-        A weight, value;
-        int c;
-    };
-    auto look = [&](int step) {
-        const int64_t r = first + int64_t(step) * GPC;
-        Ahead h{A(0), A(-INFINITY), -1};
-        if (step < run_len && r < a.n_rows) {
-            h.weight = a.weight ? A(__ldg(a.weight + r)) : A(1);
-            if (gl < a.K) {
-                h.c = __ldg(a.index + r * a.K + gl);
-                h.value = A(__ldg(a.teacher + r * a.K + gl));
+    extern __shared__ __align__(16) unsigned char scratch[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % LPR;
+    const int rows = kRows * run_len, KP = a.KP;  // of this warp in all; row b is row b % kRows of step b / kRows
+    RowRecord<A> *const recs = reinterpret_cast<RowRecord<A> *>(scratch) + warp * rows;
+    EntryRecord<A> *const ents =
+        reinterpret_cast<EntryRecord<A> *>(reinterpret_cast<RowRecord<A> *>(scratch) + kRowThreads / 32 * rows) +
+        warp * rows * KP;
+    const int64_t first = int64_t(blockIdx.x) * GPC * run_len + warp * kRows;
+    auto row_of = [&](int b) { return first + int64_t(b / kRows) * GPC + b % kRows; };
+
+    for (int at = 0; at < rows * KP; at += 32) {
+        const int i = at + lane, b = i / KP, e = i % KP;
+        const int64_t r = row_of(b);
+        const bool active = i < rows * KP && r < a.n_rows;
+        const A weight = active ? (a.weight ? A(__ldg(a.weight + r)) : A(1)) : A(0);
+        const bool seen = weight != A(0);  // a row without weight is not read
+        int c = -1;
+        A value = A(-INFINITY), xc = A(-INFINITY);
+        if (seen && e < a.K) {
+            c = __ldg(a.index + r * a.K + e);
+            value = A(__ldg(a.teacher + r * a.K + e));
+            if (c >= 0 && c < a.V) xc = E::to_acc(__ldg(a.x + r * a.x_stride + c));
+        }
+        const Entries<A> en = weigh_entries<TAIL>(c, value, a.V, a.K, KP, a.inv_tau, e, KP);
+        if (i < rows * KP) {
+            ents[i] = EntryRecord<A>{en.c, en.first, en.q, en.lq, en.dup_q, xc};
+            if (e == 0) {
+                const A up = a.upstream && active ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
+                recs[b] = RowRecord<A>{weight, up * A(a.scale) * weight * a.inv_tau, en.sum_q, en.left, {}, en.bad};
             }
         }
-        return h;
-    };
-    auto pick = [&](int step, const Ahead &h) {
-        const int64_t r = first + int64_t(step) * GPC;
-        return h.weight != A(0) && h.c >= 0 && h.c < a.V ? E::to_acc(__ldg(a.x + r * a.x_stride + h.c)) : A(-INFINITY);
-    };
-    Ahead now = look(0), next = look(1);
-    A xc = pick(0, now);
+    }
+    __syncwarp();
+
     for (int step = 0; step < run_len; ++step) {
-        const int64_t r = first + int64_t(step) * GPC;
+        const int b = step * kRows + lane / LPR;
+        const int64_t r = row_of(b);
         const bool active = r < a.n_rows;
         if (!__any_sync(kAll, active)) break;
         const int64_t rr = active ? r : 0;
-        const A weight = now.weight;
-        const bool seen = weight != A(0);  // a row without weight is not read
+        RowRecord<A> &rec = recs[b];
+        const EntryRecord<A> *const ent = ents + b * KP;
         const T *row = a.x + rr * a.x_stride;
         const RowVectors<T, MODE> rv(row, a.V);
         uint4 v[NV];
-        rv.template load_all<LPR>(v, gl, seen);
-        const A next_xc = pick(step + 1, next);
-        const Ahead after = look(step + 2);
-        const int c = seen ? now.c : -1;
-        const A value = now.value;
-        const Entries<A> en = weigh_entries<LPR, TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, gl);
+        rv.template load_all<LPR>(v, gl, rec.weight != A(0));
         if (TAIL) {
             for (int e = 0; e < a.K; ++e) {
-                const int token = __shfl_sync(kAll, en.c, e, LPR);
+                const int token = ent[e].c;
                 const int at = rv.place(token < 0 ? 0 : token), i = at / VE;
                 if (token >= 0 && i % LPR == gl) {
 #pragma unroll
@@ -310,15 +334,14 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
                 }
             }
         }
-        RowStats<A> st;
-        st.clear();
+        A max = A(-INFINITY), sum = A(0);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) st.max = M::max_of(st.max, E::vec_max(v[j]));
+        for (int j = 0; j < NV; ++j) max = M::max_of(max, E::vec_max(v[j]));
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) st.max = M::max_of(st.max, __shfl_xor_sync(kAll, st.max, o));
+        for (int o = LPR / 2; o > 0; o >>= 1) max = M::max_of(max, __shfl_xor_sync(kAll, max, o));
         // A term is the same number in the sum and in the gradient, so the rounding of the shift leaves their ratio; it
-        // is undone where the sum's logarithm is taken.
-        const TermsAt<T> at(st.max, a.kappa);
+        // is undone where the sum stands beside another row's or its logarithm is taken.
+        const TermsAt<T> at(max, a.kappa);
         A term[NV][VE];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -333,23 +356,21 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
 #pragma unroll
             for (int k = 0; k < VE; ++k) {
                 term[j][k] = M::exp2_of(term[j][k]);
-                st.s += term[j][k];
+                sum += term[j][k];
             }
         }
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) st.s += __shfl_xor_sync(kAll, st.s, o);
+        for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
         const A undo = at.plain ? M::exp2_of(-M::fma_of(at.max, a.kappa, -at.shift)) : A(1);
-        st.s *= undo;
-        const A up = a.upstream && active ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
-        const RowResult<A> res = solve_row<LPR, TAIL>(st, en, xc, a.kappa, a.inv_tau, weight, up * A(a.scale), a.KP);
-        if (active && gl == 0) {
-            if (a.row_loss) a.row_loss[r] = res.loss;
-            sum += double(res.loss);
-        }
+        const bool holds = gl < KP && ent[gl < KP ? gl : 0].own;
+        const A xc = holds ? ent[gl].xc : A(-INFINITY);
+        const RowSums<A> sums = all_sums<TAIL>(max, sum * undo, xc, a.kappa, KP, LPR);
+        if (gl == 0) rec.sums = sums;
         if (a.gx) {
+            const RowFactors<A> f = gradient_factors<TAIL>(sums, rec.sum_q, rec.left, rec.bad, rec.gain, a.kappa);
             T *out = a.gx + rr * a.g_stride;
             const bool same = MODE != kAny || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-            const A factor = res.factor * undo;
+            const A factor = f.factor * undo;
             if (active) {
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
@@ -360,13 +381,26 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
                 }
             }
             __syncwarp();
-            write_entry<T>(out, en, xc, res, a.kappa, seen);
+            if (active && holds) write_entry<T>(out, ent[gl].c, ent[gl].dup_q, xc, f, a.kappa);
         }
-        now = next, next = after, xc = next_xc;
+    }
+    __syncwarp();
+
+    double total = 0.0;
+    for (int at = 0; at < rows * KP; at += 32) {
+        const int i = at + lane, b = i / KP, e = i % KP;
+        const bool here = i < rows * KP && row_of(b) < a.n_rows;
+        const EntryRecord<A> en = here ? ents[i] : EntryRecord<A>{};
+        const RowRecord<A> rec = here ? recs[b] : RowRecord<A>{};
+        const A loss = divergence<TAIL>(rec.sums, en.q, en.lq, en.xc, rec.left, rec.bad, rec.weight, a.inv_tau, KP, KP);
+        if (here && e == 0) {
+            if (a.row_loss) a.row_loss[row_of(b)] = loss;
+            total += double(loss);
+        }
     }
     if (a.partial) {
-        sum = sum_cta(sum);
-        if (threadIdx.x == 0) a.partial[blockIdx.x] = sum * a.scale;
+        total = sum_cta(total);
+        if (threadIdx.x == 0) a.partial[blockIdx.x] = total * a.scale;
     }
 }
 
@@ -402,7 +436,7 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
         }
         int *const listed = listed_of[LANES == 32 ? warp : 0];
         const A xc = c >= 0 && c < a.V ? E::to_acc(__ldg(row + c)) : A(-INFINITY);
-        const Entries<A> en = weigh_entries<32, TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, lane);
+        const Entries<A> en = weigh_entries<TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, lane, 32);
         if (me < 32) listed[lane] = en.c >= 0 ? rv.place(en.c) : -1;
         if (LANES == 32)
             __syncwarp();
@@ -453,9 +487,11 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
         }
         st.s = st.sum(a.kappa);
         const A up = a.upstream ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
-        const RowResult<A> res = solve_row<32, TAIL>(st, en, xc, a.kappa, a.inv_tau, weight, up * A(a.scale), a.KP);
-        loss = res.loss;
+        const RowSums<A> sums = all_sums<TAIL>(st.max, st.s, en.first ? xc : A(-INFINITY), a.kappa, a.KP, 32);
+        loss = divergence<TAIL>(sums, en.q, en.lq, xc, en.left, en.bad, weight, a.inv_tau, a.KP, 32);
         if (me == 0 && a.row_loss) a.row_loss[r] = loss;
+        const RowFactors<A> f =
+            gradient_factors<TAIL>(sums, en.sum_q, en.left, en.bad, up * A(a.scale) * weight * a.inv_tau, a.kappa);
         if (out) {
             rv.template sweep<LANES>(me, seen, [&](int at, uint4(&v)[NV]) {
 #pragma unroll
@@ -465,7 +501,7 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
                         A e[E::VE];
                         E::unpack(v[j], e);
 #pragma unroll
-                        for (int k = 0; k < E::VE; ++k) e[k] = M::exp2_of((e[k] - res.top) * a.kappa) * res.factor;
+                        for (int k = 0; k < E::VE; ++k) e[k] = M::exp2_of((e[k] - f.rest_top) * a.kappa) * f.factor;
                         rv.store(out, i, same, e);
                     }
                 }
@@ -474,7 +510,7 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
                 __syncwarp();
             else
                 __syncthreads();
-            if (me < 32) write_entry<T>(out, en, xc, res, a.kappa, seen);
+            if (me < 32 && en.first) write_entry<T>(out, en.c, en.dup_q, xc, f, a.kappa);
         }
     }
     if (a.partial) {
@@ -504,11 +540,18 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const double *__restr
 template <typename T, int LPR, int NV, bool ALIGNED>
 int64_t launch_distill_rows(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 {
+    using A = typename Elt<T>::acc;
     constexpr int GPC = kRowThreads / LPR;
-    // runs of rows where there are enough for every SM: the first row of a run has nothing asked for ahead
+    // runs of rows where there are enough for every SM: what is done for all rows of a warp at once needs several
     const int run_len = a.n_rows > int64_t(GPC) * kNumSMs * 32 ? 8 : 1;
     const int64_t grid = (a.n_rows + int64_t(GPC) * run_len - 1) / (int64_t(GPC) * run_len);
-    auto go = [&](auto kernel) { kernel<<<unsigned(grid), kRowThreads, 0, s>>>(a, run_len); };
+    // (at most 8 warps x 256 entries: K <= LPR)
+    const size_t smem = size_t(GPC) * run_len * (sizeof(RowRecord<A>) + a.KP * sizeof(EntryRecord<A>));
+    auto go = [&](auto kernel) {
+        if (smem > 48 * 1024)
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        kernel<<<unsigned(grid), kRowThreads, smem, s>>>(a, run_len);
+    };
     if constexpr (ALIGNED) {
         if (a.V == LPR * NV * Elt<T>::VE)
             tail ? go(distill_rows_kernel<T, LPR, NV, kFull, true>) : go(distill_rows_kernel<T, LPR, NV, kFull, false>);
