@@ -580,7 +580,7 @@ int64_t launch_distill_stream(const DistillArgs<T> &a, bool tail, cudaStream_t s
 template <typename T, bool ALIGNED>
 int64_t launch_distill_t(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 {
-    constexpr int VE = Elt<T>::VE, NV = 64 / VE < 16 ? 64 / VE : 16;
+    constexpr int VE = Elt<T>::VE, NV = 32 / VE < 16 ? 32 / VE : 16;
     const int nv = ALIGNED ? a.V / VE : (a.V + 2 * VE - 2) / VE;
     // Few lanes a row, many elements a lane: what a row costs beside its elements (about 400 instructions of a warp) is
     // shared by the rows of a warp. 64 elements a lane is what registers hold; every entry has a lane.
@@ -590,6 +590,7 @@ int64_t launch_distill_t(const DistillArgs<T> &a, bool tail, cudaStream_t s)
         if (nv <= 16 * NV && a.K <= 16) return launch_distill_rows<T, 16, NV, ALIGNED>(a, tail, s);
         if (nv <= 64) return launch_distill_rows<T, 32, 2, ALIGNED>(a, tail, s);
         if (nv <= 128) return launch_distill_rows<T, 32, 4, ALIGNED>(a, tail, s);
+        if (nv <= 32 * 64 / VE) return launch_distill_rows<T, 32, 64 / VE, ALIGNED>(a, tail, s);
     }
     if (nv <= 32 * NV) return launch_distill_rows<T, 32, NV, ALIGNED>(a, tail, s);
     // a warp carries a longer row where there are rows enough for the SMs' warps
