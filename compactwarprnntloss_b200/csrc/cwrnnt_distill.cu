@@ -238,15 +238,16 @@ __device__ __forceinline__ void write_entry(T *out, int c, typename Elt<T>::acc 
 }
 
 // Sum over the CTA of one double per thread, in a fixed order, in thread 0.
+template <int THREADS>
 __device__ __forceinline__ double sum_cta(double v)
 {
-    __shared__ double parts[kRowThreads / 32];
+    __shared__ double parts[THREADS / 32];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = v;
     __syncthreads();
     v = 0.0;
-    for (int w = 0; w < kRowThreads / 32; ++w) v += parts[w];
+    for (int w = 0; w < THREADS / 32; ++w) v += parts[w];
     return v;
 }
 
@@ -399,23 +400,22 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
         }
     }
     if (a.partial) {
-        total = sum_cta(total);
+        total = sum_cta<kRowThreads>(total);
         if (threadIdx.x == 0) a.partial[blockIdx.x] = total * a.scale;
     }
 }
 
-// Rows that registers do not hold: a warp each (LANES = 32) or a CTA each (LANES = 256). Every warp holds the row's
+// Rows that registers do not hold: a warp each (LANES = 32) or a CTA each. Every warp holds the row's
 // entries in its lanes. The sums run along the row, then the gradient does, reading the row a second time from L2.
 template <typename T, int LANES, int MODE, bool TAIL>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(LANES == 32 ? kRowThreads : LANES)
 distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
 {
     using E = Elt<T>;
     using A = typename E::acc;
     using M = Base2<A>;
-    constexpr int NV = 4, kWarps = kRowThreads / 32;
+    constexpr int NV = 4, kWarps = (LANES == 32 ? kRowThreads : LANES) / 32;
     __shared__ RowStats<A> parts[LANES == 32 ? 1 : kWarps];
-    __shared__ int listed_of[LANES == 32 ? kWarps : 1][32];  // places of the listed tokens; -1: none
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int me = LANES == 32 ? lane : threadIdx.x;
     const int64_t r = LANES == 32 ? int64_t(blockIdx.x) * kWarps + warp : int64_t(blockIdx.x);
@@ -434,39 +434,23 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
             c = __ldg(a.index + r * a.K + lane);
             value = A(__ldg(a.teacher + r * a.K + lane));
         }
-        int *const listed = listed_of[LANES == 32 ? warp : 0];
         const A xc = c >= 0 && c < a.V ? E::to_acc(__ldg(row + c)) : A(-INFINITY);
         const Entries<A> en = weigh_entries<TAIL>(c, value, a.V, a.K, a.KP, a.inv_tau, lane, 32);
-        if (me < 32) listed[lane] = en.c >= 0 ? rv.place(en.c) : -1;
-        if (LANES == 32)
-            __syncwarp();
-        else
-            __syncthreads();
-
-        // the next of this lane's vectors, from vector `from` on, that holds a listed token
-        auto next_listed = [&](int from) {
-            int next = 0x7fffffff;
-            for (int e = 0; e < a.K; ++e) {
-                const int i = listed[e] / E::VE;
-                if (listed[e] >= 0 && i % LANES == me && i >= from && i < next) next = i;
-            }
-            return next;
-        };
+        const int place = en.c >= 0 ? rv.place(en.c) : -1;  // of this lane's entry
         RowStats<A> st;
         st.clear();
         if (seen) {
-            int next = TAIL ? next_listed(0) : 0x7fffffff;
             rv.template sweep<LANES>(me, true, [&](int at, uint4(&v)[NV]) {
-                if (TAIL && next < at + NV * LANES) {
-                    const int past = at + NV * LANES;
-                    for (int e = 0; e < a.K; ++e) {
-                        const int i = listed[e] / E::VE;
-                        if (listed[e] < 0 || i % LANES != me || i < at || i >= past) continue;
+                if (TAIL) {  // the listed tokens among these vectors of this warp's lanes
+                    const int i = place / E::VE - (at - me);
+                    unsigned hits = __ballot_sync(0xffffffffu, place >= 0 && i >= 0 && i < NV * LANES &&
+                                                                   (LANES == 32 || i % LANES / 32 == warp));
+                    for (; hits; hits &= hits - 1) {
+                        const int p = __shfl_sync(0xffffffffu, place, __ffs(hits) - 1);
 #pragma unroll
                         for (int j = 0; j < NV; ++j)
-                            if (i == at + j * LANES) blank_element<T>(v[j], listed[e] % E::VE);
+                            if (p / E::VE == at + j * LANES) blank_element<T>(v[j], p % E::VE);
                     }
-                    next = next_listed(past);
                 }
                 A m = st.max;
 #pragma unroll
@@ -478,12 +462,10 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
             });
         }
         join_lanes<32, false>(st, a.kappa);
-        if (LANES > 32) {  // the warps' parts, joined in their order: the same bits in every thread
+        if constexpr (LANES > 32) {
             if (lane == 0) parts[warp] = st;
             __syncthreads();
-            st = parts[0];
-#pragma unroll 1
-            for (int w = 1; w < kWarps; ++w) st.template join<false>(parts[w], a.kappa);
+            st = join_warps<kWarps, false>(parts, a.kappa);
         }
         st.s = st.sum(a.kappa);
         const A up = a.upstream ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
@@ -502,7 +484,8 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
                         E::unpack(v[j], e);
 #pragma unroll
                         for (int k = 0; k < E::VE; ++k) e[k] = M::exp2_of((e[k] - f.rest_top) * a.kappa) * f.factor;
-                        rv.store(out, i, same, e);
+                        // (evict-first: the rows have to stay in L2 for this second reading, their gradients do not)
+                        rv.template store<true>(out, i, same, e);
                     }
                 }
             });
@@ -514,7 +497,7 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
         }
     }
     if (a.partial) {
-        const double sum = sum_cta(me == 0 ? double(loss) : 0.0);
+        const double sum = sum_cta<kWarps * 32>(me == 0 ? double(loss) : 0.0);
         if (threadIdx.x == 0) a.partial[blockIdx.x] = sum * a.scale;
     }
 }
@@ -567,12 +550,13 @@ int64_t launch_distill_rows(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 template <typename T, int LANES, bool ALIGNED>
 int64_t launch_distill_stream(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 {
-    constexpr int rows = kRowThreads / LANES, MODE = ALIGNED ? kAligned : kAny;
+    constexpr int rows = LANES == 32 ? kRowThreads / 32 : 1, threads = LANES == 32 ? kRowThreads : LANES;
+    constexpr int MODE = ALIGNED ? kAligned : kAny;
     const int64_t grid = (a.n_rows + rows - 1) / rows;
     if (tail)
-        distill_stream_kernel<T, LANES, MODE, true><<<unsigned(grid), kRowThreads, 0, s>>>(a);
+        distill_stream_kernel<T, LANES, MODE, true><<<unsigned(grid), threads, 0, s>>>(a);
     else
-        distill_stream_kernel<T, LANES, MODE, false><<<unsigned(grid), kRowThreads, 0, s>>>(a);
+        distill_stream_kernel<T, LANES, MODE, false><<<unsigned(grid), threads, 0, s>>>(a);
     return grid;
 }
 
@@ -595,6 +579,8 @@ int64_t launch_distill_t(const DistillArgs<T> &a, bool tail, cudaStream_t s)
     if (nv <= 32 * NV) return launch_distill_rows<T, 32, NV, ALIGNED>(a, tail, s);
     // a warp carries a longer row where there are rows enough for the SMs' warps
     if (nv <= 2048 && a.n_rows >= kNumSMs * 32) return launch_distill_stream<T, 32, ALIGNED>(a, tail, s);
+    // a CTA carries it otherwise; a larger one only where SMs would stay empty (2047 x 32003 f32: 0.19 against 0.17 ms)
+    if (nv > 1024 && a.n_rows <= kNumSMs) return launch_distill_stream<T, kFewRowLanes, ALIGNED>(a, tail, s);
     return launch_distill_stream<T, kRowThreads, ALIGNED>(a, tail, s);
 }
 

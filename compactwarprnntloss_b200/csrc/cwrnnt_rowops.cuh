@@ -6,6 +6,7 @@
 namespace cwrnnt {
 
 constexpr int kRowThreads = 256;  // threads of a CTA in the row operators
+constexpr int kFewRowLanes = 512; // lanes of a long row where there are fewer rows than SMs
 
 // ------------------------------------------------------------------------------------------------ rows as vectors
 // A row is read in 16-byte vectors that lie on 16-byte boundaries, whatever V and the row stride. What lies before the
@@ -129,13 +130,19 @@ struct RowVectors {
     }
     // Stores vector i of a row of gradients. `same`: the output row has the input row's alignment, so that vector i is
     // one 16-byte store; else element by element.
+    template <bool FIRST_OUT = false>
     __device__ __forceinline__ void store(T *out, int i, bool same, const typename Elt<T>::acc (&e)[VE]) const
     {
         const uint4 v = Elt<T>::pack(e);
-        if (MODE != kAny || (same && whole(i)))
-            *(reinterpret_cast<uint4 *>(out + lead) + i) = v;
-        else
+        uint4 *const to = reinterpret_cast<uint4 *>(out + lead) + i;
+        if (MODE != kAny || (same && whole(i))) {
+            if (FIRST_OUT)
+                st_stream(to, v);
+            else
+                *to = v;
+        } else {
             store_edge(out, first(i), V, v);
+        }
     }
 };
 
@@ -257,6 +264,27 @@ __device__ __forceinline__ void join_lanes(RowStats<A> &st, A kappa)
         st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
         if (ENT) st.t += __shfl_xor_sync(0xffffffffu, st.t, o);
     }
+}
+
+// The same over the warps of a CTA, whose joined statistics lie in `parts`: added up in the warps' order, the same bits in
+// every thread.
+template <int WARPS, bool ENT, typename A>
+__device__ __forceinline__ RowStats<A> join_warps(const RowStats<A> *parts, A kappa)
+{
+    RowStats<A> st;
+    st.clear();
+    A m = parts[0].max;
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) m = Base2<A>::max_of(m, parts[w].max);
+#pragma unroll 1
+    for (int w = 0; w < WARPS; ++w) {
+        RowStats<A> part = parts[w];
+        part.template raise<ENT>(m, kappa);
+        st.s += part.s;
+        if (ENT) st.t += part.t;
+    }
+    st.max = m;
+    return st;
 }
 
 // How a row's (or a thread's) terms are formed at a fixed maximum: as x*kappa - shift, or from the difference to the

@@ -249,22 +249,24 @@ scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
 
 __host__ __device__ constexpr int stream_candidates(int lanes) { return lanes == 32 ? 96 : 512; }
 
-// Rows that registers do not hold: a warp each (LANES = 32) or a CTA each (LANES = 256). The statistics run along, with
+// Rows that registers do not hold: a warp each (LANES = 32) or a CTA each. The statistics run along, with
 // four vectors of every lane in flight. The selection reads the row again, from L1 or L2.
 template <typename T, int LANES, int MODE, bool ENT>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(LANES == 32 ? kRowThreads : LANES)
 scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
 {
     using E = Elt<T>;
     using A = typename E::acc;
     using M = Base2<A>;
     using Key = TopKey<A>;
-    constexpr int NV = 4, kWarps = kRowThreads / 32, kCap = stream_candidates(LANES), kBars = 64;
+    constexpr int NV = 4, kWarps = (LANES == 32 ? kRowThreads : LANES) / 32, kCap = stream_candidates(LANES);
+    constexpr int kBars = 64, kBarLanes = LANES / kBars;
     constexpr unsigned kAll = 0xffffffffu;
     extern __shared__ __align__(16) unsigned char scratch[];  // kCap keys per row of the CTA, when top_k > 0
     __shared__ RowStats<A> parts[LANES == 32 ? 1 : kWarps];
     __shared__ A bars[LANES == 32 ? 1 : kBars];
     __shared__ int counter;
+    __shared__ A bar_of_row;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int me = LANES == 32 ? lane : threadIdx.x;
     const int64_t r = LANES == 32 ? int64_t(blockIdx.x) * kWarps + warp : int64_t(blockIdx.x);
@@ -288,15 +290,14 @@ scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
     });
     const A own = st.max;
     join_lanes<32, ENT>(st, a.kappa);
-    if (LANES > 32) {  // the warps' parts, joined in their order: the same bits in every thread
-        A four = M::max_of(own, __shfl_xor_sync(kAll, own, 1));
-        four = M::max_of(four, __shfl_xor_sync(kAll, four, 2));
+    if constexpr (LANES > 32) {
+        A few = own;  // the maximum of each 64th of the lanes
+#pragma unroll
+        for (int o = 1; o < kBarLanes; o *= 2) few = M::max_of(few, __shfl_xor_sync(kAll, few, o));
         if (lane == 0) parts[warp] = st;
-        if (lane % 4 == 0) bars[threadIdx.x / 4] = four;
+        if (lane % kBarLanes == 0) bars[threadIdx.x / kBarLanes] = few;
         __syncthreads();
-        st = parts[0];
-#pragma unroll 1
-        for (int w = 1; w < kWarps; ++w) st.template join<ENT>(parts[w], a.kappa);
+        st = join_warps<kWarps, ENT>(parts, a.kappa);
     }
     const RowLog<A> log(st, a.kappa);
     if (me == 0) {
@@ -306,20 +307,16 @@ scores_stream_kernel(const __grid_constant__ ScoresArgs<T> a)
     if (me < a.n_targets) emit_target(a, row, r, log, __ldg(a.targets + r * a.n_targets + me), me);
     if (a.top_k == 0) return;
 
-    A bar = A(INFINITY);
-    if (LANES == 32) {
+    A bar;
+    if constexpr (LANES == 32) {
         bar = bar_of<32>(early, late, a.top_k);
-    } else {  // of 64 groups of four lanes
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const A mine = bars[lane + 32 * h];
-            int above = 0;
-#pragma unroll 8
-            for (int j = 0; j < kBars; ++j) above += bars[j] > mine;
-            if (above < a.top_k) bar = fmin(bar, mine);
+    } else {
+        if (warp == 0) {
+            bar = bar_of<32>(bars[lane], bars[lane + 32], a.top_k > 16 ? a.top_k : 17);  // of all 64
+            if (lane == 0) bar_of_row = bar;
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) bar = fmin(bar, __shfl_xor_sync(kAll, bar, o));
+        __syncthreads();
+        bar = bar_of_row;
     }
     int n = 0;
     rv.template sweep<LANES>(me, true, [&](int at, const uint4(&v)[NV]) {
@@ -524,13 +521,14 @@ cudaError_t launch_scores_rows(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
 template <typename T, int LANES, bool ALIGNED>
 cudaError_t launch_scores_stream(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
 {
-    constexpr int rows = kRowThreads / LANES, MODE = ALIGNED ? kAligned : kAny;
+    constexpr int rows = LANES == 32 ? kRowThreads / 32 : 1, threads = LANES == 32 ? kRowThreads : LANES;
+    constexpr int MODE = ALIGNED ? kAligned : kAny;
     const size_t smem = a.top_k > 0 ? rows * stream_candidates(LANES) * sizeof(TopKey<typename Elt<T>::acc>) : 0;
     const unsigned grid = unsigned((a.n_rows + rows - 1) / rows);
     if (ent)
-        scores_stream_kernel<T, LANES, MODE, true><<<grid, kRowThreads, smem, s>>>(a);
+        scores_stream_kernel<T, LANES, MODE, true><<<grid, threads, smem, s>>>(a);
     else
-        scores_stream_kernel<T, LANES, MODE, false><<<grid, kRowThreads, smem, s>>>(a);
+        scores_stream_kernel<T, LANES, MODE, false><<<grid, threads, smem, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -552,6 +550,8 @@ cudaError_t launch_scores_t(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
     if (nv <= 256) return launch_scores_rows<T, 32, 8, ALIGNED>(a, ent, s);
     // a warp carries a longer row where there are rows enough for the SMs' warps
     if (nv <= 2048 && a.n_rows >= kNumSMs * 32) return launch_scores_stream<T, 32, ALIGNED>(a, ent, s);
+    // a CTA carries it otherwise; a larger one only where SMs would stay empty (2051 x 50257 f16: 0.10 against 0.08 ms)
+    if (nv > 1024 && a.n_rows <= kNumSMs) return launch_scores_stream<T, kFewRowLanes, ALIGNED>(a, ent, s);
     return launch_scores_stream<T, kRowThreads, ALIGNED>(a, ent, s);
 }
 
