@@ -30,9 +30,9 @@ struct DistillArgs {
     T *gx;  // null: loss only
     int64_t n_rows, x_stride, g_stride;
     int V, K, KP;  // KP: K up to a power of two
-    A kappa;       // log2(e) / tau
-    A inv_tau;     // 1 / tau
-    double scale;  // of the summed loss and of the gradient
+    A kappa;         // log2(e) / tau
+    double inv_tau;  // 1 / tau
+    double scale;    // of the summed loss and of the gradient
     const C *teacher, *weight, *upstream;
     int upstream_stride;
     const int32_t *index;
@@ -59,8 +59,23 @@ __device__ __forceinline__ double exp_mid(double a)
     p = fma(p, r, 1.0);
     return p * __hiloint2double((int(n) + 1023) << 20, 0);
 }
-__device__ __forceinline__ double teacher_exp(double a, float) { return exp_mid(a); }
-__device__ __forceinline__ double teacher_exp(double a, double) { return exp(a); }
+// ln s to the same accuracy: one step of Newton's method from the single-precision logarithm.
+__device__ __forceinline__ double ln_mid(double s)
+{
+    const float y = logf(float(s));
+    return fabsf(y) < 1e30f ? y + fma(s, exp_mid(-double(y)), -1.0) : double(y);
+}
+// A row's divergence is a small difference of its entries' logarithms: what is done once a row or entry is done in double.
+template <typename A>
+__device__ __forceinline__ double exp_of(double a)
+{
+    return sizeof(A) == 8 ? exp(a) : exp_mid(a);
+}
+template <typename A>
+__device__ __forceinline__ double ln_of(double s)
+{
+    return sizeof(A) == 8 ? log(s) : ln_mid(s);
+}
 
 // Sums and maxima over the KP lanes (a power of two, at most `width`) that hold a row's entries, the first of the row's
 // `width` lanes; the result in all of them. All lanes of a warp call these together.
@@ -83,15 +98,15 @@ struct Entries {
     int c;       // token, -1: none
     bool first;  // no earlier entry names the same token
     bool bad;    // some token of the row lies outside it
-    A q, lq;     // teacher's probability and its logarithm
-    A sum_q;     // over the row
-    A left;      // one minus that, at least 0
-    A dup_q;     // q of all entries with this token, added up in their order
+    double q, lq;  // teacher's probability and its logarithm
+    A sum_q;       // over the row
+    double left;   // one minus that, at least 0
+    A dup_q;       // q of all entries with this token, added up in their order
 };
 
 // All lanes of a warp call this together; lane `e` of a row's lanes holds entry e: token `c`, value `a` (-1, -inf: none).
 template <bool TAIL, typename A>
-__device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, int KP, A inv_tau, int e, int width)
+__device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, int KP, double inv_tau, int e, int width)
 {
     constexpr unsigned kAll = 0xffffffffu;
     using M = Base2<A>;
@@ -101,27 +116,26 @@ __device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, in
     en.c = c < 0 || c >= V ? -1 : c;
     if (en.c < 0) a = A(-INFINITY);
     if (TAIL) {
-        en.lq = a;
-        const double q = teacher_exp(double(a), A(0));
-        const double sum = entry_sum(q, KP, width);
-        en.q = A(q);
+        en.lq = double(a);
+        en.q = exp_of<A>(en.lq);
+        const double sum = entry_sum(en.q, KP, width);
         en.sum_q = A(sum);
-        en.left = A(fmax(0.0, 1.0 - sum));
+        en.left = fmax(0.0, 1.0 - sum);
     } else {
-        const A z = a * inv_tau;
-        const A m = entry_max(z, KP, width);
-        const A w = m == A(-INFINITY) ? A(0) : M::exp2_of((z - m) * A(kLog2e));
-        const A s = entry_sum(w, KP, width);
-        en.lq = s == A(0) ? A(-INFINITY) : z - m - M::ln_of(s);
-        en.q = s == A(0) ? A(0) : M::ratio(w, s);
-        en.sum_q = s == A(0) ? A(0) : s / s;
-        en.left = A(0);
+        const double z = double(a) * inv_tau;
+        const double m = entry_max(z, KP, width);
+        const double w = m == -INFINITY ? 0.0 : exp_of<A>(z - m);
+        const double s = entry_sum(w, KP, width);
+        en.lq = s == 0.0 ? -INFINITY : z - m - ln_of<A>(s);
+        en.q = s == 0.0 ? 0.0 : w / s;
+        en.sum_q = s == 0.0 ? A(0) : A(s / s);
+        en.left = 0.0;
     }
     en.first = en.c >= 0;
     en.dup_q = A(0);
     for (int o = 0; o < K; ++o) {
         const int other = __shfl_sync(kAll, en.c, o, width);
-        const A oq = __shfl_sync(kAll, en.q, o, width);
+        const A oq = __shfl_sync(kAll, A(en.q), o, width);
         const bool mine = other == en.c;
         en.dup_q += mine ? oq : A(0);
         en.first = en.first && !(mine && o < e);
@@ -170,7 +184,7 @@ __device__ __forceinline__ RowSums<A> all_sums(A max, A sum, A mine, A kappa, in
     if (TAIL) {
         s.all_max = M::max_of(max, entry_max(mine, KP, width));
         const A base = s.all_max == A(-INFINITY) ? A(0) : s.all_max;
-        const A listed = entry_sum(M::exp2_of((mine - base) * kappa), KP, width);
+        const A listed = entry_sum(A(exp2((mine - base) * kappa)), KP, width);
         s.all_sum = listed + (max == A(-INFINITY) ? sum : sum * M::exp2_of((max - base) * kappa));
     }
     return s;
@@ -210,22 +224,21 @@ __device__ __forceinline__ RowFactors<A> gradient_factors(const RowSums<A> &s, A
 
 // A row's weighted divergence. Lane e of the row's `width` lanes holds entry e: its q, lq and the student's logit xc there.
 template <bool TAIL, typename A>
-__device__ __forceinline__ A divergence(const RowSums<A> &s, A q, A lq, A xc, A left, bool bad, A weight, A inv_tau, int KP,
-                                        int width)
+__device__ __forceinline__ A divergence(const RowSums<A> &s, double q, double lq, A xc, double left, bool bad, A weight,
+                                        double inv_tau, int KP, int width)
 {
-    using M = Base2<A>;
     const bool nothing = s.nothing();
-    const A ln_s = nothing ? A(0) : M::ln_of(s.all_sum);
-    A each = A(0);
-    if (q > A(0)) each = q * (lq - log_prob_of(xc, s.all_max, inv_tau, ln_s));
+    const double max = double(s.all_max), ln_s = nothing ? 0.0 : ln_of<A>(double(s.all_sum));
+    double each = 0.0;
+    if (q > 0.0) each = q * (lq - ((double(xc) - max) * inv_tau - ln_s));
     each = entry_sum(each, KP, width);
-    if (TAIL && !s.no_rest() && left > A(0)) {
-        const A ln_rest = (s.rest_max - s.all_max) * inv_tau + (M::ln_of(s.rest_sum) - ln_s);
-        each += left * (M::ln_of(left) - ln_rest);
+    if (TAIL && !s.no_rest() && left > 0.0) {
+        const double ln_rest = (double(s.rest_max) - max) * inv_tau + (ln_of<A>(double(s.rest_sum)) - ln_s);
+        each += left * (ln_of<A>(left) - ln_rest);
     }
-    if (nothing) each = A(0);
-    if (bad || ln_s != ln_s) each = A(NAN);  // (with no entry at all, a NaN logit would go unseen)
-    return weight == A(0) ? A(0) : weight * each;
+    if (nothing) each = 0.0;
+    if (bad || ln_s != ln_s) each = NAN;  // (with no entry at all, a NaN logit would go unseen)
+    return weight == A(0) ? A(0) : A(double(weight) * each);
 }
 
 // The gradient at an entry that no earlier one names the same token as.
@@ -256,11 +269,13 @@ template <typename A>
 struct EntryRecord {
     int c;    // token, -1: none
     int own;  // no earlier entry of the row names it
-    A q, lq, dup_q, xc;
+    A dup_q, xc;
+    double q, lq;
 };
 template <typename A>
 struct RowRecord {
-    A weight, gain, sum_q, left;
+    double left;
+    A weight, gain, sum_q;
     RowSums<A> sums;
     int bad;
 };
@@ -303,10 +318,10 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
         }
         const Entries<A> en = weigh_entries<TAIL>(c, value, a.V, a.K, KP, a.inv_tau, e, KP);
         if (i < rows * KP) {
-            ents[i] = EntryRecord<A>{en.c, en.first, en.q, en.lq, en.dup_q, xc};
+            ents[i] = EntryRecord<A>{en.c, en.first, en.dup_q, xc, en.q, en.lq};
             if (e == 0) {
                 const A up = a.upstream && active ? A(__ldg(a.upstream + r * a.upstream_stride)) : A(1);
-                recs[b] = RowRecord<A>{weight, up * A(a.scale) * weight * a.inv_tau, en.sum_q, en.left, {}, en.bad};
+                recs[b] = RowRecord<A>{en.left, weight, up * A(a.scale) * weight * A(a.inv_tau), en.sum_q, {}, en.bad};
             }
         }
     }
@@ -368,7 +383,7 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
         const RowSums<A> sums = all_sums<TAIL>(max, sum * undo, xc, a.kappa, KP, LPR);
         if (gl == 0) rec.sums = sums;
         if (a.gx) {
-            const RowFactors<A> f = gradient_factors<TAIL>(sums, rec.sum_q, rec.left, rec.bad, rec.gain, a.kappa);
+            const RowFactors<A> f = gradient_factors<TAIL>(sums, rec.sum_q, A(rec.left), rec.bad, rec.gain, a.kappa);
             T *out = a.gx + rr * a.g_stride;
             const bool same = MODE != kAny || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
             const A factor = f.factor * undo;
@@ -473,7 +488,7 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
         loss = divergence<TAIL>(sums, en.q, en.lq, xc, en.left, en.bad, weight, a.inv_tau, a.KP, 32);
         if (me == 0 && a.row_loss) a.row_loss[r] = loss;
         const RowFactors<A> f =
-            gradient_factors<TAIL>(sums, en.sum_q, en.left, en.bad, up * A(a.scale) * weight * a.inv_tau, a.kappa);
+            gradient_factors<TAIL>(sums, en.sum_q, A(en.left), en.bad, up * A(a.scale) * weight * A(a.inv_tau), a.kappa);
         if (out) {
             rv.template sweep<LANES>(me, seen, [&](int at, uint4(&v)[NV]) {
 #pragma unroll
@@ -596,7 +611,7 @@ cudaError_t launch_distill_of(const cwrnnt_rows &p, bool tail, const void *x, co
     a.n_rows = p.n_rows, a.x_stride = p.x_stride, a.g_stride = p.grad_stride;
     a.V = p.V, a.K = p.n_list;
     for (a.KP = 1; a.KP < a.K;) a.KP *= 2;
-    a.inv_tau = typename Elt<T>::acc(1.0 / p.temperature);
+    a.inv_tau = 1.0 / p.temperature;
     a.kappa = typename Elt<T>::acc(kLog2e / p.temperature);
     a.scale = scale;
     a.teacher = static_cast<const C *>(teacher), a.weight = static_cast<const C *>(weight);
