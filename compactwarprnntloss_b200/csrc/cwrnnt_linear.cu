@@ -5,7 +5,7 @@
 // dz at once (reading dy). Storing z in float instead costs more traffic than the product takes, storing it in 16 bits
 // costs digits of act'(z).
 //
-// One kernel for the four products: tiles of 128 x BN outputs, 64 elements of the sum a step. Operands come by tiled TMA
+// One kernel for the four products: tiles of 128 x 64 or 128 and 256 x 256 outputs, 64 elements of the sum a step. Operands come by tiled TMA
 // into a ring of 128-byte-swizzled stages; tcgen05.mma sums in TMEM in float. The forward product takes both operands
 // along the sum (K-major), dx takes W and dW takes both operands across it (MN-major): no operand is ever transposed in
 // memory. Warp 0 issues the loads, warp 1 the products; four or eight more warps carry the previous tile out of the other half
@@ -526,7 +526,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             const int end = n0 + BN < sh.N ? n0 + BN : sh.N;
             int col = n0 + share * step;
             const bool mine = row0 < sh.M && col < end;
-            if (BN >= 64 && mine) c.ask(row0, col);
+            if (mine) c.ask(row0, col);
             const bool ok = tc::mbar_wait(&sum_full[half], half_phase, &ctl.gave_up);
             tc::fence_after();
             __syncwarp();
@@ -541,34 +541,14 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         tc::mbar_arrive(&sum_empty[half]);
                 }
             };
-            if constexpr (BN >= 64) {
-                if (!mine) release();
-                for (; mine && col < end; col += kShares * step) {
-                    const int next = col + kShares * step;
-                    c.piece(d + uint32_t(col - n0), row0, split * sh.part_rows + row0, col, ok, next < end ? next : -1,
-                            release);
-                }
-            } else {
-                const int64_t row = row0 + lane;
-                uint32_t r[32];
-                tc::tmem_load32(d, r);
-                tc::tmem_load_wait();
-                release();
-                if (row < sh.M) {
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int left = sh.N - (n0 + g * 8);
-                        if (left <= 0) break;
-                        float v[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = ok ? __uint_as_float(r[g * 8 + i]) : NAN;
-                        finish_in_place<T>(ep, v, row, n0 + g * 8, left < 8 ? left : 8);
-                    }
-                }
+            if (!mine) release();
+            for (; mine && col < end; col += kShares * step) {
+                const int next = col + kShares * step;
+                c.piece(d + uint32_t(col - n0), row0, split * sh.part_rows + row0, col, ok, next < end ? next : -1, release);
             }
             if (++half == 2) half = 0, half_phase ^= 1;
         }
-        if (lane == 0) tc::stores_done();
+        if (lane == 0) tc::stores_read();
     }
     __syncwarp();
     tc::fence_before();
@@ -582,36 +562,29 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     }
 }
 
-// A few rows of x (a decoding step): one warp per COLS output columns, all rows at once, the weights read once and straight
-// from memory. Tiles of 128 rows would multiply zeros, and their set-up takes longer than this product
-// (8 x 1024 x 640 bf16: 5.2 against 8.4 us). kFewRows rows are the most that one pass carries; a second dimension of
-// CTAs carries more. Four columns a warp read x a quarter as often, where there are columns enough for all SMs.
+// A few rows of x (a decoding step): one warp per output column, all rows at once, the weights read once and straight
+// from memory. Tiles of 128 rows would multiply zeros, and their set-up takes longer than this product. kFewRows rows are
+// the most that one pass carries; a second dimension of CTAs carries more.
 constexpr int kFewRows = 8;
-constexpr int kRowsAtMost = 16;  // products of more rows take tiles
-template <typename T, bool VEC, int COLS>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 few_rows_kernel(const T *__restrict__ x, int64_t x_ld, const T *__restrict__ w, int64_t w_ld, int M, int N, int K,
                 const __grid_constant__ Epilogue ep)
 {
     using E = Elt<T>;
-    const int lane = threadIdx.x & 31, n0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * COLS, m0 = blockIdx.y * kFewRows;
-    if (n0 >= N) return;
+    const int lane = threadIdx.x & 31, n = blockIdx.x * 8 + (threadIdx.x >> 5), m0 = blockIdx.y * kFewRows;
+    if (n >= N) return;
     const int rows = M - m0 < kFewRows ? M - m0 : kFewRows;
-    const T *wn[COLS], *xm = x + int64_t(m0) * x_ld;
-#pragma unroll
-    for (int j = 0; j < COLS; ++j) wn[j] = w + int64_t(n0 + j < N ? n0 + j : n0) * w_ld;
-    float sum[COLS][kFewRows] = {};
+    const T *wn = w + int64_t(n) * w_ld, *xm = x + int64_t(m0) * x_ld;
+    float sum[kFewRows] = {};
     constexpr int kStep = VEC ? 8 : 1;
 #pragma unroll 2
     for (int k = lane * kStep; k < K; k += 32 * kStep) {
-        float a[COLS][kStep], b[kStep];
-#pragma unroll
-        for (int j = 0; j < COLS; ++j) {
-            if constexpr (VEC)
-                E::unpack(__ldg(reinterpret_cast<const uint4 *>(wn[j] + k)), a[j]);
-            else
-                a[j][0] = E::to_acc(__ldg(wn[j] + k));
-        }
+        float a[kStep], b[kStep];
+        if constexpr (VEC)
+            E::unpack(__ldg(reinterpret_cast<const uint4 *>(wn + k)), a);
+        else
+            a[0] = E::to_acc(__ldg(wn + k));
 #pragma unroll
         for (int r = 0; r < kFewRows; ++r) {
             if (r < rows) {
@@ -620,39 +593,34 @@ few_rows_kernel(const T *__restrict__ x, int64_t x_ld, const T *__restrict__ w, 
                 else
                     b[0] = E::to_acc(__ldg(xm + r * x_ld + k));
 #pragma unroll
-                for (int j = 0; j < COLS; ++j)
-#pragma unroll
-                    for (int i = 0; i < kStep; ++i) sum[j][r] = fmaf(a[j][i], b[i], sum[j][r]);
+                for (int i = 0; i < kStep; ++i) sum[r] = fmaf(a[i], b[i], sum[r]);
             }
         }
     }
-    float mine = 0.0f;  // lane j * kFewRows + r keeps column j of row r
+    float mine = 0.0f;  // lane r keeps row r
 #pragma unroll
-    for (int j = 0; j < COLS; ++j)
+    for (int r = 0; r < kFewRows; ++r) {
 #pragma unroll
-        for (int r = 0; r < kFewRows; ++r) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum[j][r] += __shfl_xor_sync(0xffffffffu, sum[j][r], o);
-            if (lane == j * kFewRows + r) mine = sum[j][r];
-        }
-    const int n = n0 + lane / kFewRows, r = lane % kFewRows;
-    if (lane < COLS * kFewRows && r < rows && n < N) {
-        const int64_t row = m0 + r;
+        for (int o = 16; o > 0; o >>= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
+        if (lane == r) mine = sum[r];
+    }
+    if (lane < rows) {
+        const int64_t row = m0 + lane;
         if (ep.bias) mine += E::to_acc(__ldg(static_cast<const T *>(ep.bias) + n));
         const float side = ep.side ? E::to_acc(__ldg(static_cast<const T *>(ep.side) + row * ep.side_ld + n)) : 0.0f;
         static_cast<T *>(ep.out)[row * ep.out_ld + n] = E::from_acc(finish_as(ep, mine, side));
     }
 }
-template <typename T, int COLS>
+template <typename T>
 cudaError_t run_few_rows(const T *x, int64_t x_ld, const T *w, int64_t w_ld, int M, int N, int K, const Epilogue &ep,
                          cudaStream_t s)
 {
-    const dim3 grid(unsigned((N + 8 * COLS - 1) / (8 * COLS)), unsigned((M + kFewRows - 1) / kFewRows));
+    const dim3 grid(unsigned((N + 7) / 8), unsigned((M + kFewRows - 1) / kFewRows));
     auto even = [](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
     if (K % 8 == 0 && even(x, x_ld) && even(w, w_ld))
-        few_rows_kernel<T, true, COLS><<<grid, 256, 0, s>>>(x, x_ld, w, w_ld, M, N, K, ep);
+        few_rows_kernel<T, true><<<grid, 256, 0, s>>>(x, x_ld, w, w_ld, M, N, K, ep);
     else
-        few_rows_kernel<T, false, COLS><<<grid, 256, 0, s>>>(x, x_ld, w, w_ld, M, N, K, ep);
+        few_rows_kernel<T, false><<<grid, 256, 0, s>>>(x, x_ld, w, w_ld, M, N, K, ep);
     return cudaGetLastError();
 }
 
@@ -790,8 +758,9 @@ bool make_map(CUtensorMap *map, const void *p, int64_t rows, int64_t cols, int64
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Products of a few rows need no tiles (and no copies for TMA).
-bool takes_few_rows(int64_t M, bool across) { return !across && M <= kRowsAtMost; }
+// Products of a few rows need no tiles (and no copies for TMA), as long as re-reading the rows of x for every column does
+// not take longer than a tile's set-up: 8 rows, us: 1024 x 640 5.0 (tiles 8.4), 1024 x 2048 7.7 (9.8), 4096 x 4096 28 (24).
+bool takes_few_rows(int64_t M, int64_t N, int64_t len) { return M <= 16 && N * len <= (int64_t(1) << 22); }
 
 // How a product of M x N outputs and a sum of `len` is cut: the width of its tiles and the parts of its sum.
 struct Cut {
@@ -800,17 +769,16 @@ struct Cut {
     int64_t tiles(int64_t M, int N) const { return ((M + rows() - 1) / rows()) * ((N + bn - 1) / bn); }
     int at_once() const { return bn == 256 ? kNumSMs / 2 : kNumSMs; }
 };
-Cut cut_product(int64_t M, int N, int64_t len, bool b_mn)
+Cut cut_product(int64_t M, int N, int64_t len)
 {
     const int steps = int((len + kBK - 1) / kBK);
     // Widths by what the waves of tiles cost, in clocks: a step takes what its operands take from L2 (about 60 bytes a
     // clock and SM), or its product; a tile takes its set-up and its epilogue, which hides behind the next tile's steps
     // only. Measured at 1000 x 1024 x 640 (width 64: one wave) and 40009 x 640 x 512 (pairs: 37 us, width 128: 52 us).
-    const int least = b_mn ? 64 : 32;
     Cut c{0, 1, steps};
     int64_t best = 0;
-    for (const int bn : {256, 128, 64, 32}) {
-        if (bn < least || (bn > least && bn / 2 >= N)) continue;
+    for (const int bn : {256, 128, 64}) {
+        if (bn > 64 && bn / 2 >= N) continue;
         const Cut t{bn, 1, steps};
         const int64_t waves = (t.tiles(M, N) + t.at_once() - 1) / t.at_once();
         const int loads = (kBM + (bn == 256 ? 128 : bn)) * kBK * 2 / 60, product = bn == 256 ? 512 : 2 * bn * 2;
@@ -885,7 +853,6 @@ cudaError_t run_product_bn(int bn, const Matrix &a, const Matrix &b, const Shape
     case 128: return run_product<T, 128, A_MN, B_MN>(a, b, sh, ep, s);
     case 64: return run_product<T, 64, A_MN, B_MN>(a, b, sh, ep, s);
     }
-    if constexpr (!B_MN) return run_product<T, 32, A_MN, B_MN>(a, b, sh, ep, s);
     return cudaErrorInvalidValue;
 }
 
@@ -893,12 +860,10 @@ cudaError_t run_product_bn(int bn, const Matrix &a, const Matrix &b, const Shape
 template <typename T>
 cudaError_t product(const Matrix &a, const Matrix &b, int64_t M, int N, int64_t len, Epilogue ep, float *part, cudaStream_t s)
 {
-    if (takes_few_rows(M, a.mn || b.mn)) {
-        const T *x = static_cast<const T *>(a.p), *w = static_cast<const T *>(b.p);
-        if (N >= 2048) return run_few_rows<T, 4>(x, a.ld, w, b.ld, int(M), N, int(len), ep, s);
-        return run_few_rows<T, 1>(x, a.ld, w, b.ld, int(M), N, int(len), ep, s);
-    }
-    const Cut c = cut_product(M, N, len, b.mn);
+    if (!a.mn && !b.mn && takes_few_rows(M, N, len))
+        return run_few_rows<T>(static_cast<const T *>(a.p), a.ld, static_cast<const T *>(b.p), b.ld, int(M), N, int(len), ep,
+                               s);
+    const Cut c = cut_product(M, N, len);
     Shape sh{};
     sh.M = M, sh.N = N;
     sh.steps = int((len + kBK - 1) / kBK);
@@ -948,20 +913,20 @@ LinearPlan plan_linear(const cwrnnt_linear &p, bool backward)
         at += align_up(bytes, 256);
         return here;
     };
-    const bool copies = backward || !takes_few_rows(p.n_rows, false);
+    const bool copies = backward || !takes_few_rows(p.n_rows, p.n_out, p.n_in);
     q.x = take(copies ? copy_bytes(p.n_rows, p.n_in, p.x_stride) : 0);
     q.w = take(copies ? copy_bytes(p.n_out, p.n_in, p.w_stride) : 0);
     auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
     int64_t parts = 0;
     if (!backward || p.activation != CWRNNT_ACT_NONE)
-        parts = part_bytes(p.n_rows, p.n_out, cut_product(p.n_rows, p.n_out, p.n_in, false));
+        parts = part_bytes(p.n_rows, p.n_out, cut_product(p.n_rows, p.n_out, p.n_in));
     if (backward) {
         if (p.activation != CWRNNT_ACT_NONE)
             q.dz = take(p.n_rows * padded(p.n_out) * 2);
         else
             q.g = take(copy_bytes(p.n_rows, p.n_out, p.g_stride));
-        parts = most(parts, part_bytes(p.n_rows, p.n_in, cut_product(p.n_rows, p.n_in, p.n_out, true)));
-        parts = most(parts, part_bytes(p.n_out, p.n_in, cut_product(p.n_out, p.n_in, p.n_rows, true)));
+        parts = most(parts, part_bytes(p.n_rows, p.n_in, cut_product(p.n_rows, p.n_in, p.n_out)));
+        parts = most(parts, part_bytes(p.n_out, p.n_in, cut_product(p.n_out, p.n_in, p.n_rows)));
         q.sums = take(4 * (kMostRuns + (p.n_rows + 31) / 32) * int64_t(p.n_out));
     }
     q.part = take(parts);
@@ -1001,7 +966,7 @@ cudaError_t linear_forward(const cwrnnt_linear &p, const void *x, const void *w,
 {
     const LinearPlan q = plan_linear(p, false);
     Matrix a{x, p.n_rows, p.n_in, p.x_stride, false}, b{w, p.n_out, p.n_in, p.w_stride, false};
-    if (!takes_few_rows(p.n_rows, false)) {
+    if (!takes_few_rows(p.n_rows, p.n_out, p.n_in)) {
         CWRNNT_TRY(readable<T>(a, ws + q.x, s));
         CWRNNT_TRY(readable<T>(b, ws + q.w, s));
     }
@@ -1031,8 +996,8 @@ cudaError_t linear_backward(const cwrnnt_linear &p, const void *x, const void *w
         ep.mode = kSlope, ep.act = p.activation, ep.bias = bias;
         ep.side = g, ep.side_ld = p.g_stride;
         ep.out = ws + q.dz, ep.out_ld = padded(p.n_out);
-        const Cut c = cut_product(p.n_rows, p.n_out, p.n_in, false);
-        if (grad_b && c.splits == 1 && c.bn >= 64 && !takes_few_rows(p.n_rows, false)) ep.sums = sums, runs = (p.n_rows + 31) / 32;
+        const Cut c = cut_product(p.n_rows, p.n_out, p.n_in);
+        if (grad_b && c.splits == 1 && !takes_few_rows(p.n_rows, p.n_out, p.n_in)) ep.sums = sums, runs = (p.n_rows + 31) / 32;
         CWRNNT_TRY(product<T>(mx, mw, p.n_rows, p.n_out, p.n_in, ep, part, s));
         dz.p = ws + q.dz, dz.ld = padded(p.n_out);
     } else {

@@ -107,9 +107,8 @@ __device__ __forceinline__ void store_2d(const CUtensorMap *map, const void *src
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// This thread's stores have read their shared memory / have reached global memory.
+// This thread's stores have read their shared memory.
 __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // Shared memory written by this thread is visible to the copies issued behind the next barrier.
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
