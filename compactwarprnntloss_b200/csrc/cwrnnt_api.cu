@@ -679,10 +679,12 @@ int cwrnnt_distill(const cwrnnt_rows *p, int32_t tail, const void *x, const void
     return e == cudaSuccess ? CWRNNT_OK : fail_launch("distill", e);
 }
 
-int64_t cwrnnt_linear_workspace_bytes(const cwrnnt_linear *p, int32_t backward)
+int64_t cwrnnt_linear_workspace_bytes(const cwrnnt_linear *p, int32_t pass)
 {
-    if (check_linear(p) != CWRNNT_OK || (backward && p->g_stride < p->n_out)) return -1;
-    return linear_workspace(*p, backward != 0);
+    if (check_linear(p) != CWRNNT_OK || pass < CWRNNT_LINEAR_FORWARD || pass > CWRNNT_LINEAR_FORWARD_RESIDUAL ||
+        (pass == CWRNNT_LINEAR_BACKWARD && p->g_stride < p->n_out))
+        return -1;
+    return linear_workspace(*p, pass == CWRNNT_LINEAR_BACKWARD, pass == CWRNNT_LINEAR_FORWARD_RESIDUAL);
 }
 
 int cwrnnt_linear_forward(const cwrnnt_linear *p, const void *x, const void *weight, const void *bias,
@@ -692,9 +694,11 @@ int cwrnnt_linear_forward(const cwrnnt_linear *p, const void *x, const void *wei
     int st = check_linear(p);
     if (st) return st;
     if (p->n_rows == 0) return CWRNNT_OK;
-    if (!linear_base(x, p->x_stride) || !linear_base(weight, p->w_stride) || !y) return CWRNNT_ERR_ARGUMENT;
+    if (!linear_base(x, p->x_stride) || !linear_base(weight, p->w_stride) || !y ||
+        (residual && !linear_base(residual, p->n_out)))
+        return CWRNNT_ERR_ARGUMENT;
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
-        workspace_bytes < linear_workspace(*p, false))
+        workspace_bytes < linear_workspace(*p, false, residual != nullptr))
         return CWRNNT_ERR_WORKSPACE;
     cudaError_t e = launch_linear(*p, x, weight, bias, residual, workspace, y, reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? CWRNNT_OK : fail_launch("linear_forward", e);
@@ -716,7 +720,7 @@ int cwrnnt_linear_backward(const cwrnnt_linear *p, const void *x, const void *we
     }
     if (!linear_base(x, p->x_stride) || !linear_base(weight, p->w_stride) || !linear_base(grad_y, p->g_stride))
         return CWRNNT_ERR_ARGUMENT;
-    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < linear_workspace(*p, true))
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < linear_workspace(*p, true, false))
         return CWRNNT_ERR_WORKSPACE;
     e = launch_linear_grad(*p, x, weight, bias, grad_y, workspace, grad_x, grad_weight, grad_bias, s);
     return e == cudaSuccess ? CWRNNT_OK : fail_launch("linear_backward", e);

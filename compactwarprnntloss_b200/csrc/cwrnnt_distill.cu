@@ -131,14 +131,17 @@ __device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, in
         en.sum_q = s == 0.0 ? A(0) : A(s / s);
         en.left = 0.0;
     }
-    en.first = en.c >= 0;
-    en.dup_q = A(0);
-    for (int o = 0; o < K; ++o) {
-        const int other = __shfl_sync(kAll, en.c, o, width);
-        const A oq = __shfl_sync(kAll, A(en.q), o, width);
-        const bool mine = other == en.c;
-        en.dup_q += mine ? oq : A(0);
-        en.first = en.first && !(mine && o < e);
+    const int lane = threadIdx.x & 31;
+    const unsigned row = (width == 32 ? kAll : (1u << width) - 1u) << (lane / width * width);
+    const unsigned same = __match_any_sync(kAll, en.c) & row;  // the row's entries with this token
+    en.first = en.c >= 0 && __ffs(same) - 1 == lane;
+    en.dup_q = A(en.q);
+    if (__any_sync(kAll, en.c >= 0 && (same & (same - 1)) != 0)) {
+        en.dup_q = A(0);
+        for (int o = 0; o < K; ++o) {
+            const A oq = __shfl_sync(kAll, A(en.q), o, width);
+            en.dup_q += same >> (lane / width * width + o) & 1 ? oq : A(0);
+        }
     }
     return en;
 }

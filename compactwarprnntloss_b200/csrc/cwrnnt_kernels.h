@@ -99,7 +99,7 @@ cudaError_t launch_distill(const cwrnnt_rows &p, bool tail, const void *x, const
                            double *partial, void *row_loss, void *loss, void *grad_x, cudaStream_t s);
 
 // Linear layers on the tensor cores: forward, gradients, and the workspace of either.
-int64_t linear_workspace(const cwrnnt_linear &p, bool backward);
+int64_t linear_workspace(const cwrnnt_linear &p, bool backward, bool residual);
 cudaError_t launch_linear(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *residual,
                           void *workspace, void *y, cudaStream_t s);
 cudaError_t launch_linear_grad(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *g,

@@ -74,9 +74,11 @@ struct Epilogue {
     const void *side;   // kStore: residual [M, side_ld] or null; kSlope: dy [M, side_ld]
     void *out;          // [M, out_ld]; kPart: float [splits * rows of tiles, out_ld]
     int64_t side_ld, out_ld;
-    bool tma_out, tma_side;  // rows of out / side lie on 16-byte boundaries: they go by TMA
+    bool tma_out;            // rows of out lie on 16-byte boundaries: they go by TMA (rows of side always do)
     bool vec;                // all 16-byte accesses allowed, columns in whole groups of 8
     float *sums;             // kSlope: sums over each 32 rows of dz, [rows / 32, N], or null
+    void *low;               // kSlope: what dz loses in its rounding, rounded again, as `out`; or null
+    __host__ __device__ int pieces() const { return 1 + (side != nullptr) + (low != nullptr); }
 };
 
 // What becomes of an element of the product once the bias is added: an activation, or (kSlopeOf + activation) the upstream
@@ -93,6 +95,14 @@ __device__ __forceinline__ float finish_as(const Epilogue &ep, float v, float si
 {
     if (ep.mode == kSlope) return side * slope(ep.act, v);
     return activate(ep.act, v) + side;
+}
+
+// What v loses when it is rounded to T, rounded to T.
+template <typename T>
+__device__ __forceinline__ T low_part(float v)
+{
+    const float high = Elt<T>::to_acc(Elt<T>::from_acc(v));
+    return Elt<T>::from_acc(fabsf(high) < INFINITY ? v - high : 0.0f);
 }
 
 // Columns [col, col + 8) of one row straight from and to global memory, `n` of them inside the matrix.
@@ -125,13 +135,20 @@ __device__ __forceinline__ void finish_in_place(const Epilogue &ep, float (&v)[8
         for (int c = 0; c < 8; ++c)
             if (c < n) out[c] = E::from_acc(v[c]);
     }
+    if (ep.low) {
+        T *low = static_cast<T *>(ep.low) + row * ep.out_ld + col;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c < n) low[c] = low_part<T>(v[c]);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------- kernel
 struct Shape {
     int64_t M;
     int N;
-    int steps;  // steps of kBK along the sum, in all
+    int steps;       // steps of kBK along the sum, in all
+    int half_steps;  // of them, those of A's first part: A may be the sum of two matrices (0: it is one)
     int steps_per_split, splits;
     int64_t tiles_m;
     int tiles_n;
@@ -183,14 +200,20 @@ struct Layout {
     static constexpr int kCarriers = BN >= 128 ? 8 : 4;  // warps of the epilogue
     static constexpr int kThreads = 64 + 32 * kCarriers;
     static constexpr uint32_t kColumns = 2 * BN;         // two sums in TMEM
-    static constexpr int stages(bool side)
+    // `pieces`: of each carrier, one on its way out, one in where there is a side, another out where dz has a low part
+    static constexpr int stages(int pieces)
     {
-        const int n = (227 * 1024 - int(sizeof(Control)) - kCarriers * kPiece * (side ? 2 : 1)) / kStage;
+        const int n = (227 * 1024 - int(sizeof(Control)) - kCarriers * kPiece * pieces) / kStage;
         return n < kMaxStages ? n : kMaxStages;
     }
-    static constexpr int bytes(bool side)
+    static constexpr int bytes(int pieces)
     {
-        return stages(side) * kStage + kCarriers * kPiece * (side ? 2 : 1) + int(sizeof(Control));
+        return stages(pieces) * kStage + kCarriers * kPiece * pieces + int(sizeof(Control));
+    }
+    static constexpr int most_bytes()
+    {
+        const int a = bytes(1), b = bytes(2), c = bytes(3);
+        return a > b ? (a > c ? a : c) : (b > c ? b : c);
     }
 };
 
@@ -210,8 +233,8 @@ struct Carrier {
     const Epilogue &ep;
     const int64_t M;
     const int N;
-    const CUtensorMap *map_out, *map_side;
-    unsigned char *out_piece, *side_piece;
+    const CUtensorMap *map_out, *map_side, *map_low;
+    unsigned char *out_piece, *side_piece, *low_piece;
     float *bias;  // 64 of them
     uint64_t *side_bar;
     volatile int *gave_up;
@@ -222,7 +245,7 @@ struct Carrier {
     // what the piece at (row0, col) needs
     __device__ __forceinline__ void ask(int row0, int col)
     {
-        if (ep.side && ep.tma_side && lane == 0) {
+        if (ep.side && lane == 0) {
             tc::mbar_expect(side_bar, kPiece);
             tc::load_2d(side_piece, map_side, side_bar, col, row0);
         }
@@ -262,6 +285,12 @@ struct Carrier {
             uint4 w = E::pack(v);
             if (!ok) w = make_uint4(~0u, ~0u, ~0u, ~0u);  // a wait that ran out leaves NaN
             *piece_group(out_piece, lane, g) = w;
+            if constexpr (KIND == kSlopeOf + CWRNNT_ACT_TANH || KIND == kSlopeOf + CWRNNT_ACT_SILU) {
+                E::unpack(w, s);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = fabsf(s[i]) < INFINITY ? v[i] - s[i] : 0.0f;
+                *piece_group(low_piece, lane, g) = E::pack(v);
+            }
         }
     }
     template <typename Release>
@@ -279,6 +308,18 @@ struct Carrier {
             *piece_group(out_piece, lane, g) = w;
         }
     }
+    // The piece's rows added up: columns 2 * lane and 2 * lane + 1. (Rows behind the matrix are zero: their upstream
+    // gradient is.)
+    __device__ __forceinline__ void add_rows(unsigned char *piece, float &s0, float &s1) const
+    {
+#pragma unroll 8
+        for (int k = 0; k < 32; ++k) {
+            const uint32_t w = reinterpret_cast<const uint32_t *>(piece_group(piece, k, lane >> 2))[lane & 3];
+            float v[8];
+            E::unpack(make_uint4(w, 0u, 0u, 0u), v);
+            s0 += v[0], s1 += v[1];
+        }
+    }
     // `d`: TMEM address of the piece's first column in this warp's lanes; `release`: gives the tile's sums back
     template <typename Release>
     __device__ __forceinline__ void piece(uint32_t d, int row0, int64_t out_row0, int col, bool ok, int next_col,
@@ -287,22 +328,8 @@ struct Carrier {
         if (ep.mode != kPart) {
             bias[lane] = next_bias[0], bias[32 + lane] = next_bias[1];
             if (ep.side) {
-                if (ep.tma_side) {
-                    ok = tc::mbar_wait(side_bar, side_phase, gave_up) && ok;
-                    side_phase ^= 1;
-                } else {
-                    // rows off the boundaries: each row of the piece as 64 consecutive elements
-                    T *s = reinterpret_cast<T *>(side_piece);
-                    for (int r = 0; r < 32; ++r)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int c = h * 32 + lane;
-                            T v = E::from_acc(0.0f);
-                            if (row0 + r < M && col + c < N)
-                                v = __ldg(static_cast<const T *>(ep.side) + int64_t(row0 + r) * ep.side_ld + col + c);
-                            s[r * 64 + (((c >> 3) ^ (r & 7)) << 3) + (c & 7)] = v;
-                        }
-                }
+                ok = tc::mbar_wait(side_bar, side_phase, gave_up) && ok;
+                side_phase ^= 1;
             }
         }
         if (lane == 0) tc::stores_read();  // the last piece has left the buffer
@@ -339,17 +366,14 @@ struct Carrier {
 #undef CWRNNT_KIND
         if (ep.tma_out) tc::fence_async();
         __syncwarp();
-        if (ep.tma_out && lane == 0) tc::store_2d(map_out, out_piece, col, int(out_row0));
+        if (ep.tma_out && lane == 0) {
+            tc::store_2d(map_out, out_piece, col, int(out_row0));
+            if (ep.low) tc::store_2d(map_low, low_piece, col, int(out_row0));
+        }
+        float s0 = 0.0f, s1 = 0.0f;
+        if (ep.sums) add_rows(out_piece, s0, s1);
+        if (ep.sums && ep.low) add_rows(low_piece, s0, s1);
         if (ep.sums) {
-            // rows behind the matrix are zero here: their upstream gradient is
-            float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll 8
-            for (int k = 0; k < 32; ++k) {
-                const uint32_t w = reinterpret_cast<const uint32_t *>(piece_group(out_piece, k, lane >> 2))[lane & 3];
-                float v[8];
-                E::unpack(make_uint4(w, 0u, 0u, 0u), v);
-                s0 += v[0], s1 += v[1];
-            }
             float *to = ep.sums + int64_t(row0 / 32) * N + col + 2 * lane;
             if (col + 2 * lane < N) to[0] = s0;
             if (col + 2 * lane + 1 < N) to[1] = s1;
@@ -373,13 +397,14 @@ template <typename T, int BN, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(Layout<BN>::kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
               const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_side,
+              const __grid_constant__ CUtensorMap map_low,
               const __grid_constant__ Shape sh, const __grid_constant__ Epilogue ep)
 {
     using L = Layout<BN>;
     // stages, pieces, control: the stages start on a 1024-byte boundary, as the swizzle wants it
     extern __shared__ __align__(1024) unsigned char stages[];
     unsigned char *const pieces = stages + sh.stages * L::kStage;
-    Control &ctl = *reinterpret_cast<Control *>(pieces + L::kCarriers * kPiece * (ep.side ? 2 : 1));
+    Control &ctl = *reinterpret_cast<Control *>(pieces + L::kCarriers * kPiece * ep.pieces());
     uint64_t *const full = ctl.full, *const empty = ctl.empty;
     uint64_t *const sum_full = ctl.sum_full, *const sum_empty = ctl.sum_empty;
     const bool placed = (tc::smem_addr(stages) & 1023) == 0;  // else every role gives up at once
@@ -429,9 +454,12 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 const int k0 = sh.first_step(split), k1 = k0 + sh.count_steps(split);
                 const int row = (int(m) * kCtas + rank) * kBM;
                 const int col = n * BN + rank * (sh.width(n, BN, kCtas) / 2);
-                for (int k = k0; ok && k < k1; ++k) {
+                for (int t_k = k0; ok && t_k < k1; ++t_k) {
                     ok = tc::mbar_wait(&empty[at], phase ^ 1, &ctl.gave_up);
                     if (!ok) break;
+                    const bool low = sh.half_steps > 0 && t_k >= sh.half_steps;
+                    const int k = low ? t_k - sh.half_steps : t_k;
+                    const CUtensorMap *const from_a = low ? &map_low : &map_a;
                     unsigned char *a = stages + at * L::kStage, *b = a + L::kA;
                     if (rank == 0) tc::mbar_expect(&full[at], L::kStage * kCtas);
                     const uint32_t bar = kPair ? tc::peer_addr(&full[at], 0) : 0;
@@ -443,9 +471,9 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     };
                     if (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < kBM / 64; ++i) load(a + i * 8192, &map_a, row + i * 64, k * kBK);
+                        for (int i = 0; i < kBM / 64; ++i) load(a + i * 8192, from_a, row + i * 64, k * kBK);
                     } else {
-                        load(a, &map_a, k * kBK, row);
+                        load(a, from_a, k * kBK, row);
                     }
                     if (B_MN) {
 #pragma unroll
@@ -513,8 +541,9 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         constexpr int kShares = L::kCarriers / 4;
         int half = 0;
         uint32_t half_phase = 0;
-        Carrier<T> c{ep, sh.M, sh.N, &map_out, &map_side, pieces + carrier * kPiece,
-                     pieces + (L::kCarriers + carrier) * kPiece, ctl.bias[carrier], &ctl.side_full[carrier], &ctl.gave_up,
+        Carrier<T> c{ep, sh.M, sh.N, &map_out, &map_side, &map_low, pieces + carrier * kPiece,
+                     pieces + (L::kCarriers + carrier) * kPiece, pieces + (2 * L::kCarriers + carrier) * kPiece,
+                     ctl.bias[carrier], &ctl.side_full[carrier], &ctl.gave_up,
                      0, lane, {}};
         const int step = ep.mode == kPart ? 32 : 64;
         for (int64_t t = t0; t < total; t += dt) {
@@ -608,7 +637,9 @@ few_rows_kernel(const T *__restrict__ x, int64_t x_ld, const T *__restrict__ w, 
         const int64_t row = m0 + lane;
         if (ep.bias) mine += E::to_acc(__ldg(static_cast<const T *>(ep.bias) + n));
         const float side = ep.side ? E::to_acc(__ldg(static_cast<const T *>(ep.side) + row * ep.side_ld + n)) : 0.0f;
-        static_cast<T *>(ep.out)[row * ep.out_ld + n] = E::from_acc(finish_as(ep, mine, side));
+        mine = finish_as(ep, mine, side);
+        static_cast<T *>(ep.out)[row * ep.out_ld + n] = E::from_acc(mine);
+        if (ep.low) static_cast<T *>(ep.low)[row * ep.out_ld + n] = low_part<T>(mine);
     }
 }
 template <typename T>
@@ -656,10 +687,11 @@ __global__ void __launch_bounds__(256) restride_kernel(const T *__restrict__ src
     }
 }
 
-// Column sums: each CTA adds up a run of rows of 256 columns in float; the runs' sums are added in order afterwards.
+// Column sums (of a matrix, or of one in two parts): each CTA adds up a run of rows of 256 columns in float; the runs' sums are added in order afterwards.
 constexpr int kSumRows = 8;
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ g, int64_t ld, int64_t rows, int cols,
+__global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ high,
+                                                          const T *__restrict__ low, int64_t ld, int64_t rows, int cols,
                                                           int64_t run, float *__restrict__ part)
 {
     using E = Elt<T>;
@@ -668,7 +700,8 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ 
     const int col = blockIdx.x * 256 + tx * 8;
     float acc[8] = {};
     const int64_t first = int64_t(blockIdx.y) * run, end = first + run < rows ? first + run : rows;
-    if (col < cols) {
+    for (const T *g : {high, low}) {
+        if (!g || col >= cols) break;
         for (int64_t r = first + ty; r < end; r += kSumRows) {
             float v[8];
             if (col + 8 <= cols) {
@@ -762,28 +795,31 @@ bool make_map(CUtensorMap *map, const void *p, int64_t rows, int64_t cols, int64
 // not take longer than a tile's set-up: 8 rows, us: 1024 x 640 5.0 (tiles 8.4), 1024 x 2048 7.7 (9.8), 4096 x 4096 28 (24).
 bool takes_few_rows(int64_t M, int64_t N, int64_t len) { return M <= 16 && N * len <= (int64_t(1) << 22); }
 
-// How a product of M x N outputs and a sum of `len` is cut: the width of its tiles and the parts of its sum.
+int steps_of(int64_t len) { return int((len + kBK - 1) / kBK); }
+
+// How a product of M x N outputs and a sum of `steps` steps is cut: the width of its tiles and the parts of its sum.
 struct Cut {
     int bn, splits, steps_per_split;
     int rows() const { return bn == 256 ? 2 * kBM : kBM; }  // of a tile (of both CTAs of a pair)
     int64_t tiles(int64_t M, int N) const { return ((M + rows() - 1) / rows()) * ((N + bn - 1) / bn); }
     int at_once() const { return bn == 256 ? kNumSMs / 2 : kNumSMs; }
 };
-Cut cut_product(int64_t M, int N, int64_t len)
+Cut cut_product(int64_t M, int N, int steps)
 {
-    const int steps = int((len + kBK - 1) / kBK);
-    // Widths by what the waves of tiles cost, in clocks: a step takes what its operands take from L2 (about 60 bytes a
-    // clock and SM), or its product; a tile takes its set-up and its epilogue, which hides behind the next tile's steps
-    // only. Measured at 1000 x 1024 x 640 (width 64: one wave) and 40009 x 640 x 512 (pairs: 37 us, width 128: 52 us).
+    // The width by what its waves of tiles take, in ns: a launch, and for each wave the steps or the epilogue, whichever is
+    // longer. Measured with each width forced: 4000 x 512 x 64 (one step) 6.0 / 5.1 / 7.9 us at 64 / 128 / 256,
+    // 40009 x 640 x 64 33.6 / 21.3 / 24.8, 40009 x 640 x 512 72 / 42 / 34, 4000 x 1024 x 640 19.4 / 12.7 / 11.5.
+    struct Width {
+        int bn, launch, step, epilogue;
+    };
+    constexpr Width widths[] = {{256, 5500, 520, 3100}, {128, 4000, 420, 1600}, {64, 4500, 390, 1350}};
     Cut c{0, 1, steps};
     int64_t best = 0;
-    for (const int bn : {256, 128, 64}) {
-        if (bn > 64 && bn / 2 >= N) continue;
-        const Cut t{bn, 1, steps};
-        const int64_t waves = (t.tiles(M, N) + t.at_once() - 1) / t.at_once();
-        const int loads = (kBM + (bn == 256 ? 128 : bn)) * kBK * 2 / 60, product = bn == 256 ? 512 : 2 * bn * 2;
-        const int64_t epilogue = bn * 18, main = steps * int64_t(loads > product ? loads : product);
-        const int64_t cost = waves * (main > epilogue ? main : epilogue) + epilogue;
+    for (const Width &w : widths) {
+        if (w.bn > 64 && w.bn / 2 >= N) continue;
+        const Cut t{w.bn, 1, steps};
+        const int64_t waves = (t.tiles(M, N) + t.at_once() - 1) / t.at_once(), main = int64_t(steps) * w.step;
+        const int64_t cost = w.launch + waves * (main > w.epilogue ? main : w.epilogue);
         if (c.bn == 0 || cost < best) c = t, best = cost;
     }
     // split long sums of few tiles, at least eight steps a part
@@ -809,40 +845,44 @@ struct Matrix {  // [rows, cols], `mn`: its columns are the output's and its row
     const void *p;
     int64_t rows, cols, ld;
     bool mn;
+    const void *low = nullptr;  // another matrix of the same shape to be added to it, or none
 };
 
 template <typename T, int BN, bool A_MN, bool B_MN>
 cudaError_t run_product(const Matrix &a, const Matrix &b, Shape sh, const Epilogue &ep, cudaStream_t s)
 {
     using L = Layout<BN>;
-    CUtensorMap ma, mb, mo{}, ms{};
+    CUtensorMap ma, mb, mo{}, ms{}, ml{};
     bool good = make_map<T>(&ma, a.p, a.rows, a.cols, a.ld, A_MN ? kBK : kBM) &&
                 make_map<T>(&mb, b.p, b.rows, b.cols, b.ld, B_MN ? kBK : L::kRowsB);
     if (ep.mode == kPart)
         good = good && make_map<float>(&mo, ep.out, sh.splits * part_rows(sh.M), sh.N, ep.out_ld, 32);
     else if (ep.tma_out)
         good = good && make_map<T>(&mo, ep.out, sh.M, sh.N, ep.out_ld, 32);
-    if (ep.side && ep.tma_side) good = good && make_map<T>(&ms, ep.side, sh.M, sh.N, ep.side_ld, 32);
+    if (ep.side) good = good && make_map<T>(&ms, ep.side, sh.M, sh.N, ep.side_ld, 32);
+    // the low part of A, or of dz on its way out (never both)
+    if (a.low) good = good && make_map<T>(&ml, a.low, a.rows, a.cols, a.ld, A_MN ? kBK : kBM);
+    if (ep.low) good = good && make_map<T>(&ml, ep.low, sh.M, sh.N, ep.out_ld, 32);
     if (!good) return cudaErrorInvalidValue;
-    const bool side = ep.side != nullptr;
-    sh.stages = L::stages(side);
+    const int pieces = ep.pieces();
+    sh.stages = L::stages(pieces);
     auto kernel = linear_kernel<T, BN, A_MN, B_MN>;
     // the attribute belongs to the device that is current
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes(false) > L::bytes(true) ? L::bytes(false) : L::bytes(true));
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::most_bytes());
     if (e != cudaSuccess) return e;
     const int ctas = L::kPair ? 2 : 1;
     const int64_t total = sh.tiles_m * sh.tiles_n * sh.splits * ctas;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(total < kNumSMs ? total : kNumSMs));
     cfg.blockDim = dim3(L::kThreads);
-    cfg.dynamicSmemBytes = L::bytes(side);
+    cfg.dynamicSmemBytes = L::bytes(pieces);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = L::kPair ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, ms, sh, ep);
+    return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, ms, ml, sh, ep);
 }
 
 template <typename T, bool A_MN, bool B_MN>
@@ -863,18 +903,20 @@ cudaError_t product(const Matrix &a, const Matrix &b, int64_t M, int N, int64_t 
     if (!a.mn && !b.mn && takes_few_rows(M, N, len))
         return run_few_rows<T>(static_cast<const T *>(a.p), a.ld, static_cast<const T *>(b.p), b.ld, int(M), N, int(len), ep,
                                s);
-    const Cut c = cut_product(M, N, len);
+    const int steps = steps_of(len) * (a.low ? 2 : 1);
+    const Cut c = cut_product(M, N, steps);
     Shape sh{};
     sh.M = M, sh.N = N;
-    sh.steps = int((len + kBK - 1) / kBK);
+    sh.steps = steps;
+    sh.half_steps = a.low ? steps / 2 : 0;
     sh.steps_per_split = c.steps_per_split, sh.splits = c.splits;
     sh.tiles_m = (M + c.rows() - 1) / c.rows(), sh.tiles_n = (N + c.bn - 1) / c.bn;
     sh.part_rows = part_rows(M);
     auto on16 = [](const void *p, int64_t ld) {
         return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0);
     };
-    ep.tma_out = on16(ep.out, ep.out_ld), ep.tma_side = on16(ep.side, ep.side_ld);
-    ep.vec = N % 8 == 0 && ep.tma_out && ep.tma_side;
+    ep.tma_out = on16(ep.out, ep.out_ld);
+    ep.vec = N % 8 == 0 && ep.tma_out && on16(ep.side, ep.side_ld);
     Epilogue here = ep;
     if (c.splits > 1) {
         here = Epilogue{};
@@ -901,10 +943,17 @@ int64_t copy_bytes(int64_t rows, int64_t cols, int64_t ld)
 }
 constexpr int kMostRuns = 256;
 
+// dz is rounded to the operands' type for its two products. Rounded once it would cost their results as much again as
+// their own rounding does, so it goes into them as two parts; relu's is exact as it is.
+int parts_of(const cwrnnt_linear &p)
+{
+    return p.activation == CWRNNT_ACT_TANH || p.activation == CWRNNT_ACT_SILU ? 2 : 1;
+}
+
 struct LinearPlan {
-    int64_t x, w, g, dz, part, sums, total;  // offsets
+    int64_t x, w, g, dz, low, side, part, sums, total;  // offsets
 };
-LinearPlan plan_linear(const cwrnnt_linear &p, bool backward)
+LinearPlan plan_linear(const cwrnnt_linear &p, bool backward, bool residual)
 {
     LinearPlan q{};
     int64_t at = 0;
@@ -913,20 +962,20 @@ LinearPlan plan_linear(const cwrnnt_linear &p, bool backward)
         at += align_up(bytes, 256);
         return here;
     };
+    q.side = take(residual ? copy_bytes(p.n_rows, p.n_out, p.n_out) : 0);
     const bool copies = backward || !takes_few_rows(p.n_rows, p.n_out, p.n_in);
     q.x = take(copies ? copy_bytes(p.n_rows, p.n_in, p.x_stride) : 0);
     q.w = take(copies ? copy_bytes(p.n_out, p.n_in, p.w_stride) : 0);
     auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
     int64_t parts = 0;
     if (!backward || p.activation != CWRNNT_ACT_NONE)
-        parts = part_bytes(p.n_rows, p.n_out, cut_product(p.n_rows, p.n_out, p.n_in));
+        parts = part_bytes(p.n_rows, p.n_out, cut_product(p.n_rows, p.n_out, steps_of(p.n_in)));
     if (backward) {
-        if (p.activation != CWRNNT_ACT_NONE)
-            q.dz = take(p.n_rows * padded(p.n_out) * 2);
-        else
-            q.g = take(copy_bytes(p.n_rows, p.n_out, p.g_stride));
-        parts = most(parts, part_bytes(p.n_rows, p.n_in, cut_product(p.n_rows, p.n_in, p.n_out)));
-        parts = most(parts, part_bytes(p.n_out, p.n_in, cut_product(p.n_out, p.n_in, p.n_rows)));
+        q.g = take(copy_bytes(p.n_rows, p.n_out, p.g_stride));
+        if (p.activation != CWRNNT_ACT_NONE) q.dz = take(p.n_rows * padded(p.n_out) * 2);
+        if (parts_of(p) == 2) q.low = take(p.n_rows * padded(p.n_out) * 2);
+        parts = most(parts, part_bytes(p.n_rows, p.n_in, cut_product(p.n_rows, p.n_in, steps_of(p.n_out) * parts_of(p))));
+        parts = most(parts, part_bytes(p.n_out, p.n_in, cut_product(p.n_out, p.n_in, steps_of(p.n_rows) * parts_of(p))));
         q.sums = take(4 * (kMostRuns + (p.n_rows + 31) / 32) * int64_t(p.n_out));
     }
     q.part = take(parts);
@@ -964,7 +1013,7 @@ template <typename T>
 cudaError_t linear_forward(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *residual,
                            char *ws, void *y, cudaStream_t s)
 {
-    const LinearPlan q = plan_linear(p, false);
+    const LinearPlan q = plan_linear(p, false, residual != nullptr);
     Matrix a{x, p.n_rows, p.n_in, p.x_stride, false}, b{w, p.n_out, p.n_in, p.w_stride, false};
     if (!takes_few_rows(p.n_rows, p.n_out, p.n_in)) {
         CWRNNT_TRY(readable<T>(a, ws + q.x, s));
@@ -972,7 +1021,9 @@ cudaError_t linear_forward(const cwrnnt_linear &p, const void *x, const void *w,
     }
     Epilogue ep{};
     ep.mode = kStore, ep.act = p.activation, ep.bias = bias;
-    ep.side = residual, ep.side_ld = p.n_out;
+    Matrix r{residual, p.n_rows, p.n_out, p.n_out, false};
+    if (residual && !takes_few_rows(p.n_rows, p.n_out, p.n_in)) CWRNNT_TRY(readable<T>(r, ws + q.side, s));
+    ep.side = r.p, ep.side_ld = r.ld;
     ep.out = y, ep.out_ld = p.n_out;
     return product<T>(a, b, p.n_rows, p.n_out, p.n_in, ep, reinterpret_cast<float *>(ws + q.part), s);
 }
@@ -981,7 +1032,7 @@ template <typename T>
 cudaError_t linear_backward(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *g,
                             char *ws, void *grad_x, void *grad_w, void *grad_b, cudaStream_t s)
 {
-    const LinearPlan q = plan_linear(p, true);
+    const LinearPlan q = plan_linear(p, true, false);
     float *part = reinterpret_cast<float *>(ws + q.part);
     Matrix mx{x, p.n_rows, p.n_in, p.x_stride, false}, mw{w, p.n_out, p.n_in, p.w_stride, false};
     Matrix dz{g, p.n_rows, p.n_out, p.g_stride, false};
@@ -991,17 +1042,19 @@ cudaError_t linear_backward(const cwrnnt_linear &p, const void *x, const void *w
     // column sums: of the epilogue's pieces of 32 rows where it forms dz, else of runs of rows of the matrix
     float *sums = reinterpret_cast<float *>(ws + q.sums), *folded = sums + (p.n_rows + 31) / 32 * int64_t(p.n_out);
     int64_t runs = 0;
+    CWRNNT_TRY(readable<T>(dz, ws + q.g, s));
     if (act) {
         Epilogue ep{};
         ep.mode = kSlope, ep.act = p.activation, ep.bias = bias;
-        ep.side = g, ep.side_ld = p.g_stride;
+        ep.side = dz.p, ep.side_ld = dz.ld;
         ep.out = ws + q.dz, ep.out_ld = padded(p.n_out);
-        const Cut c = cut_product(p.n_rows, p.n_out, p.n_in);
-        if (grad_b && c.splits == 1 && !takes_few_rows(p.n_rows, p.n_out, p.n_in)) ep.sums = sums, runs = (p.n_rows + 31) / 32;
+        const bool tiles = !takes_few_rows(p.n_rows, p.n_out, p.n_in) &&
+                           cut_product(p.n_rows, p.n_out, steps_of(p.n_in)).splits == 1;
+        if (tiles && grad_b) ep.sums = sums, runs = (p.n_rows + 31) / 32;
+        ep.low = parts_of(p) == 2 ? ws + q.low : nullptr;
         CWRNNT_TRY(product<T>(mx, mw, p.n_rows, p.n_out, p.n_in, ep, part, s));
         dz.p = ws + q.dz, dz.ld = padded(p.n_out);
-    } else {
-        CWRNNT_TRY(readable<T>(dz, ws + q.g, s));
+        dz.low = ep.low;
     }
     if (grad_b) {
         const int64_t across = (p.n_out + 255) / 256;
@@ -1013,7 +1066,7 @@ cudaError_t linear_backward(const cwrnnt_linear &p, const void *x, const void *w
             if (runs > kMostRuns) runs = kMostRuns;
             const int64_t run = (p.n_rows + runs - 1) / runs;
             column_sums_kernel<T><<<dim3(unsigned(across), unsigned(runs)), 256, 0, s>>>(
-                static_cast<const T *>(dz.p), dz.ld, p.n_rows, p.n_out, run, sums);
+                static_cast<const T *>(dz.p), static_cast<const T *>(dz.low), dz.ld, p.n_rows, p.n_out, run, sums);
             CWRNNT_TRY(cudaGetLastError());
         }
         if (runs > kMostRuns) {
@@ -1045,7 +1098,10 @@ cudaError_t linear_backward(const cwrnnt_linear &p, const void *x, const void *w
 
 }  // namespace
 
-int64_t linear_workspace(const cwrnnt_linear &p, bool backward) { return plan_linear(p, backward).total; }
+int64_t linear_workspace(const cwrnnt_linear &p, bool backward, bool residual)
+{
+    return plan_linear(p, backward, residual).total;
+}
 
 cudaError_t launch_linear(const cwrnnt_linear &p, const void *x, const void *w, const void *bias, const void *residual,
                           void *workspace, void *y, cudaStream_t s)

@@ -446,7 +446,7 @@ cwrnnt_linear describe_linear(const torch::Tensor &x, const torch::Tensor &weigh
 }
 
 torch::Tensor linear_forward(const torch::Tensor &x_, const torch::Tensor &weight_, const OptTensor &bias,
-                             const OptTensor &residual, int64_t activation)
+                             const OptTensor &residual_, int64_t activation)
 {
     CHECK_CUDA(x_);
     CHECK_CUDA(weight_);
@@ -454,12 +454,14 @@ torch::Tensor linear_forward(const torch::Tensor &x_, const torch::Tensor &weigh
     const c10::cuda::CUDAGuard guard(x_.device());
     const auto x = readable(x_), weight = readable(weight_);
     const cwrnnt_linear p = describe_linear(x, weight, bias, activation);
+    OptTensor residual = residual_;
+    if (residual && residual->dim() == 2) residual = readable(*residual);
     if (residual)
         TORCH_CHECK(residual->dim() == 2 && residual->size(0) == p.n_rows && residual->size(1) == p.n_out &&
                         residual->scalar_type() == x.scalar_type() && residual->device() == x.device() &&
                         residual->is_contiguous(),
                     "residual must be [rows, n_out], contiguous, of the type and device of x");
-    const int64_t bytes = cwrnnt_linear_workspace_bytes(&p, 0);
+    const int64_t bytes = cwrnnt_linear_workspace_bytes(&p, residual ? CWRNNT_LINEAR_FORWARD_RESIDUAL : CWRNNT_LINEAR_FORWARD);
     TORCH_CHECK(bytes >= 0, "invalid linear layer");
     auto ws = torch::empty({bytes}, x.options().dtype(torch::kUInt8));
     auto y = torch::empty({x.size(0), weight.size(0)}, x.options());
@@ -483,7 +485,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(const torch::Tensor 
                     g.device() == x.device(),
                 "the upstream gradient must be [rows, n_out], of the type and device of x");
     p.g_stride = leading(g);
-    const int64_t bytes = cwrnnt_linear_workspace_bytes(&p, 1);
+    const int64_t bytes = cwrnnt_linear_workspace_bytes(&p, CWRNNT_LINEAR_BACKWARD);
     TORCH_CHECK(bytes >= 0, "invalid linear layer");
     auto ws = torch::empty({bytes}, x.options().dtype(torch::kUInt8));
     OptTensor gx, gw, gb;

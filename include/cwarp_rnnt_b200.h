@@ -418,12 +418,12 @@ CWRNNT_API int cwrnnt_distill(const cwrnnt_rows *p, int32_t tail, const void *x,
  * with float sums; x, weight, bias, residual, y and all gradients are of p->dtype, CWRNNT_F16 or CWRNNT_BF16 (other
  * types are refused: the tensor cores have no product of theirs). cwrnnt_linear_backward writes, for the upstream
  * gradient grad_y, whichever of grad_x, grad_weight and grad_bias are not NULL (the residual's is grad_y itself);
- * nothing but the inputs is kept for it, and dz = grad_y * act'(z) is rounded to the type before its products, as the
- * tensor cores take it. x, weight and grad_y may have rows further apart than their length; where such a stride is a
+ * nothing but the inputs is kept for it. x, weight and grad_y may have rows further apart than their length; where such a stride is a
  * multiple of 8 elements the matrix must start on a 16-byte boundary, other strides are copied first (into the
- * workspace). bias, residual and all outputs are contiguous. Sums are split and joined in a fixed order: results
+ * workspace). bias, residual and all outputs are contiguous; a residual of n_out a multiple of 8 starts on a 16-byte
+ * boundary. Sums are split and joined in a fixed order: results
  * repeat bit for bit. Every wait inside the kernels is bounded (two seconds); a tile whose wait runs out is NaN.
- * workspace: cwrnnt_linear_workspace_bytes(p, backward) bytes, 256-byte aligned; not shared by calls that may overlap.
+ * workspace: cwrnnt_linear_workspace_bytes(p, pass) bytes, 256-byte aligned; not shared by calls that may overlap.
  */
 #define CWRNNT_ACT_SILU 3 /* z / (1 + exp(-z)); cwrnnt_linear_* only */
 typedef struct {
@@ -435,7 +435,10 @@ typedef struct {
     int32_t dtype;      /* CWRNNT_F16 or CWRNNT_BF16                                 */
     int32_t activation; /* CWRNNT_ACT_*                                              */
 } cwrnnt_linear;
-CWRNNT_API int64_t cwrnnt_linear_workspace_bytes(const cwrnnt_linear *p, int32_t backward);
+#define CWRNNT_LINEAR_FORWARD 0
+#define CWRNNT_LINEAR_BACKWARD 1
+#define CWRNNT_LINEAR_FORWARD_RESIDUAL 2 /* a forward pass with a residual */
+CWRNNT_API int64_t cwrnnt_linear_workspace_bytes(const cwrnnt_linear *p, int32_t pass);
 CWRNNT_API int cwrnnt_linear_forward(const cwrnnt_linear *p, const void *x, const void *weight, const void *bias,
                                      const void *residual, void *workspace, int64_t workspace_bytes, void *y,
                                      cwrnnt_stream_t stream);

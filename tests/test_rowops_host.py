@@ -124,6 +124,9 @@ def test_linear_pointers_and_workspaces():
     assert f(_linear(), one, one, None, None, one, n, None, None) == 1
     assert f(_linear(), odd, one, None, None, one, n, one, None) == 1      # off a 16-byte boundary
     assert f(_linear(), one, odd, None, None, one, n, one, None) == 1
+    assert f(_linear(), one, one, None, odd, one, 1 << 40, one, None) == 1
+    assert L.cwrnnt_linear_workspace_bytes(_linear(), 3) < 0 and L.cwrnnt_linear_workspace_bytes(_linear(), -1) < 0
+    assert L.cwrnnt_linear_workspace_bytes(_linear(n_out=47), 2) >= 64 * 48 * 2  # a copy of the residual
     assert f(_linear(), one, one, None, None, None, n, one, None) == 2
     assert f(_linear(), one, one, None, None, odd, n, one, None) == 2
     assert f(_linear(), one, one, None, None, one, n - 1, one, None) == 2
