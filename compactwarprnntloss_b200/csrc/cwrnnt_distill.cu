@@ -168,11 +168,11 @@ __device__ __forceinline__ void blank_element(uint4 &v, int c)
     v = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A row's maximum and sum 2^((x - max) * kappa): of the tokens that are not listed (rest) and of all. Without a tail the
-// two are the same.
+// A row's maximum and sum 2^((x - max) * kappa): of the tokens that are not listed (rest) and of all; `listed`: the listed
+// tokens' part of all_sum. Without a tail rest and all are the same.
 template <typename A>
 struct RowSums {
-    A rest_max, rest_sum, all_max, all_sum;
+    A rest_max, rest_sum, all_max, all_sum, listed;
     __device__ __forceinline__ bool nothing() const { return all_max == A(-INFINITY) && all_sum == all_sum; }
     __device__ __forceinline__ bool no_rest() const { return rest_max == A(-INFINITY) && rest_sum == rest_sum; }
 };
@@ -183,12 +183,12 @@ template <bool TAIL, typename A>
 __device__ __forceinline__ RowSums<A> all_sums(A max, A sum, A mine, A kappa, int KP, int width)
 {
     using M = Base2<A>;
-    RowSums<A> s{max, sum, max, sum};
+    RowSums<A> s{max, sum, max, sum, A(0)};
     if (TAIL) {
         s.all_max = M::max_of(max, entry_max(mine, KP, width));
         const A base = s.all_max == A(-INFINITY) ? A(0) : s.all_max;
-        const A listed = entry_sum(A(exp2((mine - base) * kappa)), KP, width);
-        s.all_sum = listed + (max == A(-INFINITY) ? sum : sum * M::exp2_of((max - base) * kappa));
+        s.listed = entry_sum(A(exp2((mine - base) * kappa)), KP, width);
+        s.all_sum = s.listed + (max == A(-INFINITY) ? sum : sum * M::exp2_of((max - base) * kappa));
     }
     return s;
 }
@@ -226,12 +226,17 @@ __device__ __forceinline__ RowFactors<A> gradient_factors(const RowSums<A> &s, A
 }
 
 // A row's weighted divergence. Lane e of the row's `width` lanes holds entry e: its q, lq and the student's logit xc there.
+// Both parts of the sum are joined in double: where the rest is nearly all, ln p_rest is as small as the listed tokens'
+// share, and the rounding of a joined float would be all that is left of it.
 template <bool TAIL, typename A>
 __device__ __forceinline__ A divergence(const RowSums<A> &s, double q, double lq, A xc, double left, bool bad, A weight,
                                         double inv_tau, int KP, int width)
 {
     const bool nothing = s.nothing();
-    const double max = double(s.all_max), ln_s = nothing ? 0.0 : ln_of<A>(double(s.all_sum));
+    const double max = double(s.all_max);
+    double all = double(s.all_sum);
+    if (TAIL) all = double(s.listed) + double(s.rest_sum) * exp_of<A>((double(s.rest_max) - max) * inv_tau);
+    const double ln_s = nothing ? 0.0 : ln_of<A>(all);
     double each = 0.0;
     if (q > 0.0) each = q * (lq - ((double(xc) - max) * inv_tau - ln_s));
     each = entry_sum(each, KP, width);

@@ -204,6 +204,20 @@ def test_a_confident_student_keeps_the_digits_of_the_rest():
     _run(x, val, idx)
 
 
+@pytest.mark.parametrize("V,dtype", [(4096, "f16"), (40001, "f32"), (65536, "bf16")])
+def test_a_rest_that_is_nearly_all_keeps_the_digits_of_its_logarithm(V, dtype):
+    """The listed tokens hold a few V-ths of a flat student: -ln p_rest is about their share P of it, and a rest summed to
+    SUM32 moves it by P SUM32 only. The listed ln p move by SUM32 (x / tau - max / tau is taken in double), each times its
+    q. Beside these there are the double steps (an exponential and three logarithms to 2^-33 each) and one rounding."""
+    x, _, idx = _case(21, 64, V, 2, DT[dtype], spread=0.1)
+    val = torch.full((64, 2), 4.0 / V).log()
+    rows = distill_loss(x.to(DEV), val.to(DEV), idx.to(DEV), reduction="none").double().cpu()
+    want = torch.from_numpy(ro.distill(x.double().numpy(), val.double().numpy(), idx.numpy(), None, True, 1.0)[0])
+    p = torch.softmax(x.double(), 1).gather(1, idx.long())
+    bound = ro.SUM32 * (val.double().exp().sum(1) + p.sum(1)) + 2.0 ** -31 + 2.0 ** -24 * want.abs()
+    assert ((rows - want).abs() <= bound).all(), ((rows - want).abs() / bound).max()
+
+
 def test_empty_batches_and_leading_axes():
     x, val, idx = _case(8, 24, 60, 3, torch.float32)
     a = distill_loss(x.view(2, 3, 4, 60).to(DEV), val.view(2, 3, 4, 3).to(DEV), idx.view(2, 3, 4, 3).to(DEV), reduction="none")
