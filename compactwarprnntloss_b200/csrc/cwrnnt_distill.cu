@@ -12,8 +12,9 @@
 // the listed probabilities it would lose all its digits where the student is sure of a listed token, and its gradient
 // divides nothing by a small number.
 //
-// Bound: HBM, 2 * V * sizeof(element) bytes a row: rows of up to 512 vectors (8 KB) stay in registers between the sums
-// and the gradient; longer ones take a CTA each, whose second reading comes from L2.
+// Bound: HBM, 2 * V * sizeof(element) bytes a row (314340 x 1024 bf16, two entries: 0.26 ms, 5.0 TB/s; 2047 x 32003 f32,
+// 32 entries: 0.135 ms, 3.9 TB/s). Rows of up to 2048 elements (1024 doubles) stay in registers between the sums
+// and the gradient; longer ones take a warp or a CTA each, whose second reading comes from L2.
 // The summed loss is added up in a fixed order: rows in their CTA, then the CTAs' sums in a second small kernel.
 #include "cwrnnt_kernels.h"
 #include "cwrnnt_rowops.cuh"
@@ -291,7 +292,8 @@ struct RowRecord {
 // Rows of at most LPR * NV vectors and at most LPR entries. Group g of a CTA takes the rows first + g, + GPC, .. run_len
 // times. What a row needs beside its elements would cost a warp more instructions than the elements do, so the warp does
 // that for all of its rows at once, before and after they pass: an entry to a lane. The terms of a row's sum stay in
-// registers for its gradient. (314340 x 1024 bf16, two entries a row: 0.30 ms with that work done row by row.)
+// registers for its gradient. (314340 x 1024 bf16, two entries a row: 0.26 ms; 0.30 with that work done row by row. The
+// double steps of a row are a good part of a warp's 613 instructions a row: it issues in 73 of 100 cycles.)
 template <typename T, int LPR, int NV, int MODE, bool TAIL>
 __global__ void __launch_bounds__(kRowThreads)
 distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
@@ -589,8 +591,9 @@ int64_t launch_distill_t(const DistillArgs<T> &a, bool tail, cudaStream_t s)
 {
     constexpr int VE = Elt<T>::VE, NV = 32 / VE < 16 ? 32 / VE : 16;
     const int nv = ALIGNED ? a.V / VE : (a.V + 2 * VE - 2) / VE;
-    // Few lanes a row, many elements a lane: what a row costs beside its elements (about 400 instructions of a warp) is
-    // shared by the rows of a warp. 64 elements a lane is what registers hold; every entry has a lane.
+    // Few lanes a row, many elements a lane: what a row costs beside its elements is shared by the rows of a warp. 32
+    // elements a lane where several rows share a warp (64: 0.30 against 0.25 ms on 314340 x 1024 bf16, for want of warps);
+    // every entry has a lane.
     if constexpr (sizeof(T) <= 4) {
         if (nv <= 4 * NV && a.K <= 4) return launch_distill_rows<T, 4, NV, ALIGNED>(a, tail, s);
         if (nv <= 8 * NV && a.K <= 8) return launch_distill_rows<T, 8, NV, ALIGNED>(a, tail, s);

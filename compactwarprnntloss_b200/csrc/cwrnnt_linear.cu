@@ -3,16 +3,22 @@
 //     dx = dz W,   dW = dz^T x,   db = sum over rows of dz,   dr = dy.
 // Nothing but the inputs is kept for the gradients: z is multiplied out again, and the epilogue of that product writes
 // dz at once (reading dy). Storing z in float instead costs more traffic than the product takes, storing it in 16 bits
-// costs digits of act'(z).
+// costs digits of act'(z). dz goes into its two products as the sum of two 16-bit matrices, the second what the first
+// loses in its rounding: with the first alone the gradients would be off by half as much again as their own rounding.
 //
-// One kernel for the four products: tiles of 128 x 64 or 128 and 256 x 256 outputs, 64 elements of the sum a step. Operands come by tiled TMA
-// into a ring of 128-byte-swizzled stages; tcgen05.mma sums in TMEM in float. The forward product takes both operands
-// along the sum (K-major), dx takes W and dW takes both operands across it (MN-major): no operand is ever transposed in
-// memory. Warp 0 issues the loads, warp 1 the products; four or eight more warps carry the previous tile out of the other half
-// of TMEM meanwhile, through swizzled shared memory and TMA stores (residual and dy come the same way). CTAs are persistent; output columns run fastest, so that concurrent CTAs share their rows of x in L2.
-// Products with few tiles and long sums (dW) are split along the sum; the parts are float in the workspace, added in
-// a fixed order by a second kernel that carries the same epilogue.
+// One kernel for the four products: tiles of 128 x 64 or 128 outputs, or of 256 x 256 shared by two CTAs, 64 elements of
+// the sum a step. Operands come by tiled TMA into a ring of 128-byte-swizzled stages; tcgen05.mma sums in TMEM in float.
+// The forward product takes both operands along the sum (K-major), dx takes W and dW takes both operands across it
+// (MN-major): no operand is ever transposed in memory. Warp 0 issues the loads, warp 1 the products; four or eight more
+// warps carry the previous tile out of the other half of TMEM meanwhile, through swizzled shared memory and TMA stores
+// (residual and dy come the same way). CTAs are persistent; output columns run fastest, so that concurrent CTAs share
+// their rows of x in L2. Products with few tiles and long sums (dW) are split along the sum; the parts are float in the
+// workspace, added in a fixed order by a second kernel that carries the same epilogue.
 // TMA wants rows at multiples of 16 bytes: matrices of other strides are copied to such a stride first.
+//
+// Bound: the tensor cores under the power limit for large products (314340 x 1024 x 640 bf16: 0.37 ms, 1.1 PFLOP/s, as
+// fast as the library's product without an epilogue); for short sums what a tile's operands take from L2 and, with tanh
+// or silu, the epilogue's instructions (40009 x 640 x 512 f16: 36 us plain, 54 with tanh and residual).
 #include "cwrnnt_kernels.h"
 #include "cwrnnt_tc.cuh"
 
@@ -34,36 +40,72 @@ __device__ __forceinline__ float rcp(float v)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// tanh to about 2^-22 relative: 1 - 2 / (1 + e^2z), and its series where that would cancel.
-__device__ __forceinline__ float tanh_full(float z)
+// Two elements at a time: sm_100 adds and multiplies pairs of floats in one instruction, and the epilogue of a product of
+// few steps is bound by the instructions it issues (40009 x 640 x 512, an element at a time and by pairs: tanh 51 and 47 us,
+// the gradient of silu 96 and 62).
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// The clamps let a NaN through.
+__device__ __forceinline__ float at_least(float v, float low)
 {
-    const float e = ex2_approx(fabsf(z) * 2.8853900817779268f);
-    const float t = copysignf(1.0f - 2.0f * rcp(1.0f + e), z);
-    const float s = z * z;
-    const float p = z * (1.0f + s * (-0.33333333333f + s * (0.13333333333f - 0.05396825397f * s)));
-    return fabsf(z) < 0.15f ? p : t;
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(low));
+    return r;
 }
-__device__ __forceinline__ float activate(int act, float z)
+__device__ __forceinline__ float at_most(float v, float high)
 {
-    if (act == CWRNNT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-    if (act == CWRNNT_ACT_TANH) return tanh_full(z);
-    if (act == CWRNNT_ACT_SILU) return z == -INFINITY ? 0.0f : z * rcp(1.0f + ex2_approx(-1.4426950408889634f * z));
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(high));
+    return r;
+}
+template <int ACT>
+__device__ __forceinline__ float2 activate(float2 z)
+{
+    if (ACT == CWRNNT_ACT_RELU) return make_float2(at_least(z.x, 0.0f), at_least(z.y, 0.0f));
+    if (ACT == CWRNNT_ACT_TANH) {  // to about 2^-20 relative: 1 - 2 / (1 + e^2z), and its series where that would cancel
+        const float2 m = __fmul2_rn(z, both(2.8853900817779268f));
+        const float2 e = __fadd2_rn(make_float2(ex2_approx(m.x), ex2_approx(m.y)), both(1.0f));
+        const float2 t = __ffma2_rn(make_float2(rcp(e.x), rcp(e.y)), both(-2.0f), both(1.0f));
+        const float2 s = __fmul2_rn(z, z);
+        float2 p = __ffma2_rn(s, both(-0.05396825397f), both(0.13333333333f));
+        p = __ffma2_rn(s, p, both(-0.33333333333f));
+        p = __ffma2_rn(__fmul2_rn(s, p), z, z);
+        return make_float2(fabsf(z.x) < 0.25f ? p.x : t.x, fabsf(z.y) < 0.25f ? p.y : t.y);
+    }
+    if (ACT == CWRNNT_ACT_SILU) {  // below -104 the logistic function is zero in float, and so is the product
+        z = make_float2(at_least(z.x, -104.0f), at_least(z.y, -104.0f));
+        const float2 m = __fmul2_rn(z, both(-1.4426950408889634f));
+        const float2 e = __fadd2_rn(make_float2(ex2_approx(m.x), ex2_approx(m.y)), both(1.0f));
+        return __fmul2_rn(z, make_float2(rcp(e.x), rcp(e.y)));
+    }
     return z;
 }
-__device__ __forceinline__ float slope(int act, float z)
+// dy times the activation's slope.
+template <int ACT>
+__device__ __forceinline__ float2 through(float2 z, float2 dy)
 {
-    if (act == CWRNNT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    if (act == CWRNNT_ACT_TANH) {  // 4 e / (1 + e)^2, e = exp(-2 |z|): no cancellation far out
-        const float e = ex2_approx(fabsf(z) * -2.8853900817779268f), r = rcp(1.0f + e);
-        return 4.0f * e * r * r;
+    if (ACT == CWRNNT_ACT_RELU) {
+        const float2 s = make_float2(z.x > 0.0f ? 1.0f : (z.x != z.x ? z.x : 0.0f), z.y > 0.0f ? 1.0f : (z.y != z.y ? z.y : 0.0f));
+        return __fmul2_rn(dy, s);
     }
-    if (act == CWRNNT_ACT_SILU) {  // s (1 + z (1 - s)), s the logistic function
-        if (fabsf(z) == INFINITY) return z > 0.0f ? 1.0f : 0.0f;
-        const float e = ex2_approx(-1.4426950408889634f * fabsf(z)), r = rcp(1.0f + e);
-        const float big = r, small = e * r;  // the larger and the smaller of s and 1 - s
-        return z >= 0.0f ? big * (1.0f + z * small) : small * (1.0f + z * big);
+    if (ACT == CWRNNT_ACT_TANH) {  // 4 e / (1 + e)^2, e = exp(-2 |z|): no cancellation far out
+        const float2 m = __fmul2_rn(z, both(2.8853900817779268f));
+        const float2 e = make_float2(ex2_approx(-fabsf(m.x)), ex2_approx(-fabsf(m.y)));
+        const float2 d = __fadd2_rn(e, both(1.0f)), r = make_float2(rcp(d.x), rcp(d.y));
+        return __fmul2_rn(dy, __fmul2_rn(__fmul2_rn(e, r), __fmul2_rn(r, both(4.0f))));
     }
-    return 1.0f;
+    if (ACT == CWRNNT_ACT_SILU) {  // s (1 + z (1 - s)), s the logistic function; 0 and 1 beyond -104 and 104
+        z = make_float2(at_most(at_least(z.x, -104.0f), 104.0f), at_most(at_least(z.y, -104.0f), 104.0f));
+        const float2 m = __fmul2_rn(z, both(-1.4426950408889634f));
+        const float2 d = __fadd2_rn(make_float2(ex2_approx(m.x), ex2_approx(m.y)), both(1.0f));
+        const float2 s = make_float2(rcp(d.x), rcp(d.y)), other = __ffma2_rn(s, both(-1.0f), both(1.0f));
+        return __fmul2_rn(dy, __fmul2_rn(s, __ffma2_rn(z, other, both(1.0f))));
+    }
+    return dy;
+}
+template <int ACT>
+__device__ __forceinline__ float2 finish_one(bool slope, float2 z, float2 side)
+{
+    return slope ? through<ACT>(z, side) : __fadd2_rn(activate<ACT>(z), side);
 }
 
 // ---------------------------------------------------------------------------------------------------------- epilogue
@@ -85,16 +127,23 @@ struct Epilogue {
 // gradient times the activation's slope.
 constexpr int kSlopeOf = 8;
 template <int KIND, bool SIDE>
-__device__ __forceinline__ float finish(float v, float side)
+__device__ __forceinline__ float2 finish(float2 v, float2 side)
 {
-    if (KIND >= kSlopeOf) return side * slope(KIND - kSlopeOf, v);
-    v = activate(KIND, v);
-    return SIDE ? v + side : v;
+    if constexpr (KIND >= kSlopeOf) {
+        return through<KIND - kSlopeOf>(v, side);
+    } else {
+        v = activate<KIND>(v);
+        return SIDE ? __fadd2_rn(v, side) : v;
+    }
 }
 __device__ __forceinline__ float finish_as(const Epilogue &ep, float v, float side)
 {
-    if (ep.mode == kSlope) return side * slope(ep.act, v);
-    return activate(ep.act, v) + side;
+    const bool slope = ep.mode == kSlope;
+    const float2 z = make_float2(v, 0.0f), s = make_float2(side, 0.0f);
+    if (ep.act == CWRNNT_ACT_RELU) return finish_one<CWRNNT_ACT_RELU>(slope, z, s).x;
+    if (ep.act == CWRNNT_ACT_TANH) return finish_one<CWRNNT_ACT_TANH>(slope, z, s).x;
+    if (ep.act == CWRNNT_ACT_SILU) return finish_one<CWRNNT_ACT_SILU>(slope, z, s).x;
+    return finish_one<CWRNNT_ACT_NONE>(slope, z, s).x;
 }
 
 // What v loses when it is rounded to T, rounded to T.
@@ -103,6 +152,19 @@ __device__ __forceinline__ T low_part(float v)
 {
     const float high = Elt<T>::to_acc(Elt<T>::from_acc(v));
     return Elt<T>::from_acc(fabsf(high) < INFINITY ? v - high : 0.0f);
+}
+
+// All bits of the halves of a word that are finite.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_mask(uint32_t w)
+{
+    if constexpr (Elt<T>::kBf16) {
+        const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162 *>(&w);
+        return __hlt2_mask(__habs2(h), __nv_bfloat162(__ushort_as_bfloat16(0x7f80), __ushort_as_bfloat16(0x7f80)));
+    } else {
+        const __half2 h = *reinterpret_cast<const __half2 *>(&w);
+        return __hlt2_mask(__habs2(h), __half2(__ushort_as_half(0x7c00), __ushort_as_half(0x7c00)));
+    }
 }
 
 // Columns [col, col + 8) of one row straight from and to global memory, `n` of them inside the matrix.
@@ -277,19 +339,25 @@ struct Carrier {
             float v[8], s[8] = {};
             const float4 b0 = *reinterpret_cast<const float4 *>(bias + g * 8);
             const float4 b1 = *reinterpret_cast<const float4 *>(bias + g * 8 + 4);
-            const float b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+            const float2 b[4] = {{b0.x, b0.y}, {b0.z, b0.w}, {b1.x, b1.y}, {b1.z, b1.w}};
             if (SIDE) E::unpack(side[g], s);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = finish<KIND, SIDE>(__uint_as_float(r[g / 4][g % 4 * 8 + i]) + b[i], s[i]);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t *z = &r[g / 4][g % 4 * 8 + 2 * i];
+                const float2 sum = __fadd2_rn(make_float2(__uint_as_float(z[0]), __uint_as_float(z[1])), b[i]);
+                const float2 f = finish<KIND, SIDE>(sum, make_float2(s[2 * i], s[2 * i + 1]));
+                v[2 * i] = f.x, v[2 * i + 1] = f.y;
+            }
             uint4 w = E::pack(v);
             if (!ok) w = make_uint4(~0u, ~0u, ~0u, ~0u);  // a wait that ran out leaves NaN
             *piece_group(out_piece, lane, g) = w;
             if constexpr (KIND == kSlopeOf + CWRNNT_ACT_TANH || KIND == kSlopeOf + CWRNNT_ACT_SILU) {
                 E::unpack(w, s);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = fabsf(s[i]) < INFINITY ? v[i] - s[i] : 0.0f;
-                *piece_group(low_piece, lane, g) = E::pack(v);
+                for (int i = 0; i < 8; ++i) v[i] -= s[i];
+                const uint4 low = E::pack(v);
+                *piece_group(low_piece, lane, g) = make_uint4(low.x & finite_mask<T>(w.x), low.y & finite_mask<T>(w.y),
+                                                              low.z & finite_mask<T>(w.z), low.w & finite_mask<T>(w.w));
             }
         }
     }
@@ -687,7 +755,8 @@ __global__ void __launch_bounds__(256) restride_kernel(const T *__restrict__ src
     }
 }
 
-// Column sums (of a matrix, or of one in two parts): each CTA adds up a run of rows of 256 columns in float; the runs' sums are added in order afterwards.
+// Column sums (of a matrix, or of one in two parts): each CTA adds up a run of rows of 256 columns in float; the runs' sums
+// are added in order afterwards.
 constexpr int kSumRows = 8;
 template <typename T>
 __global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ high,
@@ -792,7 +861,7 @@ bool make_map(CUtensorMap *map, const void *p, int64_t rows, int64_t cols, int64
 }
 
 // Products of a few rows need no tiles (and no copies for TMA), as long as re-reading the rows of x for every column does
-// not take longer than a tile's set-up: 8 rows, us: 1024 x 640 5.0 (tiles 8.4), 1024 x 2048 7.7 (9.8), 4096 x 4096 28 (24).
+// not take longer than a tile's set-up: 8 rows, us: 1024 x 640 5.0 (tiles 8.4), 1024 x 2048 7.7 (9.8), 4096 x 4096 28 (14).
 bool takes_few_rows(int64_t M, int64_t N, int64_t len) { return M <= 16 && N * len <= (int64_t(1) << 22); }
 
 int steps_of(int64_t len) { return int((len + kBK - 1) / kBK); }

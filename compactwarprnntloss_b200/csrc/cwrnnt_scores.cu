@@ -10,7 +10,10 @@
 //
 // Bound: HBM. Forward reads V * sizeof(element) per row, backward reads and writes that much. Rows of up to 256 vectors
 // (4 KB) stay in the registers of the lanes that share them, longer ones run through a warp or a CTA each with their
-// statistics alongside; the selection of the largest entries reads those again, from L1 or L2.
+// statistics alongside; the selection of the largest entries reads those again, from L1 or L2. Without a selection the
+// traffic is the bound (314340 x 1024 f32, two targets and the entropy: 0.22 ms, 6.0 TB/s; its gradient 0.44 ms, 5.8
+// TB/s), with one and with short rows the instructions (80003 x 4096 bf16, sixteen largest: 0.19 ms, 3.4 TB/s;
+// 2051 x 50257 f16, twenty: 0.07 ms, 3.0 TB/s; 600011 x 128 f16, four: 0.11 ms, 1.4 TB/s).
 //
 // Selection: of the lanes' own maxima, the largest value that at least k of them reach is a lower bound of the row's
 // k-th largest entry. The entries at or above it - about as many as k - are collected in shared memory and ranked by
