@@ -567,6 +567,8 @@ std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> token_scores_ad(const tor
     return {lp, ent, top, index};
 }
 
+bool being_captured() { return at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None; }
+
 class DistillFn : public torch::autograd::Function<DistillFn> {
 public:
     static torch::Tensor forward(AutogradContext *ctx, const torch::Tensor &x, const torch::Tensor &teacher,
@@ -580,6 +582,7 @@ public:
         ctx->saved_data["temperature"] = temperature;
         ctx->saved_data["scale"] = scale;
         if (grad) ctx->saved_data["grad"] = *grad;
+        ctx->saved_data["captured"] = being_captured();
         return reduced ? *loss : *rows;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
@@ -587,9 +590,10 @@ public:
         variable_list out(9);
         const auto g = grads[0].detach();
         const auto eager = ctx->saved_data.find("grad");
-        if (eager != ctx->saved_data.end()) {
+        if (eager != ctx->saved_data.end() && ctx->saved_data["captured"].toBool() == being_captured()) {
             // computed during forward for an upstream gradient of 1; handed over once (a second backward over a
-            // retained graph recomputes it below)
+            // retained graph recomputes it below, and so does one that is captured without its forward: replayed, it
+            // would scale the one gradient again and again)
             out[0] = eager->second.toTensor();
             ctx->saved_data.erase(eager);
             if (out[0].numel()) rnnt_scale_grad(out[0], g);

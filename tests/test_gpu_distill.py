@@ -250,6 +250,29 @@ def test_captured_and_replayed_on_new_contents():
         assert abs(float(loss) - want.mean()) <= 2 * ro.SUM32 * lmag.mean() + 2.0 ** -24 * abs(want.mean())
 
 
+def test_backward_captured_without_its_forward():
+    """Every replay gives the gradient for the upstream gradient of that moment, not the last one's multiple."""
+    x, val, idx = (t.to(DEV) for t in _case(22, 40, 300, 3, torch.float32))
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        leaf = x.clone().requires_grad_(True)
+        loss = distill_loss(leaf, val, idx, reduction="sum")
+        up = torch.full((), 2.0, device=DEV)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        g, = torch.autograd.grad([loss], [leaf], [up], retain_graph=True)
+    other = x.clone().requires_grad_(True)
+    want, = torch.autograd.grad(distill_loss(other, val, idx, reduction="sum"), [other])
+    for factor in (2.0, 2.0, -0.5):
+        up.fill_(factor)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(g, factor * want)
+
+
 def test_teacher_entries_from_token_scores():
     """The two operators together: the teacher's best tokens from token_scores are what distill_loss takes."""
     x, _, _ = _case(12, 33, 500, 1, torch.bfloat16)
