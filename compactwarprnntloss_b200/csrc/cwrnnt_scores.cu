@@ -13,7 +13,7 @@
 // statistics alongside; the selection of the largest entries reads those again, from L1 or L2. Without a selection the
 // traffic is the bound (314340 x 1024 f32, two targets and the entropy: 0.22 ms, 6.0 TB/s; its gradient 0.44 ms, 5.8
 // TB/s), with one and with short rows the instructions (80003 x 4096 bf16, sixteen largest: 0.19 ms, 3.4 TB/s;
-// 2051 x 50257 f16, twenty: 0.07 ms, 3.0 TB/s; 600011 x 128 f16, four: 0.11 ms, 1.4 TB/s).
+// 2051 x 50257 f16, twenty: 0.07 ms, 3.0 TB/s; 600011 x 128 f16, four: 0.09 ms, 2.0 TB/s).
 //
 // Selection: of the lanes' own maxima, the largest value that at least k of them reach is a lower bound of the row's
 // k-th largest entry. The entries at or above it - about as many as k - are collected in shared memory and ranked by
@@ -85,7 +85,14 @@ struct Candidate<__half> : ShortCandidate<__half> {};
 template <>
 struct Candidate<__nv_bfloat16> : ShortCandidate<__nv_bfloat16> {};
 
-__host__ __device__ constexpr int candidates_of(int lpr) { return 4 * lpr; }
+// (A row of fewer vectors than k has no bar, all of its entries are candidates: up to a vector for each of the lanes, which
+// are at least k.)
+template <typename T>
+__host__ __device__ constexpr int candidates_of(int lpr)
+{
+    const int most = lpr * (Elt<T>::VE > 4 ? Elt<T>::VE : 4);
+    return most > 32 ? most : 32;
+}
 
 // A lower bound of a row's k-th largest entry that about k entries reach: of the maxima of its lanes (of their two halves,
 // where k is more than half the lanes), the smallest that fewer than k exceed. All lanes of a warp call this together.
@@ -154,7 +161,7 @@ scores_rows_kernel(const __grid_constant__ ScoresArgs<T> a, int run_len)
     using Cand = Candidate<T>;
     using Word = typename Cand::Word;
     constexpr int GPC = kRowThreads / LPR;
-    constexpr int kCap = candidates_of(LPR);
+    constexpr int kCap = candidates_of<T>(LPR);
     constexpr unsigned kAll = 0xffffffffu;
     extern __shared__ __align__(16) unsigned char scratch[];  // kCap candidates per group, when top_k > 0
     const int gl = threadIdx.x % LPR, group = threadIdx.x / LPR, lane = threadIdx.x & 31;
@@ -507,7 +514,7 @@ cudaError_t launch_scores_rows(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
     constexpr int GPC = kRowThreads / LPR;
     const int run_len = a.n_rows > int64_t(GPC) * kNumSMs * 32 ? 4 : 1;
     const int64_t grid = (a.n_rows + int64_t(GPC) * run_len - 1) / (int64_t(GPC) * run_len);
-    const size_t smem = a.top_k > 0 ? GPC * candidates_of(LPR) * sizeof(typename Candidate<T>::Word) : 0;
+    const size_t smem = a.top_k > 0 ? GPC * candidates_of<T>(LPR) * sizeof(typename Candidate<T>::Word) : 0;
     auto go = [&](auto kernel) {
         kernel<<<unsigned(grid), kRowThreads, smem, s>>>(a, run_len);
         return cudaGetLastError();
@@ -539,8 +546,10 @@ template <typename T, bool ALIGNED>
 cudaError_t launch_scores_t(const ScoresArgs<T> &a, bool ent, cudaStream_t s)
 {
     const int nv = vectors_of<T>(a.V, ALIGNED);
-    // the bar of the selection is taken among the lanes' maxima: at least twice as many lanes as entries, up to a warp
-    const int lanes = 2 * a.top_k;
+    // The bar of the selection is taken among the maxima of the lanes' halves: at least as many lanes as entries, up to a
+    // warp, and no more than that, as what a row costs beside its elements is shared by the rows of a warp (600011 x 128
+    // f16, four best: 112 us with 8 lanes a row, 93 with 4).
+    const int lanes = a.top_k;
     if constexpr (sizeof(T) <= 4) {
         if (nv <= 16 && lanes <= 4) return launch_scores_rows<T, 4, 4, ALIGNED>(a, ent, s);
         if (nv <= 16 && lanes <= 8) return launch_scores_rows<T, 8, 2, ALIGNED>(a, ent, s);

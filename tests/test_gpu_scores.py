@@ -97,6 +97,18 @@ def test_every_list_length(k, V, dtype):
     _run(_logits(k, 3, V, DT[dtype]), _targets(k, 3, V, 32), k, True, tau=1.7)
 
 
+@pytest.mark.parametrize("k", [2, 4, 8, 16, 32])
+@pytest.mark.parametrize("dtype", ["f16", "f32", "f64"])
+def test_rows_of_about_as_many_vectors_as_entries_wanted(k, dtype):
+    """Fewer vectors than entries: every entry is a candidate, and the largest may all lie in one vector."""
+    per = 16 // torch.empty(0, dtype=DT[dtype]).element_size()
+    for V in {max(k, (k + d) * per + e) for d in (-1, 0, 1) for e in (-1, 0, 1)}:
+        x = _logits(V, 11, V, DT[dtype])
+        x[1] = x[1].sort(descending=True)[0]
+        x[2] = x[2].sort()[0]
+        _run(x, None, k, True)
+
+
 @pytest.mark.parametrize("V,dtype", [(40, "f16"), (128, "bf16"), (1024, "f32"), (1023, "bf16"), (4096, "f16"),
                                      (6000, "f32"), (20011, "bf16")])
 def test_equal_entries_go_to_the_lowest_index(V, dtype):
