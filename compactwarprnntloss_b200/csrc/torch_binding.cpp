@@ -582,6 +582,7 @@ public:
         ctx->saved_data["temperature"] = temperature;
         ctx->saved_data["scale"] = scale;
         if (grad) ctx->saved_data["grad"] = *grad;
+        const c10::cuda::CUDAGuard guard(x.device());
         ctx->saved_data["captured"] = being_captured();
         return reduced ? *loss : *rows;
     }
