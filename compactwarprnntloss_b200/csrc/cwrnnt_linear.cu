@@ -16,8 +16,8 @@
 // workspace, added in a fixed order by a second kernel that carries the same epilogue.
 // TMA wants rows at multiples of 16 bytes: matrices of other strides are copied to such a stride first.
 //
-// Bound: the tensor cores under the power limit for large products (314340 x 1024 x 640 bf16: 0.37 ms, 1.1 PFLOP/s, as
-// fast as the library's product without an epilogue); for short sums what a tile's operands take from L2 and, with tanh
+// Bound: the tensor cores under the power limit for large products (314340 x 1024 x 640 bf16: 0.37 ms, 1.1 PFLOP/s,
+// within a tenth of the library's bare product); for short sums what a tile's operands take from L2 and, with tanh
 // or silu, the epilogue's instructions (40009 x 640 x 512 f16: 36 us plain, 54 with tanh and residual).
 #include "cwrnnt_kernels.h"
 #include "cwrnnt_tc.cuh"

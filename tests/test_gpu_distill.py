@@ -273,6 +273,30 @@ def test_backward_captured_without_its_forward():
         assert torch.equal(g, factor * want)
 
 
+@pytest.mark.parametrize("V,dtype", [(1000, "bf16"), (9000, "f32")])
+def test_two_streams_at_once(V, dtype):
+    """Teacher's pass, loss and gradient on two streams that overlap: each the bits of a call on its own."""
+    def step(x, teacher):
+        t = token_scores(teacher, top_k=8)
+        leaf = x.clone().requires_grad_(True)
+        loss = distill_loss(leaf, t.top_log_probs, t.top_indices)
+        g, = torch.autograd.grad(loss, [leaf])
+        return t.top_log_probs, t.top_indices, loss.detach(), g
+
+    data = [[_case(seed + k, 700, V, 1, DT[dtype])[0].to(DEV) for k in (0, 1)] for seed in (30, 40)]
+    want = [step(*d) for d in data]
+    streams = [torch.cuda.Stream(DEV) for _ in data]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, d in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(step(*d))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
 def test_teacher_entries_from_token_scores():
     """The two operators together: the teacher's best tokens from token_scores are what distill_loss takes."""
     x, _, _ = _case(12, 33, 500, 1, torch.bfloat16)
