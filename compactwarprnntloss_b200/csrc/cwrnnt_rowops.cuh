@@ -149,7 +149,9 @@ struct RowVectors {
 // ---------------------------------------------------------------------------------------------- softmax of a row
 // With temperature tau and kappa = log2(e)/tau, a term of the row's softmax is 2^(x*kappa - shift): one FFMA and one
 // ex2 in float (relative error near 2^-22). The shift is the row's (or thread's) maximum in these units, rounded to
-// float once; where the sum's logarithm is taken, that rounding is undone. Double takes exp2 and log2 of the library.
+// float once; where the sum's logarithm is taken, that rounding is undone. Beyond 2^24 (2^53 in double) the rounding moves
+// the shift by whole units: a row masked with -1e10 would be off by 2^440 before it is undone. There a term is formed from
+// the difference, 2^((x - max) * kappa), which has no shift to round. Double takes exp2 and log2 of the library.
 template <typename A>
 struct Base2;
 template <>
@@ -161,8 +163,8 @@ struct Base2<float> {
     static __device__ __forceinline__ float ratio(float a, float b) { return __fdividef(a, b); }  // b in [2^-126, 2^126]
     // below this exponent a term is zero; it keeps 0 * (-inf) out of sum p log p
     static constexpr float kFloor = -1000.0f;
-    // largest shift that x*kappa - shift is formed with; beyond it (rows of the type's lowest value) x*kappa overflows
-    static constexpr float kMostShift = 1e38f;
+    // largest shift that x*kappa - shift is formed with: its rounding is below one there, a factor of two at most
+    static constexpr float kMostShift = 16777216.0f;
 };
 template <>
 struct Base2<double> {
@@ -172,7 +174,7 @@ struct Base2<double> {
     static __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
     static __device__ __forceinline__ double ratio(double a, double b) { return a / b; }
     static constexpr double kFloor = -5000.0;
-    static constexpr double kMostShift = 1e307;
+    static constexpr double kMostShift = 9007199254740992.0;
 };
 
 constexpr double kLn2 = 0.6931471805599453;
@@ -198,8 +200,10 @@ struct RowStats {
     __device__ __forceinline__ void raise(A new_max, A kappa)
     {
         using M = Base2<A>;
-        const A to = shift_of(new_max, kappa);
-        const A by = extreme(to) ? (max - new_max) * kappa : shift_of(max, kappa) - to;  // <= 0, or NaN
+        const A from = shift_of(max, kappa), to = shift_of(new_max, kappa);
+        A by = from - to;  // <= 0, or NaN
+        // sums formed from differences know no shift: theirs is the maximum itself
+        if (extreme(from) || extreme(to)) by = (max - new_max) * kappa - excess_of(max, kappa) + excess_of(new_max, kappa);
         // nothing summed yet: the sums stay zero whatever the difference is
         const A f = s == A(0) ? A(1) : M::exp2_of(by);
         if (ENT && s != A(0)) t = f == A(0) ? A(0) : (t + s * by) * f;
@@ -219,12 +223,13 @@ struct RowStats {
     // no finite entry (and no NaN either)
     __device__ __forceinline__ bool nothing() const { return max == A(-INFINITY) && s == s; }
     // log2 of the factor by which the rounding of the shift has made the sums too large
-    __device__ __forceinline__ A excess(A kappa) const
+    static __device__ __forceinline__ A excess_of(A max, A kappa)
     {
         const A shift = shift_of(max, kappa);
         if (extreme(shift) || max == A(-INFINITY)) return A(0);
         return Base2<A>::fma_of(max, kappa, -shift);
     }
+    __device__ __forceinline__ A excess(A kappa) const { return excess_of(max, kappa); }
     // sum 2^((x - max) * kappa)
     __device__ __forceinline__ A sum(A kappa) const { return s * Base2<A>::exp2_of(-excess(kappa)); }
 };
@@ -288,7 +293,7 @@ __device__ __forceinline__ RowStats<A> join_warps(const RowStats<A> *parts, A ka
 }
 
 // How a row's (or a thread's) terms are formed at a fixed maximum: as x*kappa - shift, or from the difference to the
-// maximum where that product overflows (rows of the type's lowest value). `floored`: a floor under x is far below any term
+// maximum where the shift's rounding would count (rows of a mask's value, up to the type's lowest). `floored`: a floor under x is far below any term
 // that counts, so it may keep 0 * (-inf) out of sum p log p.
 template <typename T>
 struct TermsAt {
