@@ -98,7 +98,7 @@ template <typename A>
 struct Entries {
     int c;       // token, -1: none
     bool first;  // no earlier entry names the same token
-    bool bad;    // some token of the row lies outside it
+    bool bad;    // some token of the row lies outside it, or the teacher gives no probability (NaN) to one
     double q, lq;  // teacher's probability and its logarithm
     A sum_q;       // over the row
     double left;   // one minus that, at least 0
@@ -112,8 +112,6 @@ __device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, in
     constexpr unsigned kAll = 0xffffffffu;
     using M = Base2<A>;
     Entries<A> en;
-    const unsigned outside = __ballot_sync(kAll, c >= V) >> ((threadIdx.x & 31) / width * width);
-    en.bad = (outside & (width == 32 ? kAll : (1u << width) - 1u)) != 0;
     en.c = c < 0 || c >= V ? -1 : c;
     if (en.c < 0) a = A(-INFINITY);
     if (TAIL) {
@@ -134,6 +132,8 @@ __device__ __forceinline__ Entries<A> weigh_entries(int c, A a, int V, int K, in
     }
     const int lane = threadIdx.x & 31;
     const unsigned row = (width == 32 ? kAll : (1u << width) - 1u) << (lane / width * width);
+    // (a NaN would go unseen otherwise: it compares false with everything, and fmax drops it)
+    en.bad = (__ballot_sync(kAll, c >= V || a != a || (!TAIL && a == A(INFINITY))) & row) != 0;
     const unsigned same = __match_any_sync(kAll, en.c) & row;  // the row's entries with this token
     en.first = en.c >= 0 && __ffs(same) - 1 == lane;
     en.dup_q = A(en.q);

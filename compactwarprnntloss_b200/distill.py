@@ -24,7 +24,8 @@ def distill_loss(x: torch.Tensor, teacher: torch.Tensor, indices: torch.Tensor, 
 
     teacher, indices   x.shape[:-1] + (K,), 1 <= K <= 32: the teacher's values (float32, float64 for float64 logits)
                        and their tokens (int32). A negative index is an unused slot; a token named twice counts twice;
-                       an index of V or more makes the row's loss and gradient NaN.
+                       an index of V or more makes the row's loss and gradient NaN, and so does a NaN at a used slot
+                       (without a tail, where the values are renormalised, a +inf as well).
     tail               True: the values are log-probabilities, taken at `temperature`; every token that is not listed
                        belongs to one more class. D = sum q (ln q - ln p) over the listed tokens and that class.
                        False: the values are logits or log-probabilities, q = softmax(values / temperature) over the

@@ -355,7 +355,8 @@ CWRNNT_API int cwrnnt_joint_backward(const cwrnnt_problem *p, int32_t activation
  * a token twice, or none (a negative index). A row without a finite logit (a mask that leaves nothing) has
  * log-probabilities of -inf, entropy 0, a divergence of 0 and a zero gradient; a row with a NaN or +inf logit gives
  * NaN (its best entries are still found: NaN first, then by value). An index of V or more is never followed: its
- * log-probability, or the divergence and gradient of its row, is NaN.
+ * log-probability, or the divergence and gradient of its row, is NaN. So are they where the teacher's value at a used
+ * entry is NaN, or +inf in a list that is renormalised.
  */
 #define CWRNNT_MAX_LIST 32 /* most targets, top entries or teacher entries of a row */
 typedef struct {
