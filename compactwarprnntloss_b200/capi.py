@@ -18,6 +18,7 @@ ST_BAD_LENGTH, ST_ROW_MISMATCH, ST_BAD_LABEL, ST_FWD_BWD_GAP = 0x01, 0x02, 0x04,
 MAX_COLUMNS = 4096
 STATIC_MAX_ROWS, STATIC_MAX_SEQUENCES = 131072, 1024
 MAX_LIST = 32
+UPSTREAM_UNLESS_ONE = -1
 ERR_CAPACITY = 5
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float64: F64}

@@ -661,7 +661,12 @@ int cwrnnt_distill(const cwrnnt_rows *p, int32_t tail, const void *x, const void
     int st = check_rows(p);
     if (st) return st;
     if (p->n_list < 1 || p->top_k != 0 || (tail != 0 && tail != 1)) return CWRNNT_ERR_ARGUMENT;
-    if (upstream_stride != 0 && upstream_stride != 1) return CWRNNT_ERR_ARGUMENT;
+    if (upstream_stride == CWRNNT_UPSTREAM_UNLESS_ONE) {
+        // a gradient that is there already, made anew: there is nothing else to write
+        if (row_loss || loss || (p->n_rows > 0 && (!upstream || !grad_x))) return CWRNNT_ERR_ARGUMENT;
+    } else if (upstream_stride != 0 && upstream_stride != 1) {
+        return CWRNNT_ERR_ARGUMENT;
+    }
     if (grad_x && p->grad_stride < p->V) return CWRNNT_ERR_ARGUMENT;
     if (p->n_rows > 0 && (!x || !teacher || !indices)) return CWRNNT_ERR_ARGUMENT;
     if (loss && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8 != 0 ||

@@ -36,6 +36,7 @@ struct DistillArgs {
     double scale;    // of the summed loss and of the gradient
     const C *teacher, *weight, *upstream;
     int upstream_stride;
+    bool unless_one;  // gx holds the gradient for an upstream gradient of 1 already: nothing to do if it is that
     const int32_t *index;
     C *row_loss;
     double *partial;  // one sum per CTA
@@ -310,6 +311,7 @@ distill_rows_kernel(const __grid_constant__ DistillArgs<T> a, int run_len)
     EntryRecord<A> *const ents =
         reinterpret_cast<EntryRecord<A> *>(reinterpret_cast<RowRecord<A> *>(scratch) + kRowThreads / 32 * rows) +
         warp * rows * KP;
+    if (a.unless_one && __ldg(a.upstream) == typename E::cost(1)) return;
     const int64_t first = int64_t(blockIdx.x) * GPC * run_len + warp * kRows;
     auto row_of = [&](int b) { return first + int64_t(b / kRows) * GPC + b % kRows; };
 
@@ -445,6 +447,7 @@ distill_stream_kernel(const __grid_constant__ DistillArgs<T> a)
     const int me = LANES == 32 ? lane : threadIdx.x;
     const int64_t r = LANES == 32 ? int64_t(blockIdx.x) * kWarps + warp : int64_t(blockIdx.x);
     const bool active = r < a.n_rows;
+    if (a.unless_one && __ldg(a.upstream) == typename E::cost(1)) return;
     A loss = A(0);
     if (active) {
         const A weight = a.weight ? A(__ldg(a.weight + r)) : A(1);
@@ -626,7 +629,8 @@ cudaError_t launch_distill_of(const cwrnnt_rows &p, bool tail, const void *x, co
     a.kappa = typename Elt<T>::acc(kLog2e / p.temperature);
     a.scale = scale;
     a.teacher = static_cast<const C *>(teacher), a.weight = static_cast<const C *>(weight);
-    a.upstream = static_cast<const C *>(upstream), a.upstream_stride = upstream_stride;
+    a.upstream = static_cast<const C *>(upstream), a.upstream_stride = upstream_stride == 1 ? 1 : 0;
+    a.unless_one = upstream_stride == CWRNNT_UPSTREAM_UNLESS_ONE;
     a.index = index;
     a.row_loss = static_cast<C *>(row_loss);
     a.partial = loss ? partial : nullptr;

@@ -367,11 +367,13 @@ torch::Tensor token_scores_backward(const torch::Tensor &x, const OptTensor &tar
     return gx;
 }
 
-// Returns (row_loss [R]?, loss []?, grad_x [R,V]?).
+// Returns (row_loss [R]?, loss []?, grad_x [R,V]?). `made`: the gradient for an upstream gradient of 1, to be made anew in
+// its place if that is something else.
 std::tuple<OptTensor, OptTensor, OptTensor> distill(const torch::Tensor &x, const torch::Tensor &teacher,
                                                     const torch::Tensor &indices, const OptTensor &weight,
                                                     const OptTensor &upstream, bool tail, double temperature,
-                                                    double scale, bool want_rows, bool want_loss, bool want_grad)
+                                                    double scale, bool want_rows, bool want_loss, bool want_grad,
+                                                    const OptTensor &made = {})
 {
     TORCH_CHECK(teacher.dim() == 2 && indices.dim() == 2 && teacher.size(1) == indices.size(1) && indices.size(1) > 0,
                 "teacher values and indices must both be [rows, K], K >= 1");
@@ -392,10 +394,10 @@ std::tuple<OptTensor, OptTensor, OptTensor> distill(const torch::Tensor &x, cons
         loss = torch::empty({}, costs);
         ws = torch::empty({cwrnnt_distill_workspace_bytes(&p)}, x.options().dtype(torch::kUInt8));
     }
-    if (want_grad) gx = torch::empty({x.size(0), x.size(1)}, x.options());
+    if (want_grad) gx = made ? *made : torch::empty({x.size(0), x.size(1)}, x.options());
+    const int32_t stride = made ? CWRNNT_UPSTREAM_UNLESS_ONE : upstream && upstream->numel() > 1 ? 1 : 0;
     check_status(cwrnnt_distill(&p, tail ? 1 : 0, x.data_ptr(), teacher.data_ptr(),
-                                static_cast<const int32_t *>(indices.data_ptr()), ptr(weight), ptr(upstream),
-                                upstream && upstream->numel() > 1 ? 1 : 0, scale, ptr(ws), ws ? ws->numel() : 0,
+                                static_cast<const int32_t *>(indices.data_ptr()), ptr(weight), ptr(upstream), stride, scale, ptr(ws), ws ? ws->numel() : 0,
                                 ptr(rows), ptr(loss), ptr(gx), current_stream()),
                  "cwrnnt_distill");
     return {rows, loss, gx};
@@ -590,6 +592,12 @@ public:
     {
         variable_list out(9);
         const auto g = grads[0].detach();
+        auto make = [&](const OptTensor &made) {
+            const auto saved = ctx->get_saved_variables();
+            return *std::get<2>(distill(saved[0].detach(), saved[1], saved[2], some(saved[3]), g.contiguous(),
+                                        ctx->saved_data["tail"].toBool(), ctx->saved_data["temperature"].toDouble(),
+                                        ctx->saved_data["scale"].toDouble(), false, false, true, made));
+        };
         const auto eager = ctx->saved_data.find("grad");
         if (eager != ctx->saved_data.end() && ctx->saved_data["captured"].toBool() == being_captured()) {
             // computed during forward for an upstream gradient of 1; handed over once (a second backward over a
@@ -597,12 +605,15 @@ public:
             // would scale the one gradient again and again)
             out[0] = eager->second.toTensor();
             ctx->saved_data.erase(eager);
-            if (out[0].numel()) rnnt_scale_grad(out[0], g);
+            // Of a mean over many rows float16 keeps few digits of a gradient and none below 2^-25 (a token of probability
+            // 1e-2 of 300 000 rows); a loss scale comes too late for them. So that gradient is made anew unless the
+            // factor is 1. The other types have the range, and their one more rounding is half a step.
+            if (out[0].scalar_type() == torch::ScalarType::Half)
+                out[0] = make(out[0]);
+            else if (out[0].numel())
+                rnnt_scale_grad(out[0], g);
         } else {
-            const auto saved = ctx->get_saved_variables();
-            out[0] = *std::get<2>(distill(saved[0].detach(), saved[1], saved[2], some(saved[3]), g.contiguous(),
-                                          ctx->saved_data["tail"].toBool(), ctx->saved_data["temperature"].toDouble(),
-                                          ctx->saved_data["scale"].toDouble(), false, false, true));
+            out[0] = make({});
         }
         return once_differentiable(std::move(out), "distill_loss");
     }

@@ -34,8 +34,10 @@ def distill_loss(x: torch.Tensor, teacher: torch.Tensor, indices: torch.Tensor, 
     reduction          'mean': sum of the weighted rows / mean_denominator (0: the number of rows); 'sum'; 'none' or
                        None: one value a row. No factor temperature^2 is applied.
     eager_grad         True: with 'mean' and 'sum' the gradient is computed inside the forward call, in the same pass;
-                       `backward` only scales it (nothing is touched when the upstream gradient is 1). False: it is
-                       computed by `backward`, and not at all if that never comes.
+                       `backward` only scales it (nothing is touched when the upstream gradient is 1). float16
+                       gradients are not scaled, which would lose what lies below their range, but computed once more
+                       where the upstream gradient is not 1 (a loss scale); x has to be unchanged until then. False: it
+                       is computed by `backward`, and not at all if that never comes.
 
     Neither teacher nor weight is differentiated. A row whose logits are all -inf contributes nothing."""
     assert reduction in ["mean", "sum", "none"] or reduction is None

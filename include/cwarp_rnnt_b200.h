@@ -400,13 +400,17 @@ CWRNNT_API int cwrnnt_token_scores_backward(const cwrnnt_rows *p, const void *x,
  *   tail = 0  the teacher's values are renormalised, q = softmax(teacher / tau) over the list; D = sum q (ln q - ln p)
  *   weight    [n_rows] costs type or NULL (1): a row's factor; rows of weight 0 are not read
  *   upstream, upstream_stride   costs type: the gradient of row r's weighted divergence is multiplied by
- *             upstream[r * upstream_stride] (stride 0 or 1; NULL: 1)
+ *             upstream[r * upstream_stride] (stride 0 or 1; NULL: 1). CWRNNT_UPSTREAM_UNLESS_ONE: one factor for all
+ *             rows, and grad_x, which holds the gradient for a factor of 1 from an earlier call, is left as it is where the
+ *             factor is 1 (no row_loss, no loss). A stored gradient of a 16-bit type is not multiplied instead: what lay
+ *             below the type's range or digits before the factor cannot be had back
  *   scale     factor of the summed loss and of the gradient (1 / rows for a mean)
  *   row_loss  [n_rows] costs type or NULL: weight * D
  *   loss      1 element of the costs type or NULL: scale * sum(weight * D), added up in a fixed order
  *   grad_x    [n_rows, V] or NULL, fully written: upstream * scale * weight * dD/dx
  *   workspace cwrnnt_distill_workspace_bytes(p) bytes, 8-byte aligned; only needed for `loss`
  */
+#define CWRNNT_UPSTREAM_UNLESS_ONE (-1)
 CWRNNT_API int64_t cwrnnt_distill_workspace_bytes(const cwrnnt_rows *p);
 CWRNNT_API int cwrnnt_distill(const cwrnnt_rows *p, int32_t tail, const void *x, const void *teacher,
                               const int32_t *indices, const void *weight, const void *upstream,

@@ -1,0 +1,25 @@
+"""CPU-side checks of the row operators' and the linear layers' argument checks and host plans."""
+import ctypes
+
+import pytest
+
+from compactwarprnntloss_b200 import capi
+
+ONE = ctypes.c_void_p(256)  # never followed: the call is refused first, or has no rows
+
+
+def _rows(**kw):
+    d = dict(n_rows=10, x_stride=64, grad_stride=64, temperature=1.0, V=64, dtype=capi.F16, n_list=2, top_k=0)
+    d.update(kw)
+    return ctypes.byref(capi.Rows(**d))
+
+
+@pytest.mark.parametrize("upstream,row_loss,loss,grad", [(None, None, None, ONE), (ONE, ONE, None, ONE), (ONE, None, ONE, ONE),
+                                                         (ONE, None, None, None)])
+def test_a_gradient_is_made_anew_from_a_factor_and_into_a_gradient_only(upstream, row_loss, loss, grad):
+    call = capi.lib().cwrnnt_distill
+    for stride in (capi.UPSTREAM_UNLESS_ONE,):
+        assert call(_rows(), 1, ONE, ONE, ONE, None, upstream, stride, 1.0, ONE, 1 << 20, row_loss, loss, grad, None) == 1
+    assert call(_rows(n_rows=0), 1, None, None, None, None, None, capi.UPSTREAM_UNLESS_ONE, 1.0, None, 0, None, None, None,
+                None) == 0
+    assert call(_rows(), 1, ONE, ONE, ONE, None, ONE, -2, 1.0, ONE, 1 << 20, None, None, ONE, None) == 1
