@@ -569,7 +569,15 @@ std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> token_scores_ad(const tor
     return {lp, ent, top, index};
 }
 
-bool being_captured() { return at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None; }
+// The capture that the current stream is in, 0: none.
+int64_t current_capture()
+{
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return 0;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    C10_CUDA_CHECK(cudaStreamGetCaptureInfo(at::cuda::getCurrentCUDAStream(), &status, &id));
+    return static_cast<int64_t>(id);
+}
 
 class DistillFn : public torch::autograd::Function<DistillFn> {
 public:
@@ -585,7 +593,7 @@ public:
         ctx->saved_data["scale"] = scale;
         if (grad) ctx->saved_data["grad"] = *grad;
         const c10::cuda::CUDAGuard guard(x.device());
-        ctx->saved_data["captured"] = being_captured();
+        ctx->saved_data["capture"] = current_capture();
         return reduced ? *loss : *rows;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
@@ -599,10 +607,10 @@ public:
                                         ctx->saved_data["scale"].toDouble(), false, false, true, made));
         };
         const auto eager = ctx->saved_data.find("grad");
-        if (eager != ctx->saved_data.end() && ctx->saved_data["captured"].toBool() == being_captured()) {
+        if (eager != ctx->saved_data.end() && ctx->saved_data["capture"].toInt() == current_capture()) {
             // computed during forward for an upstream gradient of 1; handed over once (a second backward over a
-            // retained graph recomputes it below, and so does one that is captured without its forward: replayed, it
-            // would scale the one gradient again and again)
+            // retained graph recomputes it below, and so does one that is captured without its forward, or in a graph
+            // of its own: replayed by itself, it would scale the one gradient again and again)
             out[0] = eager->second.toTensor();
             ctx->saved_data.erase(eager);
             // Of a mean over many rows float16 keeps few digits of a gradient and none below 2^-25 (a token of probability
