@@ -518,6 +518,13 @@ variable_list once_differentiable(variable_list grads, const char *name)
 }
 OptTensor some(const torch::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
+// None of them has a forward-mode derivative either. A tensor with a tangent need not require a gradient, so the autograd
+// functions may not see it, and the tangent would be dropped and read as zero.
+void refuse_tangent(const OptTensor &t, const char *name)
+{
+    TORCH_CHECK(!(t && t->defined() && t->_fw_grad(0).defined()), name, " has no forward-mode derivative");
+}
+
 class TokenScoresFn : public torch::autograd::Function<TokenScoresFn> {
 public:
     // outputs: those of (log_probs, entropy, top_log_probs, top_indices) that were asked for
@@ -558,6 +565,7 @@ public:
 std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> token_scores_ad(const torch::Tensor &x, const OptTensor &targets,
                                                                        int64_t top_k, bool entropy, double temperature)
 {
+    refuse_tangent(x, "token_scores");
     if (!(at::GradMode::is_enabled() && x.requires_grad())) {
         auto [lp, ent, top, index, stats] = token_scores(x, targets, top_k, entropy, temperature, false);
         return {lp, ent, top, index};
@@ -630,6 +638,7 @@ public:
 torch::Tensor distill_ad(const torch::Tensor &x, const torch::Tensor &teacher, const torch::Tensor &indices,
                          const OptTensor &weight, bool tail, double temperature, double scale, bool reduced, bool eager)
 {
+    refuse_tangent(x, "distill_loss");
     if (at::GradMode::is_enabled() && x.requires_grad())
         return DistillFn::apply(x, teacher, indices, weight, tail, temperature, scale, reduced, eager);
     auto [rows, loss, grad] =
@@ -671,6 +680,7 @@ public:
 torch::Tensor linear_ad(const torch::Tensor &x, const torch::Tensor &weight, const OptTensor &bias,
                         const OptTensor &residual, int64_t activation)
 {
+    for (const OptTensor &t : {OptTensor(x), OptTensor(weight), bias, residual}) refuse_tangent(t, "fused_linear");
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) ||
                                        (residual && residual->requires_grad())))
         return LinearFn::apply(x, weight, bias, residual, activation);

@@ -39,7 +39,8 @@ def distill_loss(x: torch.Tensor, teacher: torch.Tensor, indices: torch.Tensor, 
                        where the upstream gradient is not 1 (a loss scale); x has to be unchanged until then. False: it
                        is computed by `backward`, and not at all if that never comes.
 
-    Neither teacher nor weight is differentiated. A row whose logits are all -inf contributes nothing."""
+    Neither teacher nor weight is differentiated. A row whose logits are all -inf contributes nothing. Reverse
+    mode, once: second and forward-mode derivatives of x are refused."""
     assert reduction in ["mean", "sum", "none"] or reduction is None
     assert x.dim() >= 1 and x.size(-1) >= 1
     lead = x.shape[:-1]

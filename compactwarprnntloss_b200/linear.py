@@ -24,7 +24,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
                  residual: Optional[torch.Tensor] = None, *, activation: Optional[str] = None) -> torch.Tensor:
     """act(x W^T + bias) + residual: x [..., n_in], weight [n_out, n_in], bias [n_out], residual [..., n_out], all of
     one type (float16 or bfloat16) on one device. activation: None, 'relu', 'tanh' or 'silu'. Differentiable in all
-    four tensors; rows of x and weight may be strided."""
+    four tensors, in reverse mode, once (second and forward-mode derivatives are refused); rows of x and weight may be
+    strided."""
     assert activation in LINEAR_ACTIVATIONS
     assert x.dim() >= 1 and weight.dim() == 2 and x.size(-1) == weight.size(1)
     assert x.dtype in (torch.float16, torch.bfloat16), "fused_linear takes float16 and bfloat16"

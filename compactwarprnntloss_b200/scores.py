@@ -49,7 +49,8 @@ def token_scores(x: torch.Tensor, targets: Optional[torch.Tensor] = None, *, top
     top_k        number of best alternatives, 0 <= top_k <= min(V, 32)
     entropy      whether to compute the rows' entropy
 
-    A row whose logits are all -inf has log-probabilities of -inf, entropy 0 and a zero gradient."""
+    A row whose logits are all -inf has log-probabilities of -inf, entropy 0 and a zero gradient. Reverse mode, once:
+    second and forward-mode derivatives are refused."""
     assert x.dim() >= 1 and x.size(-1) >= 1
     assert targets is not None or top_k > 0 or entropy, "nothing asked for"
     lead = x.shape[:-1]
