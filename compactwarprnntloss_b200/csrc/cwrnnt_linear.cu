@@ -891,8 +891,8 @@ Cut cut_product(int64_t M, int N, int steps)
         const int64_t cost = w.launch + waves * (main > w.epilogue ? main : w.epilogue);
         if (c.bn == 0 || cost < best) c = t, best = cost;
     }
-    // split long sums of few tiles, at least eight steps a part
-    if (c.tiles(M, N) * 2 <= kNumSMs && steps >= 32) {
+    // split long sums of few tiles (of none where there are no rows), at least eight steps a part
+    if (M > 0 && c.tiles(M, N) * 2 <= kNumSMs && steps >= 32) {
         // wide tiles again: parts give the SMs their work
         c.bn = N > 128 && M > 128 ? 256 : (N > 64 ? 128 : 64);
         int64_t parts = c.at_once() / c.tiles(M, N);

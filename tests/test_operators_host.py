@@ -47,3 +47,16 @@ def test_tangents_are_refused():
                 call()
         with pytest.raises(RuntimeError, match="CUDA"):  # no tangent: the next check
             token_scores(x, t)
+
+
+@pytest.mark.parametrize("n_in", [1, 64, 640, 1984, 1985, 2048, 20000])
+@pytest.mark.parametrize("n_out", [1, 48, 1024, 2048, 50257])
+def test_layers_without_rows_have_a_workspace(n_in, n_out):
+    """No rows are no tiles; how a long sum is split over few tiles is not to divide by their number."""
+    L = capi.lib()
+    for act in range(4):
+        p = ctypes.byref(capi.Linear(0, n_in, n_in, n_out, n_in, n_out, capi.BF16, act))
+        for which in range(3):
+            assert L.cwrnnt_linear_workspace_bytes(p, which) >= 256
+        assert L.cwrnnt_linear_forward(p, None, None, None, None, None, 0, None, None) == 0
+        assert L.cwrnnt_linear_backward(p, None, None, None, None, None, 0, None, None, None, None) == 0
