@@ -376,12 +376,12 @@ struct Carrier {
             *piece_group(out_piece, lane, g) = w;
         }
     }
-    // The piece's rows added up: columns 2 * lane and 2 * lane + 1. (Rows behind the matrix are zero: their upstream
-    // gradient is.)
-    __device__ __forceinline__ void add_rows(unsigned char *piece, float &s0, float &s1) const
+    // The piece's first n rows added up: columns 2 * lane and 2 * lane + 1. (Rows behind the matrix are no sum of anything:
+    // their upstream gradient is zero, but their z is NaN where a weight is infinite.)
+    __device__ __forceinline__ void add_rows(unsigned char *piece, int n, float &s0, float &s1) const
     {
 #pragma unroll 8
-        for (int k = 0; k < 32; ++k) {
+        for (int k = 0; k < n; ++k) {
             const uint32_t w = reinterpret_cast<const uint32_t *>(piece_group(piece, k, lane >> 2))[lane & 3];
             float v[8];
             E::unpack(make_uint4(w, 0u, 0u, 0u), v);
@@ -439,8 +439,9 @@ struct Carrier {
             if (ep.low) tc::store_2d(map_low, low_piece, col, int(out_row0));
         }
         float s0 = 0.0f, s1 = 0.0f;
-        if (ep.sums) add_rows(out_piece, s0, s1);
-        if (ep.sums && ep.low) add_rows(low_piece, s0, s1);
+        const int rows = M - row0 < 32 ? int(M - row0) : 32;
+        if (ep.sums) add_rows(out_piece, rows, s0, s1);
+        if (ep.sums && ep.low) add_rows(low_piece, rows, s0, s1);
         if (ep.sums) {
             float *to = ep.sums + int64_t(row0 / 32) * N + col + 2 * lane;
             if (col + 2 * lane < N) to[0] = s0;
