@@ -447,6 +447,7 @@ scores_grad_kernel(const ScoresGradArgs<T> a)
         c1 = -gh * A(kLn2);
     }
     c0 *= scale, c1 *= scale;
+    if (nothing) c0 = c1 = A(0);  // (whatever an upstream gradient of -inf's is: zero times a NaN is none)
     if (active) {
         for (int at = 0; at < rv.count; at += LPR * NV) {
 #pragma unroll
