@@ -922,6 +922,12 @@ template <typename T, int BN, bool A_MN, bool B_MN>
 cudaError_t run_product(const Matrix &a, const Matrix &b, Shape sh, const Epilogue &ep, cudaStream_t s)
 {
     using L = Layout<BN>;
+    auto kernel = linear_kernel<T, BN, A_MN, B_MN>;
+    // The attribute belongs to the device that is current. This comes before the tensor maps: the driver's encoder wants a
+    // context bound to the calling thread, which the runtime does with its first call that needs one (a thread of autograd's,
+    // or of the caller's, may not have made any).
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::most_bytes());
+    if (e != cudaSuccess) return e;
     CUtensorMap ma, mb, mo{}, ms{}, ml{};
     bool good = make_map<T>(&ma, a.p, a.rows, a.cols, a.ld, A_MN ? kBK : kBM) &&
                 make_map<T>(&mb, b.p, b.rows, b.cols, b.ld, B_MN ? kBK : L::kRowsB);
@@ -936,10 +942,6 @@ cudaError_t run_product(const Matrix &a, const Matrix &b, Shape sh, const Epilog
     if (!good) return cudaErrorInvalidValue;
     const int pieces = ep.pieces();
     sh.stages = L::stages(pieces);
-    auto kernel = linear_kernel<T, BN, A_MN, B_MN>;
-    // the attribute belongs to the device that is current
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::most_bytes());
-    if (e != cudaSuccess) return e;
     const int ctas = L::kPair ? 2 : 1;
     const int64_t total = sh.tiles_m * sh.tiles_n * sh.splits * ctas;
     cudaLaunchConfig_t cfg{};
