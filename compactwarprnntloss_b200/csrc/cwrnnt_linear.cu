@@ -4,7 +4,11 @@
 // Nothing but the inputs is kept for the gradients: z is multiplied out again, and the epilogue of that product writes
 // dz at once (reading dy). Storing z in float instead costs more traffic than the product takes, storing it in 16 bits
 // costs digits of act'(z). dz goes into its two products as the sum of two 16-bit matrices, the second what the first
-// loses in its rounding: with the first alone the gradients would be off by half as much again as their own rounding.
+// loses in its rounding: with the first alone the gradients would be off by half as much again as their own rounding. The
+// second part of a float16 dz is held 2^11 times larger, or it would be below the type's range wherever dz is (upstream
+// gradients of a mean over many rows): both parts together keep dz to 2^-22 of itself, and to 2^-36 where that is less. The
+// tensor cores take the factor out: the second part's products are summed first, and scaled by 2^-11 as the first part's
+// first product is added.
 //
 // One kernel for the four products: tiles of 128 x 64 or 128 outputs, or of 256 x 256 shared by two CTAs, 64 elements of
 // the sum a step. Operands come by tiled TMA into a ring of 128-byte-swizzled stages; tcgen05.mma sums in TMEM in float.
@@ -119,7 +123,7 @@ struct Epilogue {
     bool tma_out;            // rows of out lie on 16-byte boundaries: they go by TMA (rows of side always do)
     bool vec;                // all 16-byte accesses allowed, columns in whole groups of 8
     float *sums;             // kSlope: sums over each 32 rows of dz, [rows / 32, N], or null
-    void *low;               // kSlope: what dz loses in its rounding, rounded again, as `out`; or null
+    void *low;               // kSlope: what dz loses in its rounding, scaled and rounded again, as `out`; or null
     __host__ __device__ int pieces() const { return 1 + (side != nullptr) + (low != nullptr); }
 };
 
@@ -146,12 +150,19 @@ __device__ __forceinline__ float finish_as(const Epilogue &ep, float v, float si
     return finish_one<CWRNNT_ACT_NONE>(slope, z, s).x;
 }
 
-// What v loses when it is rounded to T, rounded to T.
+// The low part of dz is held 2^kLowShift times larger: bfloat16 has float's range; what a float16 loses is at most 16, and
+// 16 * 2^11 is in its range.
+template <typename T>
+constexpr int kLowShift = Elt<T>::kBf16 ? 0 : 11;
+template <typename T>
+constexpr float kLowScale = float(1 << kLowShift<T>);
+
+// What v loses when it is rounded to T, scaled and rounded to T.
 template <typename T>
 __device__ __forceinline__ T low_part(float v)
 {
     const float high = Elt<T>::to_acc(Elt<T>::from_acc(v));
-    return Elt<T>::from_acc(fabsf(high) < INFINITY ? v - high : 0.0f);
+    return Elt<T>::from_acc(fabsf(high) < INFINITY ? (v - high) * kLowScale<T> : 0.0f);
 }
 
 // All bits of the halves of a word that are finite.
@@ -210,7 +221,7 @@ struct Shape {
     int64_t M;
     int N;
     int steps;       // steps of kBK along the sum, in all
-    int half_steps;  // of them, those of A's first part: A may be the sum of two matrices (0: it is one)
+    int half_steps;  // of them, those of A's low part, the first ones: A may be a matrix and a low part (0: it is one)
     int steps_per_split, splits;
     int64_t tiles_m;
     int tiles_n;
@@ -237,6 +248,8 @@ struct Shape {
         const int left = steps - first_step(split);
         return left < steps_per_split ? left : steps_per_split;
     }
+    // a part of the sum that holds products of the low part only
+    __device__ __forceinline__ bool low_only(int split) const { return first_step(split) + count_steps(split) <= half_steps; }
 };
 
 // A warp of the epilogue carries 32 rows by pieces of 128 bytes (64 columns of 16 bits, 32 of a part's floats) through a
@@ -354,7 +367,11 @@ struct Carrier {
             if constexpr (KIND == kSlopeOf + CWRNNT_ACT_TANH || KIND == kSlopeOf + CWRNNT_ACT_SILU) {
                 E::unpack(w, s);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] -= s[i];
+                for (int i = 0; i < 8; i += 2) {
+                    float2 lost = __ffma2_rn(make_float2(s[i], s[i + 1]), both(-1.0f), make_float2(v[i], v[i + 1]));
+                    if (kLowShift<T> > 0) lost = __fmul2_rn(lost, both(kLowScale<T>));
+                    v[i] = lost.x, v[i + 1] = lost.y;
+                }
                 const uint4 low = E::pack(v);
                 *piece_group(low_piece, lane, g) = make_uint4(low.x & finite_mask<T>(w.x), low.y & finite_mask<T>(w.y),
                                                               low.z & finite_mask<T>(w.z), low.w & finite_mask<T>(w.w));
@@ -362,7 +379,7 @@ struct Carrier {
         }
     }
     template <typename Release>
-    __device__ __forceinline__ void columns_of_part(uint32_t d, int row0, int next_col, bool ok, Release &release)
+    __device__ __forceinline__ void columns_of_part(uint32_t d, float factor, int next_col, bool ok, Release &release)
     {
         uint32_t r[32];
         tc::tmem_load32(d, r);
@@ -372,6 +389,10 @@ struct Carrier {
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
             uint4 w = make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
+            if constexpr (kLowShift<T> > 0) {
+                w.x = __float_as_uint(__uint_as_float(w.x) * factor), w.y = __float_as_uint(__uint_as_float(w.y) * factor);
+                w.z = __float_as_uint(__uint_as_float(w.z) * factor), w.w = __float_as_uint(__uint_as_float(w.w) * factor);
+            }
             if (!ok) w = make_uint4(~0u, ~0u, ~0u, ~0u);
             *piece_group(out_piece, lane, g) = w;
         }
@@ -380,18 +401,25 @@ struct Carrier {
     // their upstream gradient is zero, but their z is NaN where a weight is infinite.)
     __device__ __forceinline__ void add_rows(unsigned char *piece, int n, float &s0, float &s1) const
     {
-#pragma unroll 8
-        for (int k = 0; k < n; ++k) {
+        auto add = [&](int k) {
             const uint32_t w = reinterpret_cast<const uint32_t *>(piece_group(piece, k, lane >> 2))[lane & 3];
             float v[8];
             E::unpack(make_uint4(w, 0u, 0u, 0u), v);
             s0 += v[0], s1 += v[1];
+        };
+        if (n == 32) {
+#pragma unroll 8
+            for (int k = 0; k < 32; ++k) add(k);
+        } else {
+#pragma unroll 1
+            for (int k = 0; k < n; ++k) add(k);
         }
     }
-    // `d`: TMEM address of the piece's first column in this warp's lanes; `release`: gives the tile's sums back
+    // `d`: TMEM address of the piece's first column in this warp's lanes; `factor`: of a part's sums; `release`: gives the
+    // tile's sums back
     template <typename Release>
-    __device__ __forceinline__ void piece(uint32_t d, int row0, int64_t out_row0, int col, bool ok, int next_col,
-                                          Release &release)
+    __device__ __forceinline__ void piece(uint32_t d, int row0, int64_t out_row0, int col, float factor, bool ok,
+                                          int next_col, Release &release)
     {
         if (ep.mode != kPart) {
             bias[lane] = next_bias[0], bias[32 + lane] = next_bias[1];
@@ -404,7 +432,7 @@ struct Carrier {
         __syncwarp();
 #define CWRNNT_KIND(KIND, SIDE) columns<KIND, SIDE>(d, row0, next_col, ok, release)
         if (ep.mode == kPart) {
-            columns_of_part(d, row0, next_col, ok, release);
+            columns_of_part(d, factor, next_col, ok, release);
         } else if (ep.mode == kSlope) {
             if (ep.act == CWRNNT_ACT_RELU)
                 CWRNNT_KIND(kSlopeOf + CWRNNT_ACT_RELU, true);
@@ -441,7 +469,11 @@ struct Carrier {
         float s0 = 0.0f, s1 = 0.0f;
         const int rows = M - row0 < 32 ? int(M - row0) : 32;
         if (ep.sums) add_rows(out_piece, rows, s0, s1);
-        if (ep.sums && ep.low) add_rows(low_piece, rows, s0, s1);
+        if (ep.sums && ep.low) {
+            float l0 = 0.0f, l1 = 0.0f;
+            add_rows(low_piece, rows, l0, l1);
+            s0 += l0 * (1.0f / kLowScale<T>), s1 += l1 * (1.0f / kLowScale<T>);
+        }
         if (ep.sums) {
             float *to = ep.sums + int64_t(row0 / 32) * N + col + 2 * lane;
             if (col + 2 * lane < N) to[0] = s0;
@@ -526,8 +558,8 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 for (int t_k = k0; ok && t_k < k1; ++t_k) {
                     ok = tc::mbar_wait(&empty[at], phase ^ 1, &ctl.gave_up);
                     if (!ok) break;
-                    const bool low = sh.half_steps > 0 && t_k >= sh.half_steps;
-                    const int k = low ? t_k - sh.half_steps : t_k;
+                    const bool low = t_k < sh.half_steps;
+                    const int k = low ? t_k : t_k - sh.half_steps;
                     const CUtensorMap *const from_a = low ? &map_low : &map_a;
                     unsigned char *a = stages + at * L::kStage, *b = a + L::kA;
                     if (rank == 0) tc::mbar_expect(&full[at], L::kStage * kCtas);
@@ -580,6 +612,8 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 tc::fence_after();
                 const uint32_t d = tmem + uint32_t(half * BN);
                 const int steps = sh.count_steps(split);
+                // the step before which the low part's sum is scaled, if there is one here
+                const int scaled = kLowShift<T> > 0 ? sh.half_steps - sh.first_step(split) : 0;
                 for (int k = 0; ok && k < steps; ++k) {
                     ok = tc::mbar_wait(&full[at], phase, &ctl.gave_up);
                     if (!ok) break;
@@ -590,7 +624,10 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         // 16 elements of the sum: 32 bytes along a K-major row, 16 rows of an MN-major operand
                         const uint64_t da = tc::operand(a + i * (A_MN ? 2048 : 32), A_MN ? 8192 : 16, 1024);
                         const uint64_t db = tc::operand(b + i * (B_MN ? 2048 : 32), B_MN ? 8192 : 16, 1024);
-                        tc::mma_f16<kPair>(d, da, db, idesc, k > 0 || i > 0);
+                        if (kLowShift<T> > 0 && i == 0 && k > 0 && k == scaled)
+                            tc::mma_f16_scaled<kPair, kLowShift<T>>(d, da, db, idesc);
+                        else
+                            tc::mma_f16<kPair>(d, da, db, idesc, k > 0 || i > 0);
                     }
                     tc::commit<kPair>(&empty[at]);
                     if (++at == sh.stages) at = 0, phase ^= 1;
@@ -629,6 +666,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             tc::fence_after();
             __syncwarp();
             const uint32_t d = tmem + uint32_t(half * BN) + (uint32_t(quarter * 32) << 16);
+            const float factor = sh.low_only(split) ? 1.0f / kLowScale<T> : 1.0f;
             auto release = [&] {  // this half of TMEM is free for another tile's sums
                 tc::fence_before();
                 __syncwarp();
@@ -642,7 +680,8 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             if (!mine) release();
             for (; mine && col < end; col += kShares * step) {
                 const int next = col + kShares * step;
-                c.piece(d + uint32_t(col - n0), row0, split * sh.part_rows + row0, col, ok, next < end ? next : -1, release);
+                c.piece(d + uint32_t(col - n0), row0, split * sh.part_rows + row0, col, factor, ok, next < end ? next : -1,
+                        release);
             }
             if (++half == 2) half = 0, half_phase ^= 1;
         }
@@ -770,8 +809,8 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ 
     const int col = blockIdx.x * 256 + tx * 8;
     float acc[8] = {};
     const int64_t first = int64_t(blockIdx.y) * run, end = first + run < rows ? first + run : rows;
-    for (const T *g : {high, low}) {
-        if (!g || col >= cols) break;
+    for (const T *g : {low, high}) {
+        if (!g || col >= cols) continue;
         for (int64_t r = first + ty; r < end; r += kSumRows) {
             float v[8];
             if (col + 8 <= cols) {
@@ -782,6 +821,10 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ 
             }
 #pragma unroll
             for (int c = 0; c < 8; ++c) acc[c] += v[c];
+        }
+        if (g == low) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[c] *= 1.0f / kLowScale<T>;
         }
     }
 #pragma unroll
@@ -915,7 +958,7 @@ struct Matrix {  // [rows, cols], `mn`: its columns are the output's and its row
     const void *p;
     int64_t rows, cols, ld;
     bool mn;
-    const void *low = nullptr;  // another matrix of the same shape to be added to it, or none
+    const void *low = nullptr;  // another matrix of the same shape to be added to it, 2^kLowShift times too large, or none
 };
 
 template <typename T, int BN, bool A_MN, bool B_MN>

@@ -155,6 +155,21 @@ __device__ __forceinline__ void mma_f16(uint32_t tmem, uint64_t a, uint64_t b, u
                      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
                      : "memory");
 }
+// The same with D scaled first: D = A * B + D * 2^-SHIFT, SHIFT at most 15.
+template <bool PAIR, int SHIFT>
+__device__ __forceinline__ void mma_f16_scaled(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc)
+{
+    if (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}" ::"r"(tmem),
+                     "l"(a), "l"(b), "r"(idesc), "n"(SHIFT)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}" ::"r"(tmem),
+                     "l"(a), "l"(b), "r"(idesc), "n"(SHIFT)
+                     : "memory");
+}
 // The barrier (of a pair: that of both CTAs) completes when every mma issued so far by this thread has.
 template <bool PAIR>
 __device__ __forceinline__ void commit(uint64_t *bar)
