@@ -591,9 +591,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             for (int i = 0; rank == 0 && i < sh.stages; ++i) {
                 if (!(started >> i & 1)) continue;
                 const uint32_t last = i < at ? phase : phase ^ 1;
-                const uint64_t since = tc::now_ns();
-                while (!tc::mbar_try(&full[i], last) && tc::now_ns() - since < 2000000000ull) {
-                }
+                tc::mbar_drain(&full[i], last);
             }
         }
     } else if (warp == 1) {
@@ -637,9 +635,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             }
             // every product has left the tensor core before the CTA's memory goes
             tc::commit<kPair>(&ctl.drained);
-            const uint64_t since = tc::now_ns();
-            while (!tc::mbar_try(&ctl.drained, 0) && tc::now_ns() - since < 2000000000ull) {
-            }
+            tc::mbar_drain(&ctl.drained, 0);
         }
     } else {
         const int quarter = warp & 3;  // the TMEM lanes that this warp may read

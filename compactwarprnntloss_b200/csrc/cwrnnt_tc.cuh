@@ -63,20 +63,42 @@ __device__ __forceinline__ uint64_t now_ns()
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// Waits for a phase, for two seconds at most. `gave_up` is the CTA's flag (shared memory): whoever runs out of time
+// How long a wait has lasted: two seconds of the CTA's own time. The timer runs on while a CTA is off its SM (another
+// process's turn on the GPU, a debugger), and a wait that such a break alone made long is not to run out: of what passes between
+// two looks at the timer, 20 ms count at most. The waits end all the same, as every look counts what has passed.
+struct Patience {
+    static constexpr uint64_t kLimit = 2000000000ull, kMostAtOnce = 20000000ull;  // ns
+    uint64_t last, waited;
+    __host__ __device__ explicit Patience(uint64_t now) : last(now), waited(0) {}
+    __host__ __device__ bool spent(uint64_t now)
+    {
+        const uint64_t step = now - last;
+        waited += step < kMostAtOnce ? step : kMostAtOnce;
+        last = now;
+        return waited > kLimit;
+    }
+};
+// Waits for a phase, as long as its patience lasts. `gave_up` is the CTA's flag (shared memory): whoever runs out of time
 // sets it, and everyone else stops waiting then. Returns whether the phase came.
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up)
 {
     if (mbar_try(bar, parity)) return true;
-    const uint64_t start = now_ns();
+    Patience patience(now_ns());
     for (;;) {
         for (int i = 0; i < 32; ++i)
             if (mbar_try(bar, parity)) return true;
         if (*gave_up) return false;
-        if (now_ns() - start > 2000000000ull) {
+        if (patience.spent(now_ns())) {
             *gave_up = 1;
             return false;
         }
+    }
+}
+// The same for what has to come before the CTA's memory goes, whether others have given up or not.
+__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity)
+{
+    Patience patience(now_ns());
+    while (!mbar_try(bar, parity) && !patience.spent(now_ns())) {
     }
 }
 

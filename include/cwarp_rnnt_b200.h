@@ -426,7 +426,8 @@ CWRNNT_API int cwrnnt_distill(const cwrnnt_rows *p, int32_t tail, const void *x,
  * nothing but the inputs is kept for it. x, weight and grad_y may have rows further apart than their length; where such
  * a stride is a multiple of 8 elements the matrix must start on a 16-byte boundary, other strides are copied first (into
  * the workspace). bias, residual and all outputs are contiguous; a residual of n_out a multiple of 8 starts on a 16-byte
- * boundary. Sums are split and joined in a fixed order: results repeat bit for bit. Every wait inside the kernels is bounded (two seconds); a tile whose wait runs out is NaN.
+ * boundary. Sums are split and joined in a fixed order: results repeat bit for bit. Every wait inside the kernels is bounded
+ * (two seconds, not counting the time that another process has the GPU); a tile whose wait runs out is NaN.
  * workspace: cwrnnt_linear_workspace_bytes(p, pass) bytes, 256-byte aligned; not shared by calls that may overlap.
  */
 #define CWRNNT_ACT_SILU 3 /* z / (1 + exp(-z)); cwrnnt_linear_* only */
