@@ -20,9 +20,11 @@
 // workspace, added in a fixed order by a second kernel that carries the same epilogue.
 // TMA wants rows at multiples of 16 bytes: matrices of other strides are copied to such a stride first.
 //
-// Bound: the tensor cores under the power limit for large products (314340 x 1024 x 640 bf16: 0.37 ms, 1.1 PFLOP/s,
-// within a tenth of the library's bare product); for short sums what a tile's operands take from L2 and, with tanh
-// or silu, the epilogue's instructions (40009 x 640 x 512 f16: 36 us plain, 54 with tanh and residual).
+// Bound: for large products what lies between a tile's steps (314340 x 1024 x 640 bf16: 0.36 ms, 1.14 PFLOP/s, where the
+// library's bare product takes 0.34 in the same run; the tensor pipe is active 60 % of one launch's cycles, at 31 bytes a clock
+// and SM from L2) and the clock under the power limit (0.41 to 0.43 ms in a long run); with tanh or silu the epilogue's
+// instructions (40009 x 640 x 512 f16: 36 us plain, 54 with tanh and residual). Sides that are no multiple of 8 cost a copy of
+// their matrix, and an output of such a width leaves by 2-byte stores: 314340 x 1024 x 639 0.78 ms, 314340 x 1023 x 640 0.60.
 #include "cwrnnt_kernels.h"
 #include "cwrnnt_tc.cuh"
 

@@ -12,13 +12,15 @@
 // (4 KB) stay in the registers of the lanes that share them, longer ones run through a warp or a CTA each with their
 // statistics alongside; the selection of the largest entries reads those again, from L1 or L2. Without a selection the
 // traffic is the bound (314340 x 1024 f32, two targets and the entropy: 0.22 ms, 6.0 TB/s; its gradient 0.44 ms, 5.8
-// TB/s), with one and with short rows the instructions (80003 x 4096 bf16, sixteen largest: 0.19 ms, 3.4 TB/s;
-// 2051 x 50257 f16, twenty: 0.07 ms, 3.0 TB/s; 600011 x 128 f16, four: 0.09 ms, 2.0 TB/s).
+// TB/s), with one and with short rows the instructions (80003 x 4096 bf16, sixteen largest: 0.20 ms, 3.4 TB/s, 80 % of issue
+// slots; 2051 x 50257 f16, twenty: 0.07 ms, 3.0 TB/s, 73 %, the second reading from L2; 600011 x 128 f16, four: 0.09 ms, 2.0
+// TB/s).
 //
 // Selection: of the lanes' own maxima, the largest value that at least k of them reach is a lower bound of the row's
 // k-th largest entry. The entries at or above it - about as many as k - are collected in shared memory and ranked by
-// counting how many come before each. Rows with too many equal entries for that, and rows with NaN, are picked one
-// entry at a time instead.
+// counting how many come before each. Rows with too many equal entries for that, rows with NaN, and long rows that a mask
+// leaves fewer live lanes than the bar is taken from, are picked one entry at a time instead, by a warp that goes over the row
+// for each: right, but slow (2051 x 50257 f16 with ten tokens left: eight largest 2.6 ms, twenty 6.1).
 #include "cwrnnt_kernels.h"
 #include "cwrnnt_rowops.cuh"
 
@@ -64,7 +66,7 @@ __device__ __forceinline__ void emit_target(const ScoresArgs<T> &a, const T *row
     a.log_probs[r * a.n_targets + i] = lp;
 }
 
-// Candidate keys of rows held in registers: 16-bit rows fit 32 bits (at most 32 * 16 * 8 entries).
+// Candidate keys of rows held in registers: 16-bit rows fit 32 bits (at most 256 vectors of 8 entries).
 template <typename T>
 struct Candidate {
     using Key = TopKey<typename Elt<T>::acc>;

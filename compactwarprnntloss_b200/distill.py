@@ -37,7 +37,8 @@ def distill_loss(x: torch.Tensor, teacher: torch.Tensor, indices: torch.Tensor, 
                        `backward` only scales it (nothing is touched when the upstream gradient is 1). float16
                        gradients are not scaled, which would lose what lies below their range, but computed once more
                        where the upstream gradient is not 1 (a loss scale); x has to be unchanged until then. False: it
-                       is computed by `backward`, and not at all if that never comes.
+                       is computed by `backward`, and not at all if that never comes; with a loss scale on float16 that
+                       is the shorter way.
 
     Neither teacher nor weight is differentiated. A row whose logits are all -inf contributes nothing. Reverse
     mode, once: second and forward-mode derivatives of x are refused."""
