@@ -8,7 +8,8 @@
 // second part of a float16 dz is held 2^11 times larger, or it would be below the type's range wherever dz is (upstream
 // gradients of a mean over many rows): both parts together keep dz to 2^-22 of itself, and to 2^-36 where that is less. The
 // tensor cores take the factor out: the second part's products are summed first, and scaled by 2^-11 as the first part's
-// first product is added.
+// first product is added (40009 x 640 x 512 f16 tanh, all gradients: 5 us of 210, 3 of them for that one product of each tile,
+// 2 for the factor in the epilogue).
 //
 // One kernel for the four products: tiles of 128 x 64 or 128 outputs, or of 256 x 256 shared by two CTAs, 64 elements of
 // the sum a step. Operands come by tiled TMA into a ring of 128-byte-swizzled stages; tcgen05.mma sums in TMEM in float.
@@ -21,8 +22,8 @@
 // TMA wants rows at multiples of 16 bytes: matrices of other strides are copied to such a stride first.
 //
 // Bound: for large products what lies between a tile's steps (314340 x 1024 x 640 bf16: 0.36 ms, 1.14 PFLOP/s, where the
-// library's bare product takes 0.34 in the same run; the tensor pipe is active 60 % of one launch's cycles, at 31 bytes a clock
-// and SM from L2) and the clock under the power limit (0.41 to 0.43 ms in a long run); with tanh or silu the epilogue's
+// library's bare product takes 0.34 in the same run; the tensor pipe is active 60 % of one launch's cycles, with 8.6 TB/s from
+// L2) and the clock under the power limit (0.41 to 0.43 ms in a long run); with tanh or silu the epilogue's
 // instructions (40009 x 640 x 512 f16: 36 us plain, 54 with tanh and residual). Sides that are no multiple of 8 cost a copy of
 // their matrix, and an output of such a width leaves by 2-byte stores: 314340 x 1024 x 639 0.78 ms, 314340 x 1023 x 640 0.60.
 #include "cwrnnt_kernels.h"
@@ -612,23 +613,25 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 tc::fence_after();
                 const uint32_t d = tmem + uint32_t(half * BN);
                 const int steps = sh.count_steps(split);
-                // the step before which the low part's sum is scaled, if there is one here
-                const int scaled = kLowShift<T> > 0 ? sh.half_steps - sh.first_step(split) : 0;
+                // the step before which the low part's sum is scaled, if there is one here (only dz has a low part: B is
+                // MN-major then)
+                constexpr bool kScales = kLowShift<T> > 0 && B_MN;
+                const int scaled = kScales ? sh.half_steps - sh.first_step(split) : 0;
                 for (int k = 0; ok && k < steps; ++k) {
                     ok = tc::mbar_wait(&full[at], phase, &ctl.gave_up);
                     if (!ok) break;
                     tc::fence_after();
                     const uint32_t a = tc::smem_addr(stages + at * L::kStage), b = a + L::kA;
+                    // 16 elements of the sum: 32 bytes along a K-major row, 16 rows of an MN-major operand
+                    auto operand_a = [&](int i) { return tc::operand(a + i * (A_MN ? 2048 : 32), A_MN ? 8192 : 16, 1024); };
+                    auto operand_b = [&](int i) { return tc::operand(b + i * (B_MN ? 2048 : 32), B_MN ? 8192 : 16, 1024); };
+                    const bool scales = kScales && k > 0 && k == scaled;
+                    if (scales)
+                        tc::mma_f16_scaled<kPair, kLowShift<T>>(d, operand_a(0), operand_b(0), idesc);
+                    else
+                        tc::mma_f16<kPair>(d, operand_a(0), operand_b(0), idesc, k > 0);
 #pragma unroll
-                    for (int i = 0; i < kBK / 16; ++i) {
-                        // 16 elements of the sum: 32 bytes along a K-major row, 16 rows of an MN-major operand
-                        const uint64_t da = tc::operand(a + i * (A_MN ? 2048 : 32), A_MN ? 8192 : 16, 1024);
-                        const uint64_t db = tc::operand(b + i * (B_MN ? 2048 : 32), B_MN ? 8192 : 16, 1024);
-                        if (kLowShift<T> > 0 && i == 0 && k > 0 && k == scaled)
-                            tc::mma_f16_scaled<kPair, kLowShift<T>>(d, da, db, idesc);
-                        else
-                            tc::mma_f16<kPair>(d, da, db, idesc, k > 0 || i > 0);
-                    }
+                    for (int i = 1; i < kBK / 16; ++i) tc::mma_f16<kPair>(d, operand_a(i), operand_b(i), idesc, 1);
                     tc::commit<kPair>(&empty[at]);
                     if (++at == sh.stages) at = 0, phase ^= 1;
                 }
